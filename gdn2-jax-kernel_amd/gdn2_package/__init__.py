@@ -22,6 +22,7 @@ from .gdn2_fwd import (GDN2Error, GDN2ShapeError, gdn2_pallas_forward,
                        gdn2_pallas_forward_with_residuals)
 from .gdn2_pipeline import (gdn2_pallas_forward_trainable,
                             gdn2_pallas_forward_varlen_trainable)
+from .gdn2_scan import gdn2_gated_scan, gdn2_gated_scan_step
 
 __version__ = "0.1.0"
 
@@ -29,6 +30,7 @@ __all__ = [
     "gdn2_pallas_forward", "gdn2_pallas_forward_trainable",
     "gdn2_pallas_forward_with_residuals", "gdn2_pallas_forward_raw",
     "gdn2_pallas_forward_varlen", "gdn2_pallas_forward_varlen_trainable", "gdn2_decode_step",
+    "gdn2_gated_scan", "gdn2_gated_scan_step",
     "GDN2Error", "GDN2ShapeError",
     "GDN2LibraryError", "gdn2_fwd", "gdn2_bwd", "gdn2_pipeline", "__version__",
 ]

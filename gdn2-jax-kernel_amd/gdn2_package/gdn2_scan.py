@@ -1,0 +1,210 @@
+"""Gated linear recurrence, elementwise over the channels:
+
+    h_t = e^{g_t} h_{t-1} + b_t x_t
+
+    out, h_final = gdn2_gated_scan(x, g, b=None, h0=None)          # autograd
+    out, state = gdn2_gated_scan_step(x, g, b=None, state=None)    # one token
+
+The recurrent layer that hybrid stacks put between matrix-state (GDN-2) layers;
+``g`` is the log decay in GDN-2's convention and must not be positive in use (the
+sums of g over any run of tokens have to stay below 88).  ``g = -inf`` at a token
+starts a new sequence there: nothing of what came before, NaN included, enters
+it, and no gradient leaves it.  No counterpart in the reference.
+
+Arithmetic is float32.  x and b are float32 or bfloat16 (mixed or other types are
+widened to float32), g float32 (or bfloat16 with bfloat16 inputs); ``out`` has x's
+type and shape, states are float32.  Inputs may be strided as long as their
+channels are contiguous (the parts of one projection's output); others are copied.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
+
+_Strides = ctypes.c_longlong * 2
+
+
+def _types(x, g, b, what):
+    """(input type, g's type) of a call, as the GDN-2 forward chooses them."""
+    for t in (x, g) if b is None else (x, g, b):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: x, g, b must be torch tensors")
+        if t.shape != x.shape:
+            raise GDN2ShapeError(f"{what}: g and b must have x's shape {tuple(x.shape)}; got "
+                                 f"{tuple(t.shape)}")
+        if t.device != x.device or t.device.type != "cuda":
+            raise GDN2Error(f"{what}: inputs must live on one ROCm device; no CPU path")
+        if not t.is_floating_point():
+            raise GDN2Error(f"{what}: inputs must be floating point; got {t.dtype}")
+    dt = x.dtype
+    if dt not in _SUPPORTED_IN or (b is not None and b.dtype != dt):
+        dt = torch.float32
+    bf16 = dt == torch.bfloat16 and g.dtype == torch.bfloat16
+    return dt, torch.bfloat16 if bf16 else torch.float32
+
+
+def _state_in(h, shape, device, what, name):
+    if not isinstance(h, torch.Tensor):
+        raise TypeError(f"{what}: {name} must be a torch tensor")
+    if tuple(h.shape) != tuple(shape):
+        raise GDN2ShapeError(f"{what}: {name} must have shape {tuple(shape)}; got "
+                             f"{tuple(h.shape)}")
+    if h.device != device:
+        raise GDN2Error(f"{what}: {name} must live on {device}")
+    return h.to(torch.float32).contiguous()
+
+
+def _rows(x):
+    """(pointer, strides) of a (B,T,C) tensor, copied where its channels are apart.
+    The copy is returned too, to outlive the launch."""
+    if x.is_contiguous():
+        return x, x.data_ptr(), None
+    if x.stride(2) != 1 and x.shape[2] != 1:
+        x = x.contiguous()
+        return x, x.data_ptr(), None
+    return x, x.data_ptr(), _Strides(x.stride(0), x.stride(1))
+
+
+def _launch_fwd(x, g, b, h0, keep):
+    B, T, C = x.shape
+    dev, L = x.device, _lib.lib()
+    x, px, sx = _rows(x)
+    g, pg, sg = _rows(g)
+    pb = sb = None
+    if b is not None:
+        b, pb, sb = _rows(b)
+    out = torch.empty((B, T, C), dtype=x.dtype, device=dev)
+    h_final = torch.empty((B, C), dtype=torch.float32, device=dev)
+    kept = ws = None
+    if keep:
+        kept = torch.empty(L.gdn2_gated_scan_kept_bytes(B, T, C) // 4, dtype=torch.float32,
+                           device=dev)
+    nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        rc = L.gdn2_gated_scan_fwd(
+            torch.cuda.current_stream(dev).cuda_stream, B, T, C, _dtype_code(x.dtype),
+            _dtype_code(g.dtype), px, sx, pg, sg, pb, sb,
+            None if h0 is None else h0.data_ptr(), out.data_ptr(), h_final.data_ptr(),
+            kept.data_ptr() if keep and T else None, None if ws is None else ws.data_ptr(), nbytes)
+    if rc:
+        _raise(rc, f"gdn2_gated_scan_fwd (B,T,C)=({B},{T},{C})")
+    return out, h_final, kept
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, g, b, h0):
+        out, h_final, kept = _launch_fwd(x, g, b, h0, True)
+        ctx.save_for_backward(x, g, b, kept)
+        ctx.has_h0 = h0 is not None
+        ctx.set_materialize_grads(False)
+        return out, h_final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dh_final):
+        x, g, b, kept = ctx.saved_tensors
+        B, T, C = x.shape
+        dev, L = x.device, _lib.lib()
+        if T == 0:
+            zero = [None if t is None else torch.zeros_like(t) for t in (x, g, b)]
+            dh0 = None if not ctx.has_h0 or dh_final is None else dh_final.clone()
+            return (*zero, dh0)
+        x, px, sx = _rows(x)
+        g, pg, sg = _rows(g)
+        pb = sb = pd = sd = db = dh0 = ws = None
+        if b is not None:
+            b, pb, sb = _rows(b)
+            db = torch.empty((B, T, C), dtype=b.dtype, device=dev)
+        if dout is not None:
+            dout, pd, sd = _rows(dout.to(x.dtype))
+        if dh_final is not None:
+            dh_final = dh_final.to(torch.float32).contiguous()
+        dx = torch.empty((B, T, C), dtype=x.dtype, device=dev)
+        dg = torch.empty((B, T, C), dtype=g.dtype, device=dev)
+        if ctx.has_h0:
+            dh0 = torch.empty((B, C), dtype=torch.float32, device=dev)
+        nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ptr = lambda t: None if t is None else t.data_ptr()
+        with torch.cuda.device(dev):
+            rc = L.gdn2_gated_scan_bwd(
+                torch.cuda.current_stream(dev).cuda_stream, B, T, C, _dtype_code(x.dtype),
+                _dtype_code(g.dtype), px, sx, pg, sg, pb, sb, pd, sd, ptr(dh_final),
+                kept.data_ptr(), dx.data_ptr(), dg.data_ptr(), ptr(db), ptr(dh0), ptr(ws), nbytes)
+        if rc:
+            _raise(rc, f"gdn2_gated_scan_bwd (B,T,C)=({B},{T},{C})")
+        return dx, dg, db, dh0
+
+
+def gdn2_gated_scan(x, g, b=None, h0=None):
+    """h_t = e^{g_t} h_{t-1} + b_t x_t over the second axis.
+
+    x, g, b: (B,T,C) or (B,T,H,D), one shape; ``b=None`` stands for ones; h0 (B,C) or
+    (B,H,D), default zeros.  Returns ``out`` (all h_t, x's shape and type) and
+    ``h_final`` (float32, h0's shape).  Differentiable in x, g, b and h0, through out
+    and h_final; gradients come in each input's type.  T may be 0 (h_final = h0).
+    Shapes and types are checked before any launch (GDN2ShapeError, GDN2Error)."""
+    what = "gdn2_gated_scan"
+    dt, gdt = _types(x, g, b, what)
+    shape = x.shape
+    if len(shape) not in (3, 4):
+        raise GDN2ShapeError(f"{what}: expected (B,T,C) or (B,T,H,D) inputs, got {tuple(shape)}")
+    state = (shape[0], *shape[2:])
+    if h0 is not None:
+        h0 = _state_in(h0, state, x.device, what, "h0")
+    out_dt = x.dtype
+    x, g = x.to(dt), g.to(gdt)
+    b = None if b is None else b.to(dt)
+    if len(shape) == 4:
+        flat = (*shape[:2], shape[2] * shape[3])
+        x, g = x.reshape(flat), g.reshape(flat)
+        b = None if b is None else b.reshape(flat)
+        h0 = None if h0 is None else h0.reshape(flat[0], flat[2])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, g, b, h0)):
+        out, h_final = _GatedScan.apply(x, g, b, h0)
+    else:
+        out, h_final, _ = _launch_fwd(x, g, b, h0, False)
+    if out.dtype != out_dt:
+        out = out.to(out_dt)
+    if len(shape) == 4:
+        out, h_final = out.view(shape), h_final.view(state)
+    return out, h_final
+
+
+def gdn2_gated_scan_step(x, g, b=None, state=None, inplace=False):
+    """One token of ``gdn2_gated_scan`` for decoding.
+
+    x, g, b: one shape (B, ...) without a token axis; state: float32 of that shape
+    (default zeros).  Returns ``out`` (x's type) and the new state; ``inplace=True``
+    updates ``state`` itself, which must then be a contiguous float32 tensor.
+    Inference only."""
+    what = "gdn2_gated_scan_step"
+    dt, gdt = _types(x, g, b, what)
+    dev, shape = x.device, x.shape
+    if inplace:
+        if not isinstance(state, torch.Tensor) or state.dtype != torch.float32 or \
+                not state.is_contiguous():
+            raise GDN2Error(f"{what}: inplace needs a contiguous float32 state")
+    h_in = None if state is None else _state_in(state, shape, dev, what, "state").detach()
+    out_dt = x.dtype
+    x, g = x.detach().to(dt).contiguous(), g.detach().to(gdt).contiguous()
+    b = None if b is None else b.detach().to(dt).contiguous()
+    h_out = state if inplace else torch.empty(shape, dtype=torch.float32, device=dev)
+    out = torch.empty(shape, dtype=dt, device=dev)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().gdn2_gated_scan_step(
+            torch.cuda.current_stream(dev).cuda_stream, x.numel(), _dtype_code(dt),
+            _dtype_code(gdt), x.data_ptr(), g.data_ptr(), None if b is None else b.data_ptr(),
+            None if h_in is None else h_in.data_ptr(), h_out.data_ptr(), out.data_ptr())
+    if rc:
+        _raise(rc, f"{what} {tuple(shape)}")
+    return out.to(out_dt), h_out

@@ -337,6 +337,52 @@ int gdn2_bwd_intra(void* stream, int B, int T, int H, int D, int BT, const float
 int gdn2_bwd_reverse_cumsum(void* stream, long long tiles, int BT, int D, const float* dgc,
                             float* dg);
 
+/* ---- Gated linear recurrence ------------------------------------------------
+ * Elementwise over the C channels of (B,T,C) tensors (heads and their channels
+ * flattened):
+ *   h_t = e^{g_t} h_{t-1} + b_t x_t,   out_t = h_t,   h_final = h_T.
+ * No counterpart in the reference.  g is the log decay, as GDN-2's; the sums of g
+ * over any run of tokens must stay below 88 (g <= 0 in use).  g_t = -inf starts
+ * anew: h_t = b_t x_t whatever h_{t-1} holds, NaN included, and no gradient
+ * passes -- the sequences of a packed batch.  b may be NULL (all ones).  Float32
+ * arithmetic; in_dtype (GDN2_F32, GDN2_BF16) is x's, b's, out's and dout's and
+ * that of their gradients, g_dtype (GDN2_F32, or GDN2_BF16 with bfloat16 inputs)
+ * g's and dg's; states and their gradients are float32 (B,C).
+ * x, g, b and dout may be strided: *_strides points to two host integers, the
+ * elements from one batch entry and one token to the next (NULL: dense); the
+ * channels are contiguous.  out, dx, dg, db are dense.  Pointers are aligned to
+ * their elements; 4-element alignment of pointers, strides and C is faster.
+ * gdn2_set_launch_events does not reach the entry points from here on. */
+
+/* Bytes of the states kept for the backward: (ceil(T/256), B, C) float32. */
+size_t gdn2_gated_scan_kept_bytes(int B, int T, int C);
+/* Workspace of the forward and of the backward (0 for most sizes: only where the
+ * axis is split because there are few channels). */
+size_t gdn2_gated_scan_workspace_bytes(int B, int T, int C);
+
+/* h0 may be NULL (zero) and equal to h_final; kept may be NULL (inference). */
+int gdn2_gated_scan_fwd(void* stream, int B, int T, int C, int in_dtype, int g_dtype,
+                        const void* x, const long long* x_strides, const void* g,
+                        const long long* g_strides, const void* b, const long long* b_strides,
+                        const float* h0, void* out, float* h_final, float* kept, void* ws,
+                        size_t ws_bytes);
+
+/* Gradients from those of out and h_final (either may be NULL: zero), the
+ * forward's inputs and its kept states.  db is written where b is given, dh0
+ * where it is not NULL.  T >= 1. */
+int gdn2_gated_scan_bwd(void* stream, int B, int T, int C, int in_dtype, int g_dtype,
+                        const void* x, const long long* x_strides, const void* g,
+                        const long long* g_strides, const void* b, const long long* b_strides,
+                        const void* dout, const long long* dout_strides, const float* dh_final,
+                        const float* kept, void* dx, void* dg, void* db, float* dh0, void* ws,
+                        size_t ws_bytes);
+
+/* One token of n = B*C values, all dense; h_in may be NULL (zero) and equal to
+ * h_out (update in place). */
+int gdn2_gated_scan_step(void* stream, long long n, int in_dtype, int g_dtype, const void* x,
+                         const void* g, const void* b, const float* h_in, float* h_out,
+                         void* out);
+
 #ifdef __cplusplus
 }
 #endif

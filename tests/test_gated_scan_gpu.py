@@ -1,0 +1,376 @@
+"""Gated linear recurrence (gdn2_gated_scan, its backward, gdn2_gated_scan_step) against
+the recurrence in float64.
+
+Tolerances.  Every value is a sum of terms, each multiplied on its way by decays
+in (0, 1]; m is the same sum with the terms' magnitudes.  A term passes at most 16 tokens
+of a run (two roundings each, and the two of e^g), six compositions and four waves (three
+roundings each) and, more weakly the farther it comes, the steps of 256 tokens: fewer than
+128 roundings of 2^-24 where a step's decay is e^-2 or less, as all the inputs here
+have.  So 128 * 2^-24 * m; results in bfloat16 are rounded once more, 2^-8 of their value."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+EPS = 128 * 2.0 ** -24
+
+
+def recurrence(a, u, h0, fresh):
+    """All states of h_t = a_t h_{t-1} + u_t, (B,T,C) float64; `fresh`: h_t = u_t."""
+    h, out = h0.copy(), np.empty_like(u)
+    for t in range(u.shape[1]):
+        h = np.where(fresh[:, t], u[:, t], a[:, t] * np.where(fresh[:, t], 0.0, h) + u[:, t])
+        out[:, t] = h
+    return out
+
+
+def reference(x, g, b, h0, dout=None, dh_final=None):
+    """Outputs, gradients and the magnitudes of both, float64 (B,T,C)."""
+    fresh, a = np.isneginf(g), np.exp(g)
+    out = recurrence(a, b * x, h0, fresh)
+    mag = recurrence(a, np.abs(b * x), np.abs(h0), fresh)
+    if dout is None:
+        return out, mag
+    T = x.shape[1]
+
+    def back(d, e):
+        dh = np.empty_like(d)
+        for t in reversed(range(T)):
+            dh[:, t] = d[:, t] + e
+            e = np.where(fresh[:, t], 0.0, a[:, t] * dh[:, t])
+        return dh, e
+    dh, dh0 = back(dout, dh_final)
+    mdh, mdh0 = back(np.abs(dout), np.abs(dh_final))
+    before = np.concatenate([h0[:, None], out[:, :-1]], 1)
+    mbefore = np.concatenate([np.abs(h0)[:, None], mag[:, :-1]], 1)
+    before, mbefore = np.where(fresh, 0.0, before), np.where(fresh, 0.0, mbefore)
+    grads = {"x": (b * dh, np.abs(b) * mdh), "g": (a * before * dh, a * mbefore * mdh),
+             "b": (x * dh, np.abs(x) * mdh), "h0": (dh0, mdh0)}
+    return out, mag, grads
+
+
+def check(got, ref, mag, n=1):
+    """|got - ref| <= n EPS mag (+ the rounding of a bfloat16 result)."""
+    half = 2.0 ** -8 if got.dtype == torch.bfloat16 else 0.0
+    got = got.detach().double().cpu().numpy()
+    excess = np.abs(got - ref) - (n * EPS * mag + half * np.abs(ref) + 1e-30)
+    assert np.isfinite(got).all() and excess.max() <= 0.0, float(excess.max())
+
+
+def inputs(B, T, C, dtype, gdtype, dev, seed, low=0.01):
+    """Tensors on the device and their float64 values (after rounding to the type)."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((B, T, C))
+    g = -low - rng.exponential(0.5, (B, T, C)) * rng.uniform(0.01, 1.0, C)
+    b = rng.uniform(0.0, 1.0, (B, T, C))
+    h0 = rng.standard_normal((B, C))
+    put = lambda a, dt: torch.tensor(a, device=dev).to(dt)
+    t = [put(x, dtype), put(g, gdtype), put(b, dtype), put(h0, torch.float32)]
+    return t, [v.double().cpu().numpy() for v in t]
+
+
+TYPES = [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+         (torch.bfloat16, torch.bfloat16)]
+# one token, the sides of a run, a wave and a step; channels on and off the 4- and 16-wide tiles
+SIZES = [(1, 1, 1), (2, 2, 16), (3, 5, 7), (1, 15, 20), (2, 16, 64), (1, 63, 33), (2, 64, 48),
+         (1, 65, 128), (2, 255, 30), (1, 256, 36), (3, 257, 17), (1, 1000, 100), (9, 300, 21)]
+
+
+@pytest.mark.parametrize("dtype,gdtype", TYPES)
+@pytest.mark.parametrize("B,T,C", SIZES)
+def test_forward(dev, B, T, C, dtype, gdtype):
+    import gdn2_package as gp
+    (x, g, b, h0), (xn, gn, bn, hn) = inputs(B, T, C, dtype, gdtype, dev, T + C)
+    for bt, ht in ((b, h0), (None, None), (b, None)):
+        out, hf = gp.gdn2_gated_scan(x, g, bt, h0=ht)
+        ref, mag = reference(xn, gn, np.ones_like(bn) if bt is None else bn,
+                             np.zeros_like(hn) if ht is None else hn)
+        assert out.dtype == dtype and out.shape == x.shape and hf.dtype == torch.float32
+        check(out, ref, mag)
+        check(hf, ref[:, -1], mag[:, -1])
+
+
+@pytest.mark.parametrize("dtype,gdtype", TYPES)
+@pytest.mark.parametrize("B,T,C", SIZES)
+def test_backward(dev, B, T, C, dtype, gdtype):
+    import gdn2_package as gp
+    ts, (xn, gn, bn, hn) = inputs(B, T, C, dtype, gdtype, dev, T + C + 1)
+    rng = np.random.default_rng(5)
+    dout = torch.tensor(rng.standard_normal((B, T, C)), device=dev).to(dtype)
+    dhf = torch.tensor(rng.standard_normal((B, C)), device=dev).float()
+    for gate, state in ((True, True), (False, False)):
+        use = {"x": ts[0], "g": ts[1]}
+        if gate:
+            use["b"] = ts[2]
+        if state:
+            use["h0"] = ts[3]
+        leaf = {n: t.clone().requires_grad_() for n, t in use.items()}
+        out, hf = gp.gdn2_gated_scan(leaf["x"], leaf["g"], leaf.get("b"), h0=leaf.get("h0"))
+        got = torch.autograd.grad((out, hf), list(leaf.values()), (dout, dhf))
+        _, _, ref = reference(xn, gn, bn if gate else np.ones_like(bn),
+                              hn if state else np.zeros_like(hn), dout.double().cpu().numpy(),
+                              dhf.double().cpu().numpy())
+        for n, t in zip(leaf, got):
+            assert t.dtype == leaf[n].dtype and t.shape == leaf[n].shape
+            check(t, *ref[n], n=2)   # products of two sums
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,C", [(1, 2048, 16), (1, 5000, 20), (1, 4097, 7), (2, 9001, 40)])
+def test_split_axis(dev, B, T, C, dtype):
+    """Few channels and a long axis: segments with a summary pass before the walk."""
+    import gdn2_package as gp
+    from gdn2_package import _lib
+    assert _lib.lib().gdn2_gated_scan_workspace_bytes(B, T, C) > 0
+    ts, (xn, gn, bn, hn) = inputs(B, T, C, dtype, torch.float32, dev, T)
+    leaf = [t.clone().requires_grad_() for t in ts]
+    out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+    dout, dhf = torch.randn_like(out), torch.randn_like(hf)
+    got = torch.autograd.grad((out, hf), leaf, (dout, dhf))
+    ref, mag, grads = reference(xn, gn, bn, hn, dout.double().cpu().numpy(),
+                                dhf.double().cpu().numpy())
+    check(out, ref, mag)
+    check(hf, ref[:, -1], mag[:, -1])
+    for n, t in zip(("x", "g", "b", "h0"), got):
+        check(t, *grads[n], n=2)
+
+
+def test_gradient_against_differences(dev):
+    """<gradient, direction> against central differences of the float64 recurrence."""
+    import gdn2_package as gp
+    B, T, C = 2, 70, 9
+    ts, vals = inputs(B, T, C, torch.float32, torch.float32, dev, 11)
+    rng = np.random.default_rng(12)
+    dout, dhf = rng.standard_normal((B, T, C)), rng.standard_normal((B, C))
+    f32 = lambda a: torch.tensor(a, device=dev).float()
+    dout, dhf = (f32(a).double().cpu().numpy() for a in (dout, dhf))
+    leaf = [t.clone().requires_grad_() for t in ts]
+    out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+    got = torch.autograd.grad((out, hf), leaf, (f32(dout), f32(dhf)))
+    _, _, grads = reference(*vals, dout, dhf)
+
+    def loss(v):
+        o = recurrence(np.exp(v[1]), v[2] * v[0], v[3], np.zeros(v[0].shape, bool))
+        return (o * dout).sum() + (o[:, -1] * dhf).sum()
+    step = 1e-5
+    for i, n in enumerate(("x", "g", "b", "h0")):
+        d = rng.standard_normal(vals[i].shape)
+        up, down = list(vals), list(vals)
+        up[i], down[i] = vals[i] + step * d, vals[i] - step * d
+        diff = (loss(up) - loss(down)) / (2 * step)
+        mine = float((got[i].double().cpu().numpy() * d).sum())
+        # the kernel's bound along d, and the differences' own step^2 and rounding (1e-6)
+        tol = 2 * EPS * float((grads[n][1] * np.abs(d)).sum()) + 1e-6 * (1 + abs(diff))
+        assert abs(mine - diff) <= tol, (n, mine, diff, tol)
+
+
+@pytest.mark.parametrize("T,C", [(600, 24), (2500, 5)])
+def test_fresh_starts(dev, T, C):
+    """g = -inf starts a sequence: equal to separate calls, NaN and infinities before
+    it stay there, and no gradient crosses it."""
+    import gdn2_package as gp
+    (x, g, b, h0), _ = inputs(1, T, C, torch.float32, torch.float32, dev, T)
+    cuts = [0, 1, 2, 130, 255, 256, 257, 400, T]
+    g[:, cuts[1:-1]] = -torch.inf
+    x[:, 131:140] = torch.nan
+    x[:, 200, 0] = torch.inf
+    leaf = [t.clone().requires_grad_() for t in (x, g, b, h0)]
+    out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+    dout = torch.randn_like(out)
+    got = torch.autograd.grad((out, hf), leaf, (dout, torch.zeros_like(hf)))
+    for s, e in zip(cuts[:-1], cuts[1:]):
+        if s <= 130 < e:
+            continue
+        first = h0[:1].double().cpu().numpy() if s == 0 else np.zeros((1, C))
+        part = [v[:, s:e].double().cpu().numpy() for v in (x, g, b)]
+        ref, mag, grads = reference(*part, first, dout[:, s:e].double().cpu().numpy(),
+                                    np.zeros((1, C)))
+        check(out[:, s:e], ref, mag)
+        for n, t in zip(("x", "g", "b"), got):
+            check(t[:, s:e], *grads[n], n=2)
+    assert torch.isnan(out[:, 131:255]).all() and torch.isfinite(out[:, 255:]).all()
+    assert torch.isfinite(got[3]).all()
+
+
+def test_decays_that_underflow(dev):
+    """Finite decays below the exponent's range give zero factors, not fresh starts; long
+    runs whose products underflow stay finite."""
+    import gdn2_package as gp
+    B, T, C = 1, 700, 20
+    (x, g, b, h0), (xn, gn, bn, hn) = inputs(B, T, C, torch.float32, torch.float32, dev, 3)
+    g[:, ::3] = -300.0
+    g[:, 1::3, :5] = -1e30
+    gn = g.double().cpu().numpy()
+    leaf = [t.clone().requires_grad_() for t in (x, g, b, h0)]
+    out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+    dout = torch.randn_like(out)
+    got = torch.autograd.grad(out, leaf, dout)
+    ref, mag, grads = reference(xn, gn, bn, hn, dout.double().cpu().numpy(), np.zeros((B, C)))
+    check(out, ref, mag)
+    for n, t in zip(("x", "g", "b", "h0"), got):
+        check(t, *grads[n], n=2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strided_inputs(dev, dtype):
+    """The parts of one projection's output, a sliced time axis, a transposed copy, a
+    shared (broadcast) g and an odd storage offset."""
+    import gdn2_package as gp
+    B, T, H, D = 2, 300, 3, 8
+    C = H * D
+    proj = torch.randn((B, T, 3 * C), device=dev).to(dtype)
+    x, g, b = proj[..., :C], -proj[..., C:2 * C].abs() - 0.01, proj[..., 2 * C:]
+    want = gp.gdn2_gated_scan(x.contiguous(), g.contiguous(), b.contiguous())
+    for got in (gp.gdn2_gated_scan(x, g, b),
+                gp.gdn2_gated_scan(x.transpose(1, 2).contiguous().transpose(1, 2), g, b)):
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+    o4, h4 = gp.gdn2_gated_scan(*(t.unflatten(-1, (H, D)) for t in (x, g, b)))
+    assert o4.shape == (B, T, H, D) and h4.shape == (B, H, D)
+    assert torch.equal(o4.flatten(2), want[0]) and torch.equal(h4.flatten(1), want[1])
+    got = gp.gdn2_gated_scan(*(t[:, 40:200] for t in (x, g, b)))
+    want = gp.gdn2_gated_scan(*(t[:, 40:200].contiguous() for t in (x, g, b)))
+    assert all(torch.equal(a, e) for a, e in zip(got, want))
+    odd = torch.randn(B * T * C + 1, device=dev).to(dtype)[1:].view(B, T, C)
+    got = gp.gdn2_gated_scan(odd, g, b)
+    want = gp.gdn2_gated_scan(odd.clone(), g, b)
+    assert all(torch.allclose(a, e, rtol=2.0 ** -7, atol=1e-5) for a, e in zip(got, want))
+
+
+def test_gradient_of_a_shared_decay(dev):
+    """One g for all the channels of a head: its gradient is the sum over them."""
+    import gdn2_package as gp
+    B, T, H, D = 2, 100, 3, 16
+    x = torch.randn((B, T, H, D), device=dev)
+    g1 = (-torch.rand((B, T, H, 1), device=dev) - 0.01).requires_grad_()
+    out, _ = gp.gdn2_gated_scan(x, g1.expand(B, T, H, D))
+    out.square().sum().backward()
+    g2 = g1.detach().expand(B, T, H, D).clone().requires_grad_()
+    out2, _ = gp.gdn2_gated_scan(x, g2)
+    out2.square().sum().backward()
+    assert torch.equal(out, out2)
+    ref = g2.grad.double().sum(-1, keepdim=True)
+    mag = g2.grad.double().abs().sum(-1, keepdim=True)
+    assert ((g1.grad.double() - ref).abs() <= D * 2.0 ** -24 * mag).all()
+
+
+@pytest.mark.parametrize("dtype,gdtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (32, 768), (5, 2, 12)])
+def test_step(dev, shape, dtype, gdtype):
+    import gdn2_package as gp
+    rng = np.random.default_rng(1)
+    put = lambda a, dt: torch.tensor(a, device=dev).to(dt)
+    x, b = put(rng.standard_normal(shape), dtype), put(rng.uniform(0, 1, shape), dtype)
+    g, h = put(-rng.exponential(0.5, shape), gdtype), put(rng.standard_normal(shape), torch.float32)
+    g.view(-1)[0] = -torch.inf
+    hn = h.double().cpu().numpy().copy()
+    h.view(-1)[0] = torch.nan          # dropped by the fresh start
+    hn.reshape(-1)[0] = 0.0
+    before = h.clone()
+    xn, bn, gn = (t.double().cpu().numpy() for t in (x, b, g))
+    for bt in (b, None):
+        out, new = gp.gdn2_gated_scan_step(x, g, bt, state=h)
+        u = xn * (bn if bt is not None else 1.0)
+        check(new, np.exp(gn) * hn + u, np.exp(gn) * np.abs(hn) + np.abs(u))
+        check(out, np.exp(gn) * hn + u, np.exp(gn) * np.abs(hn) + np.abs(u))
+        assert torch.equal(h.isnan(), before.isnan()) and new.data_ptr() != h.data_ptr()
+    out2, same = gp.gdn2_gated_scan_step(x, g, None, state=h, inplace=True)
+    assert same.data_ptr() == h.data_ptr() and torch.equal(h, new) and torch.equal(out, out2)
+    out3, new3 = gp.gdn2_gated_scan_step(x, g, b)
+    check(new3, xn * bn, np.abs(xn * bn))
+
+
+def test_prefix_then_steps_equal_the_scan(dev):
+    import gdn2_package as gp
+    B, T, C = 2, 40, 12
+    (x, g, b, h0), (xn, gn, bn, hn) = inputs(B, T, C, torch.float32, torch.float32, dev, 2)
+    _, h = gp.gdn2_gated_scan(x[:, :30], g[:, :30], b[:, :30], h0=h0)
+    ref, mag = reference(xn, gn, bn, hn)
+    for t in range(30, T):
+        out, h = gp.gdn2_gated_scan_step(x[:, t], g[:, t], b[:, t], state=h)
+        check(out, ref[:, t], mag[:, t])
+
+
+def test_other_types_and_empty_axis(dev):
+    import gdn2_package as gp
+    x = torch.randn((2, 9, 8), device=dev, dtype=torch.float16).requires_grad_()
+    g = -torch.rand((2, 9, 8), device=dev)
+    out, hf = gp.gdn2_gated_scan(x, g, torch.ones_like(x, dtype=torch.bfloat16))
+    assert out.dtype == torch.float16 and hf.dtype == torch.float32
+    out.float().sum().backward()
+    assert x.grad.dtype == torch.float16
+    h0 = torch.randn((2, 8), device=dev, requires_grad=True)
+    out, hf = gp.gdn2_gated_scan(x[:, :0], g[:, :0], h0=h0)
+    assert out.shape == (2, 0, 8) and torch.equal(hf, h0)
+    hf.sum().backward()
+    assert torch.equal(h0.grad, torch.ones_like(h0))
+    with torch.no_grad():
+        _, hf = gp.gdn2_gated_scan(x[:, :0], g[:, :0])
+    assert torch.equal(hf, torch.zeros((2, 8), device=dev))
+
+
+def test_only_one_output_used(dev):
+    """The cotangent of the output that is not used counts as zero."""
+    import gdn2_package as gp
+    (x, g, b, h0), (xn, gn, bn, hn) = inputs(1, 300, 8, torch.float32, torch.float32, dev, 8)
+    zero = np.zeros_like(hn)
+    for pick in (0, 1):
+        leaf = [t.clone().requires_grad_() for t in (x, g, b, h0)]
+        res = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])[pick]
+        res.sum().backward()
+        one = np.ones_like(xn)
+        _, _, ref = reference(xn, gn, bn, hn, one if pick == 0 else 0 * one,
+                              zero if pick == 0 else zero + 1)
+        for n, t in zip(("x", "g", "b", "h0"), leaf):
+            check(t.grad, *ref[n], n=2)
+
+
+def test_other_stream_and_graph(dev):
+    """On a stream that is not the current default, and replayed from a captured graph."""
+    import gdn2_package as gp
+    x, b = torch.randn((2, 700, 40), device=dev), torch.rand((2, 700, 40), device=dev)
+    g = -torch.rand((2, 700, 40), device=dev) - 0.01
+    want = gp.gdn2_gated_scan(x, g, b)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = gp.gdn2_gated_scan(x, g, b)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, e) for a, e in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = gp.gdn2_gated_scan(x, g, b)
+    for k in range(3):
+        x.normal_()
+        want = gp.gdn2_gated_scan(x, g, b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(got, want)), k
+
+
+def test_refusals(dev):
+    import gdn2_package as gp
+    x = torch.randn((2, 5, 8), device=dev)
+    g = -torch.rand_like(x)
+    for bad in (lambda: gp.gdn2_gated_scan(x[0], g[0]),
+                lambda: gp.gdn2_gated_scan(x, g[:, :4]),
+                lambda: gp.gdn2_gated_scan(x, g, g[..., :4]),
+                lambda: gp.gdn2_gated_scan(x, g, h0=torch.zeros((2, 7), device=dev)),
+                lambda: gp.gdn2_gated_scan(x[:0], g[:0]),
+                lambda: gp.gdn2_gated_scan_step(x, g, state=x[0])):
+        with pytest.raises(gp.GDN2ShapeError):
+            bad()
+    for bad in (lambda: gp.gdn2_gated_scan(x.cpu(), g.cpu()),
+                lambda: gp.gdn2_gated_scan(x, g.cpu()),
+                lambda: gp.gdn2_gated_scan(x.int(), g),
+                lambda: gp.gdn2_gated_scan(x, g, h0=torch.zeros((2, 8))),
+                lambda: gp.gdn2_gated_scan_step(x, g, inplace=True),
+                lambda: gp.gdn2_gated_scan_step(x, g, state=x.bfloat16(), inplace=True)):
+        with pytest.raises(gp.GDN2Error):
+            bad()
+    with pytest.raises(TypeError):
+        gp.gdn2_gated_scan(x, [1.0])
+    leaf = x.clone().requires_grad_()
+    out, _ = gp.gdn2_gated_scan(leaf, g)
+    first, = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):   # no second derivative, and it says so
+        first.sum().backward()
