@@ -48,6 +48,7 @@ ERR_SCRATCH = -11
 NOALLOC_SCRATCH_BYTES = 128 << 20
 
 _c_int, _c_float, _c_size, _vp = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+_c_ll = ctypes.c_longlong
 
 # name -> (restype, argtypes); exactly the entry points of include/gdn2.h
 SIGNATURES = {
@@ -94,6 +95,16 @@ SIGNATURES = {
     "gdn2_gated_scan_fwd": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 11 + [_c_size]),
     "gdn2_gated_scan_bwd": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 15 + [_c_size]),
     "gdn2_gated_scan_step": (_c_int, [_vp, ctypes.c_longlong, _c_int, _c_int] + [_vp] * 6),
+    "gdn2_rms_norm": (_c_int, [_vp] + [_c_int] * 5 + [_vp, _c_ll, _vp, _c_ll, _vp, _c_float]
+                      + [_vp] * 3),
+    "gdn2_rms_norm_int8": (_c_int, [_vp] + [_c_int] * 5 + [_vp, _c_ll, _vp, _c_ll, _vp, _c_float,
+                                                           _vp, _c_ll, _vp, _vp]),
+    "gdn2_rms_norm_bwd_workspace_bytes": (_c_size, [_c_int] * 2),
+    "gdn2_rms_norm_bwd": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 9 + [_c_size]),
+    "gdn2_quantize_int8": (_c_int, [_vp] + [_c_int] * 3 + [_vp, _c_ll, _vp, _c_ll, _vp]),
+    "gdn2_dequantize_int8": (_c_int, [_vp] + [_c_int] * 3 + [_vp, _c_ll, _vp, _vp]),
+    "gdn2_int8_matmul": (_c_int, [_vp] + [_c_int] * 4 + [_vp, _c_ll, _vp, _vp, _c_ll]
+                         + [_vp] * 3),
 }
 
 

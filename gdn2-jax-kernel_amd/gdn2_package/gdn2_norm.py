@@ -1,0 +1,147 @@
+"""RMS norm with the residual's addition:
+
+    y, h = gdn2_rms_norm(x, weight, residual=None, eps=1e-6)        # autograd
+
+h = x + residual, rounded to the residual's type (the residual stream), and
+y = h w / sqrt(mean(h^2) + eps) over the last axis, the norm of h as it is returned.
+Without a residual h is x itself.  ``gdn2_int8.gdn2_rms_norm_int8`` gives y in
+8 bits.  No counterpart in the reference.
+
+Float32 arithmetic.  x is float32 or bfloat16 (other types are widened to float32),
+the residual has x's type or is float32 (a bfloat16 residual of a float32 x is
+widened), the weight (C,) is float32 or bfloat16.  Rows may be strided as long as
+their values are contiguous.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
+
+
+def _tensor(t, name, what):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what}: {name} must be a torch tensor")
+    if t.device.type != "cuda":
+        raise GDN2Error(f"{what}: {name} must live on the ROCm device; no CPU path")
+
+
+def _as_rows(x):
+    """x as (M, C) rows of contiguous values; a copy only where there is no such view."""
+    C = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, C) if C else x.reshape(0, 0)
+    return x if x.stride(1) == 1 or C == 1 else x.contiguous()
+
+
+def _row_stride(x):
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _prepare(x, weight, residual, eps, what):
+    """(x, residual, weight) of supported types, checked; rows are not formed yet."""
+    _tensor(x, "x", what)
+    _tensor(weight, "weight", what)
+    if x.dim() < 1 or tuple(weight.shape) != tuple(x.shape[-1:]):
+        raise GDN2ShapeError(f"{what}: weight must have the shape of x's last axis; got "
+                             f"{tuple(weight.shape)} for x {tuple(x.shape)}")
+    if not x.is_floating_point() or not weight.is_floating_point():
+        raise GDN2Error(f"{what}: x and weight must be floating point")
+    if weight.device != x.device:
+        raise GDN2Error(f"{what}: weight must live on {x.device}")
+    if not float(eps) >= 0.0:
+        raise GDN2Error(f"{what}: eps = {eps!r} must not be negative")
+    if residual is not None:
+        _tensor(residual, "residual", what)
+        if residual.shape != x.shape:
+            raise GDN2ShapeError(f"{what}: residual must have x's shape {tuple(x.shape)}; got "
+                                 f"{tuple(residual.shape)}")
+        if residual.device != x.device or not residual.is_floating_point():
+            raise GDN2Error(f"{what}: residual must be floating point, on {x.device}")
+    if x.dtype not in _SUPPORTED_IN:
+        x = x.float()
+    if weight.dtype not in _SUPPORTED_IN:
+        weight = weight.float()
+    if residual is not None and residual.dtype != x.dtype:
+        residual = residual.float()
+    return x, weight.contiguous(), residual
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, keep):
+        M, C = x.shape
+        dev = x.device
+        y = torch.empty((M, C), dtype=x.dtype, device=dev)
+        h = None if residual is None else torch.empty((M, C), dtype=residual.dtype, device=dev)
+        rstd = torch.empty(M, dtype=torch.float32, device=dev) if keep else None
+        ptr = lambda t: None if t is None else t.data_ptr()
+        with torch.cuda.device(dev):
+            rc = _lib.lib().gdn2_rms_norm(
+                torch.cuda.current_stream(dev).cuda_stream, M, C, _dtype_code(x.dtype),
+                _dtype_code(x.dtype if h is None else h.dtype), _dtype_code(weight.dtype),
+                x.data_ptr(), _row_stride(x), ptr(residual),
+                0 if h is None else _row_stride(residual), weight.data_ptr(), eps, y.data_ptr(),
+                ptr(h), ptr(rstd))
+        if rc:
+            _raise(rc, f"gdn2_rms_norm (M,C)=({M},{C})")
+        if keep:
+            ctx.save_for_backward(x if h is None else h, weight, rstd)
+            ctx.x_dtype, ctx.has_residual = x.dtype, h is not None
+            ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        M, C = h.shape
+        dev, L = h.device, _lib.lib()
+        h = h.contiguous()
+        dy = None if dy is None else dy.to(ctx.x_dtype).contiguous()
+        dh = None if dh is None else dh.to(h.dtype).contiguous()
+        dx = torch.empty((M, C), dtype=ctx.x_dtype, device=dev)
+        dr = torch.empty((M, C), dtype=h.dtype, device=dev) \
+            if ctx.has_residual and h.dtype != ctx.x_dtype else None
+        dw = torch.empty(C, dtype=weight.dtype, device=dev)
+        nbytes = L.gdn2_rms_norm_bwd_workspace_bytes(M, C)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ptr = lambda t: None if t is None else t.data_ptr()
+        with torch.cuda.device(dev):
+            rc = L.gdn2_rms_norm_bwd(
+                torch.cuda.current_stream(dev).cuda_stream, M, C, _dtype_code(ctx.x_dtype),
+                _dtype_code(h.dtype), _dtype_code(weight.dtype), h.data_ptr(), weight.data_ptr(),
+                rstd.data_ptr(), ptr(dy), ptr(dh), dx.data_ptr(), ptr(dr), dw.data_ptr(),
+                ws.data_ptr(), nbytes)
+        if rc:
+            _raise(rc, f"gdn2_rms_norm_bwd (M,C)=({M},{C})")
+        return dx, dw, (dx if dr is None else dr) if ctx.has_residual else None, None, None
+
+
+def gdn2_rms_norm(x, weight, residual=None, eps=1e-6):
+    """(y, h) with h = x + residual (x itself without one) and y = h w / sqrt(mean(h^2) + eps).
+
+    x (..., C) with C <= 16384, weight (C,), residual of x's shape.  y has x's shape and type,
+    h the residual's.  Differentiable in x, weight and residual, through y and h.  Shapes
+    and types are checked before any launch (GDN2ShapeError, GDN2Error)."""
+    what = "gdn2_rms_norm"
+    shape, out_dt, h_dt = x.shape if isinstance(x, torch.Tensor) else None, None, None
+    xs, ws, rs = _prepare(x, weight, residual, eps, what)
+    out_dt, h_dt = x.dtype, None if residual is None else residual.dtype
+    rows = _as_rows(xs)
+    r_rows = None if rs is None else _as_rows(rs)
+    if torch.is_grad_enabled() and (xs.requires_grad or ws.requires_grad or
+                                    (rs is not None and rs.requires_grad)):
+        res = _RmsNorm.apply(rows, ws, r_rows, float(eps), True)
+    else:
+        res = _RmsNorm.forward(None, rows, ws, r_rows, float(eps), False)
+    y, h = (res, None) if rs is None else res
+    y = y.view(shape)
+    if y.dtype != out_dt:
+        y = y.to(out_dt)
+    if h is None:
+        return y, x
+    h = h.view(shape)
+    return y, h if h.dtype == h_dt else h.to(h_dt)

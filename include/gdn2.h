@@ -383,6 +383,60 @@ int gdn2_gated_scan_step(void* stream, long long n, int in_dtype, int g_dtype, c
                          const void* g, const void* b, const float* h_in, float* h_out,
                          void* out);
 
+/* ---- RMS norm with the residual's addition ----------------------------------
+ * Over M rows of C <= 16384 values (no counterpart in the reference):
+ *   h = x + residual, rounded to the residual's type;   y = h w / sqrt(mean h^2 + eps).
+ * residual may be NULL: then h = x, and h (the output) may be NULL.  x_dtype is
+ * x's, y's, dy's and dx's, r_dtype (x_dtype, or GDN2_F32) the residual's, h's, dh's and
+ * dr's, w_dtype the weight's and dw's.  x and residual have rows of contiguous values,
+ * *_stride elements apart; all else is dense.  Float32 arithmetic.  Pointers are aligned
+ * to their elements (faster: 16 bytes, with row strides of 16 bytes and C % 8 == 0).
+ * eps >= 0, GDN2_ERR_SHAPE otherwise. */
+
+/* rstd (M) float32 is for the backward, or NULL. */
+int gdn2_rms_norm(void* stream, int M, int C, int x_dtype, int r_dtype, int w_dtype,
+                  const void* x, long long x_stride, const void* residual,
+                  long long r_stride, const void* weight, float eps, void* y, void* h,
+                  float* rstd);
+
+/* Gradients from those of y and h (dy, dh: either may be NULL, zero): dx, and dr, the
+ * residual's (NULL where it has x's type: it equals dx), and dw.  h is the forward's
+ * (x without a residual). */
+size_t gdn2_rms_norm_bwd_workspace_bytes(int M, int C);
+int gdn2_rms_norm_bwd(void* stream, int M, int C, int x_dtype, int r_dtype, int w_dtype,
+                      const void* h, const void* weight, const float* rstd, const void* dy,
+                      const void* dh, void* dx, void* dr, void* dw, void* ws,
+                      size_t ws_bytes);
+
+/* y in 8 bits with a scale for each row: with t = h w and m = max |t|, q = round(127 t / m)
+ * (ties to even) and scale = m / (127 sqrt(mean h^2 + eps)).  A row whose m is below 1e-36
+ * has q = 0 and scale 0; one that holds NaN or an infinity q = 0 and scale NaN.  q is 16-byte
+ * aligned, its rows q_stride = C rounded up to a multiple of 16 bytes apart, the bytes
+ * between zero. */
+int gdn2_rms_norm_int8(void* stream, int M, int C, int x_dtype, int r_dtype, int w_dtype,
+                       const void* x, long long x_stride, const void* residual,
+                       long long r_stride, const void* weight, float eps, void* q,
+                       long long q_stride, float* scale, void* h);
+
+/* ---- Rows in 8 bits and their products --------------------------------------- */
+
+/* Rows of x (C <= 32768) in 8 bits: as gdn2_rms_norm_int8 with t = x, scale = m / 127. */
+int gdn2_quantize_int8(void* stream, int M, int C, int x_dtype, const void* x,
+                       long long x_stride, void* q, long long q_stride, float* scale);
+
+/* out = q scale, (M,C) dense; rows of q are q_stride bytes apart. */
+int gdn2_dequantize_int8(void* stream, int M, int C, int out_dtype, const void* q,
+                         long long q_stride, const float* scale, void* out);
+
+/* out[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n] (bias float32 or
+ * NULL), out (M,N) dense of out_dtype; x (M,K) and w (N,K) signed 8-bit integers, sums
+ * exact in 32 bits (1 <= K <= 131071).  x and w are 16-byte aligned, their rows *_stride
+ * bytes apart, a multiple of 16 and at least K rounded up to one: the bytes between
+ * are read and count for nothing. */
+int gdn2_int8_matmul(void* stream, int M, int N, int K, int out_dtype, const void* x,
+                     long long x_stride, const float* x_scale, const void* w,
+                     long long w_stride, const float* w_scale, const float* bias, void* out);
+
 #ifdef __cplusplus
 }
 #endif
