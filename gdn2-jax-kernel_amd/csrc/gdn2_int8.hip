@@ -4,17 +4,22 @@
 // bits (K <= 131071), so no order of theirs can change a result; the scales are applied in
 // float32 and the result is rounded once.
 //
-// Tiled kernel: BM x BN outputs a workgroup, 64-byte slices of k staged through LDS by
-// global_load_lds in four buffers (three in flight), v_mfma_i32_16x16x64_i8.  The 16-byte
-// pieces of a row are permuted within it by the row number, so that the eight lanes
-// that LDS serves together read eight different bank groups; as the DMA writes LDS in lane
-// order, the lanes' global addresses are permuted instead.  The weight is the left operand,
-// its rows dealt to the fragments so that a lane ends up with eight neighbouring columns of
-// one output row, stored as 16 bytes of bfloat16.
+// Tiled kernel: BM x BN outputs a workgroup, slices of 128 bytes of k staged through LDS by
+// global_load_lds in a ring, v_mfma_i32_16x16x64_i8 (the 32x32x32 form reaches 3.4 P/s from
+// registers, this one 4.0).  Half a slice is multiplied while the other's fragments are
+// read.  Slices of whole cache lines: with 64 bytes 128 x 128 tiles reach 1.65 P/s at
+// 8192 x 8192 x 8192, with 128 2.04 (the traffic from L2 bounds them, not LDS, which is
+// read without conflicts, nor the matrix cores, 51% busy).  The 16-byte pieces of a row are
+// permuted within it by the row number, so that the eight lanes that LDS serves together read
+// different banks; as the DMA writes LDS in lane order, the lanes' global addresses are permuted
+// instead.  The weight is the left operand, its rows dealt to the fragments so that a lane
+// ends up with eight neighbouring columns of one output row.  Several workgroups share a CU, so
+// that one's start and stores pass under another's products (one that walks over many
+// tiles and loads ahead instead waits for its stores: 65536 x 4608 x 768 418 us against 372).
 //
-// Few rows (M <= 64): the weight's traffic is all that counts.  A workgroup takes 16
-// weight rows and its eight waves the slices of k in turn, straight from memory to
-// registers; their sums meet in LDS.
+// Few rows: the weight's traffic is all that counts.  A workgroup takes 16 weight rows and
+// its eight waves the slices of k in turn, straight from memory to registers; their sums meet
+// in LDS.
 //
 // k past K: rows are readable up to a multiple of 16 bytes, loads are clamped there, and
 // the activations' bytes from K on are zeroed in the last slice.
@@ -53,22 +58,115 @@ __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {
   return v;
 }
 
-constexpr int kBK = 64, kStages = 4;
+// Bytes of k of a slice: whole 128-byte lines.
+constexpr int kBK = 128;
 
-// Place of piece c of row r within its 64-byte row: activations' fragments read rows
-// i = 0..15, the weight's rows 8 (i / 4) + i % 4 (+ 4).
-__device__ __forceinline__ int swz_x(int r) { return (r >> 1) & 3; }
-__device__ __forceinline__ int swz_w(int r) { return ((r >> 1) & 1) | ((r >> 2) & 2); }
+// Place of 16-byte piece c of row r within its slice: piece c ^ swz(r).  Activations'
+// fragments read rows i = 0..15, the weight's rows 8 (i / 4) + i % 4 (+ 4).
+__device__ __forceinline__ int swz_x(int r) { return r & 7; }
+__device__ __forceinline__ int swz_w(int r) { return (r & 3) | ((r >> 1) & 4); }
 
-template <int BM, int BN, int WR, int WC, typename TO>
-__global__ void __launch_bounds__(64 * WR * WC) int8_mm(MmArgs a) {
-  constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC;   // waves, and a wave's tile
-  constexpr int MI = WM / 16, NI = WN / 16;
-  constexpr int STAGE = (BM + BN) * kBK;
-  constexpr int NL = STAGE / 1024 / NW;                     // DMA instructions of a wave
+// The 16-byte pieces of two halves of a row's columns, as lanes 16 lg + li hold them for rows
+// li = 0..15 (t0: the first half, t1: the second), dealt so that t0 holds both halves of the
+// rows 0..7 and t1 those of the rows 8..15: lanes li and li ^ 8 exchange a piece.  Each of
+// the two stores that follow then writes 128 bytes of eight rows, not 64 of sixteen.
+__device__ __forceinline__ void whole_lines(i32x4& t0, i32x4& t1, bool high) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int give = high ? t0[d] : t1[d];
+    const int got = __builtin_amdgcn_update_dpp(0, give, 0x128, 0xF, 0xF, false);   // row_ror:8
+    t0[d] = high ? got : t0[d];
+    t1[d] = high ? t1[d] : got;
+  }
+}
+
+// Scale, convert and store a wave's part: the fragment pair j, j + 1 of tile i holds row li,
+// columns 32 (j / 2) + 8 lg + e.  m, n: its first row and column; sx(row), sw(column) and
+// bias(column) give the scales of places within the part.
+template <typename TO, int NI, int MI, typename SX, typename SW, typename BI>
+__device__ __forceinline__ void store_part(const MmArgs& a, const i32x4 (&acc)[NI][MI], int m,
+                                           int n, int li, int lg, SX sx, SW sw, BI bias) {
+  const bool high = li >= 8;
+  const bool whole = a.vec && n + 16 * NI <= a.N && m + 16 * MI <= a.M;
+  // all scales before the first store, which could alias them for all the compiler knows
+  float s[MI], sc[NI / 2][8], bi[NI / 2][8];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) s[i] = sx(16 * i + li);
+#pragma unroll
+  for (int j = 0; j < NI / 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      sc[j][e] = sw(32 * j + 8 * lg + e);
+      bi[j][e] = a.bias ? bias(32 * j + 8 * lg + e) : 0.f;
+    }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    float y[NI / 2][8];
+#pragma unroll
+    for (int j = 0; j < NI; j += 2)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[j / 2][e] = (float)acc[j + e / 4][i][e % 4] * s[i] * sc[j / 2][e];
+        if (a.bias) y[j / 2][e] += bi[j / 2][e];
+      }
+    TO* row = (TO*)a.out + (long long)(m + 16 * i) * a.N + n;
+    if (whole && (sizeof(TO) == 4 || NI % 4 == 0)) {
+      // two halves of 128 bytes: float32 the two pieces of 8 values, bfloat16 two fragment pairs
+      constexpr int STEP = sizeof(TO) == 4 ? 1 : 2;
+#pragma unroll
+      for (int j = 0; j + STEP <= NI / 2; j += STEP) {
+        i32x4 t0, t1;
+        if constexpr (sizeof(TO) == 4) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            t0[d] = __float_as_int(y[j][d]);
+            t1[d] = __float_as_int(y[j][4 + d]);
+          }
+        } else {
+          t0 = __builtin_bit_cast(i32x4, make_op(y[j], (bf16x8*)nullptr));
+          t1 = __builtin_bit_cast(i32x4, make_op(y[j + STEP - 1], (bf16x8*)nullptr));
+        }
+        whole_lines(t0, t1, high);
+        const int c = sizeof(TO) == 4 ? 32 * j + 8 * lg + 4 * high : 32 * j + 8 * lg + 32 * high;
+        i32x4* p0 = reinterpret_cast<i32x4*>(row + (long long)(li & 7) * a.N + c);
+        i32x4* p1 = reinterpret_cast<i32x4*>(row + (long long)(8 + (li & 7)) * a.N + c);
+        *p0 = t0;
+        *p1 = t1;
+      }
+    } else if (m + 16 * i + li < a.M) {
+      TO* p = row + (long long)li * a.N + 8 * lg;
+#pragma unroll
+      for (int j = 0; j < NI / 2; ++j) {
+        if (a.vec && n + 32 * j + 8 * lg + 8 <= a.N) {
+          store4(p + 32 * j, f32x4{y[j][0], y[j][1], y[j][2], y[j][3]});
+          store4(p + 32 * j + 4, f32x4{y[j][4], y[j][5], y[j][6], y[j][7]});
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + 32 * j + 8 * lg + e < a.N) p[32 * j + e] = from_f<TO>(y[j][e]);
+        }
+      }
+    }
+  }
+}
+
+// BM x BN outputs; WR x WC waves; ST slices of k in LDS; PER_CU workgroups on a CU.
+template <int BM_, int BN_, int WR_, int WC_, int ST_, int PER_CU_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, ST = ST_, PER_CU = PER_CU_;
+  static constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC;   // waves, and a wave's part
+  static constexpr int MI = WM / 16, NI = WN / 16;
+  static constexpr int STAGE = (BM + BN) * kBK;
+  static constexpr int NL = STAGE / 1024 / NW;                     // DMA instructions of a wave
   static_assert(STAGE % (1024 * NW) == 0 && NI % 2 == 0 && BM % 16 == 0, "tile");
-  __shared__ __attribute__((aligned(16))) char lds[kStages][STAGE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+};
+
+template <typename C, typename TO>
+__global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) int8_mm(MmArgs a) {
+  constexpr int BM = C::BM, BN = C::BN, NW = C::NW, MI = C::MI, NI = C::NI, NL = C::NL;
+  constexpr int ST = C::ST;
+  __shared__ __attribute__((aligned(16))) char lds[ST * C::STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, lg = lane >> 4;
 
   // tiles: neighbours on one XCD, four rows of tiles before the next column
@@ -78,12 +176,12 @@ __global__ void __launch_bounds__(64 * WR * WC) int8_mm(MmArgs a) {
   const int rows = a.tm - 4 * group < 4 ? a.tm - 4 * group : 4;
   const int m0 = (4 * group + in_group % rows) * BM, n0 = (in_group / rows) * BN;
 
-  // this lane's source of each DMA: row and piece of the staged tile
+  // this lane's source of each DMA: row and piece of the slice
   const char* src[NL];
   int at[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int r = (wave * NL + i) * 16 + lane / 4, p = lane % 4;
+    const int r = (wave * NL + i) * 8 + lane / 8, p = lane % 8;
     if (r < BM) {
       const int m = m0 + r < a.M ? m0 + r : a.M - 1;
       src[i] = (const char*)a.x + m * a.ldx;
@@ -95,8 +193,8 @@ __global__ void __launch_bounds__(64 * WR * WC) int8_mm(MmArgs a) {
     }
   }
   const int last = (a.K + 15) / 16 * 16 - 16;   // the last readable piece of a row
-  auto load = [&](int kb) {
-    char* dst = lds[kb % kStages] + wave * NL * 1024;
+  auto load = [&](int kb, int buf) {
+    char* dst = lds + buf * C::STAGE + wave * NL * 1024;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int k = kb * kBK + at[i];
@@ -104,86 +202,82 @@ __global__ void __launch_bounds__(64 * WR * WC) int8_mm(MmArgs a) {
     }
   };
 
-  const int wm = (wave / WC) * WM, wn = (wave % WC) * WN;
+  // this lane's fragments in a slice; the slice's second half is 64 bytes on (^ 64)
+  const int wm = (wave / C::WC) * C::WM, wn = (wave % C::WC) * C::WN;
+  int rw[NI], rx[MI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int r = wn + (j / 2) * 32 + (li / 4) * 8 + (j & 1) * 4 + li % 4;
+    rw[j] = (BM + r) * kBK + 16 * (lg ^ swz_w(r));
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r = wm + i * 16 + li;
+    rx[i] = r * kBK + 16 * (lg ^ swz_x(r));
+  }
+  struct Frags {
+    i32x4 w[NI], x[MI];
+  };
+  auto read = [&](Frags& f, int buf, int half) {
+    const char* s = lds + buf * C::STAGE;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) f.w[j] = *reinterpret_cast<const i32x4*>(s + (rw[j] ^ half));
+#pragma unroll
+    for (int i = 0; i < MI; ++i) f.x[i] = *reinterpret_cast<const i32x4*>(s + (rx[i] ^ half));
+  };
   i32x4 acc[NI][MI];
 #pragma unroll
   for (int j = 0; j < NI; ++j)
 #pragma unroll
     for (int i = 0; i < MI; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+  auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[j][i] = mma8(f.w[j], f.x[i], acc[j][i]);
+  };
 
   const int nk = (a.K + kBK - 1) / kBK;
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s)
-    if (s < nk) load(s);
+  for (int s = 0; s < ST; ++s)
+    if (s < nk) load(s, s);
+  if (nk >= ST)
+    wait_vmcnt<(ST - 1) * NL>();
+  else
+    wait_vmcnt<0>();
+  lds_barrier();
+  // a half slice is multiplied while the next one is read
+  Frags f0, f1;
+  read(f0, 0, 0);
+  int buf = 0;
   for (int kb = 0; kb < nk; ++kb) {
-    // slice kb has arrived once only the later ones (kStages - 2 of them) are in flight
-    if (kb + kStages - 1 <= nk)
-      wait_vmcnt<(kStages - 2) * NL>();
-    else
-      wait_vmcnt<0>();
-    lds_barrier();   // also: every wave is done with slice kb - 1, whose buffer is next
-    if (kb + kStages - 1 < nk) load(kb + kStages - 1);
-    const char* sx = lds[kb % kStages];
-    const char* sw = sx + BM * kBK;
-    i32x4 fw[NI], fx[MI];
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int r = wn + (j / 2) * 32 + (li / 4) * 8 + (j & 1) * 4 + li % 4;
-      fw[j] = *reinterpret_cast<const i32x4*>(sw + r * kBK + 16 * (lg ^ swz_w(r)));
-    }
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int r = wm + i * 16 + li;
-      fx[i] = *reinterpret_cast<const i32x4*>(sx + r * kBK + 16 * (lg ^ swz_x(r)));
-    }
+    read(f1, buf, 64);
     if (kb * kBK + kBK > a.K) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fx[i] = keep_bytes(fx[i], a.K - kb * kBK - 16 * lg);
+      for (int i = 0; i < MI; ++i) {
+        f0.x[i] = keep_bytes(f0.x[i], a.K - kb * kBK - 16 * lg);
+        f1.x[i] = keep_bytes(f1.x[i], a.K - kb * kBK - 64 - 16 * lg);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < NI; ++j)
-#pragma unroll
-      for (int i = 0; i < MI; ++i) acc[j][i] = mma8(fw[j], fx[i], acc[j][i]);
+    multiply(f0);
+    // slice kb + 1 has arrived once only the ST - 2 later ones are in flight; every wave has
+    // read slice kb, whose buffer is free
+    if (kb + ST <= nk)
+      wait_vmcnt<(ST - 2) * NL>();
+    else
+      wait_vmcnt<0>();
+    lds_barrier();
+    if (kb + ST < nk) load(kb + ST, buf);
+    buf = buf + 1 == ST ? 0 : buf + 1;
+    read(f0, buf, 0);   // after the last slice: stale data that nothing uses
+    multiply(f1);
   }
 
-  // lane: row m = li of tile i, columns 8 lg .. 8 lg + 7 of the tile pair j, j + 1
-  TO* out = (TO*)a.out;
-#pragma unroll
-  for (int j = 0; j < NI; j += 2) {
-    const int n = n0 + wn + j * 16 + lg * 8;
-    float sw[8], bias[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int ne = n + e < a.N ? n + e : a.N - 1;
-      sw[e] = a.sw[ne];
-      bias[e] = a.bias ? a.bias[ne] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + wm + i * 16 + li;
-      if (m >= a.M) continue;
-      const float s = a.sx[m];
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = (float)acc[j + e / 4][i][e % 4] * s * sw[e];
-        if (a.bias) y[e] += bias[e];
-      }
-      TO* p = out + (long long)m * a.N + n;
-      if (a.vec && n + 8 <= a.N) {
-        if constexpr (sizeof(TO) == 2) {
-          *reinterpret_cast<bf16x8*>(p) = make_op(y, (bf16x8*)nullptr);
-        } else {
-          store4(p, f32x4{y[0], y[1], y[2], y[3]});
-          store4(p + 4, f32x4{y[4], y[5], y[6], y[7]});
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < a.N) p[e] = from_f<TO>(y[e]);
-      }
-    }
-  }
+  const int m = m0 + wm, n = n0 + wn;
+  store_part<TO>(
+      a, acc, m, n, li, lg, [&](int r) { return a.sx[m + r < a.M ? m + r : a.M - 1]; },
+      [&](int c) { return a.sw[n + c < a.N ? n + c : a.N - 1]; },
+      [&](int c) { return a.bias[n + c < a.N ? n + c : a.N - 1]; });
 }
 
 // 16 weight rows and all of x's (up to 16 MT) a workgroup; wave w takes the slices of 128
@@ -194,13 +288,13 @@ __global__ void __launch_bounds__(512) int8_mm_rows(MmArgs a) {
   __shared__ int sum[NW][MT][16][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int li = lane & 15, lg = lane >> 4;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
   const int n = n0 + li < a.N ? n0 + li : a.N - 1;
   const char* w = (const char*)a.w + n * a.ldw;
   const char* x[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int m = i * 16 + li < a.M ? i * 16 + li : a.M - 1;
+    const int m = m0 + i * 16 + li < a.M ? m0 + i * 16 + li : a.M - 1;
     x[i] = (const char*)a.x + m * a.ldx;
   }
   const int last = (a.K + 15) / 16 * 16 - 16;
@@ -235,11 +329,11 @@ __global__ void __launch_bounds__(512) int8_mm_rows(MmArgs a) {
     for (int r = 0; r < 4; ++r) sum[wave][i][li][4 * lg + r] = acc[i][r];
   __syncthreads();
   for (int e = threadIdx.x; e < MT * 256; e += 64 * NW) {
-    const int m = e / 16, c = e % 16;
+    const int ml = e / 16, c = e % 16, m = m0 + ml;
     if (m < a.M && n0 + c < a.N) {
       int s = 0;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) s += sum[k][m / 16][m % 16][c];
+      for (int k = 0; k < NW; ++k) s += sum[k][ml / 16][ml % 16][c];
       float y = (float)s * a.sx[m] * a.sw[n0 + c];
       if (a.bias) y += a.bias[n0 + c];
       ((TO*)a.out)[(long long)m * a.N + n0 + c] = from_f<TO>(y);
@@ -247,35 +341,51 @@ __global__ void __launch_bounds__(512) int8_mm_rows(MmArgs a) {
   }
 }
 
-template <int BM, int BN, int WR, int WC, typename TO>
+template <typename C, typename TO>
 void launch_tiles(hipStream_t st, MmArgs a) {
-  a.tm = (a.M + BM - 1) / BM;
-  a.tn = (a.N + BN - 1) / BN;
+  a.tm = (a.M + C::BM - 1) / C::BM;
+  a.tn = (a.N + C::BN - 1) / C::BN;
   a.chunk = (a.tm * a.tn + 7) / 8;
-  hipLaunchKernelGGL((int8_mm<BM, BN, WR, WC, TO>), dim3(8u * (unsigned)a.chunk),
-                     dim3(64 * WR * WC), 0, st, a);
+  hipLaunchKernelGGL((int8_mm<C, TO>), dim3(8u * (unsigned)a.chunk), dim3(64 * C::NW), 0, st, a);
+}
+template <int MT, typename TO>
+void launch_rows(hipStream_t st, const MmArgs& a) {
+  hipLaunchKernelGGL((int8_mm_rows<MT, TO>),
+                     dim3((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+                     dim3(512), 0, st, a);
 }
 
 template <typename TO>
 hipError_t launch_mm(hipStream_t st, const MmArgs& a) {
-  const long long cus = num_cus();
+  // (M x N x K, bfloat16 results, one kernel, us)
+  const int cus = num_cus();
   auto tiles = [&](int bm, int bn) {
     return (((long long)a.M + bm - 1) / bm) * (((long long)a.N + bn - 1) / bn);
   };
-  if (a.M <= 64) {
-    const dim3 grid((unsigned)((a.N + 15) / 16)), block(512);
-    if (a.M <= 16)
-      hipLaunchKernelGGL((int8_mm_rows<1, TO>), grid, block, 0, st, a);
-    else if (a.M <= 32)
-      hipLaunchKernelGGL((int8_mm_rows<2, TO>), grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL((int8_mm_rows<4, TO>), grid, block, 0, st, a);
-  } else if (tiles(256, 256) >= cus) {
-    launch_tiles<256, 256, 2, 4, TO>(st, a);
-  } else if (tiles(128, 128) >= cus) {
-    launch_tiles<128, 128, 2, 2, TO>(st, a);
+  // Few rows, or few columns of few rows: 1 x 4608 x 768 2.9 (64 x 64 tiles: 4.0),
+  // 8 x 8192 x 8192 14.3 (18.7), 32 x 4096 x 4096 7.6 (10.6), 500 x 200 x 300 2.8 (4.0),
+  // 128 x 64 x 8192 12.3 (18.4); but 64 x 4608 x 768 5.2 (4.6), 300 x 1024 x 8192 33.9 (19.1).
+  if (a.M <= 16) {
+    launch_rows<1, TO>(st, a);
+  } else if (a.M <= 32 || tiles(32, 16) <= cus) {
+    launch_rows<2, TO>(st, a);
+    // All tiles at once on the CUs, three each: 512 x 4096 x 4096 16.4 (128 x 128: 24.0),
+    // 1024 x 2048 x 2048 10.0 (14.3); but 2048 x 2048 x 1024, 1024 tiles, 11.9 (10.5).
+  } else if (tiles(64, 64) <= 3 * cus) {
+    launch_tiles<Tile<64, 64, 2, 2, 3, 3>, TO>(st, a);
   } else {
-    launch_tiles<128, 64, 2, 2, TO>(st, a);
+    // 192 x 128 does a unit of work in 0.92 of the time of 128 x 128 (8192 x 8192 x 8192 496 and
+    // 529, 65536 x 4608 x 768 342 and 372) where the rounds of two workgroups a CU come
+    // out as well: 3000 x 3000 x 3000 40.3 and 49.7, but 4096 x 4096 x 4096 80.2 and 72.8,
+    // 16384 x 512 x 1024 17.9 and 15.0.  A last round that is not full counts half as one.
+    auto cost = [&](int bm, double unit) {
+      const double r = (double)tiles(bm, 128) / (2 * cus);
+      return (r < 1 ? 1 : (r + (double)(long long)(r + 0.999999)) / 2) * bm * unit;
+    };
+    if (cost(192, 0.92) < cost(128, 1.0))
+      launch_tiles<Tile<192, 128, 2, 2, 2, 2>, TO>(st, a);
+    else
+      launch_tiles<Tile<128, 128, 2, 2, 2, 2>, TO>(st, a);
   }
   return hipGetLastError();
 }

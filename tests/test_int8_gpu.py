@@ -135,7 +135,7 @@ def test_product(dev, M, N):
 @pytest.mark.parametrize("M,N,K", [(2050, 2100, 200), (4100, 4104, 130), (4097, 4353, 64),
                                    (65600, 70, 40), (70, 20000, 70), (64, 9000, 2000)])
 def test_product_of_many_tiles(dev, M, N, K):
-    """Enough tiles of 128 x 128 and 256 x 256 to choose them, and long thin products."""
+    """Enough tiles to choose those of 128 x 128 and of 192 x 128, and long thin products."""
     import gdn2_package as gp
     q, sx, w, sw, bias = operands(M, N, K, dev, K)
     for dt, b in ((F32, None), (BF16, bias.bfloat16())):
