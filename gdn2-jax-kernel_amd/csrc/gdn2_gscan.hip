@@ -9,15 +9,25 @@
 // e^L, is carried, so that L = -inf says that the run holds a fresh start, and sums of
 // small decays lose nothing.  Everything is held in float32.
 //
-// One workgroup walks the whole axis for 16 channels, 256 tokens at a time.  A thread
-// takes V neighbouring channels (8- or 16-byte accesses) of S consecutive tokens: it
-// composes its run in registers, the runs of a wave are composed by lane shuffles, the
-// four waves' through LDS, and the thread then walks its tokens again from the state
-// that enters them.  The data are read once, and the next 256 tokens are in flight
-// meanwhile.  The backward pass needs the state before every token: the forward pass
-// keeps the state that enters each 256 tokens (1/256 of the data), from which the
-// backward forms them again on its way from the last 256 tokens to the first, so
-// that it too reads every input once and never reads the outputs.
+// A thread takes V neighbouring channels (8- or 16-byte accesses) of 16 / V consecutive tokens:
+// it composes its run in registers, the runs of a wave are composed by lane shuffles and
+// the waves' through LDS, and the thread then walks its tokens again from the state that
+// enters them.  The data are read once and the results written once, which bounds all of it.
+//
+// Short axes: a workgroup walks along the whole axis for its tile of channels, 128 tokens at a
+// time, the next ones in flight meanwhile.  Long axes: every step (512 threads, 8192 values)
+// has a workgroup of its own and the state is handed on through memory, in one pass over the
+// data too.  Tiles are wide where there are channels enough: rows of 32 bytes, a quarter of
+// a line, keep the address path busy without moving much (8 x 8192 x 768 bfloat16, walked
+// in tiles of 16, 32 and 64 channels, which leave ever more CUs without work: 201, 150, 191 us;
+// in steps at once 167, 125, 115).  Copies reach 5.16 TB/s on this card; these reach, forward
+// and backward: 8 x 8192 x 768 bfloat16 4.4 and 4.6 TB/s, 2 x 16384 x 2048 bfloat16 4.7 and 5.0,
+// 1 x 131072 x 1024 float32 without a gate forward 5.2.
+//
+// The backward pass needs the state before every token: the forward pass keeps the state
+// that enters each step (under 1% of the data), from which the backward forms them again on
+// its way from the last step to the first, so that it too reads every input once and never
+// reads the outputs.
 #include <limits.h>
 
 #include "gdn2.h"
@@ -26,9 +36,8 @@
 namespace gdn2 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kTile = 16;      // channels of a workgroup
-constexpr int kBlock = 256;    // tokens of a step of the walk, and between kept states
+constexpr int kThreads = 256;  // of the elementwise kernels
+constexpr int kMinTile = 16;   // channels of the narrowest workgroup
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Strides are in elements; channels are contiguous.
@@ -42,9 +51,9 @@ struct ScanArgs {
   const float* dh_final;  // (B, C) or null
   void *out, *dx, *dg, *db;            // (B, T, C) dense
   float *h_final, *dh0;                // (B, C)
-  float* kept;                         // (ceil(T / kBlock), B, C) or null
-  float* seg;                          // (nseg, 2, B, C): L and H (or D) of each segment
-  int B, T, C, nct, nseg, seg_blocks;  // channel tiles; segments of seg_blocks steps
+  float* kept;                         // (steps, B, C) or null
+  void* ws;
+  int B, T, C, nct;                    // nct: channel tiles
   int chunk;                           // work items of one XCD
 };
 
@@ -84,36 +93,36 @@ __device__ __forceinline__ void put(T* p, const float (&f)[V]) {
   }
 }
 
-// Where a workgroup and a thread work.
-template <int V>
+// Where a workgroup and a thread work: NT threads, CT channels, V neighbouring ones a
+// thread, 16 values of a step for each.
+template <int V, int CT, int NT_>
 struct Place {
-  static constexpr int LPR = kTile / V;              // lanes across the channels
+  static constexpr int NT = NT_, NW = NT / 64;       // threads, waves
+  static constexpr int BLOCK = 16 * NT / CT;         // tokens of a step
+  static constexpr int LPR = CT / V;                 // lanes across the channels
   static constexpr int TLW = 64 / LPR;               // runs of a wave
-  static constexpr int S = kBlock * LPR / kThreads;  // tokens of a run
-  int lane, wave, tl, c, b, seg;
+  static constexpr int S = 16 / V;                   // tokens of a run
+  static_assert(LPR <= 64 && TLW * NW * S == BLOCK, "a step is the workgroup's runs");
+  int lane, wave, tl, ci, c, b;
   bool on;       // the channels exist
   bool idle;     // the workgroup has no work
-  int blk0, blk1;
+  int blocks;    // steps of the axis
   __device__ Place(const ScanArgs& a) {
     // neighbouring channel tiles share cache lines: consecutive items on one XCD
-    const int item = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
-    const int units = a.B * a.nct;
-    idle = (blockIdx.x >> 3) >= a.chunk || item >= units * a.nseg;
-    seg = item / units;
-    const int unit = item - seg * units;
+    const int unit = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
+    idle = (int)(blockIdx.x >> 3) >= a.chunk || unit >= a.B * a.nct;
     b = unit / a.nct;
     lane = threadIdx.x & 63;
     wave = threadIdx.x >> 6;
     tl = lane / LPR;
-    c = (unit - b * a.nct) * kTile + (lane % LPR) * V;
+    ci = (lane % LPR) * V;
+    c = (unit - b * a.nct) * CT + ci;
     on = c < a.C;
     if (!on) c = 0;   // loads stay in bounds, nothing is stored
-    blk0 = seg * a.seg_blocks;
-    const int n = (a.T + kBlock - 1) / kBlock;
-    blk1 = blk0 + a.seg_blocks < n ? blk0 + a.seg_blocks : n;
+    blocks = (a.T + BLOCK - 1) / BLOCK;
   }
   // first token of the thread's run in step blk
-  __device__ int first(int blk) const { return blk * kBlock + (wave * TLW + tl) * S; }
+  __device__ int first(int blk) const { return blk * BLOCK + (wave * TLW + tl) * S; }
   __device__ size_t bc(const ScanArgs& a) const { return (size_t)b * a.C + c; }
 };
 
@@ -197,34 +206,43 @@ __device__ __forceinline__ float token(float a, float h, float u) {
   return fmaf(a, a < 0.f ? 0.f : h, u);
 }
 
-// The state that enters segment `seg`, from the earlier segments' compositions.
-template <int V>
-__device__ __forceinline__ void enter(const ScanArgs& a, size_t bc, int from, int to, int step,
-                                      float (&h)[V]) {
-  const size_t n = (size_t)a.B * a.C;
-  for (int s = from; s != to; s += step) {
-    const float* p = a.seg + 2 * n * s + bc;
+// A wave's composition in LDS: e^L (negative for a fresh start), and H or D.
+template <int NW, int CT>
+struct Totals {
+  float a[2][NW][CT], h[2][NW][CT];   // two buffers: one barrier a step
+  template <int V>
+  __device__ __forceinline__ void put_(int buf, int wave, int ci, const float (&L)[V],
+                                       const float (&H)[V]) {
+    float f[V];
 #pragma unroll
-    for (int c = 0; c < V; ++c) h[c] = carry_through(p[c], h[c], p[n + c]);
+    for (int c = 0; c < V; ++c) f[c] = L[c] == kNegInf ? -1.f : exp2_(L[c]);
+    put<float, V>(&a[buf][wave][ci], f);
+    put<float, V>(&h[buf][wave][ci], H);
   }
-}
+  // h <- e^L h + H of wave k
+  template <int V>
+  __device__ __forceinline__ void pass(int buf, int k, int ci, float (&x)[V]) const {
+    const auto av = *reinterpret_cast<const typename Raw<float, V>::type*>(&a[buf][k][ci]);
+    const auto hv = *reinterpret_cast<const typename Raw<float, V>::type*>(&h[buf][k][ci]);
+    float af[V], hf[V];
+    widen<float, V>(av, af);
+    widen<float, V>(hv, hf);
+#pragma unroll
+    for (int c = 0; c < V; ++c) x[c] = fmaf(af[c], af[c] < 0.f ? 0.f : x[c], hf[c]);
+  }
+};
 
-// Forward.  SUMMARY: only the composition of each segment, into a.seg.
-template <typename TX, typename TG, bool GATE, int V, bool SUMMARY>
-__global__ void __launch_bounds__(kThreads) gscan_fwd(ScanArgs a) {
-  using P = Place<V>;
-  constexpr int S = P::S, LPR = P::LPR;
-  __shared__ float sL[2][4][kTile], sH[2][4][kTile];
+// Forward.
+template <typename TX, typename TG, bool GATE, int V, int CT>
+__global__ void __launch_bounds__(8 * CT) gscan_fwd(ScanArgs a) {
+  using P = Place<V, CT, 8 * CT>;
+  constexpr int S = P::S, LPR = P::LPR, NW = P::NW;
+  __shared__ __attribute__((aligned(16))) Totals<NW, CT> tot;
   const P w(a);
   if (w.idle) return;
-  const int ci = (w.lane % LPR) * V;   // channel within the tile
-  float h[V], Ls[V];
+  float h[V];
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    h[c] = !SUMMARY && a.h0 ? a.h0[w.bc(a) + c] : 0.f;
-    Ls[c] = 0.f;
-  }
-  if (!SUMMARY) enter<V>(a, w.bc(a), 0, w.seg, 1, h);
+  for (int c = 0; c < V; ++c) h[c] = a.h0 ? a.h0[w.bc(a) + c] : 0.f;
   Run<TX, V, S> x;
   Run<TG, V, S> g;
   std::conditional_t<GATE, Run<TX, V, S>, None> b;
@@ -234,12 +252,12 @@ __global__ void __launch_bounds__(kThreads) gscan_fwd(ScanArgs a) {
     g.load(a.g, w.b, w.c, t, a.T);
     if constexpr (GATE) b.load(a.b, w.b, w.c, t, a.T);
   };
-  load(w.blk0);
-  for (int blk = w.blk0; blk < w.blk1; ++blk) {
+  load(0);
+  for (int blk = 0; blk < w.blocks; ++blk) {
     const int t = w.first(blk);
     Factors<V, S> f;
     factors<TX, TG, GATE, V, S>(f, x, g, b, t, a.T);
-    if (blk + 1 < w.blk1) load(blk + 1);
+    if (blk + 1 < w.blocks) load(blk + 1);
     float L[V], H[V], TL[V], TH[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) {
@@ -248,70 +266,47 @@ __global__ void __launch_bounds__(kThreads) gscan_fwd(ScanArgs a) {
     }
     wave_compose<V, LPR, false>(L, H, TL, TH, w.lane);
     const int buf = blk & 1;
-    if (w.lane >= 64 - LPR) {
-#pragma unroll
-      for (int c = 0; c < V; ++c) {
-        sL[buf][w.wave][ci + c] = TL[c];
-        sH[buf][w.wave][ci + c] = TH[c];
-      }
-    }
-    if (!SUMMARY && a.kept && w.on && w.wave == 0 && w.tl == 0)
+    if (w.lane >= 64 - LPR) tot.template put_<V>(buf, w.wave, w.ci, TL, TH);
+    if (a.kept && w.on && w.wave == 0 && w.tl == 0)
       put<float, V>(a.kept + (size_t)blk * a.B * a.C + w.bc(a), h);
     lds_barrier();   // the other buffer is written next: one barrier a step
     float mine[V];
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-      mine[c] = h[c];
+    for (int c = 0; c < V; ++c) mine[c] = h[c];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float l = sL[buf][k][ci + c];
-        if (k == w.wave) mine[c] = h[c];
-        h[c] = carry_through(l, h[c], sH[buf][k][ci + c]);
-        if (SUMMARY) Ls[c] += l;
-      }
+    for (int k = 0; k < NW; ++k) {
+      if (k == w.wave)
+#pragma unroll
+        for (int c = 0; c < V; ++c) mine[c] = h[c];
+      tot.template pass<V>(buf, k, w.ci, h);
     }
-    if constexpr (!SUMMARY) {
 #pragma unroll
-      for (int c = 0; c < V; ++c) mine[c] = carry_through(L[c], mine[c], H[c]);
-      TX* out = (TX*)a.out + (long long)w.b * a.T * a.C + w.c;
+    for (int c = 0; c < V; ++c) mine[c] = carry_through(L[c], mine[c], H[c]);
+    TX* out = (TX*)a.out + (long long)w.b * a.T * a.C + w.c;
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
+    for (int i = 0; i < S; ++i) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) mine[c] = token(f.a[i][c], mine[c], f.u[i][c]);
-        if (w.on && t + i < a.T) put<TX, V>(out + (long long)(t + i) * a.C, mine);
-      }
+      for (int c = 0; c < V; ++c) mine[c] = token(f.a[i][c], mine[c], f.u[i][c]);
+      if (w.on && t + i < a.T) put<TX, V>(out + (long long)(t + i) * a.C, mine);
     }
   }
-  if (w.on && w.wave == 0 && w.tl == 0) {
-    if constexpr (SUMMARY) {
-      const size_t n = (size_t)a.B * a.C;
-      put<float, V>(a.seg + 2 * n * w.seg + w.bc(a), Ls);
-      put<float, V>(a.seg + 2 * n * w.seg + n + w.bc(a), h);
-    } else if (w.seg == a.nseg - 1) {
-      put<float, V>(a.h_final + w.bc(a), h);
-    }
-  }
+  if (w.on && w.wave == 0 && w.tl == 0) put<float, V>(a.h_final + w.bc(a), h);
 }
 
 // Backward.  With e the gradient that reaches the state after token t from later tokens
 // (dh_final after the last): dh = dout_t + e, dx = b dh, db = x dh, dg = a h_{t-1} dh,
 // and a dh goes on to the token before; a run maps the e entering it from the right to
-// e^L e + D.  SUMMARY: only L and D of each segment.
-template <typename TX, typename TG, bool GATE, int V, bool SUMMARY>
-__global__ void __launch_bounds__(kThreads) gscan_bwd(ScanArgs a) {
-  using P = Place<V>;
-  constexpr int S = P::S, LPR = P::LPR;
-  __shared__ float sL[2][4][kTile], sH[2][4][kTile], sD[2][4][kTile];
+// e^L e + D.
+template <typename TX, typename TG, bool GATE, int V, int CT>
+__global__ void __launch_bounds__(8 * CT) gscan_bwd(ScanArgs a) {
+  using P = Place<V, CT, 8 * CT>;
+  constexpr int S = P::S, LPR = P::LPR, NW = P::NW;
+  __shared__ __attribute__((aligned(16))) Totals<NW, CT> fwd, rev;
   const P w(a);
   if (w.idle) return;
-  const int ci = (w.lane % LPR) * V;
-  float e[V], Ls[V];
+  float e[V];
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    e[c] = !SUMMARY && a.dh_final ? a.dh_final[w.bc(a) + c] : 0.f;
-    Ls[c] = 0.f;
-  }
-  if (!SUMMARY) enter<V>(a, w.bc(a), a.nseg - 1, w.seg, -1, e);
+  for (int c = 0; c < V; ++c) e[c] = a.dh_final ? a.dh_final[w.bc(a) + c] : 0.f;
   const bool has_dout = a.dout.p != nullptr;
   Run<TX, V, S> x, d;
   Run<TG, V, S> g;
@@ -323,37 +318,21 @@ __global__ void __launch_bounds__(kThreads) gscan_bwd(ScanArgs a) {
     const int t = w.first(blk);
     g.load(a.g, w.b, w.c, t, a.T);
     if (has_dout) d.load(a.dout, w.b, w.c, t, a.T);
-    if constexpr (!SUMMARY) {
-      x.load(a.x, w.b, w.c, t, a.T);
-      if constexpr (GATE) b.load(a.b, w.b, w.c, t, a.T);
+    x.load(a.x, w.b, w.c, t, a.T);
+    if constexpr (GATE) b.load(a.b, w.b, w.c, t, a.T);
 #pragma unroll
-      for (int c = 0; c < V; ++c) h[c] = a.kept[(size_t)blk * a.B * a.C + w.bc(a) + c];
-    }
+    for (int c = 0; c < V; ++c) h[c] = a.kept[(size_t)blk * a.B * a.C + w.bc(a) + c];
   };
-  load(w.blk1 - 1);
-  for (int blk = w.blk1 - 1; blk >= w.blk0; --blk) {
+  load(w.blocks - 1);
+  for (int blk = w.blocks - 1; blk >= 0; --blk) {
     const int t = w.first(blk);
     Factors<V, S> f;
     float xv[S][V], bv[S][V], dv[S][V], hw[V];
-    if constexpr (SUMMARY) {
+    factors<TX, TG, GATE, V, S>(f, x, g, b, t, a.T);
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        float gv[V];
-        widen<TG, V>(g.r[i], gv);
-#pragma unroll
-        for (int c = 0; c < V; ++c) {
-          const float l = t + i < a.T ? gv[c] * kLog2e : 0.f;
-          f.a[i][c] = l == kNegInf ? -1.f : exp2_(l);
-          f.L[c] = (i == 0 ? 0.f : f.L[c]) + l;
-        }
-      }
-    } else {
-      factors<TX, TG, GATE, V, S>(f, x, g, b, t, a.T);
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        widen<TX, V>(x.r[i], xv[i]);
-        if constexpr (GATE) widen<TX, V>(b.r[i], bv[i]);
-      }
+    for (int i = 0; i < S; ++i) {
+      widen<TX, V>(x.r[i], xv[i]);
+      if constexpr (GATE) widen<TX, V>(b.r[i], bv[i]);
     }
 #pragma unroll
     for (int i = 0; i < S; ++i) {
@@ -364,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) gscan_bwd(ScanArgs a) {
     }
 #pragma unroll
     for (int c = 0; c < V; ++c) hw[c] = h[c];
-    if (blk > w.blk0) load(blk - 1);
+    if (blk > 0) load(blk - 1);
     float L[V], H[V], R[V], D[V], TL[V], TH[V], TD[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) {
@@ -372,85 +351,346 @@ __global__ void __launch_bounds__(kThreads) gscan_bwd(ScanArgs a) {
 #pragma unroll
       for (int i = S - 1; i >= 0; --i)
         D[c] = f.a[i][c] < 0.f ? 0.f : f.a[i][c] * (dv[i][c] + D[c]);
-      R[c] = f.L[c];
-      if constexpr (!SUMMARY) {
-        L[c] = f.L[c];
-        H[c] = f.H[c];
-      }
+      R[c] = L[c] = f.L[c];
+      H[c] = f.H[c];
     }
     const int buf = blk & 1;
-    if constexpr (!SUMMARY) {
-      wave_compose<V, LPR, false>(L, H, TL, TH, w.lane);
-      if (w.lane >= 64 - LPR) {
-#pragma unroll
-        for (int c = 0; c < V; ++c) sH[buf][w.wave][ci + c] = TH[c];
-      }
-    }
+    wave_compose<V, LPR, false>(L, H, TL, TH, w.lane);
+    if (w.lane >= 64 - LPR) fwd.template put_<V>(buf, w.wave, w.ci, TL, TH);
     wave_compose<V, LPR, true>(R, D, TL, TD, w.lane);
-    if (w.lane < LPR) {
-#pragma unroll
-      for (int c = 0; c < V; ++c) {
-        sL[buf][w.wave][ci + c] = TL[c];
-        sD[buf][w.wave][ci + c] = TD[c];
-      }
-    }
+    if (w.lane < LPR) rev.template put_<V>(buf, w.wave, w.ci, TL, TD);
     lds_barrier();
     float mine[V];
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-      mine[c] = e[c];
+    for (int c = 0; c < V; ++c) mine[c] = e[c];
 #pragma unroll
-      for (int k = 3; k >= 0; --k) {
-        const float l = sL[buf][k][ci + c];
-        if (k == w.wave) mine[c] = e[c];
-        e[c] = carry_through(l, e[c], sD[buf][k][ci + c]);
-        if (SUMMARY) Ls[c] += l;
+    for (int k = NW - 1; k >= 0; --k) {
+      if (k == w.wave)
+#pragma unroll
+        for (int c = 0; c < V; ++c) mine[c] = e[c];
+      rev.template pass<V>(buf, k, w.ci, e);
+    }
+#pragma unroll
+    for (int k = 0; k < NW - 1; ++k)
+      if (k < w.wave) fwd.template pass<V>(buf, k, w.ci, hw);
+    float before[S][V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      float hc = carry_through(L[c], hw[c], H[c]);
+      mine[c] = carry_through(R[c], mine[c], D[c]);
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        before[i][c] = hc;
+        hc = token(f.a[i][c], hc, f.u[i][c]);
       }
     }
-    if constexpr (!SUMMARY) {
-      float before[S][V];
+    const long long o = (long long)w.b * a.T * a.C + w.c;
+#pragma unroll
+    for (int i = S - 1; i >= 0; --i) {
+      float dx[V], dg[V], db[V];
 #pragma unroll
       for (int c = 0; c < V; ++c) {
-        float hc = hw[c];
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          if (k < w.wave) hc = carry_through(sL[buf][k][ci + c], hc, sH[buf][k][ci + c]);
-        hc = carry_through(L[c], hc, H[c]);
-        mine[c] = carry_through(R[c], mine[c], D[c]);
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          before[i][c] = hc;
-          hc = token(f.a[i][c], hc, f.u[i][c]);
-        }
+        const float dh = dv[i][c] + mine[c], av = f.a[i][c];
+        mine[c] = av < 0.f ? 0.f : av * dh;
+        dg[c] = av < 0.f ? 0.f : mine[c] * before[i][c];
+        dx[c] = GATE ? bv[i][c] * dh : dh;
+        db[c] = xv[i][c] * dh;
       }
-      const long long o = (long long)w.b * a.T * a.C + w.c;
-#pragma unroll
-      for (int i = S - 1; i >= 0; --i) {
-        float dx[V], dg[V], db[V];
-#pragma unroll
-        for (int c = 0; c < V; ++c) {
-          const float dh = dv[i][c] + mine[c], av = f.a[i][c];
-          mine[c] = av < 0.f ? 0.f : av * dh;
-          dg[c] = av < 0.f ? 0.f : mine[c] * before[i][c];
-          dx[c] = GATE ? bv[i][c] * dh : dh;
-          db[c] = xv[i][c] * dh;
-        }
-        if (w.on && t + i < a.T) {
-          const long long at = o + (long long)(t + i) * a.C;
-          put<TX, V>((TX*)a.dx + at, dx);
-          put<TG, V>((TG*)a.dg + at, dg);
-          if constexpr (GATE) put<TX, V>((TX*)a.db + at, db);
-        }
+      if (w.on && t + i < a.T) {
+        const long long at = o + (long long)(t + i) * a.C;
+        put<TX, V>((TX*)a.dx + at, dx);
+        put<TG, V>((TG*)a.dg + at, dg);
+        if constexpr (GATE) put<TX, V>((TX*)a.db + at, db);
       }
     }
   }
-  if (w.on && w.wave == 0 && w.tl == 0) {
-    if constexpr (SUMMARY) {
-      const size_t n = (size_t)a.B * a.C;
-      put<float, V>(a.seg + 2 * n * w.seg + w.bc(a), Ls);
-      put<float, V>(a.seg + 2 * n * w.seg + n + w.bc(a), e);
-    } else if (w.seg == 0 && a.dh0) {
-      put<float, V>(a.dh0 + w.bc(a), e);
+  if (w.on && w.wave == 0 && w.tl == 0 && a.dh0) put<float, V>(a.dh0 + w.bc(a), e);
+}
+
+// ---- The axis cut into its steps, all in one launch --------------------------------
+// A workgroup takes 128 tokens of 64 channels (or 256 of 32, 512 of 16).  It publishes its composition as soon as it
+// has it, finds the state that enters it from the steps before, and publishes the one
+// that leaves it.  Steps are dealt by a ticket, the earliest of all channels first: a
+// workgroup waits only for ones with smaller tickets, which have started and which in their
+// turn never wait for it, so every wait ends whatever else the GPU runs.  The entering state
+// is always the same sequence of operations -- the nearest published state, carried through
+// the published compositions after it, each rounded the same wherever it is done -- so
+// results do not depend on what was found first.
+//
+// A published value is 64 bits written at once, {e^L or a tag, H or the state}; the memory is
+// filled with kNone before the launch, whose upper word is no such float.
+constexpr unsigned long long kNone = ~0ull;
+constexpr int kWindow = 4;      // steps looked back over at a time
+struct Chain {
+  unsigned long long *comp, *state;   // (steps, B, C) each
+  unsigned* ticket;
+};
+
+__device__ __forceinline__ unsigned long long pack(float hi, float lo) {
+  return ((unsigned long long)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+}
+__device__ __forceinline__ float upper(unsigned long long v) {
+  return __uint_as_float((unsigned)(v >> 32));
+}
+__device__ __forceinline__ float lower(unsigned long long v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ void publish(unsigned long long* p, float hi, float lo) {
+  __hip_atomic_store(p, pack(hi, lo), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// h through a composition (a = e^L, negative for a fresh start)
+__device__ __forceinline__ float through(float a, float h, float u) {
+  return fmaf(a, a < 0.f ? 0.f : h, u);
+}
+
+// The state that enters step blk (REV: from the right), for one channel a lane; `start` is
+// the one that enters the first.  at: the channel's place; on: it exists.
+template <bool REV>
+__device__ __forceinline__ float entering(const Chain& ch, size_t n, size_t at, bool on, int blk,
+                                          int blocks, float start) {
+  while (true) {
+    unsigned long long s[kWindow], m[kWindow];
+#pragma unroll
+    for (int d = 0; d < kWindow; ++d) {
+      const int j = REV ? blk + 1 + d : blk - 1 - d;
+      const bool in = REV ? j < blocks : j >= 0;
+      const size_t o = (size_t)(in ? j : blk) * n + at;
+      s[d] = __hip_atomic_load(ch.state + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      m[d] = __hip_atomic_load(ch.comp + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (!in || !on) s[d] = pack(0.f, start);
+      if (!on) m[d] = 0;
+    }
+    float h = 0.f;
+    int found = -1;
+#pragma unroll
+    for (int d = 0; d < kWindow; ++d) {
+      if (found == -1) {
+        if (__all(s[d] != kNone)) {
+          found = d;
+          h = lower(s[d]);
+        } else if (!__all(m[d] != kNone)) {
+          found = -2;   // a gap: look again
+        }
+      }
+    }
+    if (found >= 0) {
+#pragma unroll
+      for (int d = kWindow - 2; d >= 0; --d)
+        if (d < found) h = through(upper(m[d]), h, lower(m[d]));
+      return h;
+    }
+    __builtin_amdgcn_s_sleep(2);
+  }
+}
+
+// One wave, a channel a lane: publish the workgroup's composition, find the entering state,
+// publish the leaving one.  Returns both.
+template <bool REV, int NW, int CT>
+__device__ __forceinline__ void link(const Chain& ch, const Totals<NW, CT>& tot, size_t n,
+                                     size_t at, bool on, int blk, int blocks, float start, int lane,
+                                     float& in, float& out) {
+  float A = 1.f, H = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const int k = REV ? NW - 1 - i : i;
+    const float ak = tot.a[0][k][lane % CT], hk = tot.h[0][k][lane % CT];
+    H = through(ak, H, hk);
+    A = ak < 0.f || A < 0.f ? -1.f : A * ak;
+  }
+  if (A != A) A = __uint_as_float(0x7fc00000u);   // any NaN but kNone's
+  // the steps after this one, if any, read these
+  const bool first = REV ? blk == blocks - 1 : blk == 0, last = REV ? blk == 0 : blk == blocks - 1;
+  const size_t o = (size_t)blk * n + at;
+  if (!last && !first && on) publish(ch.comp + o, A, H);
+  in = first ? start : entering<REV>(ch, n, at, on, blk, blocks, start);
+  out = through(A, in, H);
+  if (!last && on) publish(ch.state + o, 0.f, out);
+}
+
+// The step and channels of a ticket.
+template <int V, int CT>
+struct Step : Place<V, CT, 512> {
+  int blk;
+  __device__ Step(const ScanArgs& a, int item, bool rev) : Place<V, CT, 512>(a) {
+    const int units = a.B * a.nct;
+    blk = item / units;
+    const int unit = item - blk * units;
+    if (rev) blk = this->blocks - 1 - blk;
+    this->b = unit / a.nct;
+    this->c = (unit - this->b * a.nct) * CT + this->ci;
+    this->on = this->c < a.C;
+    if (!this->on) this->c = 0;
+  }
+};
+// The channel of lane `lane` in the tile of ticket `item`; C, where the tile is narrower.
+template <int CT>
+__device__ __forceinline__ int tile_channel(const ScanArgs& a, int item, int lane) {
+  return lane < CT ? (item % (a.B * a.nct)) % a.nct * CT + lane : a.C;
+}
+__device__ __forceinline__ int next_ticket(unsigned* ticket, int* shared) {
+  if (threadIdx.x == 0) *shared = (int)atomicAdd(ticket, 1u);
+  __syncthreads();
+  return *shared;
+}
+
+__global__ void __launch_bounds__(kThreads) chain_clear(unsigned long long* p, size_t n,
+                                                        unsigned* ticket) {
+  const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i < n) p[i] = kNone;
+  if (i == 0) *ticket = 0;
+}
+
+template <typename TX, typename TG, bool GATE, int V, int CT>
+__global__ void __launch_bounds__(512, 4) chain_fwd(ScanArgs a, Chain ch) {
+  using P = Place<V, CT, 512>;
+  constexpr int S = P::S, LPR = P::LPR, NW = P::NW;
+  __shared__ __attribute__((aligned(16))) Totals<NW, CT> tot;
+  __shared__ __attribute__((aligned(16))) float s_in[CT];
+  __shared__ int s_ticket;
+  const Step<V, CT> w(a, next_ticket(ch.ticket, &s_ticket), false);
+  Run<TX, V, S> x;
+  Run<TG, V, S> g;
+  std::conditional_t<GATE, Run<TX, V, S>, None> b;
+  const int t = w.first(w.blk);
+  g.load(a.g, w.b, w.c, t, a.T);
+  x.load(a.x, w.b, w.c, t, a.T);
+  if constexpr (GATE) b.load(a.b, w.b, w.c, t, a.T);
+  Factors<V, S> f;
+  factors<TX, TG, GATE, V, S>(f, x, g, b, t, a.T);
+  float L[V], H[V], TL[V], TH[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    L[c] = f.L[c];
+    H[c] = f.H[c];
+  }
+  wave_compose<V, LPR, false>(L, H, TL, TH, w.lane);
+  if (w.lane >= 64 - LPR) tot.template put_<V>(0, w.wave, w.ci, TL, TH);
+  lds_barrier();
+  if (w.wave == 0) {
+    // lane = channel of the tile
+    const int unit_c = tile_channel<CT>(a, s_ticket, w.lane);
+    const bool on = unit_c < a.C;
+    const size_t n = (size_t)a.B * a.C, at = (size_t)w.b * a.C + (on ? unit_c : 0);
+    float in, out;
+    link<false, NW, CT>(ch, tot, n, at, on, w.blk, w.blocks, a.h0 && on ? a.h0[at] : 0.f, w.lane, in,
+                        out);
+    if (w.lane < CT) s_in[w.lane] = in;
+    if (on && a.kept) a.kept[(size_t)w.blk * n + at] = in;
+    if (on && w.blk == w.blocks - 1) a.h_final[at] = out;
+  }
+  lds_barrier();
+  float mine[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) mine[c] = s_in[w.ci + c];
+#pragma unroll
+  for (int k = 0; k < NW - 1; ++k)
+    if (k < w.wave) tot.template pass<V>(0, k, w.ci, mine);
+#pragma unroll
+  for (int c = 0; c < V; ++c) mine[c] = carry_through(L[c], mine[c], H[c]);
+  TX* out = (TX*)a.out + (long long)w.b * a.T * a.C + w.c;
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) mine[c] = token(f.a[i][c], mine[c], f.u[i][c]);
+    if (w.on && t + i < a.T) put<TX, V>(out + (long long)(t + i) * a.C, mine);
+  }
+}
+
+template <typename TX, typename TG, bool GATE, int V, int CT>
+__global__ void __launch_bounds__(512, 4) chain_bwd(ScanArgs a, Chain ch) {
+  using P = Place<V, CT, 512>;
+  constexpr int S = P::S, LPR = P::LPR, NW = P::NW;
+  __shared__ __attribute__((aligned(16))) Totals<NW, CT> fwd, rev;
+  __shared__ __attribute__((aligned(16))) float s_in[CT];
+  __shared__ int s_ticket;
+  const Step<V, CT> w(a, next_ticket(ch.ticket, &s_ticket), true);
+  const bool has_dout = a.dout.p != nullptr;
+  Run<TX, V, S> x, d;
+  Run<TG, V, S> g;
+  std::conditional_t<GATE, Run<TX, V, S>, None> b;
+  const int t = w.first(w.blk);
+  g.load(a.g, w.b, w.c, t, a.T);
+  if (has_dout) d.load(a.dout, w.b, w.c, t, a.T);
+  x.load(a.x, w.b, w.c, t, a.T);
+  if constexpr (GATE) b.load(a.b, w.b, w.c, t, a.T);
+  float hw[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) hw[c] = a.kept[(size_t)w.blk * a.B * a.C + w.bc(a) + c];
+  Factors<V, S> f;
+  factors<TX, TG, GATE, V, S>(f, x, g, b, t, a.T);
+  float dv[S][V];
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    if (has_dout) widen<TX, V>(d.r[i], dv[i]);
+#pragma unroll
+    for (int c = 0; c < V; ++c)
+      if (!has_dout || t + i >= a.T) dv[i][c] = 0.f;
+  }
+  float L[V], H[V], R[V], D[V], TL[V], TH[V], TD[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    D[c] = 0.f;
+#pragma unroll
+    for (int i = S - 1; i >= 0; --i)
+      D[c] = f.a[i][c] < 0.f ? 0.f : f.a[i][c] * (dv[i][c] + D[c]);
+    R[c] = L[c] = f.L[c];
+    H[c] = f.H[c];
+  }
+  wave_compose<V, LPR, true>(R, D, TL, TD, w.lane);
+  if (w.lane < LPR) rev.template put_<V>(0, w.wave, w.ci, TL, TD);
+  wave_compose<V, LPR, false>(L, H, TL, TH, w.lane);
+  if (w.lane >= 64 - LPR) fwd.template put_<V>(0, w.wave, w.ci, TL, TH);
+  lds_barrier();
+  if (w.wave == 0) {
+    const int unit_c = tile_channel<CT>(a, s_ticket, w.lane);
+    const bool on = unit_c < a.C;
+    const size_t n = (size_t)a.B * a.C, at = (size_t)w.b * a.C + (on ? unit_c : 0);
+    float in, out;
+    link<true, NW, CT>(ch, rev, n, at, on, w.blk, w.blocks, a.dh_final && on ? a.dh_final[at] : 0.f,
+                       w.lane, in, out);
+    if (w.lane < CT) s_in[w.lane] = in;
+    if (on && w.blk == 0 && a.dh0) a.dh0[at] = out;
+  }
+  // meanwhile the other waves form the states before their tokens
+  float before[S][V];
+#pragma unroll
+  for (int k = 0; k < NW - 1; ++k)
+    if (k < w.wave) fwd.template pass<V>(0, k, w.ci, hw);
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    float hc = carry_through(L[c], hw[c], H[c]);
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      before[i][c] = hc;
+      hc = token(f.a[i][c], hc, f.u[i][c]);
+    }
+  }
+  lds_barrier();
+  float mine[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) mine[c] = s_in[w.ci + c];
+#pragma unroll
+  for (int k = NW - 1; k > 0; --k)
+    if (k > w.wave) rev.template pass<V>(0, k, w.ci, mine);
+#pragma unroll
+  for (int c = 0; c < V; ++c) mine[c] = carry_through(R[c], mine[c], D[c]);
+  const long long o = (long long)w.b * a.T * a.C + w.c;
+#pragma unroll
+  for (int i = S - 1; i >= 0; --i) {
+    float dx[V], dg[V], db[V], xv[V], bv[V];
+    widen<TX, V>(x.r[i], xv);
+    if constexpr (GATE) widen<TX, V>(b.r[i], bv);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const float dh = dv[i][c] + mine[c], av = f.a[i][c];
+      mine[c] = av < 0.f ? 0.f : av * dh;
+      dg[c] = av < 0.f ? 0.f : mine[c] * before[i][c];
+      dx[c] = GATE ? bv[c] * dh : dh;
+      db[c] = xv[c] * dh;
+    }
+    if (w.on && t + i < a.T) {
+      const long long at = o + (long long)(t + i) * a.C;
+      put<TX, V>((TX*)a.dx + at, dx);
+      put<TG, V>((TG*)a.dg + at, dg);
+      if constexpr (GATE) put<TX, V>((TX*)a.db + at, db);
     }
   }
 }
@@ -483,18 +723,39 @@ __global__ void __launch_bounds__(kThreads) gscan_none(size_t n, const float* h_
 
 // ---------------------------------------------------------------- host side
 
-int blocks_of(int T) { return T / kBlock + (T % kBlock != 0); }
-
-// Segments of the axis: where the (batch, channel tile) units leave most of the GPU
-// idle, the axis is cut and a summary pass over the segments comes first.
-int segments(int B, int T, int C) {
-  const long long units = (long long)B * ((C + kTile - 1) / kTile);
-  const int n = blocks_of(T);
-  if (n < 8 || units >= 96) return 1;
-  long long want = (256 + units - 1) / units;
-  if (want > n / 4) want = n / 4;
-  const int per = (int)((n + want - 1) / want);
-  return (n + per - 1) / per;
+// How a call is spread over the GPU: a walk along the axis by workgroups of ct channels, or
+// (chain) all steps at once.
+struct Split {
+  bool chain;
+  int ct, nct;
+  int block, blocks;   // tokens of a step, steps
+  size_t ws;
+};
+Split split(int B, int T, int C, int in_dtype) {
+  Split s;
+  auto units = [&](int ct) { return (long long)B * ((C + ct - 1) / ct); };
+  auto cut = [&](bool chain, int ct) {
+    s.chain = chain;
+    s.ct = ct;
+    s.nct = (C + ct - 1) / ct;
+    s.block = chain ? 16 * 512 / ct : 128;
+    s.blocks = T / s.block + (T % s.block != 0);
+    s.ws = chain ? 256 + (size_t)s.blocks * B * C * 16 : 0;
+  };
+  // Short axes: one launch, no ticket.  16 x 512 x 1024 bfloat16 forward and backward 18 and 35
+  // us, in steps at once 27 and 38; 16 x 2048 x 4096 303 and 582, in steps at once 289 and 510.
+  if (T <= 512 || (T <= 1024 && units(64) >= 256)) {
+    cut(false, units(64) >= 192 ? 64 : 16);
+    return s;
+  }
+  // Rows of a tile fill a 128-byte line.  With few channels the time goes by the hand-over from
+  // step to step (1.1 us for every four) and narrower tiles have longer steps: bfloat16 forward
+  // 1 x 65536 x 768 in tiles of 64, 32, 16 channels 152, 129, 165 us, 1 x 16384 x 128 35, 23,
+  // 18; float32 1 x 32768 x 256 forward and backward 158, 107, 112.
+  const long long bc = (long long)B * C;
+  cut(true, bc >= 1024 ? (in_dtype == GDN2_F32 ? 32 : 64) : bc >= 192 ? 32 : 16);
+  if (s.blocks * units(s.ct) >= (1ll << 30)) cut(false, 64);   // tickets past 31 bits
+  return s;
 }
 
 int validate(int B, int T, int C, int in_dtype, int g_dtype) {
@@ -502,9 +763,9 @@ int validate(int B, int T, int C, int in_dtype, int g_dtype) {
   if (in_dtype != GDN2_F32 && in_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
   if (g_dtype != GDN2_F32 && !(g_dtype == GDN2_BF16 && in_dtype == GDN2_BF16))
     return GDN2_ERR_DTYPE;
-  if (T > INT_MAX - kBlock || C > INT_MAX - kTile) return GDN2_ERR_SHAPE;
+  if (T > INT_MAX - 512 || C > INT_MAX - 64) return GDN2_ERR_SHAPE;
   // the launch's workgroups, and bytes of a tensor, within 31 and 62 bits
-  if ((double)B * ((C + kTile - 1) / kTile) > 8.0e6) return GDN2_ERR_SHAPE;
+  if ((double)B * ((C + kMinTile - 1) / kMinTile) > 8.0e6) return GDN2_ERR_SHAPE;
   if ((double)B * T * C > 1e18) return GDN2_ERR_SHAPE;
   return GDN2_OK;
 }
@@ -524,35 +785,61 @@ int check_f32(const void* p, bool optional, bool* vec) {
   return GDN2_OK;
 }
 
+template <typename TX, typename TG, bool GATE, int V, int CT>
+void launch_tile(hipStream_t st, const ScanArgs& a, bool bwd) {
+  const dim3 grid(8u * (unsigned)a.chunk), block(8 * CT);
+  if (bwd)
+    hipLaunchKernelGGL((gscan_bwd<TX, TG, GATE, V, CT>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((gscan_fwd<TX, TG, GATE, V, CT>), grid, block, 0, st, a);
+}
+template <typename TX, typename TG, bool GATE, int V, int CT>
+void launch_chain(hipStream_t st, const ScanArgs& a, bool bwd, int n) {
+  const size_t values = (size_t)n * a.B * a.C;
+  Chain ch;
+  ch.ticket = (unsigned*)a.ws;
+  ch.comp = (unsigned long long*)((char*)a.ws + 256);
+  ch.state = ch.comp + values;
+  hipLaunchKernelGGL(chain_clear, dim3((unsigned)((2 * values + kThreads - 1) / kThreads)),
+                     dim3(kThreads), 0, st, ch.comp, 2 * values, ch.ticket);
+  const dim3 grid((unsigned)(n * a.B * a.nct)), block(512);
+  if (bwd)
+    hipLaunchKernelGGL((chain_bwd<TX, TG, GATE, V, CT>), grid, block, 0, st, a, ch);
+  else
+    hipLaunchKernelGGL((chain_fwd<TX, TG, GATE, V, CT>), grid, block, 0, st, a, ch);
+}
 template <typename TX, typename TG, bool GATE, int V>
-hipError_t launch_scan(hipStream_t st, const ScanArgs& a, bool bwd) {
-  const dim3 grid(8u * (unsigned)a.chunk), block(kThreads);
-  if (bwd) {
-    if (a.nseg > 1)
-      hipLaunchKernelGGL((gscan_bwd<TX, TG, false, V, true>), grid, block, 0, st, a);
-    hipLaunchKernelGGL((gscan_bwd<TX, TG, GATE, V, false>), grid, block, 0, st, a);
+void launch_width(hipStream_t st, const ScanArgs& a, bool bwd, const Split& s) {
+  if (s.chain) {
+    if (s.ct == 64)
+      launch_chain<TX, TG, GATE, V, 64>(st, a, bwd, s.blocks);
+    else if (s.ct == 32)
+      launch_chain<TX, TG, GATE, V, 32>(st, a, bwd, s.blocks);
+    else
+      launch_chain<TX, TG, GATE, V, 16>(st, a, bwd, s.blocks);
+  } else if (s.ct == 64) {
+    launch_tile<TX, TG, GATE, V, 64>(st, a, bwd);
   } else {
-    if (a.nseg > 1)
-      hipLaunchKernelGGL((gscan_fwd<TX, TG, GATE, V, true>), grid, block, 0, st, a);
-    hipLaunchKernelGGL((gscan_fwd<TX, TG, GATE, V, false>), grid, block, 0, st, a);
+    launch_tile<TX, TG, GATE, V, 16>(st, a, bwd);
   }
-  return hipGetLastError();
 }
 template <typename TX, typename TG>
-hipError_t launch_scan(hipStream_t st, const ScanArgs& a, bool bwd, bool vec) {
+hipError_t launch_types(hipStream_t st, const ScanArgs& a, bool bwd, bool vec,
+                        const Split& s) {
   if (a.b.p)
-    return vec ? launch_scan<TX, TG, true, 4>(st, a, bwd) : launch_scan<TX, TG, true, 1>(st, a, bwd);
-  return vec ? launch_scan<TX, TG, false, 4>(st, a, bwd) : launch_scan<TX, TG, false, 1>(st, a, bwd);
+    vec ? launch_width<TX, TG, true, 4>(st, a, bwd, s) : launch_width<TX, TG, true, 1>(st, a, bwd, s);
+  else
+    vec ? launch_width<TX, TG, false, 4>(st, a, bwd, s)
+        : launch_width<TX, TG, false, 1>(st, a, bwd, s);
+  return hipGetLastError();
 }
 int launch_scan(hipStream_t st, ScanArgs& a, int in_dtype, int g_dtype, bool bwd, bool vec) {
-  a.nct = (a.C + kTile - 1) / kTile;
-  a.nseg = segments(a.B, a.T, a.C);
-  const int n = blocks_of(a.T);
-  a.seg_blocks = (n + a.nseg - 1) / a.nseg;
-  a.chunk = (a.B * a.nct * a.nseg + 7) / 8;
-  const hipError_t e = in_dtype == GDN2_F32 ? launch_scan<float, float>(st, a, bwd, vec)
-                       : g_dtype == GDN2_F32 ? launch_scan<bf16_t, float>(st, a, bwd, vec)
-                                             : launch_scan<bf16_t, bf16_t>(st, a, bwd, vec);
+  const Split s = split(a.B, a.T, a.C, in_dtype);
+  a.nct = s.nct;
+  a.chunk = (int)(((long long)a.B * a.nct + 7) / 8);
+  const hipError_t e = in_dtype == GDN2_F32 ? launch_types<float, float>(st, a, bwd, vec, s)
+                       : g_dtype == GDN2_F32 ? launch_types<bf16_t, float>(st, a, bwd, vec, s)
+                                             : launch_types<bf16_t, bf16_t>(st, a, bwd, vec, s);
   return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
@@ -580,15 +867,14 @@ using namespace gdn2;
 
 extern "C" {
 
-size_t gdn2_gated_scan_kept_bytes(int B, int T, int C) {
-  if (validate(B, T, C, GDN2_F32, GDN2_F32) != GDN2_OK) return 0;
-  return (size_t)blocks_of(T) * B * C * sizeof(float);
+size_t gdn2_gated_scan_kept_bytes(int B, int T, int C, int in_dtype) {
+  if (validate(B, T, C, in_dtype, GDN2_F32) != GDN2_OK) return 0;
+  return (size_t)split(B, T, C, in_dtype).blocks * B * C * sizeof(float);
 }
 
-size_t gdn2_gated_scan_workspace_bytes(int B, int T, int C) {
-  if (validate(B, T, C, GDN2_F32, GDN2_F32) != GDN2_OK) return 0;
-  const int nseg = segments(B, T, C);
-  return nseg > 1 ? (size_t)nseg * 2 * B * C * sizeof(float) : 0;
+size_t gdn2_gated_scan_workspace_bytes(int B, int T, int C, int in_dtype) {
+  if (validate(B, T, C, in_dtype, GDN2_F32) != GDN2_OK) return 0;
+  return split(B, T, C, in_dtype).ws;
 }
 
 int gdn2_gated_scan_fwd(void* stream, int B, int T, int C, int in_dtype, int g_dtype,
@@ -610,7 +896,7 @@ int gdn2_gated_scan_fwd(void* stream, int B, int T, int C, int in_dtype, int g_d
   a.out = out;
   a.h_final = h_final;
   a.kept = kept;
-  a.seg = (float*)ws;
+  a.ws = ws;
   a.B = B;
   a.T = T;
   a.C = C;
@@ -620,7 +906,7 @@ int gdn2_gated_scan_fwd(void* stream, int B, int T, int C, int in_dtype, int g_d
         (rc = check_rows({out, 0, 0}, in_dtype, &vec)))
       return rc;
     if (b && (rc = check_rows(a.b, in_dtype, &vec))) return rc;
-    const size_t need = gdn2_gated_scan_workspace_bytes(B, T, C);
+    const size_t need = gdn2_gated_scan_workspace_bytes(B, T, C, in_dtype);
     if ((rc = check_f32(need ? ws : nullptr, need == 0, &vec))) return rc;
     if (ws_bytes < need) return GDN2_ERR_WORKSPACE;
   }
@@ -659,7 +945,7 @@ int gdn2_gated_scan_bwd(void* stream, int B, int T, int C, int in_dtype, int g_d
   a.dg = dg;
   a.db = db;
   a.dh0 = dh0;
-  a.seg = (float*)ws;
+  a.ws = ws;
   a.B = B;
   a.T = T;
   a.C = C;
@@ -676,7 +962,7 @@ int gdn2_gated_scan_bwd(void* stream, int B, int T, int C, int in_dtype, int g_d
   if ((rc = check_f32(kept, false, &vec)) || (rc = check_f32(dh_final, true, &vec)) ||
       (rc = check_f32(dh0, true, &vec)))
     return rc;
-  const size_t need = gdn2_gated_scan_workspace_bytes(B, T, C);
+  const size_t need = gdn2_gated_scan_workspace_bytes(B, T, C, in_dtype);
   if ((rc = check_f32(need ? ws : nullptr, need == 0, &vec))) return rc;
   if (ws_bytes < need) return GDN2_ERR_WORKSPACE;
   return launch_scan((hipStream_t)stream, a, in_dtype, g_dtype, true, vec);

@@ -90,8 +90,8 @@ SIGNATURES = {
     "gdn2_bwd_intra": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 6 + [_c_float]
                        + [_vp] * 5 + [_c_size]),
     "gdn2_bwd_reverse_cumsum": (_c_int, [_vp, ctypes.c_longlong, _c_int, _c_int, _vp, _vp]),
-    "gdn2_gated_scan_kept_bytes": (_c_size, [_c_int] * 3),
-    "gdn2_gated_scan_workspace_bytes": (_c_size, [_c_int] * 3),
+    "gdn2_gated_scan_kept_bytes": (_c_size, [_c_int] * 4),
+    "gdn2_gated_scan_workspace_bytes": (_c_size, [_c_int] * 4),
     "gdn2_gated_scan_fwd": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 11 + [_c_size]),
     "gdn2_gated_scan_bwd": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 15 + [_c_size]),
     "gdn2_gated_scan_step": (_c_int, [_vp, ctypes.c_longlong, _c_int, _c_int] + [_vp] * 6),

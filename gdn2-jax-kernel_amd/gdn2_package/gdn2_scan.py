@@ -72,7 +72,7 @@ def _rows(x):
 
 def _launch_fwd(x, g, b, h0, keep):
     B, T, C = x.shape
-    dev, L = x.device, _lib.lib()
+    dev, L, code = x.device, _lib.lib(), _dtype_code(x.dtype)
     x, px, sx = _rows(x)
     g, pg, sg = _rows(g)
     pb = sb = None
@@ -82,14 +82,14 @@ def _launch_fwd(x, g, b, h0, keep):
     h_final = torch.empty((B, C), dtype=torch.float32, device=dev)
     kept = ws = None
     if keep:
-        kept = torch.empty(L.gdn2_gated_scan_kept_bytes(B, T, C) // 4, dtype=torch.float32,
+        kept = torch.empty(L.gdn2_gated_scan_kept_bytes(B, T, C, code) // 4, dtype=torch.float32,
                            device=dev)
-    nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C)
+    nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C, code)
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     with torch.cuda.device(dev):
         rc = L.gdn2_gated_scan_fwd(
-            torch.cuda.current_stream(dev).cuda_stream, B, T, C, _dtype_code(x.dtype),
+            torch.cuda.current_stream(dev).cuda_stream, B, T, C, code,
             _dtype_code(g.dtype), px, sx, pg, sg, pb, sb,
             None if h0 is None else h0.data_ptr(), out.data_ptr(), h_final.data_ptr(),
             kept.data_ptr() if keep and T else None, None if ws is None else ws.data_ptr(), nbytes)
@@ -112,7 +112,7 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dout, dh_final):
         x, g, b, kept = ctx.saved_tensors
         B, T, C = x.shape
-        dev, L = x.device, _lib.lib()
+        dev, L, code = x.device, _lib.lib(), _dtype_code(x.dtype)
         if T == 0:
             zero = [None if t is None else torch.zeros_like(t) for t in (x, g, b)]
             dh0 = None if not ctx.has_h0 or dh_final is None else dh_final.clone()
@@ -131,13 +131,13 @@ class _GatedScan(torch.autograd.Function):
         dg = torch.empty((B, T, C), dtype=g.dtype, device=dev)
         if ctx.has_h0:
             dh0 = torch.empty((B, C), dtype=torch.float32, device=dev)
-        nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C)
+        nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C, code)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
         with torch.cuda.device(dev):
             rc = L.gdn2_gated_scan_bwd(
-                torch.cuda.current_stream(dev).cuda_stream, B, T, C, _dtype_code(x.dtype),
+                torch.cuda.current_stream(dev).cuda_stream, B, T, C, code,
                 _dtype_code(g.dtype), px, sx, pg, sg, pb, sb, pd, sd, ptr(dh_final),
                 kept.data_ptr(), dx.data_ptr(), dg.data_ptr(), ptr(db), ptr(dh0), ptr(ws), nbytes)
         if rc:

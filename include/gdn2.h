@@ -354,11 +354,11 @@ int gdn2_bwd_reverse_cumsum(void* stream, long long tiles, int BT, int D, const 
  * their elements; 4-element alignment of pointers, strides and C is faster.
  * gdn2_set_launch_events does not reach the entry points from here on. */
 
-/* Bytes of the states kept for the backward: (ceil(T/256), B, C) float32. */
-size_t gdn2_gated_scan_kept_bytes(int B, int T, int C);
-/* Workspace of the forward and of the backward (0 for most sizes: only where the
- * axis is split because there are few channels). */
-size_t gdn2_gated_scan_workspace_bytes(int B, int T, int C);
+/* Bytes of the states kept for the backward (float32, one for every 128 to 512
+ * tokens) and of the workspace of the forward and of the backward (0 for short
+ * axes, where a workgroup walks along the whole axis). */
+size_t gdn2_gated_scan_kept_bytes(int B, int T, int C, int in_dtype);
+size_t gdn2_gated_scan_workspace_bytes(int B, int T, int C, int in_dtype);
 
 /* h0 may be NULL (zero) and equal to h_final; kept may be NULL (inference). */
 int gdn2_gated_scan_fwd(void* stream, int B, int T, int C, int in_dtype, int g_dtype,

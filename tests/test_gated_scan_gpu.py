@@ -3,9 +3,9 @@ the recurrence in float64.
 
 Tolerances.  Every value is a sum of terms, each multiplied on its way by decays
 in (0, 1]; m is the same sum with the terms' magnitudes.  A term passes at most 16 tokens
-of a run (two roundings each, and the two of e^g), six compositions and four waves (three
-roundings each) and, more weakly the farther it comes, the steps of 256 tokens: fewer than
-128 roundings of 2^-24 where a step's decay is e^-2 or less, as all the inputs here
+of a run (two roundings each, and the two of e^g), six compositions and eight waves (three
+roundings each) and, more weakly the farther it comes, the steps of 128 tokens or more: fewer
+than 128 roundings of 2^-24 where a step's decay is e^-1 or less, as all the inputs here
 have.  So 128 * 2^-24 * m; results in bfloat16 are rounded once more, 2^-8 of their value."""
 import numpy as np
 import pytest
@@ -116,12 +116,15 @@ def test_backward(dev, B, T, C, dtype, gdtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("B,T,C", [(1, 2048, 16), (1, 5000, 20), (1, 4097, 7), (2, 9001, 40)])
-def test_split_axis(dev, B, T, C, dtype):
-    """Few channels and a long axis: segments with a summary pass before the walk."""
+@pytest.mark.parametrize("B,T,C", [(1, 2048, 16), (1, 5000, 20), (1, 4097, 7), (2, 9001, 40),
+                                   (1, 513, 64), (3, 1025, 200), (2, 1537, 192), (1, 1500, 999),
+                                   (2, 700, 1000), (17, 640, 100), (1, 2049, 1024)])
+def test_steps_at_once(dev, B, T, C, dtype):
+    """Long axes: every step has its workgroup, tiles of 16, 32 and 64 channels."""
     import gdn2_package as gp
     from gdn2_package import _lib
-    assert _lib.lib().gdn2_gated_scan_workspace_bytes(B, T, C) > 0
+    code = _lib.GDN2_F32 if dtype == torch.float32 else _lib.GDN2_BF16
+    assert _lib.lib().gdn2_gated_scan_workspace_bytes(B, T, C, code) > 0
     ts, (xn, gn, bn, hn) = inputs(B, T, C, dtype, torch.float32, dev, T)
     leaf = [t.clone().requires_grad_() for t in ts]
     out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
@@ -133,6 +136,35 @@ def test_split_axis(dev, B, T, C, dtype):
     check(hf, ref[:, -1], mag[:, -1])
     for n, t in zip(("x", "g", "b", "h0"), got):
         check(t, *grads[n], n=2)
+
+
+@pytest.mark.parametrize("B,T,C", [(1, 20000, 128), (2, 6000, 300), (4, 2000, 1024)])
+def test_same_results_every_time(dev, B, T, C):
+    """The hand-over from step to step leaves no trace of who was first."""
+    import gdn2_package as gp
+    ts, _ = inputs(B, T, C, torch.float32, torch.float32, dev, 1)
+    leaf = [t.requires_grad_() for t in ts]
+    dout = torch.randn((B, T, C), device=dev)
+    first = None
+    for _ in range(4):
+        out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+        res = (out, hf, *torch.autograd.grad((out, hf), leaf, (dout, torch.ones_like(hf))))
+        first = first or res
+        assert all(torch.equal(a, e) for a, e in zip(res, first))
+
+
+def test_nan_of_any_payload_does_not_stop_the_hand_over(dev):
+    """NaN whose bits are all ones (memory filled with 0xFF) in every input."""
+    import gdn2_package as gp
+    B, T, C = 1, 1200, 96
+    x = torch.full((B, T, C), -1, dtype=torch.int32, device=dev).view(torch.float32)
+    fine = torch.rand((B, T, C), device=dev)
+    for args in ((x, -fine), (fine, x), (fine, -fine, x), (x, x, x)):
+        leaf = [t.clone().requires_grad_() for t in args]
+        out, hf = gp.gdn2_gated_scan(*leaf)
+        grads = torch.autograd.grad((out, hf), leaf, (x, x[:, 0]))
+        assert torch.isnan(out).all() and torch.isnan(hf).all()
+        assert all(torch.isnan(t).all() for t in grads)
 
 
 def test_gradient_against_differences(dev):
@@ -164,7 +196,7 @@ def test_gradient_against_differences(dev):
         assert abs(mine - diff) <= tol, (n, mine, diff, tol)
 
 
-@pytest.mark.parametrize("T,C", [(600, 24), (2500, 5)])
+@pytest.mark.parametrize("T,C", [(500, 24), (2500, 5), (1300, 1100)])
 def test_fresh_starts(dev, T, C):
     """g = -inf starts a sequence: equal to separate calls, NaN and infinities before
     it stay there, and no gradient crosses it."""
