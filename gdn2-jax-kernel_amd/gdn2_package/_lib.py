@@ -137,5 +137,21 @@ def lib():
     return _LIB
 
 
+# The current stream's handle: torch's own short form where it has one.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(name: str, device, *args) -> int:
+    """Call entry point ``name`` on the current stream of ``device`` (which is made
+    the current device for the call where it is not) and return its code."""
+    fn = getattr(_LIB or lib(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        return fn(_raw_stream(index), *args)
+    with torch.cuda.device(index):
+        return fn(_raw_stream(index), *args)
+
+
 def strerror(code: int) -> str:
     return lib().gdn2_strerror(code).decode()

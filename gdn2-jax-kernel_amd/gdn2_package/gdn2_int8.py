@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
-from .gdn2_norm import _as_rows, _prepare, _row_stride, _tensor
+from .gdn2_norm import _as, _as_rows, _prepare, _row_stride, _tensor
 
 
 def _empty_q(shape, dev):
@@ -38,21 +38,20 @@ def gdn2_rms_norm_int8(x, weight, residual=None, eps=1e-6):
     what = "gdn2_rms_norm_int8"
     xs, ws, rs = _prepare(x, weight, residual, eps, what)
     shape, dev = xs.shape, xs.device
-    rows = _as_rows(xs.detach())
+    rows = _as_rows(xs)
     M, C = rows.shape
     q, ld = _empty_q(shape, dev)
     scale = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
     h = r_rows = None
     if rs is not None:
-        r_rows = _as_rows(rs.detach())
+        r_rows = _as_rows(rs)
         h = torch.empty(shape, dtype=rs.dtype, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().gdn2_rms_norm_int8(
-            torch.cuda.current_stream(dev).cuda_stream, M, C, _dtype_code(rows.dtype),
-            _dtype_code(rows.dtype if h is None else h.dtype), _dtype_code(ws.dtype),
-            rows.data_ptr(), _row_stride(rows), None if h is None else r_rows.data_ptr(),
-            0 if h is None else _row_stride(r_rows), ws.data_ptr(), float(eps), q.data_ptr(), ld,
-            scale.data_ptr(), None if h is None else h.data_ptr())
+    rc = _lib.launch(
+        "gdn2_rms_norm_int8", dev, M, C, _dtype_code(rows.dtype),
+        _dtype_code(rows.dtype if h is None else h.dtype), _dtype_code(ws.dtype),
+        rows.data_ptr(), _row_stride(rows), None if h is None else r_rows.data_ptr(),
+        0 if h is None else _row_stride(r_rows), ws.data_ptr(), float(eps), q.data_ptr(), ld,
+        scale.data_ptr(), None if h is None else h.data_ptr())
     if rc:
         _raise(rc, f"{what} (M,C)=({M},{C})")
     if h is None:
@@ -69,17 +68,15 @@ def gdn2_quantize_int8(x):
         raise GDN2ShapeError(f"{what}: expected rows, got a scalar")
     if not x.is_floating_point():
         raise GDN2Error(f"{what}: x must be floating point; got {x.dtype}")
-    x = x.detach()
     if x.dtype not in _SUPPORTED_IN:
         x = x.float()
     rows = _as_rows(x)
     M, C = rows.shape
     q, ld = _empty_q(x.shape, x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = _lib.lib().gdn2_quantize_int8(
-            torch.cuda.current_stream(x.device).cuda_stream, M, C, _dtype_code(rows.dtype),
-            rows.data_ptr(), _row_stride(rows), q.data_ptr(), ld, scale.data_ptr())
+    rc = _lib.launch(
+        "gdn2_quantize_int8", x.device, M, C, _dtype_code(rows.dtype),
+        rows.data_ptr(), _row_stride(rows), q.data_ptr(), ld, scale.data_ptr())
     if rc:
         _raise(rc, f"{what} (M,C)=({M},{C})")
     return q, scale
@@ -108,10 +105,9 @@ def gdn2_dequantize_int8(q, scale, dtype=torch.bfloat16):
     rows, s = _int8_rows(q, scale, ("q", "scale"), what, getattr(q, "device", None))
     M, C = rows.shape
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    with torch.cuda.device(q.device):
-        rc = _lib.lib().gdn2_dequantize_int8(
-            torch.cuda.current_stream(q.device).cuda_stream, M, C, _dtype_code(dtype),
-            rows.data_ptr(), _row_stride(rows), s.data_ptr(), out.data_ptr())
+    rc = _lib.launch(
+        "gdn2_dequantize_int8", q.device, M, C, _dtype_code(dtype),
+        rows.data_ptr(), _row_stride(rows), s.data_ptr(), out.data_ptr())
     if rc:
         _raise(rc, f"{what} (M,C)=({M},{C})")
     return out
@@ -154,15 +150,14 @@ def gdn2_int8_matmul(q, scale, weight, weight_scale, bias=None, out_dtype=torch.
             raise GDN2ShapeError(f"{what}: bias must be ({N},); got {tuple(bias.shape)}")
         if bias.device != dev or not bias.is_floating_point():
             raise GDN2Error(f"{what}: bias must be floating point, on {dev}")
-        bias = bias.detach().to(torch.float32).contiguous()
+        bias = _as(bias, torch.float32).contiguous()
     x, ldx = _wide_rows(x)
     w, ldw = _wide_rows(w)
     out = torch.empty((*q.shape[:-1], N), dtype=out_dtype, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().gdn2_int8_matmul(
-            torch.cuda.current_stream(dev).cuda_stream, M, N, K, _dtype_code(out_dtype),
-            x.data_ptr(), ldx, sx.data_ptr(), w.data_ptr(), ldw, sw.data_ptr(),
-            None if bias is None else bias.data_ptr(), out.data_ptr())
+    rc = _lib.launch(
+        "gdn2_int8_matmul", dev, M, N, K, _dtype_code(out_dtype),
+        x.data_ptr(), ldx, sx.data_ptr(), w.data_ptr(), ldw, sw.data_ptr(),
+        None if bias is None else bias.data_ptr(), out.data_ptr())
     if rc:
         _raise(rc, f"{what} (M,N,K)=({M},{N},{K})")
     return out

@@ -24,8 +24,12 @@ from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _ra
 def _tensor(t, name, what):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a torch tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise GDN2Error(f"{what}: {name} must live on the ROCm device; no CPU path")
+
+
+def _as(t, dt):
+    return t if t.dtype == dt else t.to(dt)
 
 
 def _as_rows(x):
@@ -44,7 +48,7 @@ def _prepare(x, weight, residual, eps, what):
     """(x, residual, weight) of supported types, checked; rows are not formed yet."""
     _tensor(x, "x", what)
     _tensor(weight, "weight", what)
-    if x.dim() < 1 or tuple(weight.shape) != tuple(x.shape[-1:]):
+    if x.dim() < 1 or weight.shape != x.shape[-1:]:
         raise GDN2ShapeError(f"{what}: weight must have the shape of x's last axis; got "
                              f"{tuple(weight.shape)} for x {tuple(x.shape)}")
     if not x.is_floating_point() or not weight.is_floating_point():
@@ -78,13 +82,11 @@ class _RmsNorm(torch.autograd.Function):
         h = None if residual is None else torch.empty((M, C), dtype=residual.dtype, device=dev)
         rstd = torch.empty(M, dtype=torch.float32, device=dev) if keep else None
         ptr = lambda t: None if t is None else t.data_ptr()
-        with torch.cuda.device(dev):
-            rc = _lib.lib().gdn2_rms_norm(
-                torch.cuda.current_stream(dev).cuda_stream, M, C, _dtype_code(x.dtype),
-                _dtype_code(x.dtype if h is None else h.dtype), _dtype_code(weight.dtype),
-                x.data_ptr(), _row_stride(x), ptr(residual),
-                0 if h is None else _row_stride(residual), weight.data_ptr(), eps, y.data_ptr(),
-                ptr(h), ptr(rstd))
+        rc = _lib.launch(
+            "gdn2_rms_norm", dev, M, C, _dtype_code(x.dtype),
+            _dtype_code(x.dtype if h is None else h.dtype), _dtype_code(weight.dtype),
+            x.data_ptr(), _row_stride(x), ptr(residual), 0 if h is None else _row_stride(residual),
+            weight.data_ptr(), eps, y.data_ptr(), ptr(h), ptr(rstd))
         if rc:
             _raise(rc, f"gdn2_rms_norm (M,C)=({M},{C})")
         if keep:
@@ -100,8 +102,8 @@ class _RmsNorm(torch.autograd.Function):
         M, C = h.shape
         dev, L = h.device, _lib.lib()
         h = h.contiguous()
-        dy = None if dy is None else dy.to(ctx.x_dtype).contiguous()
-        dh = None if dh is None else dh.to(h.dtype).contiguous()
+        dy = None if dy is None else _as(dy, ctx.x_dtype).contiguous()
+        dh = None if dh is None else _as(dh, h.dtype).contiguous()
         dx = torch.empty((M, C), dtype=ctx.x_dtype, device=dev)
         dr = torch.empty((M, C), dtype=h.dtype, device=dev) \
             if ctx.has_residual and h.dtype != ctx.x_dtype else None
@@ -109,12 +111,10 @@ class _RmsNorm(torch.autograd.Function):
         nbytes = L.gdn2_rms_norm_bwd_workspace_bytes(M, C)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
-        with torch.cuda.device(dev):
-            rc = L.gdn2_rms_norm_bwd(
-                torch.cuda.current_stream(dev).cuda_stream, M, C, _dtype_code(ctx.x_dtype),
-                _dtype_code(h.dtype), _dtype_code(weight.dtype), h.data_ptr(), weight.data_ptr(),
-                rstd.data_ptr(), ptr(dy), ptr(dh), dx.data_ptr(), ptr(dr), dw.data_ptr(),
-                ws.data_ptr(), nbytes)
+        rc = _lib.launch(
+            "gdn2_rms_norm_bwd", dev, M, C, _dtype_code(ctx.x_dtype), _dtype_code(h.dtype),
+            _dtype_code(weight.dtype), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), ptr(dy),
+            ptr(dh), dx.data_ptr(), ptr(dr), dw.data_ptr(), ws.data_ptr(), nbytes)
         if rc:
             _raise(rc, f"gdn2_rms_norm_bwd (M,C)=({M},{C})")
         return dx, dw, (dx if dr is None else dr) if ctx.has_residual else None, None, None

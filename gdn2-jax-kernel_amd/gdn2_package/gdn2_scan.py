@@ -34,11 +34,11 @@ def _types(x, g, b, what):
     for t in (x, g) if b is None else (x, g, b):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: x, g, b must be torch tensors")
+        if not t.is_cuda or t.device != x.device:
+            raise GDN2Error(f"{what}: inputs must live on one ROCm device; no CPU path")
         if t.shape != x.shape:
             raise GDN2ShapeError(f"{what}: g and b must have x's shape {tuple(x.shape)}; got "
                                  f"{tuple(t.shape)}")
-        if t.device != x.device or t.device.type != "cuda":
-            raise GDN2Error(f"{what}: inputs must live on one ROCm device; no CPU path")
         if not t.is_floating_point():
             raise GDN2Error(f"{what}: inputs must be floating point; got {t.dtype}")
     dt = x.dtype
@@ -48,15 +48,19 @@ def _types(x, g, b, what):
     return dt, torch.bfloat16 if bf16 else torch.float32
 
 
+def _as(t, dt):
+    return t if t is None or t.dtype == dt else t.to(dt)
+
+
 def _state_in(h, shape, device, what, name):
     if not isinstance(h, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a torch tensor")
-    if tuple(h.shape) != tuple(shape):
+    if h.shape != shape:
         raise GDN2ShapeError(f"{what}: {name} must have shape {tuple(shape)}; got "
                              f"{tuple(h.shape)}")
     if h.device != device:
         raise GDN2Error(f"{what}: {name} must live on {device}")
-    return h.to(torch.float32).contiguous()
+    return _as(h, torch.float32).contiguous()
 
 
 def _rows(x):
@@ -87,12 +91,10 @@ def _launch_fwd(x, g, b, h0, keep):
     nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C, code)
     if nbytes:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = L.gdn2_gated_scan_fwd(
-            torch.cuda.current_stream(dev).cuda_stream, B, T, C, code,
-            _dtype_code(g.dtype), px, sx, pg, sg, pb, sb,
-            None if h0 is None else h0.data_ptr(), out.data_ptr(), h_final.data_ptr(),
-            kept.data_ptr() if keep and T else None, None if ws is None else ws.data_ptr(), nbytes)
+    rc = _lib.launch(
+        "gdn2_gated_scan_fwd", dev, B, T, C, code, _dtype_code(g.dtype), px, sx, pg, sg, pb, sb,
+        None if h0 is None else h0.data_ptr(), out.data_ptr(), h_final.data_ptr(),
+        kept.data_ptr() if keep and T else None, None if ws is None else ws.data_ptr(), nbytes)
     if rc:
         _raise(rc, f"gdn2_gated_scan_fwd (B,T,C)=({B},{T},{C})")
     return out, h_final, kept
@@ -124,9 +126,9 @@ class _GatedScan(torch.autograd.Function):
             b, pb, sb = _rows(b)
             db = torch.empty((B, T, C), dtype=b.dtype, device=dev)
         if dout is not None:
-            dout, pd, sd = _rows(dout.to(x.dtype))
+            dout, pd, sd = _rows(_as(dout, x.dtype))
         if dh_final is not None:
-            dh_final = dh_final.to(torch.float32).contiguous()
+            dh_final = _as(dh_final, torch.float32).contiguous()
         dx = torch.empty((B, T, C), dtype=x.dtype, device=dev)
         dg = torch.empty((B, T, C), dtype=g.dtype, device=dev)
         if ctx.has_h0:
@@ -135,11 +137,10 @@ class _GatedScan(torch.autograd.Function):
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
-        with torch.cuda.device(dev):
-            rc = L.gdn2_gated_scan_bwd(
-                torch.cuda.current_stream(dev).cuda_stream, B, T, C, code,
-                _dtype_code(g.dtype), px, sx, pg, sg, pb, sb, pd, sd, ptr(dh_final),
-                kept.data_ptr(), dx.data_ptr(), dg.data_ptr(), ptr(db), ptr(dh0), ptr(ws), nbytes)
+        rc = _lib.launch(
+            "gdn2_gated_scan_bwd", dev, B, T, C, code, _dtype_code(g.dtype), px, sx, pg, sg, pb,
+            sb, pd, sd, ptr(dh_final), kept.data_ptr(), dx.data_ptr(), dg.data_ptr(), ptr(db),
+            ptr(dh0), ptr(ws), nbytes)
         if rc:
             _raise(rc, f"gdn2_gated_scan_bwd (B,T,C)=({B},{T},{C})")
         return dx, dg, db, dh0
@@ -158,18 +159,19 @@ def gdn2_gated_scan(x, g, b=None, h0=None):
     shape = x.shape
     if len(shape) not in (3, 4):
         raise GDN2ShapeError(f"{what}: expected (B,T,C) or (B,T,H,D) inputs, got {tuple(shape)}")
-    state = (shape[0], *shape[2:])
+    state = torch.Size((shape[0], *shape[2:]))
     if h0 is not None:
         h0 = _state_in(h0, state, x.device, what, "h0")
     out_dt = x.dtype
-    x, g = x.to(dt), g.to(gdt)
-    b = None if b is None else b.to(dt)
+    x, g, b = _as(x, dt), _as(g, gdt), _as(b, dt)
     if len(shape) == 4:
         flat = (*shape[:2], shape[2] * shape[3])
         x, g = x.reshape(flat), g.reshape(flat)
         b = None if b is None else b.reshape(flat)
         h0 = None if h0 is None else h0.reshape(flat[0], flat[2])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, g, b, h0)):
+    if torch.is_grad_enabled() and (
+            x.requires_grad or g.requires_grad or (b is not None and b.requires_grad) or
+            (h0 is not None and h0.requires_grad)):
         out, h_final = _GatedScan.apply(x, g, b, h0)
     else:
         out, h_final, _ = _launch_fwd(x, g, b, h0, False)
@@ -194,17 +196,16 @@ def gdn2_gated_scan_step(x, g, b=None, state=None, inplace=False):
         if not isinstance(state, torch.Tensor) or state.dtype != torch.float32 or \
                 not state.is_contiguous():
             raise GDN2Error(f"{what}: inplace needs a contiguous float32 state")
-    h_in = None if state is None else _state_in(state, shape, dev, what, "state").detach()
+    h_in = None if state is None else _state_in(state, shape, dev, what, "state")
     out_dt = x.dtype
-    x, g = x.detach().to(dt).contiguous(), g.detach().to(gdt).contiguous()
-    b = None if b is None else b.detach().to(dt).contiguous()
+    x, g = _as(x, dt).contiguous(), _as(g, gdt).contiguous()
+    b = None if b is None else _as(b, dt).contiguous()
     h_out = state if inplace else torch.empty(shape, dtype=torch.float32, device=dev)
     out = torch.empty(shape, dtype=dt, device=dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().gdn2_gated_scan_step(
-            torch.cuda.current_stream(dev).cuda_stream, x.numel(), _dtype_code(dt),
-            _dtype_code(gdt), x.data_ptr(), g.data_ptr(), None if b is None else b.data_ptr(),
-            None if h_in is None else h_in.data_ptr(), h_out.data_ptr(), out.data_ptr())
+    rc = _lib.launch(
+        "gdn2_gated_scan_step", dev, x.numel(), _dtype_code(dt), _dtype_code(gdt), x.data_ptr(),
+        g.data_ptr(), None if b is None else b.data_ptr(),
+        None if h_in is None else h_in.data_ptr(), h_out.data_ptr(), out.data_ptr())
     if rc:
         _raise(rc, f"{what} {tuple(shape)}")
-    return out.to(out_dt), h_out
+    return _as(out, out_dt), h_out
