@@ -20,7 +20,7 @@
 // data too.  Tiles are wide where there are channels enough: rows of 32 bytes, a quarter of
 // a line, keep the address path busy without moving much (8 x 8192 x 768 bfloat16, walked
 // in tiles of 16, 32 and 64 channels, which leave ever more CUs without work: 201, 150, 191 us;
-// in steps at once 167, 125, 115).  Copies reach 5.16 TB/s on this card; these reach, forward
+// in steps at once 175, 125, 115).  Copies reach 5.16 TB/s on this card; these reach, forward
 // and backward: 8 x 8192 x 768 bfloat16 4.4 and 4.6 TB/s, 2 x 16384 x 2048 bfloat16 4.7 and 5.0,
 // 1 x 131072 x 1024 float32 without a gate forward 5.2.
 //
@@ -408,22 +408,29 @@ __global__ void __launch_bounds__(8 * CT) gscan_bwd(ScanArgs a) {
 }
 
 // ---- The axis cut into its steps, all in one launch --------------------------------
-// A workgroup takes 128 tokens of 64 channels (or 256 of 32, 512 of 16).  It publishes its composition as soon as it
-// has it, finds the state that enters it from the steps before, and publishes the one
-// that leaves it.  Steps are dealt by a ticket, the earliest of all channels first: a
-// workgroup waits only for ones with smaller tickets, which have started and which in their
-// turn never wait for it, so every wait ends whatever else the GPU runs.  The entering state
-// is always the same sequence of operations -- the nearest published state, carried through
-// the published compositions after it, each rounded the same wherever it is done -- so
-// results do not depend on what was found first.
+// A workgroup takes 128 tokens of 64 channels (or 256 of 32).  It publishes its
+// composition as soon as it has it, finds the state that enters it from the steps before,
+// and publishes the one that leaves it.  Steps are dealt by a ticket, the earliest of all
+// tiles first (or, each tile with tickets of its own, the earliest of the tile): a workgroup
+// waits only for ones with smaller tickets, which have started and which in their turn never
+// wait for it, so every wait ends whatever else the GPU runs.
+// The entering state is always the same sequence of operations -- the nearest published
+// state, carried through the published compositions after it, each rounded the same wherever
+// it is done -- so results do not depend on what was found first.
 //
-// A published value is 64 bits written at once, {e^L or a tag, H or the state}; the memory is
-// filled with kNone before the launch, whose upper word is no such float.
+// What a step has published is 64 bits, written at once: first {e^L, H} (e^L = -1 for a fresh
+// start), then {kState, state}; before, the clearing kernel's kNone.
 constexpr unsigned long long kNone = ~0ull;
-constexpr int kWindow = 4;      // steps looked back over at a time
+constexpr float kState = -2.f;
+// Steps looked back over at a time: 8 where the registers allow (1 x 131072 x 1024 float32
+// forward 313 us, with 4 345); the backward has none to spare (8 x 8192 x 768 bfloat16 250 us,
+// with 4 194).
+template <bool REV> constexpr int kWindow = REV ? 4 : 8;
+constexpr int kTicketStride = 16; // tickets of different tiles on cache lines of their own
 struct Chain {
-  unsigned long long *comp, *state;   // (steps, B, C) each
-  unsigned* ticket;
+  unsigned long long* slot;       // (steps, B, C)
+  unsigned* ticket;               // (B tiles) kTicketStride; counted from -1, as cleared
+  int own;                        // each tile draws from its own
 };
 
 __device__ __forceinline__ unsigned long long pack(float hi, float lo) {
@@ -447,34 +454,24 @@ template <bool REV>
 __device__ __forceinline__ float entering(const Chain& ch, size_t n, size_t at, bool on, int blk,
                                           int blocks, float start) {
   while (true) {
-    unsigned long long s[kWindow], m[kWindow];
+    unsigned long long v[kWindow<REV>];
 #pragma unroll
-    for (int d = 0; d < kWindow; ++d) {
+    for (int d = 0; d < kWindow<REV>; ++d) {
       const int j = REV ? blk + 1 + d : blk - 1 - d;
       const bool in = REV ? j < blocks : j >= 0;
-      const size_t o = (size_t)(in ? j : blk) * n + at;
-      s[d] = __hip_atomic_load(ch.state + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      m[d] = __hip_atomic_load(ch.comp + o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (!in || !on) s[d] = pack(0.f, start);
-      if (!on) m[d] = 0;
+      v[d] = __hip_atomic_load(ch.slot + (size_t)(in ? j : blk) * n + at, __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+      if (!in || !on) v[d] = pack(kState, start);
     }
-    float h = 0.f;
-    int found = -1;
+    int found = -1;   // the nearest state with nothing missing before it
 #pragma unroll
-    for (int d = 0; d < kWindow; ++d) {
-      if (found == -1) {
-        if (__all(s[d] != kNone)) {
-          found = d;
-          h = lower(s[d]);
-        } else if (!__all(m[d] != kNone)) {
-          found = -2;   // a gap: look again
-        }
-      }
-    }
-    if (found >= 0) {
+    for (int d = 0; d < kWindow<REV>; ++d)
+      if (found == -1) found = upper(v[d]) == kState ? d : v[d] == kNone ? -2 : -1;
+    if (__all(found >= 0)) {
+      float h = 0.f;
 #pragma unroll
-      for (int d = kWindow - 2; d >= 0; --d)
-        if (d < found) h = through(upper(m[d]), h, lower(m[d]));
+      for (int d = kWindow<REV> - 1; d >= 0; --d)
+        if (d <= found) h = d == found ? lower(v[d]) : through(upper(v[d]), h, lower(v[d]));
       return h;
     }
     __builtin_amdgcn_s_sleep(2);
@@ -498,44 +495,50 @@ __device__ __forceinline__ void link(const Chain& ch, const Totals<NW, CT>& tot,
   if (A != A) A = __uint_as_float(0x7fc00000u);   // any NaN but kNone's
   // the steps after this one, if any, read these
   const bool first = REV ? blk == blocks - 1 : blk == 0, last = REV ? blk == 0 : blk == blocks - 1;
-  const size_t o = (size_t)blk * n + at;
-  if (!last && !first && on) publish(ch.comp + o, A, H);
+  unsigned long long* slot = ch.slot + (size_t)blk * n + at;
+  if (!last && !first && on) publish(slot, A, H);
   in = first ? start : entering<REV>(ch, n, at, on, blk, blocks, start);
   out = through(A, in, H);
-  if (!last && on) publish(ch.state + o, 0.f, out);
+  if (!last && on) publish(slot, kState, out);
 }
 
-// The step and channels of a ticket.
+// A workgroup's tile and step, by the ticket that its first thread draws.
+__device__ __forceinline__ int draw(const ScanArgs& a, const Chain& ch, int* shared) {
+  if (threadIdx.x == 0) {
+    const int units = a.B * a.nct;
+    if (ch.own) {
+      const int unit = (int)(blockIdx.x % (unsigned)units);
+      *shared = (int)(atomicAdd(ch.ticket + unit * kTicketStride, 1u) + 1u) * units + unit;
+    } else {
+      *shared = (int)(atomicAdd(ch.ticket, 1u) + 1u);
+    }
+  }
+  __syncthreads();
+  return *shared;
+}
 template <int V, int CT>
 struct Step : Place<V, CT, 512> {
-  int blk;
+  int unit, blk;
   __device__ Step(const ScanArgs& a, int item, bool rev) : Place<V, CT, 512>(a) {
     const int units = a.B * a.nct;
     blk = item / units;
-    const int unit = item - blk * units;
+    unit = item - blk * units;
     if (rev) blk = this->blocks - 1 - blk;
     this->b = unit / a.nct;
     this->c = (unit - this->b * a.nct) * CT + this->ci;
     this->on = this->c < a.C;
     if (!this->on) this->c = 0;
   }
+  // The channel of a lane of the wave that links, and C where the tile is narrower.
+  __device__ int lane_channel(const ScanArgs& a) const {
+    return this->lane < CT ? unit % a.nct * CT + this->lane : a.C;
+  }
 };
-// The channel of lane `lane` in the tile of ticket `item`; C, where the tile is narrower.
-template <int CT>
-__device__ __forceinline__ int tile_channel(const ScanArgs& a, int item, int lane) {
-  return lane < CT ? (item % (a.B * a.nct)) % a.nct * CT + lane : a.C;
-}
-__device__ __forceinline__ int next_ticket(unsigned* ticket, int* shared) {
-  if (threadIdx.x == 0) *shared = (int)atomicAdd(ticket, 1u);
-  __syncthreads();
-  return *shared;
-}
 
-__global__ void __launch_bounds__(kThreads) chain_clear(unsigned long long* p, size_t n,
-                                                        unsigned* ticket) {
-  const size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i < n) p[i] = kNone;
-  if (i == 0) *ticket = 0;
+__global__ void __launch_bounds__(kThreads) chain_clear(uint4* p, size_t n) {
+  const size_t stride = (size_t)gridDim.x * kThreads;
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += stride)
+    p[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
 }
 
 template <typename TX, typename TG, bool GATE, int V, int CT>
@@ -545,7 +548,7 @@ __global__ void __launch_bounds__(512, 4) chain_fwd(ScanArgs a, Chain ch) {
   __shared__ __attribute__((aligned(16))) Totals<NW, CT> tot;
   __shared__ __attribute__((aligned(16))) float s_in[CT];
   __shared__ int s_ticket;
-  const Step<V, CT> w(a, next_ticket(ch.ticket, &s_ticket), false);
+  const Step<V, CT> w(a, draw(a, ch, &s_ticket), false);
   Run<TX, V, S> x;
   Run<TG, V, S> g;
   std::conditional_t<GATE, Run<TX, V, S>, None> b;
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(512, 4) chain_fwd(ScanArgs a, Chain ch) {
   lds_barrier();
   if (w.wave == 0) {
     // lane = channel of the tile
-    const int unit_c = tile_channel<CT>(a, s_ticket, w.lane);
+    const int unit_c = w.lane_channel(a);
     const bool on = unit_c < a.C;
     const size_t n = (size_t)a.B * a.C, at = (size_t)w.b * a.C + (on ? unit_c : 0);
     float in, out;
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(512, 4) chain_bwd(ScanArgs a, Chain ch) {
   __shared__ __attribute__((aligned(16))) Totals<NW, CT> fwd, rev;
   __shared__ __attribute__((aligned(16))) float s_in[CT];
   __shared__ int s_ticket;
-  const Step<V, CT> w(a, next_ticket(ch.ticket, &s_ticket), true);
+  const Step<V, CT> w(a, draw(a, ch, &s_ticket), true);
   const bool has_dout = a.dout.p != nullptr;
   Run<TX, V, S> x, d;
   Run<TG, V, S> g;
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(512, 4) chain_bwd(ScanArgs a, Chain ch) {
   if (w.lane >= 64 - LPR) fwd.template put_<V>(0, w.wave, w.ci, TL, TH);
   lds_barrier();
   if (w.wave == 0) {
-    const int unit_c = tile_channel<CT>(a, s_ticket, w.lane);
+    const int unit_c = w.lane_channel(a);
     const bool on = unit_c < a.C;
     const size_t n = (size_t)a.B * a.C, at = (size_t)w.b * a.C + (on ? unit_c : 0);
     float in, out;
@@ -655,12 +658,16 @@ __global__ void __launch_bounds__(512, 4) chain_bwd(ScanArgs a, Chain ch) {
   for (int k = 0; k < NW - 1; ++k)
     if (k < w.wave) fwd.template pass<V>(0, k, w.ci, hw);
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    float hc = carry_through(L[c], hw[c], H[c]);
+  for (int c = 0; c < V; ++c) hw[c] = carry_through(L[c], hw[c], H[c]);
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      before[i][c] = hc;
-      hc = token(f.a[i][c], hc, f.u[i][c]);
+  for (int i = 0; i < S; ++i) {
+    float xv[V], bv[V];   // b x once more: kept, it would not fit the registers
+    widen<TX, V>(x.r[i], xv);
+    if constexpr (GATE) widen<TX, V>(b.r[i], bv);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      before[i][c] = hw[c];
+      hw[c] = token(f.a[i][c], hw[c], GATE ? bv[c] * xv[c] : xv[c]);
     }
   }
   lds_barrier();
@@ -723,6 +730,8 @@ __global__ void __launch_bounds__(kThreads) gscan_none(size_t n, const float* h_
 
 // ---------------------------------------------------------------- host side
 
+size_t ticket_bytes(int units) { return (size_t)units * kTicketStride * sizeof(unsigned); }
+
 // How a call is spread over the GPU: a walk along the axis by workgroups of ct channels, or
 // (chain) all steps at once.
 struct Split {
@@ -740,7 +749,7 @@ Split split(int B, int T, int C, int in_dtype) {
     s.nct = (C + ct - 1) / ct;
     s.block = chain ? 16 * 512 / ct : 128;
     s.blocks = T / s.block + (T % s.block != 0);
-    s.ws = chain ? 256 + (size_t)s.blocks * B * C * 16 : 0;
+    s.ws = chain ? ticket_bytes(B * s.nct) + ((size_t)s.blocks * B * C * 8 + 15) / 16 * 16 : 0;
   };
   // Short axes: one launch, no ticket.  16 x 512 x 1024 bfloat16 forward and backward 18 and 35
   // us, in steps at once 27 and 38; 16 x 2048 x 4096 303 and 582, in steps at once 289 and 510.
@@ -749,11 +758,11 @@ Split split(int B, int T, int C, int in_dtype) {
     return s;
   }
   // Rows of a tile fill a 128-byte line.  With few channels the time goes by the hand-over from
-  // step to step (1.1 us for every four) and narrower tiles have longer steps: bfloat16 forward
-  // 1 x 65536 x 768 in tiles of 64, 32, 16 channels 152, 129, 165 us, 1 x 16384 x 128 35, 23,
-  // 18; float32 1 x 32768 x 256 forward and backward 158, 107, 112.
-  const long long bc = (long long)B * C;
-  cut(true, bc >= 1024 ? (in_dtype == GDN2_F32 ? 32 : 64) : bc >= 192 ? 32 : 16);
+  // step to step (about 1.1 us for a window of them) and narrower tiles have longer steps: bfloat16
+  // forward and backward 8 x 8192 x 768 in tiles of 64 and 32 channels 115 + 196 and 125 + 215 us,
+  // 1 x 65536 x 768 124 + 206 and 128 + 211, 1 x 16384 x 128 27 + 37 and 18 + 26; float32
+  // 8 x 4096 x 768 88 + 147 and 87 + 148, 1 x 32768 x 256 58 + 79 and 40 + 56.
+  cut(true, in_dtype == GDN2_BF16 && (long long)B * C >= 1024 ? 64 : 32);
   if (s.blocks * units(s.ct) >= (1ll << 30)) cut(false, 64);   // tickets past 31 bits
   return s;
 }
@@ -795,13 +804,18 @@ void launch_tile(hipStream_t st, const ScanArgs& a, bool bwd) {
 }
 template <typename TX, typename TG, bool GATE, int V, int CT>
 void launch_chain(hipStream_t st, const ScanArgs& a, bool bwd, int n) {
-  const size_t values = (size_t)n * a.B * a.C;
+  // tickets, then slots, all cleared
+  const size_t tickets = ticket_bytes(a.B * a.nct), bytes = tickets + (size_t)n * a.B * a.C * 8;
   Chain ch;
+  // Drawing from one counter takes 10 ns a ticket; where all workgroups start at once that is
+  // waited for (1 x 4001 x 768 17.8 us, from the tiles' own 14.1), where they do not it keeps the
+  // tiles abreast (1 x 131072 x 1024 313 us, from the tiles' own 386).
+  ch.own = n * a.B * a.nct <= 2 * num_cus();
   ch.ticket = (unsigned*)a.ws;
-  ch.comp = (unsigned long long*)((char*)a.ws + 256);
-  ch.state = ch.comp + values;
-  hipLaunchKernelGGL(chain_clear, dim3((unsigned)((2 * values + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, st, ch.comp, 2 * values, ch.ticket);
+  ch.slot = (unsigned long long*)((char*)a.ws + tickets);
+  const size_t pieces = (bytes + 15) / 16, wgs = (pieces + kThreads - 1) / kThreads;
+  hipLaunchKernelGGL(chain_clear, dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(kThreads), 0, st,
+                     (uint4*)a.ws, pieces);
   const dim3 grid((unsigned)(n * a.B * a.nct)), block(512);
   if (bwd)
     hipLaunchKernelGGL((chain_bwd<TX, TG, GATE, V, CT>), grid, block, 0, st, a, ch);
@@ -813,10 +827,8 @@ void launch_width(hipStream_t st, const ScanArgs& a, bool bwd, const Split& s) {
   if (s.chain) {
     if (s.ct == 64)
       launch_chain<TX, TG, GATE, V, 64>(st, a, bwd, s.blocks);
-    else if (s.ct == 32)
-      launch_chain<TX, TG, GATE, V, 32>(st, a, bwd, s.blocks);
     else
-      launch_chain<TX, TG, GATE, V, 16>(st, a, bwd, s.blocks);
+      launch_chain<TX, TG, GATE, V, 32>(st, a, bwd, s.blocks);
   } else if (s.ct == 64) {
     launch_tile<TX, TG, GATE, V, 64>(st, a, bwd);
   } else {
