@@ -46,6 +46,8 @@ def _row_stride(x):
 
 def _prepare(x, weight, residual, eps, what):
     """(x, residual, weight) of supported types, checked; rows are not formed yet."""
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError(f"{what}: weight must be a torch tensor")
     _tensor(x, "x", what)
     _tensor(weight, "weight", what)
     if x.dim() < 1 or weight.shape != x.shape[-1:]:
