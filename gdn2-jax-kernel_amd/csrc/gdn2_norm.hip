@@ -11,8 +11,10 @@
 //   dh_total = rstd (dn - n mean(dn n)) + dh,   dx = dr = dh_total,   dw = sum dy n.
 //
 // All of these are bound by memory traffic: a row is read once into registers (8 values
-// a thread and chunk, 16-byte accesses), reduced over its 64, 256 or 1024 threads and
-// written from the registers.  Sums and the norm's factors are float32.
+// a thread and chunk, 16-byte accesses), reduced over its 64 to 1024 threads and
+// written from the registers.  Sums and the norm's factors are float32.  Copies reach 5.16 TB/s
+// on this card; with a residual, bfloat16: norm of 65536 x 768 75 us (5.4 TB/s), 16384 x 4096
+// 97 (5.5), 4096 x 8192 41 (6.5); in 8 bits 66 (5.3), 87 (5.4), 37 (6.4).
 #include "gdn2.h"
 #include "gdn2_common.h"
 
@@ -93,10 +95,13 @@ __device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(
 
 enum { kNorm, kNorm8, kQuant };
 
-// TPR threads take a row, NCH chunks of 8 values each; a workgroup max(256, TPR) threads.
+// Threads of a workgroup with TPR threads to a row: a row alone, or four of a wave each.
+template <int TPR> constexpr int kNT = TPR == 64 ? 256 : TPR;
+
+// TPR threads take a row, NCH chunks of 8 values each.
 template <typename TX, typename TR, int MODE, int TPR, int NCH, bool VEC>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd(NormArgs a) {
-  constexpr int NT = TPR > 256 ? TPR : 256, NW = TPR / 64;
+__global__ void __launch_bounds__(kNT<TPR>) norm_fwd(NormArgs a) {
+  constexpr int NT = kNT<TPR>, NW = TPR / 64;
   __shared__ float s_sum[NW];
   __shared__ unsigned s_max[NW];
   const int tid = threadIdx.x % TPR;
@@ -216,16 +221,48 @@ struct NormBwdArgs {
   const void *h, *w, *dy, *dh;   // h, dy, dh dense; dy or dh may be null
   const float* rstd;
   void *dx, *dr;                 // dr: null where the residual's gradient is dx itself
-  float* part;                   // (waves or workgroups of the launch, C)
+  float* part;                   // (workgroups, C)
   int M, C, w_bf16, groups;      // groups of TPR threads in the launch
 };
 
+// 8 values at column c as they are stored, so that the next row's wait in few registers.
+template <typename T, bool VEC> struct Raw8 {
+  T v[8];
+  __device__ __forceinline__ void load(const T* row, int c, int C) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < C ? row[c + e] : (T)0.f;
+  }
+  __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
+};
+template <> struct Raw8<float, true> {
+  f32x4 v[2];
+  __device__ __forceinline__ void load(const float* row, int c, int C) {
+    v[0] = c < C ? load4f(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+    v[1] = c < C ? load4f(row + c + 4) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ float operator[](int e) const { return v[e / 4][e % 4]; }
+};
+template <> struct Raw8<bf16_t, true> {
+  bf16x8 v;
+  __device__ __forceinline__ void load(const bf16_t* row, int c, int C) {
+    const bf16_t z = (bf16_t)0.f;
+    v = c < C ? *reinterpret_cast<const bf16x8*>(row + c) : bf16x8{z, z, z, z, z, z, z, z};
+  }
+  __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
+};
+
+// A group of TPR threads takes the rows group, group + groups, ...; dw gathers in its
+// registers (a thread keeps its columns), then over the workgroup's groups in LDS and, by
+// norm_dw, over the workgroups, always in the same order.  The next row is in flight while one
+// is worked on.  With a partial sum of dw for each wave and no row ahead 65536 x 768 bfloat16
+// took 95 us, 4096 x 8192 87, 2048 x 2048 19; so 76 (5.3 TB/s), 44 and 12.
 template <typename TX, typename TR, int TPR, int NCH, bool VEC>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_bwd(NormBwdArgs a) {
-  constexpr int NT = TPR > 256 ? TPR : 256, NW = TPR / 64;
+__global__ void __launch_bounds__(kNT<TPR>) norm_bwd(NormBwdArgs a) {
+  constexpr int NT = kNT<TPR>, NW = TPR / 64, NG = NT / TPR;
   __shared__ float s_sum[2][NW];
+  __shared__ float s_dw[NG > 1 ? NG : 1][NG > 1 ? NCH * TPR * 8 : 1];
   const int tid = threadIdx.x % TPR;
-  const int group = blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
+  const int group = blockIdx.x * NG + threadIdx.x / TPR;
   float w[NCH][8], dw[NCH][8];
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
@@ -233,27 +270,42 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_bwd(NormBwdArgs a)
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[j][e] = 0.f;
   }
-  int flip = 0;
-  for (long long row = group; row < a.M; row += a.groups, flip ^= 1) {
-    const float rstd = a.rstd[row];
-    float n[NCH][8], d[NCH][8], sum = 0.f;
+  Raw8<TR, VEC> rh[NCH], rg[NCH];
+  Raw8<TX, VEC> ry[NCH];
+  float r_next = 0.f;
+  auto load = [&](long long row) {
+    r_next = a.rstd[row];
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       const int c = (j * TPR + tid) * 8;
-      load8<TR, VEC>((const TR*)a.h + row * a.C, c, a.C, n[j]);
-      if (a.dy) {
-        load8<TX, VEC>((const TX*)a.dy + row * a.C, c, a.C, d[j]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[j][e] = 0.f;
-      }
+      rh[j].load((const TR*)a.h + row * a.C, c, a.C);
+      if (a.dy) ry[j].load((const TX*)a.dy + row * a.C, c, a.C);
+      if (a.dh) rg[j].load((const TR*)a.dh + row * a.C, c, a.C);
     }
+  };
+  constexpr bool AHEAD = NCH <= 2;   // the registers of wider rows are full
+  int flip = 0;
+  if (AHEAD && group < a.M) load(group);
+  for (long long row = group; row < a.M; row += a.groups, flip ^= 1) {
+    if (!AHEAD) load(row);
+    const float rstd = r_next;
+    float n[NCH][8], d[NCH][8], sum = 0.f;
+    Raw8<TR, VEC> g[NCH];
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        n[j][e] = rh[j][e] * rstd;
+        d[j][e] = a.dy ? ry[j][e] : 0.f;
+      }
+      g[j] = rg[j];
+    }
+    if (AHEAD && row + a.groups < a.M) load(row + a.groups);
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       float part = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        n[j][e] *= rstd;
         dw[j][e] = fmaf(d[j][e], n[j][e], dw[j][e]);
         d[j][e] *= w[j][e];
         part = fmaf(d[j][e], n[j][e], part);
@@ -263,7 +315,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_bwd(NormBwdArgs a)
     sum = wave_sum(sum);
     if constexpr (NW > 1) {
       if (tid % 64 == 0) s_sum[flip][tid / 64] = sum;   // two buffers: one barrier a row
-      __syncthreads();
+      lds_barrier();
       sum = 0.f;
 #pragma unroll
       for (int k = 0; k < NW; ++k) sum += s_sum[flip][k];
@@ -272,22 +324,33 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_bwd(NormBwdArgs a)
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
       const int c = (j * TPR + tid) * 8;
-      float g[8];
-      if (a.dh) {
-        load8<TR, VEC>((const TR*)a.dh + row * a.C, c, a.C, g);
-      } else {
+      float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = fmaf(rstd, d[j][e] - n[j][e] * mean, g[e]);
-      store8<TX, VEC>((TX*)a.dx + row * a.C, c, a.C, g);
-      if (a.dr) store8<TR, VEC>((TR*)a.dr + row * a.C, c, a.C, g);
+      for (int e = 0; e < 8; ++e)
+        o[e] = fmaf(rstd, d[j][e] - n[j][e] * mean, a.dh ? g[j][e] : 0.f);
+      store8<TX, VEC>((TX*)a.dx + row * a.C, c, a.C, o);
+      if (a.dr) store8<TR, VEC>((TR*)a.dr + row * a.C, c, a.C, o);
     }
   }
+  if constexpr (NG > 1) {
 #pragma unroll
-  for (int j = 0; j < NCH; ++j)
-    store8<float, VEC>(a.part + (size_t)group * a.C, (j * TPR + tid) * 8, a.C, dw[j]);
+    for (int j = 0; j < NCH; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; e += 4)
+        store4(&s_dw[threadIdx.x / TPR][(j * TPR + tid) * 8 + e],
+               f32x4{dw[j][e], dw[j][e + 1], dw[j][e + 2], dw[j][e + 3]});
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.C; c += NT) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) s += s_dw[k][c];
+      a.part[(size_t)blockIdx.x * a.C + c] = s;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NCH; ++j)
+      store8<float, VEC>(a.part + (size_t)blockIdx.x * a.C, (j * TPR + tid) * 8, a.C, dw[j]);
+  }
 }
 
 // dw[c] = sum over the partial sums, in a fixed order: 32 columns a workgroup, 32 groups of
@@ -297,8 +360,10 @@ __global__ void __launch_bounds__(1024) norm_dw(const float* part, int groups, i
   __shared__ float s[32][33];
   const int tx = threadIdx.x % 32, ty = threadIdx.x / 32, c = blockIdx.x * 32 + tx;
   float sum = 0.f;
-  if (c < C)
+  if (c < C) {
+#pragma unroll 8
     for (int g = ty; g < groups; g += 32) sum += part[(size_t)g * C + c];
+  }
   s[ty][tx] = sum;
   __syncthreads();
 #pragma unroll
@@ -341,31 +406,33 @@ void by_width(int C, F f) {
   return f(std::integral_constant<int, TPR>{}, std::integral_constant<int, NCH>{})
   if (C <= 512) GDN2_W(64, 1);
   if (C <= 1024) GDN2_W(64, 2);
-  if (C <= 2048) GDN2_W(64, 4);
+  if (C <= 2048) GDN2_W(128, 2);
   if (C <= 4096) GDN2_W(256, 2);
-  if (C <= 8192) GDN2_W(256, 4);
-  if (!WIDE || C <= 16384) GDN2_W(1024, 2);
+  if (C <= 8192) GDN2_W(512, 2);
+  if (!WIDE || C <= 16384) GDN2_W(512, 4);
   if constexpr (WIDE) GDN2_W(1024, 4);
 #undef GDN2_W
 }
-// Row groups of the backward launch: its partial sums of dw.
-int bwd_groups(int M, int C) {
-  int per = 1, tpr = 64;
-  by_width<false>(C, [&](auto t, auto) {
-    tpr = decltype(t)::value;
-    per = tpr < 256 ? 256 / tpr : 1;
-  });
-  const int waves = tpr / 64;
-  long long want = 4096 / waves;          // 16 waves a CU
-  if (want > M) want = M;
-  return (int)((want + per - 1) / per * per);
+// Workgroups of the backward launch, each with a partial sum of dw; `per`: row groups of one.
+// At most 2048 waves, two to a SIMD (4096: 65536 x 768 bfloat16 87 us, 2048 76; 16384 x 4096 113
+// and 101), and, down to one workgroup a CU, at least four rows a group.
+int bwd_workgroups(int M, int C, int* per) {
+  int tpr = 64;
+  by_width<false>(C, [&](auto t, auto) { tpr = decltype(t)::value; });
+  *per = tpr == 64 ? 4 : 1;
+  constexpr int WAVES = 2048;
+  long long groups = WAVES / (tpr / 64);
+  const long long few = M / 4 > 256 ? M / 4 : 256;
+  if (groups > few) groups = few;
+  if (groups > M) groups = M;
+  return (int)((groups + *per - 1) / *per);
 }
 
 template <typename TX, typename TR, int MODE>
 hipError_t launch_fwd(hipStream_t st, const NormArgs& a, bool vec) {
   by_width<MODE == kQuant>(a.C, [&](auto t, auto n) {
     constexpr int TPR = decltype(t)::value, NCH = decltype(n)::value;
-    constexpr int NT = TPR > 256 ? TPR : 256, ROWS = NT / TPR;
+    constexpr int NT = kNT<TPR>, ROWS = NT / TPR;
     const dim3 grid((unsigned)(((long long)a.M + ROWS - 1) / ROWS)), block(NT);
     if (vec)
       hipLaunchKernelGGL((norm_fwd<TX, TR, MODE, TPR, NCH, true>), grid, block, 0, st, a);
@@ -387,11 +454,11 @@ int launch_fwd(hipStream_t st, const NormArgs& a, int x_dtype, int r_dtype, bool
   return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 template <typename TX, typename TR>
-hipError_t launch_bwd(hipStream_t st, const NormBwdArgs& a, bool vec) {
+hipError_t launch_bwd(hipStream_t st, const NormBwdArgs& a, int wgs, bool vec) {
   by_width<false>(a.C, [&](auto t, auto n) {
     constexpr int TPR = decltype(t)::value, NCH = decltype(n)::value;
-    constexpr int NT = TPR > 256 ? TPR : 256;
-    const dim3 grid((unsigned)(a.groups / (NT / TPR))), block(NT);
+    constexpr int NT = kNT<TPR>;
+    const dim3 grid((unsigned)wgs), block(NT);
     if (vec)
       hipLaunchKernelGGL((norm_bwd<TX, TR, TPR, NCH, true>), grid, block, 0, st, a);
     else
@@ -500,7 +567,8 @@ int gdn2_dequantize_int8(void* stream, int M, int C, int out_dtype, const void* 
 
 size_t gdn2_rms_norm_bwd_workspace_bytes(int M, int C) {
   if (validate(M, C, GDN2_F32, GDN2_F32, GDN2_F32) != GDN2_OK) return 0;
-  return (size_t)bwd_groups(M, C) * C * sizeof(float);
+  int per = 1;
+  return (size_t)bwd_workgroups(M, C, &per) * C * sizeof(float);
 }
 
 int gdn2_rms_norm_bwd(void* stream, int M, int C, int x_dtype, int r_dtype, int w_dtype,
@@ -523,16 +591,18 @@ int gdn2_rms_norm_bwd(void* stream, int M, int C, int x_dtype, int r_dtype, int 
   NormBwdArgs a = {};
   a.h = h, a.w = weight, a.dy = dy, a.dh = dh, a.rstd = rstd, a.dx = dx, a.dr = dr;
   a.part = (float*)ws, a.M = M, a.C = C, a.w_bf16 = w_dtype == GDN2_BF16;
-  a.groups = bwd_groups(M, C);
+  int per = 1;
+  const int wgs = bwd_workgroups(M, C, &per);
+  a.groups = wgs * per;
   hipStream_t st = (hipStream_t)stream;
   hipError_t e = hipSuccess;
   if (M > 0)
-    e = x_dtype == GDN2_F32   ? launch_bwd<float, float>(st, a, vec)
-        : r_dtype == GDN2_F32 ? launch_bwd<bf16_t, float>(st, a, vec)
-                              : launch_bwd<bf16_t, bf16_t>(st, a, vec);
+    e = x_dtype == GDN2_F32   ? launch_bwd<float, float>(st, a, wgs, vec)
+        : r_dtype == GDN2_F32 ? launch_bwd<bf16_t, float>(st, a, wgs, vec)
+                              : launch_bwd<bf16_t, bf16_t>(st, a, wgs, vec);
   if (e != hipSuccess) return GDN2_ERR_LAUNCH;
   hipLaunchKernelGGL(norm_dw, dim3((unsigned)((C + 31) / 32)), dim3(1024), 0, st, a.part,
-                     M > 0 ? a.groups : 0, C, dw, w_dtype == GDN2_BF16);
+                     M > 0 ? wgs : 0, C, dw, w_dtype == GDN2_BF16);
   return hipGetLastError() == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 

@@ -111,8 +111,10 @@ def test_norm_refusals():
     assert bwd(dw=None) == _lib.ERR_NULL and bwd(ws=None) == _lib.ERR_NULL
     assert bwd(wsb=0) == _lib.ERR_WORKSPACE
     size = L.gdn2_rms_norm_bwd_workspace_bytes
-    assert size(10, 64) == 12 * 64 * 4          # 10 rows in groups of 4 waves
-    assert size(1 << 20, 768) == 4096 * 768 * 4 and size(1 << 20, 4096) == 1024 * 4096 * 4
+    # a row of partial sums for each workgroup: of four waves up to 1024 columns, else of a row
+    assert size(10, 64) == 3 * 64 * 4
+    assert size(1 << 20, 768) == 512 * 768 * 4 and size(1 << 20, 4096) == 512 * 4096 * 4
+    assert size(2000, 4096) == 500 * 4096 * 4 and size(300, 4096) == 256 * 4096 * 4
     assert size(0, 64) == 0 and size(4, 16385) == 0 and size(-1, 4) == 0
 
 
