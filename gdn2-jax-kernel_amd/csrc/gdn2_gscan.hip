@@ -707,19 +707,20 @@ template <typename TX, typename TG, bool GATE, int V>
 __global__ void __launch_bounds__(kThreads) gscan_step(size_t n, const TX* x, const TG* g,
                                                        const TX* b, const float* h_in,
                                                        float* h_out, TX* out) {
-  const size_t i = ((size_t)blockIdx.x * kThreads + threadIdx.x) * V;
-  if (i >= n) return;
-  float xv[V], gv[V], bv[V], h[V];
-  widen<TX, V>(*reinterpret_cast<const typename Raw<TX, V>::type*>(x + i), xv);
-  widen<TG, V>(*reinterpret_cast<const typename Raw<TG, V>::type*>(g + i), gv);
-  if constexpr (GATE) widen<TX, V>(*reinterpret_cast<const typename Raw<TX, V>::type*>(b + i), bv);
+  for (size_t i = ((size_t)blockIdx.x * kThreads + threadIdx.x) * V; i < n;
+       i += (size_t)gridDim.x * kThreads * V) {
+    float xv[V], gv[V], bv[V], h[V];
+    widen<TX, V>(*reinterpret_cast<const typename Raw<TX, V>::type*>(x + i), xv);
+    widen<TG, V>(*reinterpret_cast<const typename Raw<TG, V>::type*>(g + i), gv);
+    if constexpr (GATE) widen<TX, V>(*reinterpret_cast<const typename Raw<TX, V>::type*>(b + i), bv);
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const float u = GATE ? bv[c] * xv[c] : xv[c];
-    h[c] = carry_through(gv[c] * kLog2e, h_in ? h_in[i + c] : 0.f, u);
+    for (int c = 0; c < V; ++c) {
+      const float u = GATE ? bv[c] * xv[c] : xv[c];
+      h[c] = carry_through(gv[c] * kLog2e, h_in ? h_in[i + c] : 0.f, u);
+    }
+    put<float, V>(h_out + i, h);
+    put<TX, V>(out + i, h);
   }
-  put<float, V>(h_out + i, h);
-  put<TX, V>(out + i, h);
 }
 
 // No token: the state passes through.
@@ -763,7 +764,7 @@ Split split(int B, int T, int C, int in_dtype) {
   // 1 x 65536 x 768 124 + 206 and 128 + 211, 1 x 16384 x 128 27 + 37 and 18 + 26; float32
   // 8 x 4096 x 768 88 + 147 and 87 + 148, 1 x 32768 x 256 58 + 79 and 40 + 56.
   cut(true, in_dtype == GDN2_BF16 && (long long)B * C >= 1024 ? 64 : 32);
-  if (s.blocks * units(s.ct) >= (1ll << 30)) cut(false, 64);   // tickets past 31 bits
+  if (s.blocks * units(s.ct) >= (1ll << 22)) cut(false, 64);   // a grid's threads: 32 bits
   return s;
 }
 
@@ -773,7 +774,7 @@ int validate(int B, int T, int C, int in_dtype, int g_dtype) {
   if (g_dtype != GDN2_F32 && !(g_dtype == GDN2_BF16 && in_dtype == GDN2_BF16))
     return GDN2_ERR_DTYPE;
   if (T > INT_MAX - 512 || C > INT_MAX - 64) return GDN2_ERR_SHAPE;
-  // the launch's workgroups, and bytes of a tensor, within 31 and 62 bits
+  // a launch's threads (up to 512 for 16 channels) within 32 bits, bytes of a tensor within 62
   if ((double)B * ((C + kMinTile - 1) / kMinTile) > 8.0e6) return GDN2_ERR_SHAPE;
   if ((double)B * T * C > 1e18) return GDN2_ERR_SHAPE;
   return GDN2_OK;
@@ -858,8 +859,9 @@ int launch_scan(hipStream_t st, ScanArgs& a, int in_dtype, int g_dtype, bool bwd
 template <typename TX, typename TG>
 hipError_t launch_step(hipStream_t st, size_t n, const void* x, const void* g, const void* b,
                        const float* h_in, float* h_out, void* out, bool vec) {
-  const size_t per = (size_t)kThreads * (vec ? 4 : 1);
-  const dim3 grid((unsigned)((n + per - 1) / per)), block(kThreads);
+  // a grid's threads stay within 32 bits: the kernel walks over what lies beyond
+  const size_t per = (size_t)kThreads * (vec ? 4 : 1), wgs = (n + per - 1) / per;
+  const dim3 grid((unsigned)(wgs < 65536 ? wgs : 65536)), block(kThreads);
 #define GDN2_STEP(GATE, V)                                                                   \
   hipLaunchKernelGGL((gscan_step<TX, TG, GATE, V>), grid, block, 0, st, n, (const TX*)x,     \
                      (const TG*)g, (const TX*)b, h_in, h_out, (TX*)out)

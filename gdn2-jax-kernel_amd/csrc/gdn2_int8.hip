@@ -406,9 +406,9 @@ extern "C" int gdn2_int8_matmul(void* stream, int M, int N, int K, int out_dtype
   if (out_dtype != GDN2_F32 && out_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
   const long long row = (K + 15ll) / 16 * 16;
   if (x_stride < row || w_stride < row) return GDN2_ERR_SHAPE;
-  // tiles are counted in 31 bits, and a tile's row numbers may pass the end by 255
-  if (M > INT_MAX - 256 || N > INT_MAX - 256 ||
-      ((M + 127ll) / 128) * ((N + 63ll) / 64) > (1ll << 30))
+  // a launch's threads stay within 32 bits (128 x 128 tiles of 256, 16 columns of 512), and a
+  // tile's row numbers, which may pass the end by 255, within 31
+  if (M > INT_MAX - 256 || N > (1 << 26) || ((M + 127ll) / 128) * ((N + 127ll) / 128) > (1ll << 23))
     return GDN2_ERR_SHAPE;
   if (M == 0) return GDN2_OK;
   const size_t es = out_dtype == GDN2_F32 ? 4 : 2;

@@ -102,94 +102,97 @@ template <int TPR> constexpr int kNT = TPR == 64 ? 256 : TPR;
 template <typename TX, typename TR, int MODE, int TPR, int NCH, bool VEC>
 __global__ void __launch_bounds__(kNT<TPR>) norm_fwd(NormArgs a) {
   constexpr int NT = kNT<TPR>, NW = TPR / 64;
-  __shared__ float s_sum[NW];
-  __shared__ unsigned s_max[NW];
+  __shared__ float s_sum[2][NW];      // two buffers: a slower wave may still read the last row's
+  __shared__ unsigned s_max[2][NW];
   const int tid = threadIdx.x % TPR;
-  const long long row = (long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
-  if (row >= a.M) return;   // whole waves, and whole workgroups where a row has several
-  const TX* x = (const TX*)a.x + row * a.ldx;
-  float v[NCH][8];
+  int flip = 0;
+  // whole waves leave the loop, and whole workgroups where a row has several
+  for (long long row = (long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR; row < a.M;
+       row += (long long)gridDim.x * (NT / TPR), flip ^= 1) {
+    const TX* x = (const TX*)a.x + row * a.ldx;
+    float v[NCH][8];
 #pragma unroll
-  for (int j = 0; j < NCH; ++j) load8<TX, VEC>(x, (j * TPR + tid) * 8, a.C, v[j]);
-  if (MODE != kQuant && a.r) {
-    const TR* r = (const TR*)a.r + row * a.ldr;
-    TR* h = (TR*)a.h + row * a.C;
+    for (int j = 0; j < NCH; ++j) load8<TX, VEC>(x, (j * TPR + tid) * 8, a.C, v[j]);
+    if (MODE != kQuant && a.r) {
+      const TR* r = (const TR*)a.r + row * a.ldr;
+      TR* h = (TR*)a.h + row * a.C;
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int c = (j * TPR + tid) * 8;
-      float f[8];
-      load8<TR, VEC>(r, c, a.C, f);
+      for (int j = 0; j < NCH; ++j) {
+        const int c = (j * TPR + tid) * 8;
+        float f[8];
+        load8<TR, VEC>(r, c, a.C, f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] = to_f(from_f<TR>(v[j][e] + f[e]));
-      store8<TR, VEC>(h, c, a.C, v[j]);
-    }
-  }
-  float rstd = 1.f;
-  unsigned top = 0;
-  if constexpr (MODE != kQuant) {
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      float w[8], part = 0.f;
-      load_w<VEC>(a.w, a.w_bf16, (j * TPR + tid) * 8, a.C, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        part = fmaf(v[j][e], v[j][e], part);
-        v[j][e] *= w[e];
+        for (int e = 0; e < 8; ++e) v[j][e] = to_f(from_f<TR>(v[j][e] + f[e]));
+        store8<TR, VEC>(h, c, a.C, v[j]);
       }
-      sum += part;
     }
-    sum = wave_sum(sum);
-    if constexpr (NW > 1) {
-      if (tid % 64 == 0) s_sum[tid / 64] = sum;
-      __syncthreads();
-      sum = 0.f;
+    float rstd = 1.f, w[NCH][8];
+    unsigned top = 0;
+    if constexpr (MODE != kQuant) {
+      float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) sum += s_sum[k];
-    }
-    rstd = 1.f / sqrtf(sum / (float)a.C + a.eps);
-    if (a.rstd && tid == 0) a.rstd[row] = rstd;
-  }
-  if constexpr (MODE == kNorm) {
-    TX* y = (TX*)a.y + row * a.C;
+      for (int j = 0; j < NCH; ++j) {
+        float part = 0.f;
+        load_w<VEC>(a.w, a.w_bf16, (j * TPR + tid) * 8, a.C, w[j]);
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= rstd;
-      store8<TX, VEC>(y, (j * TPR + tid) * 8, a.C, v[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < NCH; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned u = magnitude(v[j][e]);
-        top = top > u ? top : u;
+        for (int e = 0; e < 8; ++e) {
+          part = fmaf(v[j][e], v[j][e], part);
+          if (MODE == kNorm8) v[j][e] *= w[j][e];
+        }
+        sum += part;
       }
-    top = wave_max(top);
-    if constexpr (NW > 1) {
-      if (tid % 64 == 0) s_max[tid / 64] = top;
-      __syncthreads();
+      sum = wave_sum(sum);
+      if constexpr (NW > 1) {
+        if (tid % 64 == 0) s_sum[flip][tid / 64] = sum;
+        lds_barrier();
+        sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < NW; ++k) top = top > s_max[k] ? top : s_max[k];
-    }
-    const float m = __uint_as_float(top);
-    const bool bad = top >= 0x7f800000u, zero = m < kTiny;
-    const float inv = bad || zero ? 0.f : (1.f / m) * 127.f;
-    if (tid == 0)
-      a.scale[row] = bad ? __uint_as_float(0x7fc00000u) : zero ? 0.f : m * rstd / 127.f;
-    signed char* q = a.q + row * a.ldq;
-#pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int c = (j * TPR + tid) * 8;
-      unsigned p[2] = {0, 0};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = bad ? 0 : (int)rintf(v[j][e] * inv);
-        p[e / 4] |= ((unsigned)i & 0xffu) << (8 * (e % 4));
+        for (int k = 0; k < NW; ++k) sum += s_sum[flip][k];
       }
-      // the bytes between C and the next multiple of 16 are zeroed: ldq is one
-      if (c < (int)a.ldq) *reinterpret_cast<uint2*>(q + c) = make_uint2(p[0], p[1]);
+      rstd = 1.f / sqrtf(sum / (float)a.C + a.eps);
+      if (a.rstd && tid == 0) a.rstd[row] = rstd;
+    }
+    if constexpr (MODE == kNorm) {
+      TX* y = (TX*)a.y + row * a.C;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[j][e] = v[j][e] * rstd * w[j][e];
+        store8<TX, VEC>(y, (j * TPR + tid) * 8, a.C, v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NCH; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned u = magnitude(v[j][e]);
+          top = top > u ? top : u;
+        }
+      top = wave_max(top);
+      if constexpr (NW > 1) {
+        if (tid % 64 == 0) s_max[flip][tid / 64] = top;
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < NW; ++k) top = top > s_max[flip][k] ? top : s_max[flip][k];
+      }
+      const float m = __uint_as_float(top);
+      const bool bad = top >= 0x7f800000u, zero = m < kTiny;
+      const float inv = bad || zero ? 0.f : (1.f / m) * 127.f;
+      if (tid == 0)
+        a.scale[row] = bad ? __uint_as_float(0x7fc00000u) : zero ? 0.f : m * rstd / 127.f;
+      signed char* q = a.q + row * a.ldq;
+#pragma unroll
+      for (int j = 0; j < NCH; ++j) {
+        const int c = (j * TPR + tid) * 8;
+        unsigned p[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = bad ? 0 : (int)rintf(v[j][e] * inv);
+          p[e / 4] |= ((unsigned)i & 0xffu) << (8 * (e % 4));
+        }
+        // the bytes between C and the next multiple of 16 are zeroed: ldq is one
+        if (c < (int)a.ldq) *reinterpret_cast<uint2*>(q + c) = make_uint2(p[0], p[1]);
+      }
     }
   }
 }
@@ -198,23 +201,24 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize(const signed char* q, long long ldq,
                                                   const float* scale, T* y, long long M, int C) {
   const int per = (C + 7) / 8;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / per;
-  if (row >= M) return;
-  const int c = (int)(i - row * per) * 8;
-  const float s = scale[row];
-  float f[8];
-  if constexpr (VEC) {
-    const uint2 p = *reinterpret_cast<const uint2*>(q + row * ldq + c);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < M * per;
+       i += (long long)gridDim.x * 256) {
+    const long long row = i / per;
+    const int c = (int)(i - row * per) * 8;
+    const float s = scale[row];
+    float f[8];
+    if constexpr (VEC) {
+      const uint2 p = *reinterpret_cast<const uint2*>(q + row * ldq + c);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = (float)(signed char)((e < 4 ? p.x : p.y) >> (8 * (e % 4)));
-  } else {
+      for (int e = 0; e < 8; ++e) f[e] = (float)(signed char)((e < 4 ? p.x : p.y) >> (8 * (e % 4)));
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < C ? (float)q[row * ldq + c + e] : 0.f;
+      for (int e = 0; e < 8; ++e) f[e] = c + e < C ? (float)q[row * ldq + c + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= s;
+    store8<T, VEC>(y + row * C, c, C, f);
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] *= s;
-  store8<T, VEC>(y + row * C, c, C, f);
 }
 
 struct NormBwdArgs {
@@ -381,6 +385,10 @@ __global__ void __launch_bounds__(1024) norm_dw(const float* part, int groups, i
 
 // ---------------------------------------------------------------- host side
 
+// Workgroups of a launch: the kernels walk over what lies beyond, and a grid's threads stay
+// within 32 bits.
+unsigned grid_of(long long wgs) { return (unsigned)(wgs < 65536 ? wgs : 65536); }
+
 int validate(int M, int C, int x_dtype, int r_dtype, int w_dtype, int most = kMaxWidth) {
   if (M < 0 || C < 1 || C > most) return GDN2_ERR_SHAPE;
   if (x_dtype != GDN2_F32 && x_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
@@ -433,7 +441,7 @@ hipError_t launch_fwd(hipStream_t st, const NormArgs& a, bool vec) {
   by_width<MODE == kQuant>(a.C, [&](auto t, auto n) {
     constexpr int TPR = decltype(t)::value, NCH = decltype(n)::value;
     constexpr int NT = kNT<TPR>, ROWS = NT / TPR;
-    const dim3 grid((unsigned)(((long long)a.M + ROWS - 1) / ROWS)), block(NT);
+    const dim3 grid(grid_of(((long long)a.M + ROWS - 1) / ROWS)), block(NT);
     if (vec)
       hipLaunchKernelGGL((norm_fwd<TX, TR, MODE, TPR, NCH, true>), grid, block, 0, st, a);
     else
@@ -541,17 +549,16 @@ int gdn2_dequantize_int8(void* stream, int M, int C, int out_dtype, const void* 
                          long long q_stride, const float* scale, void* out) {
   int rc = validate(M, 1, out_dtype, out_dtype, GDN2_F32);
   if (rc) return rc;
-  if (C < 1) return GDN2_ERR_SHAPE;
+  if (C < 1 || C > 0x7fffffff - 8) return GDN2_ERR_SHAPE;
   if (M == 0) return GDN2_OK;
   const long long n = (long long)M * ((C + 7ll) / 8);
-  if ((n + 255) / 256 > 0x7fffffffll) return GDN2_ERR_SHAPE;
   bool vec = C % 8 == 0, s_vec = true;
   if ((rc = check(out, out_dtype, C, false, &vec)) ||
       (rc = check(scale, GDN2_F32, 0, false, &s_vec)))
     return rc;
   if (!q) return GDN2_ERR_NULL;
   if ((uintptr_t)q % 8 || q_stride % 8) vec = false;
-  const dim3 grid((unsigned)((n + 255) / 256)), block(256);
+  const dim3 grid(grid_of((n + 255) / 256)), block(256);
   hipStream_t st = (hipStream_t)stream;
 #define GDN2_DQ(T, VEC)                                                                   \
   hipLaunchKernelGGL((dequantize<T, VEC>), grid, block, 0, st, (const signed char*)q,     \

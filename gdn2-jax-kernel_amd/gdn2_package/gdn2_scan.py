@@ -7,8 +7,8 @@
 
 The recurrent layer that hybrid stacks put between matrix-state (GDN-2) layers;
 ``g`` is the log decay in GDN-2's convention and must not be positive in use (the
-sums of g over any run of tokens have to stay below 88).  ``g = -inf`` at a token
-starts a new sequence there: nothing of what came before, NaN included, enters
+sums of g over any run of tokens have to stay below 88).  ``g = -inf`` at a token (or the
+type's lowest value, as masks have it) starts a new sequence there: nothing of what came before, NaN included, enters
 it, and no gradient leaves it.  No counterpart in the reference.
 
 Arithmetic is float32.  x and b are float32 or bfloat16 (mixed or other types are

@@ -342,9 +342,10 @@ int gdn2_bwd_reverse_cumsum(void* stream, long long tiles, int BT, int D, const 
  * flattened):
  *   h_t = e^{g_t} h_{t-1} + b_t x_t,   out_t = h_t,   h_final = h_T.
  * No counterpart in the reference.  g is the log decay, as GDN-2's; the sums of g
- * over any run of tokens must stay below 88 (g <= 0 in use).  g_t = -inf starts
- * anew: h_t = b_t x_t whatever h_{t-1} holds, NaN included, and no gradient
- * passes -- the sequences of a packed batch.  b may be NULL (all ones).  Float32
+ * over any run of tokens must stay below 88 (g <= 0 in use).  g_t = -inf (or below
+ * -2.3e38, as a mask of the type's lowest value) starts anew: h_t = b_t x_t whatever
+ * h_{t-1} holds, NaN included, and no gradient passes -- the sequences of a packed
+ * batch.  b may be NULL (all ones).  Float32
  * arithmetic; in_dtype (GDN2_F32, GDN2_BF16) is x's, b's, out's and dout's and
  * that of their gradients, g_dtype (GDN2_F32, or GDN2_BF16 with bfloat16 inputs)
  * g's and dg's; states and their gradients are float32 (B,C).
@@ -430,7 +431,8 @@ int gdn2_dequantize_int8(void* stream, int M, int C, int out_dtype, const void* 
 
 /* out[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n] (bias float32 or
  * NULL), out (M,N) dense of out_dtype; x (M,K) and w (N,K) signed 8-bit integers, sums
- * exact in 32 bits (1 <= K <= 131071).  x and w are 16-byte aligned, their rows *_stride
+ * exact in 32 bits (1 <= K <= 131071; N <= 2^26, and M N in 128 x 128 tiles at most
+ * 2^23 of them).  x and w are 16-byte aligned, their rows *_stride
  * bytes apart, a multiple of 16 and at least K rounded up to one: the bytes between
  * are read and count for nothing. */
 int gdn2_int8_matmul(void* stream, int M, int N, int K, int out_dtype, const void* x,

@@ -204,6 +204,7 @@ def test_fresh_starts(dev, T, C):
     (x, g, b, h0), _ = inputs(1, T, C, torch.float32, torch.float32, dev, T)
     cuts = [0, 1, 2, 130, 255, 256, 257, 400, T]
     g[:, cuts[1:-1]] = -torch.inf
+    g[:, cuts[2]] = torch.finfo(torch.float32).min      # masks' lowest value: as -inf
     x[:, 131:140] = torch.nan
     x[:, 200, 0] = torch.inf
     leaf = [t.clone().requires_grad_() for t in (x, g, b, h0)]
@@ -309,6 +310,18 @@ def test_step(dev, shape, dtype, gdtype):
     assert same.data_ptr() == h.data_ptr() and torch.equal(h, new) and torch.equal(out, out2)
     out3, new3 = gp.gdn2_gated_scan_step(x, g, b)
     check(new3, xn * bn, np.abs(xn * bn))
+
+
+def test_step_beyond_a_grid(dev):
+    """More values than the launch has threads."""
+    import gdn2_package as gp
+    n = 65536 * 1024 + 4000
+    x, h = torch.randn(n, device=dev).bfloat16(), torch.randn(n, device=dev)
+    g = -torch.rand(n, device=dev).bfloat16()
+    out, new = gp.gdn2_gated_scan_step(x, g, state=h)
+    for part in (slice(0, 5000), slice(n - 9000, n)):
+        a, b = gp.gdn2_gated_scan_step(x[part], g[part], state=h[part])
+        assert torch.equal(out[part], a) and torch.equal(new[part], b)
 
 
 def test_prefix_then_steps_equal_the_scan(dev):

@@ -161,6 +161,25 @@ def test_strided_rows_shapes_and_zero_rows(dev):
     assert torch.equal(wl.grad, torch.zeros_like(wl))
 
 
+@pytest.mark.parametrize("M,C", [(270000, 16), (66000, 1100)])
+def test_more_rows_than_a_grid(dev, M, C):
+    """Workgroups that take a row (or four) after another: the same as the rows alone."""
+    import gdn2_package as gp
+    x, r, w, _, _ = make(M, C, TYPES[1], dev, 1)
+    cut = 65536 * (4 if C <= 1024 else 1) - 3
+    for f in (gp.gdn2_rms_norm, gp.gdn2_rms_norm_int8):
+        whole = f(x, w, residual=r)
+        for part in (slice(0, 1000), slice(cut, None)):
+            for a, b in zip(whole, f(x[part], w, residual=r[part])):
+                assert torch.equal(a[part], b)
+    q, s = gp.gdn2_quantize_int8(x)
+    back = gp.gdn2_dequantize_int8(q, s)
+    for part in (slice(0, 1000), slice(cut, None)):
+        qp, sp = gp.gdn2_quantize_int8(x[part])
+        assert torch.equal(q[part], qp) and torch.equal(s[part], sp)
+        assert torch.equal(back[part], gp.gdn2_dequantize_int8(qp, sp))
+
+
 def test_other_types(dev):
     import gdn2_package as gp
     x, r, w, dy, dh = make(5, 48, TYPES[0], dev, 9)

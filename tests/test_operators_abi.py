@@ -129,6 +129,7 @@ def test_int8_refusals():
     assert mm(ldx=40) == _lib.ERR_SHAPE and mm(ldw=32) == _lib.ERR_SHAPE
     assert mm(M=BIG) == _lib.ERR_SHAPE and mm(N=BIG) == _lib.ERR_SHAPE
     assert mm(M=1 << 30, N=1 << 30) == _lib.ERR_SHAPE
+    assert mm(N=(1 << 26) + 1) == _lib.ERR_SHAPE and mm(M=1 << 24, N=8200) == _lib.ERR_SHAPE
     assert mm(od=4) == _lib.ERR_DTYPE and mm(M=0) == _lib.OK
     for name in ("x", "sx", "w", "sw", "out"):
         assert mm(**{name: None}) == _lib.ERR_NULL, name
@@ -141,7 +142,7 @@ def test_int8_refusals():
     assert q(dt=8) == _lib.ERR_DTYPE and q(x=None) == _lib.ERR_NULL and q(M=0) == _lib.OK
     d = lambda M=4, C=40, dt=F32, qq=P[0], s=P[1], out=P[2]: \
         L.gdn2_dequantize_int8(None, M, C, dt, qq, 48, s, out)
-    assert d(C=0) == _lib.ERR_SHAPE and d(M=BIG, C=BIG) == _lib.ERR_SHAPE
+    assert d(C=0) == _lib.ERR_SHAPE and d(C=BIG) == _lib.ERR_SHAPE
     assert d(qq=None) == _lib.ERR_NULL and d(s=None) == _lib.ERR_NULL
     assert d(dt=5) == _lib.ERR_DTYPE and d(out=P[2] + 2) == _lib.ERR_ALIGN
 
