@@ -75,39 +75,55 @@ def _prepare(x, weight, residual, eps, what):
     return x, weight.contiguous(), residual
 
 
+def _launch_fwd(x, weight, residual, eps, keep):
+    """(y, h, rstd) of x's shape; h None without a residual, rstd of each row if kept."""
+    shape, dev = x.shape, x.device
+    x = _as_rows(x)
+    M, C = x.shape
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    h = rstd = None
+    if residual is not None:
+        residual = _as_rows(residual)
+        h = torch.empty(shape, dtype=residual.dtype, device=dev)
+    if keep:
+        rstd = torch.empty(M, dtype=torch.float32, device=dev)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    rc = _lib.launch(
+        "gdn2_rms_norm", dev, M, C, _dtype_code(x.dtype),
+        _dtype_code(x.dtype if h is None else h.dtype), _dtype_code(weight.dtype), x.data_ptr(),
+        _row_stride(x), ptr(residual), 0 if h is None else _row_stride(residual),
+        weight.data_ptr(), eps, y.data_ptr(), ptr(h), ptr(rstd))
+    if rc:
+        _raise(rc, f"gdn2_rms_norm (M,C)=({M},{C})")
+    return y, h, rstd
+
+
 class _RmsNorm(torch.autograd.Function):
+    # Shapes are dealt with inside, and the wrapper that refuses second derivatives is called only
+    # where they could be asked for: every node and call of a small layer's backward counts.
     @staticmethod
-    def forward(ctx, x, weight, residual, eps, keep):
-        M, C = x.shape
-        dev = x.device
-        y = torch.empty((M, C), dtype=x.dtype, device=dev)
-        h = None if residual is None else torch.empty((M, C), dtype=residual.dtype, device=dev)
-        rstd = torch.empty(M, dtype=torch.float32, device=dev) if keep else None
-        ptr = lambda t: None if t is None else t.data_ptr()
-        rc = _lib.launch(
-            "gdn2_rms_norm", dev, M, C, _dtype_code(x.dtype),
-            _dtype_code(x.dtype if h is None else h.dtype), _dtype_code(weight.dtype),
-            x.data_ptr(), _row_stride(x), ptr(residual), 0 if h is None else _row_stride(residual),
-            weight.data_ptr(), eps, y.data_ptr(), ptr(h), ptr(rstd))
-        if rc:
-            _raise(rc, f"gdn2_rms_norm (M,C)=({M},{C})")
-        if keep:
-            ctx.save_for_backward(x if h is None else h, weight, rstd)
-            ctx.x_dtype, ctx.has_residual = x.dtype, h is not None
-            ctx.set_materialize_grads(False)
+    def forward(ctx, x, weight, residual, eps):
+        y, h, rstd = _launch_fwd(x, weight, residual, eps, True)
+        ctx.save_for_backward(x if h is None else h, weight, rstd)
+        ctx.x_dtype, ctx.has_residual = x.dtype, h is not None
+        ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dh=None):
+        grads = _RmsNorm._grads
+        return (once_differentiable(grads) if torch.is_grad_enabled() else grads)(ctx, dy, dh)
+
+    @staticmethod
+    def _grads(ctx, dy, dh):
         h, weight, rstd = ctx.saved_tensors
-        M, C = h.shape
-        dev, L = h.device, _lib.lib()
+        shape, dev, L = h.shape, h.device, _lib.lib()
+        M, C = rstd.shape[0], shape[-1]
         h = h.contiguous()
         dy = None if dy is None else _as(dy, ctx.x_dtype).contiguous()
         dh = None if dh is None else _as(dh, h.dtype).contiguous()
-        dx = torch.empty((M, C), dtype=ctx.x_dtype, device=dev)
-        dr = torch.empty((M, C), dtype=h.dtype, device=dev) \
+        dx = torch.empty(shape, dtype=ctx.x_dtype, device=dev)
+        dr = torch.empty(shape, dtype=h.dtype, device=dev) \
             if ctx.has_residual and h.dtype != ctx.x_dtype else None
         dw = torch.empty(C, dtype=weight.dtype, device=dev)
         nbytes = L.gdn2_rms_norm_bwd_workspace_bytes(M, C)
@@ -119,7 +135,7 @@ class _RmsNorm(torch.autograd.Function):
             ptr(dh), dx.data_ptr(), ptr(dr), dw.data_ptr(), ws.data_ptr(), nbytes)
         if rc:
             _raise(rc, f"gdn2_rms_norm_bwd (M,C)=({M},{C})")
-        return dx, dw, (dx if dr is None else dr) if ctx.has_residual else None, None, None
+        return dx, dw, (dx if dr is None else dr) if ctx.has_residual else None, None
 
 
 def gdn2_rms_norm(x, weight, residual=None, eps=1e-6):
@@ -129,21 +145,15 @@ def gdn2_rms_norm(x, weight, residual=None, eps=1e-6):
     h the residual's.  Differentiable in x, weight and residual, through y and h.  Shapes
     and types are checked before any launch (GDN2ShapeError, GDN2Error)."""
     what = "gdn2_rms_norm"
-    shape, out_dt, h_dt = x.shape if isinstance(x, torch.Tensor) else None, None, None
-    xs, ws, rs = _prepare(x, weight, residual, eps, what)
-    out_dt, h_dt = x.dtype, None if residual is None else residual.dtype
-    rows = _as_rows(xs)
-    r_rows = None if rs is None else _as_rows(rs)
-    if torch.is_grad_enabled() and (xs.requires_grad or ws.requires_grad or
+    xs, w, rs = _prepare(x, weight, residual, eps, what)
+    if torch.is_grad_enabled() and (xs.requires_grad or w.requires_grad or
                                     (rs is not None and rs.requires_grad)):
-        res = _RmsNorm.apply(rows, ws, r_rows, float(eps), True)
+        res = _RmsNorm.apply(xs, w, rs, float(eps))
+        y, h = (res, None) if rs is None else res
     else:
-        res = _RmsNorm.forward(None, rows, ws, r_rows, float(eps), False)
-    y, h = (res, None) if rs is None else res
-    y = y.view(shape)
-    if y.dtype != out_dt:
-        y = y.to(out_dt)
+        y, h, _ = _launch_fwd(xs, w, rs, float(eps), False)
+    if y.dtype != x.dtype:
+        y = y.to(x.dtype)
     if h is None:
         return y, x
-    h = h.view(shape)
-    return y, h if h.dtype == h_dt else h.to(h_dt)
+    return y, h if h.dtype == residual.dtype else h.to(residual.dtype)

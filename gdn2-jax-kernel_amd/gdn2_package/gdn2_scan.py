@@ -7,9 +7,10 @@
 
 The recurrent layer that hybrid stacks put between matrix-state (GDN-2) layers;
 ``g`` is the log decay in GDN-2's convention and must not be positive in use (the
-sums of g over any run of tokens have to stay below 88).  ``g = -inf`` at a token (or the
-type's lowest value, as masks have it) starts a new sequence there: nothing of what came before, NaN included, enters
-it, and no gradient leaves it.  No counterpart in the reference.
+sums of g over any run of tokens have to stay below 88).  ``g = -inf`` at a token (or
+below -2.3e38, as masks of float32's or bfloat16's lowest value are) starts a new
+sequence there: nothing of what came before, NaN included, enters it, and no gradient
+leaves it.  No counterpart in the reference.
 
 Arithmetic is float32.  x and b are float32 or bfloat16 (mixed or other types are
 widened to float32), g float32 (or bfloat16 with bfloat16 inputs); ``out`` has x's
@@ -64,26 +65,35 @@ def _state_in(h, shape, device, what, name):
 
 
 def _rows(x):
-    """(pointer, strides) of a (B,T,C) tensor, copied where its channels are apart.
-    The copy is returned too, to outlive the launch."""
+    """(pointer, strides) of a (B,T,C) or (B,T,H,D) tensor, copied where its channels are
+    apart.  The copy is returned too, to outlive the launch."""
     if x.is_contiguous():
         return x, x.data_ptr(), None
+    if x.dim() == 4:
+        x = x.reshape(*x.shape[:2], x.shape[2] * x.shape[3])
     if x.stride(2) != 1 and x.shape[2] != 1:
         x = x.contiguous()
         return x, x.data_ptr(), None
     return x, x.data_ptr(), _Strides(x.stride(0), x.stride(1))
 
 
+def _sizes(x):
+    """(shape, B, T, C)"""
+    s = x.shape
+    return s, s[0], s[1], s[2] if len(s) == 3 else s[2] * s[3]
+
+
 def _launch_fwd(x, g, b, h0, keep):
-    B, T, C = x.shape
+    shape, B, T, C = _sizes(x)
+    state = (B, *shape[2:])
     dev, L, code = x.device, _lib.lib(), _dtype_code(x.dtype)
     x, px, sx = _rows(x)
     g, pg, sg = _rows(g)
     pb = sb = None
     if b is not None:
         b, pb, sb = _rows(b)
-    out = torch.empty((B, T, C), dtype=x.dtype, device=dev)
-    h_final = torch.empty((B, C), dtype=torch.float32, device=dev)
+    out = torch.empty(shape, dtype=x.dtype, device=dev)
+    h_final = torch.empty(state, dtype=torch.float32, device=dev)
     kept = ws = None
     if keep:
         kept = torch.empty(L.gdn2_gated_scan_kept_bytes(B, T, C, code) // 4, dtype=torch.float32,
@@ -101,6 +111,8 @@ def _launch_fwd(x, g, b, h0, keep):
 
 
 class _GatedScan(torch.autograd.Function):
+    # Shapes are dealt with inside, and the wrapper that refuses second derivatives is called only
+    # where they could be asked for: every node and call of a small layer's backward counts.
     @staticmethod
     def forward(ctx, x, g, b, h0):
         out, h_final, kept = _launch_fwd(x, g, b, h0, True)
@@ -110,10 +122,15 @@ class _GatedScan(torch.autograd.Function):
         return out, h_final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout, dh_final):
+        grads = _GatedScan._grads
+        return (once_differentiable(grads) if torch.is_grad_enabled() else grads)(
+            ctx, dout, dh_final)
+
+    @staticmethod
+    def _grads(ctx, dout, dh_final):
         x, g, b, kept = ctx.saved_tensors
-        B, T, C = x.shape
+        shape, B, T, C = _sizes(x)
         dev, L, code = x.device, _lib.lib(), _dtype_code(x.dtype)
         if T == 0:
             zero = [None if t is None else torch.zeros_like(t) for t in (x, g, b)]
@@ -124,15 +141,15 @@ class _GatedScan(torch.autograd.Function):
         pb = sb = pd = sd = db = dh0 = ws = None
         if b is not None:
             b, pb, sb = _rows(b)
-            db = torch.empty((B, T, C), dtype=b.dtype, device=dev)
+            db = torch.empty(shape, dtype=b.dtype, device=dev)
         if dout is not None:
             dout, pd, sd = _rows(_as(dout, x.dtype))
         if dh_final is not None:
             dh_final = _as(dh_final, torch.float32).contiguous()
-        dx = torch.empty((B, T, C), dtype=x.dtype, device=dev)
-        dg = torch.empty((B, T, C), dtype=g.dtype, device=dev)
+        dx = torch.empty(shape, dtype=x.dtype, device=dev)
+        dg = torch.empty(shape, dtype=g.dtype, device=dev)
         if ctx.has_h0:
-            dh0 = torch.empty((B, C), dtype=torch.float32, device=dev)
+            dh0 = torch.empty((B, *shape[2:]), dtype=torch.float32, device=dev)
         nbytes = L.gdn2_gated_scan_workspace_bytes(B, T, C, code)
         if nbytes:
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -164,11 +181,6 @@ def gdn2_gated_scan(x, g, b=None, h0=None):
         h0 = _state_in(h0, state, x.device, what, "h0")
     out_dt = x.dtype
     x, g, b = _as(x, dt), _as(g, gdt), _as(b, dt)
-    if len(shape) == 4:
-        flat = (*shape[:2], shape[2] * shape[3])
-        x, g = x.reshape(flat), g.reshape(flat)
-        b = None if b is None else b.reshape(flat)
-        h0 = None if h0 is None else h0.reshape(flat[0], flat[2])
     if torch.is_grad_enabled() and (
             x.requires_grad or g.requires_grad or (b is not None and b.requires_grad) or
             (h0 is not None and h0.requires_grad)):
@@ -177,8 +189,6 @@ def gdn2_gated_scan(x, g, b=None, h0=None):
         out, h_final, _ = _launch_fwd(x, g, b, h0, False)
     if out.dtype != out_dt:
         out = out.to(out_dt)
-    if len(shape) == 4:
-        out, h_final = out.view(shape), h_final.view(state)
     return out, h_final
 
 

@@ -419,3 +419,15 @@ def test_refusals(dev):
     first, = torch.autograd.grad(out.sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):   # no second derivative, and it says so
         first.sum().backward()
+
+
+def test_second_derivative_is_refused(dev):
+    """create_graph gives the gradients, and their own gradient raises."""
+    import gdn2_package as gp
+    x = torch.randn(2, 9, 16, device=dev, requires_grad=True)
+    g = -torch.rand(2, 9, 16, device=dev)
+    plain, = torch.autograd.grad(gp.gdn2_gated_scan(x, g)[0].sum(), (x,))
+    dx, = torch.autograd.grad(gp.gdn2_gated_scan(x, g)[0].sum(), (x,), create_graph=True)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), (x,))

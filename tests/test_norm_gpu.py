@@ -207,3 +207,34 @@ def test_refusals(dev):
                 bad()
         with pytest.raises(TypeError):
             f(x, None)
+
+
+def test_second_derivative_is_refused(dev):
+    """create_graph gives the gradients, and their own gradient raises."""
+    import gdn2_package as gp
+    x = torch.randn(5, 64, device=dev, requires_grad=True)
+    w = torch.ones(64, device=dev, requires_grad=True)
+    plain, = torch.autograd.grad(gp.gdn2_rms_norm(x, w)[0].sum(), (x,))
+    dx, = torch.autograd.grad(gp.gdn2_rms_norm(x, w)[0].sum(), (x,), create_graph=True)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), (x,))
+
+
+def test_gradients_of_higher_ranks(dev):
+    """(B, T, H, D) inputs, x a part of a projection: the gradients have the inputs' shapes."""
+    import gdn2_package as gp
+    base = torch.randn(2, 7, 3, 192, device=dev)
+    r = torch.randn(2, 7, 3, 64, device=dev, requires_grad=True)
+    w = (1 + 0.1 * torch.randn(64, device=dev)).requires_grad_()
+    dy, dh = torch.randn(2, 7, 3, 64, device=dev), torch.randn(2, 7, 3, 64, device=dev)
+    got = []
+    for x in (base[..., 64:128], base[..., 64:128].reshape(42, 64)):
+        x = x.detach().requires_grad_()
+        y, h = gp.gdn2_rms_norm(x, w, r.view(x.shape))
+        assert y.shape == h.shape == x.shape
+        grads = torch.autograd.grad((y, h), (x, w, r), (dy.view(x.shape), dh.view(x.shape)))
+        assert grads[0].shape == x.shape
+        got.append(grads)
+    for a, b in zip(*got):
+        assert torch.equal(a.reshape(b.shape), b)
