@@ -114,12 +114,12 @@ def gdn2_dequantize_int8(q, scale, dtype=torch.bfloat16):
 
 
 def _wide_rows(q):
-    """(q, row stride) with rows at multiples of 16 bytes that are readable up to the next
-    multiple of 16; q itself where it is laid out so."""
+    """(q, row stride) with rows at multiples of 16 bytes, at most 16 MiB apart, that are
+    readable up to the next multiple of 16; q itself where it is laid out so."""
     M, K = q.shape
     ld = q.stride(0) if M > 1 else (K + 15) // 16 * 16
     end = (K + 15) // 16 * 16
-    if ld % 16 == 0 and ld >= end and q.data_ptr() % 16 == 0 and (
+    if ld % 16 == 0 and end <= ld <= 1 << 24 and q.data_ptr() % 16 == 0 and (
             K == end or M == 0 or
             q.untyped_storage().nbytes() >= q.storage_offset() + (M - 1) * ld + end):
         return q, ld

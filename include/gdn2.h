@@ -433,8 +433,8 @@ int gdn2_dequantize_int8(void* stream, int M, int C, int out_dtype, const void* 
  * NULL), out (M,N) dense of out_dtype; x (M,K) and w (N,K) signed 8-bit integers, sums
  * exact in 32 bits (1 <= K <= 131071; N <= 2^26, and M N in 128 x 128 tiles at most
  * 2^23 of them).  x and w are 16-byte aligned, their rows *_stride
- * bytes apart, a multiple of 16 and at least K rounded up to one: the bytes between
- * are read and count for nothing. */
+ * bytes apart, a multiple of 16, at least K rounded up to one and at most 2^24: the
+ * bytes between K and its multiple are read and count for nothing. */
 int gdn2_int8_matmul(void* stream, int M, int N, int K, int out_dtype, const void* x,
                      long long x_stride, const float* x_scale, const void* w,
                      long long w_stride, const float* w_scale, const float* bias, void* out);

@@ -182,6 +182,23 @@ def test_layouts(dev):
     assert torch.equal(gp.gdn2_int8_matmul(q, sx[:1].expand(M), w, sw, out_dtype=F32)[0], want[0])
 
 
+@pytest.mark.parametrize("M,N", [(40, 2100), (200, 13001)])
+def test_rows_far_apart(dev, M, N):
+    """Row strides up to the largest that is read in place, and past it (copied); results whose
+    rows start anywhere."""
+    import gdn2_package as gp
+    K = 100
+    q, sx, w, sw, bias = operands(M, N, K, dev, 2)
+    want = gp.gdn2_int8_matmul(q, sx, w, sw, bias, out_dtype=BF16)
+    check_product(gp.gdn2_int8_matmul(q, sx, w, sw, out_dtype=F32), *product(q, sx, w, sw))
+    for stride in (1 << 24, (1 << 24) + 16):
+        far = torch.empty((M - 1) * stride + 112, dtype=torch.int8, device=dev)
+        rows = far.as_strided((M, K), (stride, 1))
+        rows.copy_(q)
+        assert torch.equal(gp.gdn2_int8_matmul(rows, sx, w, sw, bias, out_dtype=BF16), want)
+        del far, rows
+
+
 def test_the_chain_of_a_layer(dev):
     """norm -> 8 bits -> product approximates the float layer within the steps' size."""
     import gdn2_package as gp

@@ -129,6 +129,7 @@ def test_int8_refusals():
     assert mm(ldx=40) == _lib.ERR_SHAPE and mm(ldw=32) == _lib.ERR_SHAPE
     assert mm(M=BIG) == _lib.ERR_SHAPE and mm(N=BIG) == _lib.ERR_SHAPE
     assert mm(M=1 << 30, N=1 << 30) == _lib.ERR_SHAPE
+    assert mm(ldx=(1 << 24) + 16) == _lib.ERR_SHAPE and mm(ldw=(1 << 24) + 16) == _lib.ERR_SHAPE
     assert mm(N=(1 << 26) + 1) == _lib.ERR_SHAPE and mm(M=1 << 24, N=8200) == _lib.ERR_SHAPE
     assert mm(od=4) == _lib.ERR_DTYPE and mm(M=0) == _lib.OK
     for name in ("x", "sx", "w", "sw", "out"):
