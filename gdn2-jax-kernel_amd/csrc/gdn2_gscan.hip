@@ -21,7 +21,7 @@
 // a line, keep the address path busy without moving much (8 x 8192 x 768 bfloat16, walked
 // in tiles of 16, 32 and 64 channels, which leave ever more CUs without work: 201, 150, 191 us;
 // in steps at once 175, 125, 115).  Copies reach 5.16 TB/s on this card; these reach, forward
-// and backward: 8 x 8192 x 768 bfloat16 4.4 and 4.6 TB/s, 2 x 16384 x 2048 bfloat16 4.7 and 5.0,
+// and backward: 8 x 8192 x 768 bfloat16 4.4 and 5.0 TB/s, 2 x 16384 x 2048 bfloat16 4.7 and 5.0,
 // 1 x 131072 x 1024 float32 without a gate forward 5.2.
 //
 // The backward pass needs the state before every token: the forward pass keeps the state
