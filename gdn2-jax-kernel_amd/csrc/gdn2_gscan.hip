@@ -795,6 +795,11 @@ int check_f32(const void* p, bool optional, bool* vec) {
   return GDN2_OK;
 }
 
+// Words of 64 bits, cleared 16 bytes at a time.
+int check_ws(const void* p, size_t need) {
+  return !need ? GDN2_OK : !p ? GDN2_ERR_NULL : (uintptr_t)p % 16 ? GDN2_ERR_ALIGN : GDN2_OK;
+}
+
 template <typename TX, typename TG, bool GATE, int V, int CT>
 void launch_tile(hipStream_t st, const ScanArgs& a, bool bwd) {
   const dim3 grid(8u * (unsigned)a.chunk), block(8 * CT);
@@ -921,7 +926,7 @@ int gdn2_gated_scan_fwd(void* stream, int B, int T, int C, int in_dtype, int g_d
       return rc;
     if (b && (rc = check_rows(a.b, in_dtype, &vec))) return rc;
     const size_t need = gdn2_gated_scan_workspace_bytes(B, T, C, in_dtype);
-    if ((rc = check_f32(need ? ws : nullptr, need == 0, &vec))) return rc;
+    if ((rc = check_ws(ws, need))) return rc;
     if (ws_bytes < need) return GDN2_ERR_WORKSPACE;
   }
   if ((rc = check_f32(h_final, false, &vec)) || (rc = check_f32(h0, true, &vec)) ||
@@ -977,7 +982,7 @@ int gdn2_gated_scan_bwd(void* stream, int B, int T, int C, int in_dtype, int g_d
       (rc = check_f32(dh0, true, &vec)))
     return rc;
   const size_t need = gdn2_gated_scan_workspace_bytes(B, T, C, in_dtype);
-  if ((rc = check_f32(need ? ws : nullptr, need == 0, &vec))) return rc;
+  if ((rc = check_ws(ws, need))) return rc;
   if (ws_bytes < need) return GDN2_ERR_WORKSPACE;
   return launch_scan((hipStream_t)stream, a, in_dtype, g_dtype, true, vec);
 }

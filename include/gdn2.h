@@ -352,7 +352,8 @@ int gdn2_bwd_reverse_cumsum(void* stream, long long tiles, int BT, int D, const 
  * x, g, b and dout may be strided: *_strides points to two host integers, the
  * elements from one batch entry and one token to the next (NULL: dense); the
  * channels are contiguous.  out, dx, dg, db are dense.  Pointers are aligned to
- * their elements; 4-element alignment of pointers, strides and C is faster.
+ * their elements, the workspace to 16 bytes; 4-element alignment of pointers, strides
+ * and C is faster.
  * gdn2_set_launch_events does not reach the entry points from here on. */
 
 /* Bytes of the states kept for the backward (float32, one for every 128 to 512

@@ -38,6 +38,7 @@ def test_scan_refusals(f):
     assert f(b=P[2] + 2) == _lib.ERR_ALIGN
     assert f(dt=BF16, b=P[2] + 1) == _lib.ERR_ALIGN
     assert f(ws=P[7] + 2) == _lib.ERR_ALIGN and f(kept=P[6] + 2) == _lib.ERR_ALIGN
+    assert f(ws=P[7] + 8) == _lib.ERR_ALIGN     # 64-bit words, cleared 16 bytes at a time
 
 
 def test_scan_refusals_by_direction():
