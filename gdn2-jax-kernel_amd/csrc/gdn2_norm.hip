@@ -13,8 +13,8 @@
 // All of these are bound by memory traffic: a row is read once into registers (8 values
 // a thread and chunk, 16-byte accesses), reduced over its 64 to 1024 threads and
 // written from the registers.  Sums and the norm's factors are float32.  Copies reach 5.16 TB/s
-// on this card; with a residual, bfloat16: norm of 65536 x 768 75 us (5.4 TB/s), 16384 x 4096
-// 97 (5.5), 4096 x 8192 41 (6.5); in 8 bits 66 (5.3), 87 (5.4), 37 (6.4).
+// on this card; with a residual, bfloat16: norm of 65536 x 768 73 us (5.5 TB/s), 16384 x 4096
+// 95 (5.7), 4096 x 8192 41 (6.5); in 8 bits 66 (5.3), 86 (5.5), 37 (6.4).
 #include "gdn2.h"
 #include "gdn2_common.h"
 
@@ -37,33 +37,60 @@ struct NormArgs {
   int M, C, w_bf16;
 };
 
-// 8 values at column c of a row of C.  VEC: the row is aligned and C a multiple of 8.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c, int C, float (&f)[8]) {
-  if constexpr (VEC) {
-    if (c < C) {
-      load_f<8>(row + c, f);
+// 8 values at column c of a row of C, as they are stored.  VEC: the row is aligned to 16 bytes
+// and C a multiple of 8; else the same accesses start at any value, and only a row's last piece
+// goes value by value (65536 x 767 bfloat16, norm, in 8 bits, backward: 92, 82, 135 us; all value
+// by value 291, 249, 197).
+template <typename V, typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+  V v;
+};
+template <typename V, typename T, bool VEC>
+__device__ __forceinline__ V take(const T* p) {
+  if constexpr (VEC)
+    return *reinterpret_cast<const V*>(p);
+  else
+    return reinterpret_cast<const Loose<V, T>*>(p)->v;
+}
+template <typename V, typename T, bool VEC>
+__device__ __forceinline__ void give(T* p, const V& v) {
+  if constexpr (VEC)
+    *reinterpret_cast<V*>(p) = v;
+  else
+    reinterpret_cast<Loose<V, T>*>(p)->v = v;
+}
+template <typename T, bool VEC> struct Raw8 {
+  using V = std::conditional_t<sizeof(T) == 4, f32x4, bf16x8>;
+  static constexpr int N = 16 / sizeof(T), P = 8 / N;   // values of an access, accesses
+  V v[P];
+  __device__ __forceinline__ void load(const T* row, int c, int C) {
+    if (VEC ? c < C : c + 8 <= C) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) v[i] = take<V, T, VEC>(row + c + i * N);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+      for (int e = 0; e < 8; ++e) v[e / N][e % N] = !VEC && c + e < C ? row[c + e] : (T)0.f;
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = c + e < C ? to_f(row[c + e]) : 0.f;
   }
+  __device__ __forceinline__ float operator[](int e) const { return (float)v[e / N][e % N]; }
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int c, int C, float (&f)[8]) {
+  Raw8<T, VEC> r;
+  r.load(row, c, C);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = r[e];
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* row, int c, int C, const float (&f)[8]) {
-  if constexpr (VEC) {
-    if (c < C) {
-      if constexpr (sizeof(T) == 4) {
-        store4(row + c, f32x4{f[0], f[1], f[2], f[3]});
-        store4(row + c + 4, f32x4{f[4], f[5], f[6], f[7]});
-      } else {
-        *reinterpret_cast<bf16x8*>(row + c) = make_op(f, (bf16x8*)nullptr);
-      }
+  if (VEC ? c < C : c + 8 <= C) {
+    if constexpr (sizeof(T) == 4) {
+      give<f32x4, T, VEC>(row + c, f32x4{f[0], f[1], f[2], f[3]});
+      give<f32x4, T, VEC>(row + c + 4, f32x4{f[4], f[5], f[6], f[7]});
+    } else {
+      give<bf16x8, T, VEC>(row + c, make_op(f, (bf16x8*)nullptr));
     }
-  } else {
+  } else if constexpr (!VEC) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (c + e < C) row[c + e] = from_f<T>(f[e]);
@@ -205,8 +232,8 @@ __global__ void __launch_bounds__(256) dequantize(const signed char* q, long lon
     const int c = (int)(i - row * per) * 8;
     const float s = scale[row];
     float f[8];
-    if constexpr (VEC) {
-      const uint2 p = *reinterpret_cast<const uint2*>(q + row * ldq + c);
+    if (VEC || c + 8 <= C) {
+      const uint2 p = take<uint2, signed char, VEC>(q + row * ldq + c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = (float)(signed char)((e < 4 ? p.x : p.y) >> (8 * (e % 4)));
     } else {
@@ -225,32 +252,6 @@ struct NormBwdArgs {
   void *dx, *dr;                 // dr: null where the residual's gradient is dx itself
   float* part;                   // (workgroups, C)
   int M, C, w_bf16, groups;      // groups of TPR threads in the launch
-};
-
-// 8 values at column c as they are stored, so that the next row's wait in few registers.
-template <typename T, bool VEC> struct Raw8 {
-  T v[8];
-  __device__ __forceinline__ void load(const T* row, int c, int C) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < C ? row[c + e] : (T)0.f;
-  }
-  __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
-};
-template <> struct Raw8<float, true> {
-  f32x4 v[2];
-  __device__ __forceinline__ void load(const float* row, int c, int C) {
-    v[0] = c < C ? load4f(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
-    v[1] = c < C ? load4f(row + c + 4) : f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  __device__ __forceinline__ float operator[](int e) const { return v[e / 4][e % 4]; }
-};
-template <> struct Raw8<bf16_t, true> {
-  bf16x8 v;
-  __device__ __forceinline__ void load(const bf16_t* row, int c, int C) {
-    const bf16_t z = (bf16_t)0.f;
-    v = c < C ? *reinterpret_cast<const bf16x8*>(row + c) : bf16x8{z, z, z, z, z, z, z, z};
-  }
-  __device__ __forceinline__ float operator[](int e) const { return (float)v[e]; }
 };
 
 // A group of TPR threads takes the rows group, group + groups, ...; dw gathers in its
