@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(8 * CT) gscan_bwd(ScanArgs a) {
 }
 
 // ---- The axis cut into its steps, all in one launch --------------------------------
-// A workgroup takes 128 tokens of 64 channels (or 256 of 32).  It publishes its
+// A workgroup takes 128 tokens of 64 channels (or 256 of 32, 512 of 16).  It publishes its
 // composition as soon as it has it, finds the state that enters it from the steps before,
 // and publishes the one that leaves it.  Steps are dealt by a ticket, the earliest of all
 // tiles first (or, each tile with tickets of its own, the earliest of the tile): a workgroup
@@ -762,8 +762,11 @@ Split split(int B, int T, int C, int in_dtype) {
   // step to step (about 1.1 us for a window of them) and narrower tiles have longer steps: bfloat16
   // forward and backward 8 x 8192 x 768 in tiles of 64 and 32 channels 115 + 196 and 125 + 215 us,
   // 1 x 65536 x 768 124 + 206 and 128 + 211, 1 x 16384 x 128 27 + 37 and 18 + 26; float32
-  // 8 x 4096 x 768 88 + 147 and 87 + 148, 1 x 32768 x 256 58 + 79 and 40 + 56.
-  cut(true, in_dtype == GDN2_BF16 && (long long)B * C >= 1024 ? 64 : 32);
+  // 8 x 4096 x 768 88 + 147 and 87 + 148, 1 x 32768 x 256 58 + 79 and 40 + 56.  In tiles of 32
+  // and 16 bfloat16 1 x 131072 x 128 95 + 136 and 65 + 113, 1 x 100000 x 77 80 + 105 and 53 + 70,
+  // but 2 x 60000 x 100 59 + 84 and 62 + 97, 1 x 16384 x 128 18.3 + 36.2 and 19.3 + 36.9.
+  const long long all = (long long)B * C;
+  cut(true, all <= 128 && T > 32768 ? 16 : in_dtype == GDN2_BF16 && all >= 1024 ? 64 : 32);
   if (s.blocks * units(s.ct) >= (1ll << 22)) cut(false, 64);   // a grid's threads: 32 bits
   return s;
 }
@@ -833,8 +836,10 @@ void launch_width(hipStream_t st, const ScanArgs& a, bool bwd, const Split& s) {
   if (s.chain) {
     if (s.ct == 64)
       launch_chain<TX, TG, GATE, V, 64>(st, a, bwd, s.blocks);
-    else
+    else if (s.ct == 32)
       launch_chain<TX, TG, GATE, V, 32>(st, a, bwd, s.blocks);
+    else
+      launch_chain<TX, TG, GATE, V, 16>(st, a, bwd, s.blocks);
   } else if (s.ct == 64) {
     launch_tile<TX, TG, GATE, V, 64>(st, a, bwd);
   } else {

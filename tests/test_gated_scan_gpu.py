@@ -118,7 +118,8 @@ def test_backward(dev, B, T, C, dtype, gdtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,T,C", [(1, 2048, 16), (1, 5000, 20), (1, 4097, 7), (2, 9001, 40),
                                    (1, 513, 64), (3, 1025, 200), (2, 1537, 192), (1, 1500, 999),
-                                   (2, 700, 1000), (17, 640, 100), (1, 2049, 1024)])
+                                   (2, 700, 1000), (17, 640, 100), (1, 2049, 1024),
+                                   (1, 33001, 77), (2, 32769, 64)])
 def test_steps_at_once(dev, B, T, C, dtype):
     """Long axes: every step has its workgroup, tiles of 16, 32 and 64 channels."""
     import gdn2_package as gp
@@ -138,7 +139,7 @@ def test_steps_at_once(dev, B, T, C, dtype):
         check(t, *grads[n], n=2)
 
 
-@pytest.mark.parametrize("B,T,C", [(1, 20000, 128), (2, 6000, 300), (4, 2000, 1024)])
+@pytest.mark.parametrize("B,T,C", [(1, 20000, 128), (2, 6000, 300), (4, 2000, 1024), (1, 90000, 100)])
 def test_same_results_every_time(dev, B, T, C):
     """The hand-over from step to step leaves no trace of who was first."""
     import gdn2_package as gp

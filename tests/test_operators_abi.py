@@ -64,6 +64,9 @@ def test_scan_sizes():
     assert kept(8, 8192, 768, F32) == 32 * 8 * 768 * 4
     assert ws(8, 8192, 768, F32) == 32 * 8 * 768 * 8 + 8 * 24 * 64
     assert kept(1, 600, 33, BF16) == 3 * 33 * 4
+    # few channels and many tokens: steps of 512 (tiles of 16)
+    assert kept(1, 40000, 100, F32) == 79 * 100 * 4
+    assert ws(1, 40000, 100, F32) == 79 * 100 * 8 + 7 * 64
     assert ws(1, 600, 33, BF16) == (3 * 33 * 8 + 15) // 16 * 16 + 2 * 64
     for bad in ((0, 5, 5, F32), (5, -1, 5, F32), (5, 5, 0, F32), (5, 5, 5, 9)):
         assert kept(*bad) == 0 and ws(*bad) == 0
