@@ -7,7 +7,9 @@
 // A run of tokens maps the state entering it to the one leaving it by h -> e^L h + H
 // with L the sum of its g: two runs compose as (L1 + L2, e^{L2} H1 + H2).  L, not
 // e^L, is carried, so that L = -inf says that the run holds a fresh start, and sums of
-// small decays lose nothing.  Everything is held in float32.
+// small decays lose nothing; the mark stays whatever is added to it (a NaN or +inf in another g
+// of the run would undo it, and let through what a fresh start drops).  Everything is held in
+// float32.
 //
 // A thread takes V neighbouring channels (8- or 16-byte accesses) of 16 / V consecutive tokens:
 // it composes its run in registers, the runs of a wave are composed by lane shuffles and
@@ -64,6 +66,10 @@ constexpr float kNegInf = -__builtin_inff();
 // e^l h + u, or u alone where l = -inf.
 __device__ __forceinline__ float carry_through(float l, float h, float u) {
   return l == kNegInf ? u : fmaf(exp2_(l), h, u);
+}
+// L of two runs together.
+__device__ __forceinline__ float sum_decays(float l0, float l1) {
+  return l0 == kNegInf || l1 == kNegInf ? kNegInf : l0 + l1;
 }
 
 template <typename T, int V> struct Raw;
@@ -156,7 +162,7 @@ __device__ __forceinline__ void wave_compose(float (&L)[V], float (&H)[V], float
       const float h = REV ? __shfl_down(H[c], m) : __shfl_up(H[c], m);
       if (place >= m) {
         H[c] = carry_through(L[c], h, H[c]);
-        L[c] += l;
+        L[c] = sum_decays(L[c], l);
       }
     }
   }
@@ -182,6 +188,7 @@ __device__ __forceinline__ void factors(Factors<V, S>& f, const Run<TX, V, S>& x
                                         const Run<TG, V, S>& g, const RB& b, int t, int T_len) {
 #pragma unroll
   for (int c = 0; c < V; ++c) f.L[c] = f.H[c] = 0.f;
+  bool started[V] = {};
 #pragma unroll
   for (int i = 0; i < S; ++i) {
     const bool real = t + i < T_len;
@@ -198,8 +205,12 @@ __device__ __forceinline__ void factors(Factors<V, S>& f, const Run<TX, V, S>& x
       f.a[i][c] = anew ? -1.f : exp2_(l);
       f.H[c] = fmaf(f.a[i][c], anew ? 0.f : f.H[c], f.u[i][c]);
       f.L[c] += l;
+      started[c] |= anew;
     }
   }
+#pragma unroll
+  for (int c = 0; c < V; ++c)
+    if (started[c]) f.L[c] = kNegInf;
 }
 // a h + u for one token of a run.
 __device__ __forceinline__ float token(float a, float h, float u) {

@@ -432,3 +432,56 @@ def test_second_derivative_is_refused(dev):
     assert torch.equal(dx, plain)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dx.sum(), (x,))
+
+
+# walked in tiles of 16 (4 channels a thread, and one) and 64; steps at once in tiles of 16, 32, 64
+STARTS = [(1, 500, 24), (1, 470, 5), (200, 402, 33), (48, 450, 240), (1, 33000, 64),
+          (1, 33001, 7), (1, 2500, 40), (2, 1300, 77), (1, 1400, 1100), (1, 1201, 1027)]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,C", STARTS)
+def test_no_decay_passes_a_fresh_start(dev, B, T, C, dtype, bad):
+    """NaN and +inf in g: the sequences before and after theirs are what they are alone, states
+    and gradients, wherever in a run, a wave or a step the starts and the bad tokens stand."""
+    import gdn2_package as gp
+    (x, g, b, h0), _ = inputs(B, T, C, dtype, torch.float32, dev, T)
+    # sequences start at `cuts`; bad tokens at one's end, right after its start, at several
+    # places, and all through one that is longer than a step
+    cuts, spoilt = [0, 3, 41, 100, 130, 200, 390], {1: [40], 3: [101], 5: [203, 257, 388]}
+    if T > 1200:
+        cuts += [400, 1030, 1100]
+        spoilt[7] = range(401, 1030)
+    cuts += [T - 5, T]
+    spoilt[len(cuts) - 2] = [T - 3]
+    g[:, cuts[1:-1]] = -torch.inf
+    for tokens in spoilt.values():
+        g[:, list(tokens)] = bad
+    leaf = [t.clone().requires_grad_() for t in (x, g, b, h0)]
+    out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+    dout, dhf = torch.randn_like(out), torch.randn_like(hf)
+    got = torch.autograd.grad((out, hf), leaf, (dout, dhf))
+    for i, (s, e) in enumerate(zip(cuts[:-1], cuts[1:])):
+        if i in spoilt:
+            continue
+        n64 = lambda t: t.detach().double().cpu().numpy()
+        first = n64(h0) if s == 0 else np.zeros((B, C))
+        ref, mag, grads = reference(*(n64(t[:, s:e]) for t in (x, g, b)), first,
+                                    n64(dout[:, s:e]), n64(dhf) if e == T else np.zeros((B, C)))
+        check(out[:, s:e], ref, mag)
+        for n, t in zip(("x", "g", "b"), got):
+            check(t[:, s:e], *grads[n], n=2)
+        if s == 0:
+            check(got[3], *grads["h0"], n=2)
+    assert not torch.isfinite(out[:, 40]).any() and not torch.isfinite(out[:, 389]).any()
+
+
+def test_step_after_a_bad_decay(dev):
+    import gdn2_package as gp
+    x = torch.randn((3, 20), device=dev)
+    for bad in (torch.nan, torch.inf):
+        _, h = gp.gdn2_gated_scan_step(x, torch.full_like(x, bad), state=torch.ones_like(x))
+        assert not torch.isfinite(h).any()
+        out, h = gp.gdn2_gated_scan_step(x, torch.full_like(x, -torch.inf), state=h)
+        assert torch.equal(out, x) and torch.equal(h, x)
