@@ -459,11 +459,13 @@ __device__ __forceinline__ float through(float a, float h, float u) {
   return fmaf(a, a < 0.f ? 0.f : h, u);
 }
 
-// The state that enters step blk (REV: from the right), for one channel a lane; `start` is
-// the one that enters the first.  at: the channel's place; on: it exists.
+// The state that enters step blk (REV: from the right), not the first, for one channel a lane.
+// at: the channel's place; on: it exists.  The first step publishes no composition, only its
+// state, so nothing beyond it is ever looked for, and it alone reads h0 (REV: dh_final), which
+// the last step may overwrite as soon as it has found a state.
 template <bool REV>
 __device__ __forceinline__ float entering(const Chain& ch, size_t n, size_t at, bool on, int blk,
-                                          int blocks, float start) {
+                                          int blocks) {
   while (true) {
     unsigned long long v[kWindow<REV>];
 #pragma unroll
@@ -472,7 +474,7 @@ __device__ __forceinline__ float entering(const Chain& ch, size_t n, size_t at, 
       const bool in = REV ? j < blocks : j >= 0;
       v[d] = __hip_atomic_load(ch.slot + (size_t)(in ? j : blk) * n + at, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT);
-      if (!in || !on) v[d] = pack(kState, start);
+      if (!in || !on) v[d] = pack(kState, 0.f);
     }
     int found = -1;   // the nearest state with nothing missing before it
 #pragma unroll
@@ -489,12 +491,12 @@ __device__ __forceinline__ float entering(const Chain& ch, size_t n, size_t at, 
   }
 }
 
-// One wave, a channel a lane: publish the workgroup's composition, find the entering state,
-// publish the leaving one.  Returns both.
+// One wave, a channel a lane: publish the workgroup's composition, find the entering state
+// (start's, or zero, for the first step), publish the leaving one.  Returns both.
 template <bool REV, int NW, int CT>
 __device__ __forceinline__ void link(const Chain& ch, const Totals<NW, CT>& tot, size_t n,
-                                     size_t at, bool on, int blk, int blocks, float start, int lane,
-                                     float& in, float& out) {
+                                     size_t at, bool on, int blk, int blocks, const float* start,
+                                     int lane, float& in, float& out) {
   float A = 1.f, H = 0.f;
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
@@ -508,7 +510,7 @@ __device__ __forceinline__ void link(const Chain& ch, const Totals<NW, CT>& tot,
   const bool first = REV ? blk == blocks - 1 : blk == 0, last = REV ? blk == 0 : blk == blocks - 1;
   unsigned long long* slot = ch.slot + (size_t)blk * n + at;
   if (!last && !first && on) publish(slot, A, H);
-  in = first ? start : entering<REV>(ch, n, at, on, blk, blocks, start);
+  in = !first ? entering<REV>(ch, n, at, on, blk, blocks) : start && on ? start[at] : 0.f;
   out = through(A, in, H);
   if (!last && on) publish(slot, kState, out);
 }
@@ -584,8 +586,7 @@ __global__ void __launch_bounds__(512, 4) chain_fwd(ScanArgs a, Chain ch) {
     const bool on = unit_c < a.C;
     const size_t n = (size_t)a.B * a.C, at = (size_t)w.b * a.C + (on ? unit_c : 0);
     float in, out;
-    link<false, NW, CT>(ch, tot, n, at, on, w.blk, w.blocks, a.h0 && on ? a.h0[at] : 0.f, w.lane, in,
-                        out);
+    link<false, NW, CT>(ch, tot, n, at, on, w.blk, w.blocks, a.h0, w.lane, in, out);
     if (w.lane < CT) s_in[w.lane] = in;
     if (on && a.kept) a.kept[(size_t)w.blk * n + at] = in;
     if (on && w.blk == w.blocks - 1) a.h_final[at] = out;
@@ -658,8 +659,7 @@ __global__ void __launch_bounds__(512, 4) chain_bwd(ScanArgs a, Chain ch) {
     const bool on = unit_c < a.C;
     const size_t n = (size_t)a.B * a.C, at = (size_t)w.b * a.C + (on ? unit_c : 0);
     float in, out;
-    link<true, NW, CT>(ch, rev, n, at, on, w.blk, w.blocks, a.dh_final && on ? a.dh_final[at] : 0.f,
-                       w.lane, in, out);
+    link<true, NW, CT>(ch, rev, n, at, on, w.blk, w.blocks, a.dh_final, w.lane, in, out);
     if (w.lane < CT) s_in[w.lane] = in;
     if (on && w.blk == 0 && a.dh0) a.dh0[at] = out;
   }

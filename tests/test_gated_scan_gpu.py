@@ -485,3 +485,25 @@ def test_step_after_a_bad_decay(dev):
         assert not torch.isfinite(h).any()
         out, h = gp.gdn2_gated_scan_step(x, torch.full_like(x, -torch.inf), state=h)
         assert torch.equal(out, x) and torch.equal(h, x)
+
+
+@pytest.mark.parametrize("B,T,C", [(3, 100, 40), (2, 400, 130), (1, 700, 64), (2, 1500, 33),
+                                   (1, 2049, 1024), (1, 33000, 20)])
+def test_state_updated_in_place(dev, B, T, C):
+    """h_final over h0, as the C interface allows: no step reads h0 once another may have
+    written h_final."""
+    import gdn2_package as gp
+    from gdn2_package import _lib
+    (x, g, b, h0), _ = inputs(B, T, C, torch.float32, torch.float32, dev, C)
+    want, hf = gp.gdn2_gated_scan(x, g, b, h0=h0)
+    nbytes = _lib.lib().gdn2_gated_scan_workspace_bytes(B, T, C, _lib.GDN2_F32)
+    ws, out = torch.empty(nbytes, dtype=torch.uint8, device=dev), torch.empty_like(x)
+    state = h0.clone()
+    for _ in range(4):
+        state.copy_(h0)
+        rc = _lib.launch("gdn2_gated_scan_fwd", x.device, B, T, C, _lib.GDN2_F32, _lib.GDN2_F32,
+                         x.data_ptr(), None, g.data_ptr(), None, b.data_ptr(), None,
+                         state.data_ptr(), out.data_ptr(), state.data_ptr(), None,
+                         ws.data_ptr() if nbytes else None, nbytes)
+        assert rc == _lib.OK
+        assert torch.equal(out, want) and torch.equal(state, hf)
