@@ -32,9 +32,14 @@ def _as(t, dt):
     return t if t.dtype == dt else t.to(dt)
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
 def _as_rows(x):
     """x as (M, C) rows of contiguous values; a copy only where there is no such view."""
     C = x.shape[-1]
+    if C > _INT_MAX or x.numel() > _INT_MAX * C:   # ctypes would cut them to 32 bits
+        raise GDN2ShapeError(f"gdn2: more than 2^31 - 1 rows or columns in {tuple(x.shape)}")
     if x.dim() != 2:
         x = x.reshape(-1, C) if C else x.reshape(0, 0)
     return x if x.stride(1) == 1 or C == 1 else x.contiguous()

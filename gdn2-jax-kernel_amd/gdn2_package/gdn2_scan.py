@@ -176,6 +176,8 @@ def gdn2_gated_scan(x, g, b=None, h0=None):
     shape = x.shape
     if len(shape) not in (3, 4):
         raise GDN2ShapeError(f"{what}: expected (B,T,C) or (B,T,H,D) inputs, got {tuple(shape)}")
+    if max(_sizes(x)[1:]) >= 2 ** 31:   # ctypes would cut them to 32 bits
+        raise GDN2ShapeError(f"{what}: sizes past 2^31 - 1 in {tuple(shape)}")
     state = torch.Size((shape[0], *shape[2:]))
     if h0 is not None:
         h0 = _state_in(h0, state, x.device, what, "h0")

@@ -238,3 +238,24 @@ def test_gradients_of_higher_ranks(dev):
         got.append(grads)
     for a, b in zip(*got):
         assert torch.equal(a.reshape(b.shape), b)
+
+
+def test_sizes_past_32_bits_are_refused(dev):
+    """More rows (or columns, or tokens) than the C interface counts, without memory behind them."""
+    import gdn2_package as gp
+    many = 2 ** 32 + 5
+    x, one = torch.zeros((1, 1), device=dev), torch.ones(1, device=dev)
+    rows, wide = x.expand(many, 1), x.expand(1, many)
+    q, w = x.to(torch.int8), torch.ones((4, 1), dtype=torch.int8, device=dev)
+    for bad in (lambda: gp.gdn2_rms_norm(rows, one), lambda: gp.gdn2_rms_norm_int8(rows, one),
+                lambda: gp.gdn2_rms_norm(rows, one, residual=rows),
+                lambda: gp.gdn2_quantize_int8(rows), lambda: gp.gdn2_quantize_int8(wide),
+                lambda: gp.gdn2_dequantize_int8(q.expand(many, 1), one.expand(many)),
+                lambda: gp.gdn2_dequantize_int8(q.expand(1, many), one),
+                lambda: gp.gdn2_int8_matmul(q.expand(many, 1), one.expand(many), w, one.expand(4)),
+                lambda: gp.gdn2_int8_matmul(q, one, w[:1].expand(many, 1), one.expand(many)),
+                lambda: gp.gdn2_gated_scan(x[None].expand(1, many, 1), x[None].expand(1, many, 1)),
+                lambda: gp.gdn2_gated_scan(x[None].expand(many, 1, 1), x[None].expand(many, 1, 1)),
+                lambda: gp.gdn2_gated_scan(*[x[None, None].expand(1, 2, 2 ** 16, 2 ** 17)] * 2)):
+        with pytest.raises(gp.GDN2ShapeError):
+            bad()

@@ -169,3 +169,18 @@ def test_python_refuses_host_tensors():
               lambda: gp.gdn2_quantize_int8(None), lambda: gp.gdn2_int8_matmul(1, x, x, x)):
         with pytest.raises(TypeError):
             f()
+
+
+def test_rows_past_32_bits_are_refused():
+    """ctypes keeps the low 32 bits of a size: 2^32 + 3 rows would run as 3."""
+    from gdn2_package import GDN2ShapeError, gdn2_norm
+    import torch
+    L = _lib.lib()
+    assert L.gdn2_rms_norm_bwd_workspace_bytes(2 ** 32 + 3, 8) == \
+        L.gdn2_rms_norm_bwd_workspace_bytes(3, 8)
+    one = torch.zeros((1, 1, 1))
+    for shape in ((2 ** 31, 1, 1), (2 ** 17, 2 ** 15 + 1, 1), (1, 1, 2 ** 32 + 8), (0, 3, 2 ** 31)):
+        x = one[:0].expand(shape) if 0 in shape else one.expand(shape)
+        with pytest.raises(GDN2ShapeError):
+            gdn2_norm._as_rows(x)
+    assert gdn2_norm._as_rows(one[0].expand(2 ** 31 - 1, 1)).shape == (2 ** 31 - 1, 1)
