@@ -15,6 +15,7 @@ their values are contiguous.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -33,6 +34,11 @@ def _as(t, dt):
 
 
 _INT_MAX = 2 ** 31 - 1
+
+
+def _forward_mode():
+    """Whether inputs could carry tangents (a level of forward mode is open)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
 
 
 def _as_rows(x):
@@ -147,12 +153,14 @@ def gdn2_rms_norm(x, weight, residual=None, eps=1e-6):
     """(y, h) with h = x + residual (x itself without one) and y = h w / sqrt(mean(h^2) + eps).
 
     x (..., C) with C <= 16384, weight (C,), residual of x's shape.  y has x's shape and type,
-    h the residual's.  Differentiable in x, weight and residual, through y and h.  Shapes
-    and types are checked before any launch (GDN2ShapeError, GDN2Error)."""
+    h the residual's.  Differentiable in x, weight and residual, through y and h, in reverse mode
+    (tangents of forward mode raise NotImplementedError).  Shapes and types are checked before
+    any launch (GDN2ShapeError, GDN2Error)."""
     what = "gdn2_rms_norm"
     xs, w, rs = _prepare(x, weight, residual, eps, what)
-    if torch.is_grad_enabled() and (xs.requires_grad or w.requires_grad or
-                                    (rs is not None and rs.requires_grad)):
+    # tangents go to the autograd function too, which refuses them
+    if _forward_mode() or torch.is_grad_enabled() and (
+            xs.requires_grad or w.requires_grad or (rs is not None and rs.requires_grad)):
         res = _RmsNorm.apply(xs, w, rs, float(eps))
         y, h = (res, None) if rs is None else res
     else:

@@ -26,6 +26,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
+from .gdn2_norm import _forward_mode
 
 _Strides = ctypes.c_longlong * 2
 
@@ -169,7 +170,8 @@ def gdn2_gated_scan(x, g, b=None, h0=None):
     x, g, b: (B,T,C) or (B,T,H,D), one shape; ``b=None`` stands for ones; h0 (B,C) or
     (B,H,D), default zeros.  Returns ``out`` (all h_t, x's shape and type) and
     ``h_final`` (float32, h0's shape).  Differentiable in x, g, b and h0, through out
-    and h_final; gradients come in each input's type.  T may be 0 (h_final = h0).
+    and h_final, in reverse mode (tangents of forward mode raise NotImplementedError); gradients
+    come in each input's type.  T may be 0 (h_final = h0).
     Shapes and types are checked before any launch (GDN2ShapeError, GDN2Error)."""
     what = "gdn2_gated_scan"
     dt, gdt = _types(x, g, b, what)
@@ -183,7 +185,8 @@ def gdn2_gated_scan(x, g, b=None, h0=None):
         h0 = _state_in(h0, state, x.device, what, "h0")
     out_dt = x.dtype
     x, g, b = _as(x, dt), _as(g, gdt), _as(b, dt)
-    if torch.is_grad_enabled() and (
+    # tangents go to the autograd function too, which refuses them
+    if _forward_mode() or torch.is_grad_enabled() and (
             x.requires_grad or g.requires_grad or (b is not None and b.requires_grad) or
             (h0 is not None and h0.requires_grad)):
         out, h_final = _GatedScan.apply(x, g, b, h0)

@@ -507,3 +507,21 @@ def test_state_updated_in_place(dev, B, T, C):
                          ws.data_ptr() if nbytes else None, nbytes)
         assert rc == _lib.OK
         assert torch.equal(out, want) and torch.equal(state, hf)
+
+
+def test_tangents_are_refused(dev):
+    """Forward mode is not there, and no tangent is dropped without a word."""
+    import gdn2_package as gp
+    from torch.autograd import forward_ad
+    x, b = torch.randn(2, 2, 9, 16, device=dev)
+    g, h0 = -torch.rand(2, 9, 16, device=dev), torch.randn(2, 16, device=dev)
+    want = gp.gdn2_gated_scan(x, g, b, h0=h0)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            assert all(torch.equal(a, e) for a, e in zip(gp.gdn2_gated_scan(x, g, b, h0=h0), want))
+            dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+            for call in (lambda: gp.gdn2_gated_scan(dual(x), g), lambda: gp.gdn2_gated_scan(x, dual(g)),
+                         lambda: gp.gdn2_gated_scan(x, g, dual(b)),
+                         lambda: gp.gdn2_gated_scan(x, g, h0=dual(h0))):
+                with pytest.raises(NotImplementedError):
+                    call()

@@ -259,3 +259,20 @@ def test_sizes_past_32_bits_are_refused(dev):
                 lambda: gp.gdn2_gated_scan(*[x[None, None].expand(1, 2, 2 ** 16, 2 ** 17)] * 2)):
         with pytest.raises(gp.GDN2ShapeError):
             bad()
+
+
+def test_tangents_are_refused(dev):
+    """Forward mode is not there, and no tangent is dropped without a word."""
+    import gdn2_package as gp
+    from torch.autograd import forward_ad
+    x, r = torch.randn(2, 5, 64, device=dev)
+    w = torch.ones(64, device=dev)
+    want = gp.gdn2_rms_norm(x, w, residual=r)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            assert all(torch.equal(a, b) for a, b in zip(gp.gdn2_rms_norm(x, w, residual=r), want))
+            dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+            for call in (lambda: gp.gdn2_rms_norm(dual(x), w), lambda: gp.gdn2_rms_norm(x, dual(w)),
+                         lambda: gp.gdn2_rms_norm(x.half(), w, residual=dual(r))):
+                with pytest.raises(NotImplementedError):
+                    call()
