@@ -41,6 +41,16 @@ def _forward_mode():
     return getattr(forward_ad, "_current_level", 0) >= 0
 
 
+def _gradients(grads, ctx, *cotangents):
+    """grads(ctx, *cotangents); where a graph of it is asked for, its results raise if they are
+    differentiated.  once_differentiable sees to that where a cotangent requires a gradient, but
+    the results depend on the inputs too, whatever the cotangents are."""
+    if not torch.is_grad_enabled():
+        return grads(ctx, *cotangents)
+    return once_differentiable(grads)(
+        ctx, *(c if c is None else c.detach().requires_grad_() for c in cotangents))
+
+
 def _as_rows(x):
     """x as (M, C) rows of contiguous values; a copy only where there is no such view."""
     C = x.shape[-1]
@@ -122,8 +132,7 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh=None):
-        grads = _RmsNorm._grads
-        return (once_differentiable(grads) if torch.is_grad_enabled() else grads)(ctx, dy, dh)
+        return _gradients(_RmsNorm._grads, ctx, dy, dh)
 
     @staticmethod
     def _grads(ctx, dy, dh):

@@ -22,11 +22,10 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
-from .gdn2_norm import _forward_mode
+from .gdn2_norm import _forward_mode, _gradients
 
 _Strides = ctypes.c_longlong * 2
 
@@ -124,9 +123,7 @@ class _GatedScan(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, dh_final):
-        grads = _GatedScan._grads
-        return (once_differentiable(grads) if torch.is_grad_enabled() else grads)(
-            ctx, dout, dh_final)
+        return _gradients(_GatedScan._grads, ctx, dout, dh_final)
 
     @staticmethod
     def _grads(ctx, dout, dh_final):

@@ -525,3 +525,20 @@ def test_tangents_are_refused(dev):
                          lambda: gp.gdn2_gated_scan(x, g, h0=dual(h0))):
                 with pytest.raises(NotImplementedError):
                     call()
+
+
+@pytest.mark.parametrize("full", [False, True])
+def test_a_penalty_on_the_gradient_is_refused(dev, full):
+    """A loss that holds its own gradient raises, also where the cotangent was a constant and the
+    rest of the loss could go on without the penalty's part."""
+    import gdn2_package as gp
+    x = torch.randn(2, 9, 16, device=dev, requires_grad=True)
+    g = (-torch.rand(2, 9, 16, device=dev)).requires_grad_()
+    b, h0 = (torch.rand_like(x), torch.randn(2, 16, device=dev)) if full else (None, None)
+    loss = sum(t.sum() for t in gp.gdn2_gated_scan(x, g, b, h0=h0)[:2 if full else 1])
+    dx, dg = torch.autograd.grad(loss, (x, g), create_graph=True)
+    for penalty in (dx.square().sum(), dg.square().sum()):
+        with pytest.raises(RuntimeError):
+            (loss + penalty).backward(retain_graph=True)
+    for got, want in zip(torch.autograd.grad(loss, (x, g)), (dx, dg)):
+        assert torch.equal(got, want)     # without it nothing is in the way

@@ -276,3 +276,20 @@ def test_tangents_are_refused(dev):
                          lambda: gp.gdn2_rms_norm(x.half(), w, residual=dual(r))):
                 with pytest.raises(NotImplementedError):
                     call()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_a_penalty_on_the_gradient_is_refused(dev, residual):
+    """A loss that holds its own gradient raises, also where the cotangent was a constant and the
+    rest of the loss could go on without the penalty's part."""
+    import gdn2_package as gp
+    leaf = [torch.randn(5, 64, device=dev, requires_grad=True) for _ in range(2)]
+    w = torch.ones(64, device=dev, requires_grad=True)
+    y, _ = gp.gdn2_rms_norm(leaf[0], w, residual=leaf[1] if residual else None)
+    loss = y.sum()
+    dx, dw = torch.autograd.grad(loss, (leaf[0], w), create_graph=True)
+    for penalty in (dx.square().sum(), dw.square().sum()):
+        with pytest.raises(RuntimeError):
+            (loss + penalty).backward(retain_graph=True)
+    for got, want in zip(torch.autograd.grad(loss, (leaf[0], w)), (dx, dw)):
+        assert torch.equal(got, want)     # without it nothing is in the way
