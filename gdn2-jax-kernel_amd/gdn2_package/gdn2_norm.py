@@ -2,15 +2,18 @@
 
     y, h = gdn2_rms_norm(x, weight, residual=None, eps=1e-6)        # autograd
 
-h = x + residual, rounded to the residual's type (the residual stream), and
-y = h w / sqrt(mean(h^2) + eps) over the last axis, the norm of h as it is returned.
-Without a residual h is x itself.  ``gdn2_int8.gdn2_rms_norm_int8`` gives y in
-8 bits.  No counterpart in the reference.
+h = x + residual, returned in the residual's type (the residual stream), and
+y = h w / sqrt(mean(h^2) + eps) over the last axis.  Without a residual h is x itself.
+``gdn2_int8.gdn2_rms_norm_int8`` gives y in 8 bits.  No counterpart in the reference.
 
-Float32 arithmetic.  x is float32 or bfloat16 (other types are widened to float32),
-the residual has x's type or is float32 (a bfloat16 residual of a float32 x is
-widened), the weight (C,) is float32 or bfloat16.  Rows may be strided as long as
-their values are contiguous.
+x is float32 or bfloat16, the residual has x's type or is float32, the weight (C,) is
+float32 or bfloat16: then h is rounded to the residual's type first, and y is the norm of
+h as it is returned.  Other types are widened to float32, a bfloat16 residual of a float32
+x too: then y is the norm of the float32 sum, and h is rounded to the residual's type
+only when it is returned.
+
+Float32 arithmetic: squares of values past 1.8e19 overflow, and y is 0 in such a row.
+Rows may be strided as long as their values are contiguous.
 """
 from __future__ import annotations
 

@@ -293,3 +293,33 @@ def test_a_penalty_on_the_gradient_is_refused(dev, residual):
             (loss + penalty).backward(retain_graph=True)
     for got, want in zip(torch.autograd.grad(loss, (leaf[0], w)), (dx, dw)):
         assert torch.equal(got, want)     # without it nothing is in the way
+
+
+@pytest.mark.parametrize("x_dt,r_dt", [(F32, BF16), (torch.float16, BF16), (BF16, torch.float16),
+                                       (torch.float16, torch.float16), (F32, torch.float64)])
+def test_widened_residuals(dev, x_dt, r_dt):
+    """A residual of a type that the kernels do not take: y is the norm of the float32 sum, in 8
+    bits too, and h is that sum rounded to the residual's type."""
+    import gdn2_package as gp
+    x, r, w, _, _ = make(7, 104, (x_dt, r_dt, F32), dev, 4)
+    y, h = gp.gdn2_rms_norm(x, w, residual=r)
+    q, scale, h8 = gp.gdn2_rms_norm_int8(x, w, residual=r)
+    assert y.dtype == x_dt and h.dtype == h8.dtype == r_dt
+    total = x.float() + r.float()
+    assert torch.equal(h, total.to(r_dt)) and torch.equal(h8, h)
+    ref = np64(total) * np64(w) / np.sqrt((np64(total) ** 2).mean(-1, keepdims=True) + 1e-6)
+    if x_dt == F32:
+        close(y, ref, np.abs(ref), 32)
+    want, whole = gp.gdn2_rms_norm(total, w)
+    assert whole is total and torch.equal(y, want.to(x_dt))
+    want = gp.gdn2_rms_norm_int8(total, w)
+    assert torch.equal(q, want[0]) and torch.equal(scale, want[1])
+
+
+@pytest.mark.parametrize("types", [(BF16, BF16, F32), (F32, F32, F32)])
+def test_norm_is_that_of_the_returned_stream(dev, types):
+    """Residuals that the kernels take: y is the norm of h as it is returned."""
+    import gdn2_package as gp
+    x, r, w, _, _ = make(7, 104, types, dev, 6)
+    y, h = gp.gdn2_rms_norm(x, w, residual=r)
+    assert torch.equal(y, gp.gdn2_rms_norm(h, w)[0])
