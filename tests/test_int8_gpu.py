@@ -266,3 +266,31 @@ def test_refusals(dev):
             bad()
     with pytest.raises(TypeError):
         mm(q, 1.0, w, sw)
+
+
+@pytest.mark.parametrize("K", [384, 385, 513, 1003, 2049])
+@pytest.mark.parametrize("M,N", [(500, 400), (70, 9000), (2050, 2100), (4100, 4104)])
+def test_product_of_many_slices(dev, M, N, K):
+    """K over many more slices than the ring holds, whole ones and not, in tiles of 64 x 64 (the
+    first two sizes), 128 x 128 and 192 x 128."""
+    import gdn2_package as gp
+    q, sx, w, sw, bias = operands(M, N, K, dev, K)
+    for dt, b in ((F32, bias), (BF16, None)):
+        y = gp.gdn2_int8_matmul(q, sx, w, sw, bias=b, out_dtype=dt)
+        check_product(y, *product(q, sx, w, sw, b))
+
+
+@pytest.mark.parametrize("M,N", [(40, 9000), (128, 25000), (192, 33000)])
+def test_longest_sums_in_tiles(dev, M, N):
+    """All -128 over K = 131071 in each of the three tiles."""
+    import gdn2_package as gp
+    K, ld = 131071, 131072
+    q = torch.full((M, ld), -128, dtype=torch.int8, device=dev)[:, :K]
+    w = torch.full((N, ld), -128, dtype=torch.int8, device=dev)[:, :K]
+    w[1::3] = 127
+    w[2::3] = 0
+    one = lambda n: torch.ones(n, device=dev)
+    y = gp.gdn2_int8_matmul(q, one(M), w, one(N), out_dtype=F32)
+    row = torch.empty(N, dtype=torch.float64, device=dev)
+    row[0::3], row[1::3], row[2::3] = 16384.0 * K, -16256.0 * K, 0.0
+    assert torch.equal(y, row.float().expand(M, N))
