@@ -520,7 +520,8 @@ def test_tangents_are_refused(dev):
         with torch.set_grad_enabled(grad), forward_ad.dual_level():
             assert all(torch.equal(a, e) for a, e in zip(gp.gdn2_gated_scan(x, g, b, h0=h0), want))
             dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
-            for call in (lambda: gp.gdn2_gated_scan(dual(x), g), lambda: gp.gdn2_gated_scan(x, dual(g)),
+            for call in (lambda: gp.gdn2_gated_scan(dual(x), g),
+                         lambda: gp.gdn2_gated_scan(x, dual(g)),
                          lambda: gp.gdn2_gated_scan(x, g, dual(b)),
                          lambda: gp.gdn2_gated_scan(x, g, h0=dual(h0))):
                 with pytest.raises(NotImplementedError):
@@ -542,3 +543,106 @@ def test_a_penalty_on_the_gradient_is_refused(dev, full):
             (loss + penalty).backward(retain_graph=True)
     for got, want in zip(torch.autograd.grad(loss, (x, g)), (dx, dg)):
         assert torch.equal(got, want)     # without it nothing is in the way
+
+
+@pytest.mark.parametrize("dtype,gdtype", TYPES)
+@pytest.mark.parametrize("B,T,C", [(200, 130, 33), (48, 300, 256), (256, 600, 20), (64, 1000, 200)])
+def test_walk_in_wide_tiles(dev, B, T, C, dtype, gdtype):
+    """Short axes with enough tiles of 64 channels: walked in those, 4 channels a thread and one."""
+    import gdn2_package as gp
+    from gdn2_package import _lib
+    code = _lib.GDN2_F32 if dtype == torch.float32 else _lib.GDN2_BF16
+    assert _lib.lib().gdn2_gated_scan_workspace_bytes(B, T, C, code) == 0
+    assert B * ((C + 63) // 64) >= (192 if T <= 512 else 256)
+    ts, (xn, gn, bn, hn) = inputs(B, T, C, dtype, gdtype, dev, T)
+    for names in (("x", "g", "b", "h0"), ("x", "g")):
+        leaf = {n: ts["xgb".find(n) if n != "h0" else 3].clone().requires_grad_() for n in names}
+        out, hf = gp.gdn2_gated_scan(leaf["x"], leaf["g"], leaf.get("b"), h0=leaf.get("h0"))
+        dout, dhf = torch.randn_like(out), torch.randn_like(hf)
+        got = torch.autograd.grad((out, hf), list(leaf.values()), (dout, dhf))
+        ref, mag, grads = reference(xn, gn, bn if "b" in leaf else np.ones_like(bn),
+                                    hn if "h0" in leaf else np.zeros_like(hn),
+                                    dout.double().cpu().numpy(), dhf.double().cpu().numpy())
+        check(out, ref, mag)
+        check(hf, ref[:, -1], mag[:, -1])
+        for n, t in zip(leaf, got):
+            check(t, *grads[n], n=2)
+
+
+# tiles of 16 (many tokens, few channels), 64 (bfloat16, many channels; float32: 32) and 32
+LONG = [(1, 32801, 77), (1, 32900, 64), (2, 1537, 767), (2, 1100, 512), (1, 700, 101),
+        (1, 900, 100)]
+
+
+@pytest.mark.parametrize("dtype,gdtype", TYPES)
+@pytest.mark.parametrize("B,T,C", LONG)
+def test_steps_at_once_without_a_gate(dev, B, T, C, dtype, gdtype):
+    """Every tile without a gate and with g of either type; the cotangent of one output alone."""
+    import gdn2_package as gp
+    ts, (xn, gn, bn, hn) = inputs(B, T, C, dtype, gdtype, dev, T + 1)
+    zero_out, zero_hf, ones = np.zeros_like(xn), np.zeros_like(hn), np.ones_like(bn)
+    for which in (0, 1):
+        leaf = [t.clone().requires_grad_() for t in ts[:2]]
+        res = gp.gdn2_gated_scan(*leaf)
+        cot = torch.randn_like(res[which])
+        got = torch.autograd.grad(res[which], leaf, cot)
+        cn = cot.double().cpu().numpy()
+        ref, mag, grads = reference(xn, gn, ones, zero_hf, zero_out if which else cn,
+                                    cn if which else zero_hf)
+        check(res[0], ref, mag)
+        check(res[1], ref[:, -1], mag[:, -1])
+        for n, t in zip(("x", "g"), got):
+            check(t, *grads[n], n=2)
+
+
+@pytest.mark.parametrize("dtype,gdtype", TYPES)
+@pytest.mark.parametrize("B,T,C", [(2, 1537, 767), (1, 700, 60), (1, 33000, 24)])
+def test_gated_steps_at_once_of_one_output(dev, B, T, C, dtype, gdtype):
+    """With a gate: one channel a thread in tiles of 64, g in bfloat16, one output alone."""
+    import gdn2_package as gp
+    ts, (xn, gn, bn, hn) = inputs(B, T, C, dtype, gdtype, dev, T + 2)
+    for which in (0, 1):
+        leaf = [t.clone().requires_grad_() for t in ts]
+        res = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+        cot = torch.randn_like(res[which])
+        got = torch.autograd.grad(res[which], leaf, cot)
+        cn = cot.double().cpu().numpy()
+        _, _, grads = reference(xn, gn, bn, hn, np.zeros_like(xn) if which else cn,
+                                cn if which else np.zeros_like(hn))
+        for n, t in zip(("x", "g", "b", "h0"), got):
+            check(t, *grads[n], n=2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,C", [(2, 300, 24), (200, 100, 40), (2, 1300, 768), (1, 33000, 40)])
+def test_strides_walked_and_in_steps(dev, B, T, C, dtype):
+    """The parts of one projection, rows at an odd offset and cotangents of any layout: the
+    results from dense tensors where the accesses are the same, within the bound where not."""
+    import gdn2_package as gp
+    (x, g, b, h0), (xn, gn, bn, hn) = inputs(B, T, C, dtype, dtype, dev, T + 3)
+    dout = torch.randn((B, T, C), device=dev).to(dtype)
+    wide = torch.cat([dout, dout], 2)
+
+    def run(x, g, b, dout):
+        leaf = [t.detach().requires_grad_() for t in (x, g, b, h0)]
+        out, hf = gp.gdn2_gated_scan(*leaf[:3], h0=leaf[3])
+        return (out, hf, *torch.autograd.grad((out, hf), leaf, (dout, torch.ones_like(hf))))
+    want = run(x, g, b, dout)
+    proj = torch.cat([x, g, b], 2)
+    parts = [proj[..., i * C:(i + 1) * C] for i in range(3)]
+    for got in (run(*parts, wide[..., C:]),
+                run(*(t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, g, b, dout))),
+                run(x.transpose(1, 2).contiguous().transpose(1, 2), g, b, dout)):
+        assert all(torch.equal(a, e) for a, e in zip(got, want))
+    odd = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+    got = run(odd(x), odd(g), odd(b), odd(dout))
+    ref, mag, grads = reference(xn, gn, bn, hn, dout.double().cpu().numpy(), np.ones_like(hn))
+    check(got[0], ref, mag)
+    check(got[1], ref[:, -1], mag[:, -1])
+    for n, t in zip(("x", "g", "b", "h0"), got[2:]):
+        check(t, *grads[n], n=2)
+    # a g shared by all channels, and one by all tokens
+    for shared in (g[..., :1].expand(B, T, C), g[:, :1].expand(B, T, C)):
+        one = gp.gdn2_gated_scan(x, shared, b, h0=h0)
+        two = gp.gdn2_gated_scan(x, shared.contiguous(), b, h0=h0)
+        assert all(torch.equal(a, e) for a, e in zip(one, two))
