@@ -845,9 +845,9 @@ void launch_chain(hipStream_t st, const ScanArgs& a, bool bwd, int n) {
 template <typename TX, typename TG, bool GATE, int V>
 void launch_width(hipStream_t st, const ScanArgs& a, bool bwd, const Split& s) {
   if (s.chain) {
-    if (s.ct == 64)
-      launch_chain<TX, TG, GATE, V, 64>(st, a, bwd, s.blocks);
-    else if (s.ct == 32)
+    if constexpr (sizeof(TX) == 2)   // float32 takes no steps in tiles of 64
+      if (s.ct == 64) return launch_chain<TX, TG, GATE, V, 64>(st, a, bwd, s.blocks);
+    if (s.ct == 32)
       launch_chain<TX, TG, GATE, V, 32>(st, a, bwd, s.blocks);
     else
       launch_chain<TX, TG, GATE, V, 16>(st, a, bwd, s.blocks);
