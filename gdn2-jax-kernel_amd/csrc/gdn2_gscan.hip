@@ -419,6 +419,8 @@ __global__ void __launch_bounds__(8 * CT) gscan_bwd(ScanArgs a) {
 }
 
 // ---- The axis cut into its steps, all in one launch --------------------------------
+// (The published single-pass scan with decoupled look-back, Merrill and Garland 2016, its
+// order of service by tickets.)
 // A workgroup takes 128 tokens of 64 channels (or 256 of 32, 512 of 16).  It publishes its
 // composition as soon as it has it, finds the state that enters it from the steps before,
 // and publishes the one that leaves it.  Steps are dealt by a ticket, the earliest of all
@@ -435,7 +437,9 @@ constexpr unsigned long long kNone = ~0ull;
 constexpr float kState = -2.f;
 // Steps looked back over at a time: 8 where the registers allow (1 x 131072 x 1024 float32
 // forward 313 us, with 4 345); the backward has none to spare (8 x 8192 x 768 bfloat16 250 us,
-// with 4 194).
+// with 4 194).  Even so its gated forms do not fit the 128 registers of two workgroups a CU and
+// keep 8 to 36 bytes a lane in scratch memory (12 there: 37 MB read and 31 written beyond the
+// operands' 503 and 403), as do gated bfloat16 forwards with one channel a thread (12 to 20).
 template <bool REV> constexpr int kWindow = REV ? 4 : 8;
 constexpr int kTicketStride = 16; // tickets of different tiles on cache lines of their own
 struct Chain {

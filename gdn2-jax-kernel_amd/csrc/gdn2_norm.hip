@@ -12,9 +12,11 @@
 //
 // All of these are bound by memory traffic: a row is read once into registers (8 values
 // a thread and chunk, 16-byte accesses), reduced over its 64 to 1024 threads and
-// written from the registers.  Sums and the norm's factors are float32.  Copies reach 5.16 TB/s
-// on this card; with a residual, bfloat16: norm of 65536 x 768 73 us (5.5 TB/s), 16384 x 4096
-// 95 (5.7), 4096 x 8192 41 (6.5); in 8 bits 66 (5.3), 86 (5.5), 37 (6.4).
+// written from the registers.  Sums and the norm's factors are float32.  A copy of 1 GiB reaches
+// 5.16 TB/s on this card; these, with a residual, bfloat16: norm of 65536 x 768 73 us (5.5 TB/s),
+// 16384 x 4096 95 (5.7); in 8 bits 65 (5.4), 84 (5.6).  Calls of a few hundred MB pass a copy's
+// rate because part of their data is still in the last-level cache (256 MB): 4096 x 8192, 268 MB in
+// all, 41 and 37 us (6.5 and 6.4 TB/s).
 #include "gdn2.h"
 #include "gdn2_common.h"
 
@@ -39,8 +41,9 @@ struct NormArgs {
 
 // 8 values at column c of a row of C, as they are stored.  VEC: the row is aligned to 16 bytes
 // and C a multiple of 8; else the same accesses start at any value, and only a row's last piece
-// goes value by value (65536 x 767 bfloat16, norm, in 8 bits, backward: 92, 82, 135 us; all value
-// by value 291, 249, 197).
+// goes value by value (65536 x 767 bfloat16, norm, in 8 bits, backward: 93, 82, 135 to 156 us; all
+// value by value 291, 249, 197).  The backward, with two waves a SIMD to cover it, waits for
+// that piece in three operands and a result of every row (65536 x 768 75 us).
 template <typename V, typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Loose {
   V v;
@@ -258,7 +261,9 @@ struct NormBwdArgs {
 // registers (a thread keeps its columns), then over the workgroup's groups in LDS and, by
 // norm_dw, over the workgroups, always in the same order.  The next row is in flight while one
 // is worked on.  With a partial sum of dw for each wave and no row ahead 65536 x 768 bfloat16
-// took 95 us, 4096 x 8192 87, 2048 x 2048 19; so 76 (5.3 TB/s), 44 and 12.
+// took 95 us, 4096 x 8192 87, 2048 x 2048 19; so 76 (5.3 TB/s), 44 and 12.  Rows past 8192 values
+// with a float32 stream do not fit the registers of two waves a SIMD: 12 to 44 bytes a lane go
+// through scratch memory (4096 x 16384 float32 213 us, 5.0 TB/s).
 template <typename TX, typename TR, int TPR, int NCH, bool VEC>
 __global__ void __launch_bounds__(kNT<TPR>) norm_bwd(NormBwdArgs a) {
   constexpr int NT = kNT<TPR>, NW = TPR / 64, NG = NT / TPR;

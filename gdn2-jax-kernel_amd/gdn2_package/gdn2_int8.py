@@ -5,15 +5,17 @@
     x = gdn2_dequantize_int8(q, scale, dtype=torch.bfloat16)
     y = gdn2_int8_matmul(q, scale, w, w_scale, bias=None, out_dtype=torch.bfloat16)
 
-A row t is held as q = round(127 t / max|t|) (ties to even) and scale = max|t| / 127; it
-stands for q * scale.  A row of zeros has scale 0; one that holds NaN or an infinity
+A row t is held as q = round(127 t / max|t|) (ties to even; in float32, t times 127 (1 / max|t|),
+so that a value within three roundings of a tie may go either way) and scale = max|t| / 127;
+it stands for q * scale.  A row of zeros has scale 0; one that holds NaN or an infinity
 has scale NaN and q = 0, so that all that is computed from it is NaN.  The weight of a
 linear layer, (N,K) as torch.nn.Linear holds it, is quantised once with
 ``gdn2_quantize_int8(weight)``: a scale for each output channel.
 
 Rows of q start at multiples of 16 bytes: where the width is none, q is a view of a wider
-tensor.  The product takes such rows as they are and copies others.  Inference only.  No
-counterpart in the reference.
+tensor.  The product takes such rows as they are and copies others.  Inference only: as with
+the decode step, results carry no gradient, whatever the inputs require.  No counterpart in
+the reference.
 """
 from __future__ import annotations
 
@@ -34,7 +36,7 @@ def _empty_q(shape, dev):
 
 def gdn2_rms_norm_int8(x, weight, residual=None, eps=1e-6):
     """``gdn2_rms_norm`` with y in 8 bits: (q int8 of x's shape, scale float32 of x's shape
-    without its last axis, h).  q does not depend on the order of any sum."""
+    without its last axis, h).  q does not depend on the order of any sum.  Inference only."""
     what = "gdn2_rms_norm_int8"
     xs, ws, rs = _prepare(x, weight, residual, eps, what)
     shape, dev = xs.shape, xs.device
@@ -133,7 +135,7 @@ def gdn2_int8_matmul(q, scale, weight, weight_scale, bias=None, out_dtype=torch.
 
     q (..., K) int8 with scale (...); weight (N, K) int8 with weight_scale (N,); bias (N,)
     or None.  Returns (..., N) in out_dtype (float32 or bfloat16).  The sums over K are
-    exact integers (K <= 131071), scaled in float32 and rounded once."""
+    exact integers (K <= 131071), scaled in float32 and rounded once.  Inference only."""
     what = "gdn2_int8_matmul"
     if out_dtype not in _SUPPORTED_IN:
         raise GDN2Error(f"{what}: out_dtype must be float32 or bfloat16; got {out_dtype}")

@@ -200,7 +200,8 @@ def gdn2_gated_scan_step(x, g, b=None, state=None, inplace=False):
     x, g, b: one shape (B, ...) without a token axis; state: float32 of that shape
     (default zeros).  Returns ``out`` (x's type) and the new state; ``inplace=True``
     updates ``state`` itself, which must then be a contiguous float32 tensor.
-    Inference only."""
+    Inference only: as with the decode step, results carry no gradient, whatever the
+    inputs require."""
     what = "gdn2_gated_scan_step"
     dt, gdt = _types(x, g, b, what)
     dev, shape = x.device, x.shape

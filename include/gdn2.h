@@ -411,7 +411,8 @@ int gdn2_rms_norm_bwd(void* stream, int M, int C, int x_dtype, int r_dtype, int 
                       size_t ws_bytes);
 
 /* y in 8 bits with a scale for each row: with t = h w and m = max |t|, q = round(127 t / m)
- * (ties to even) and scale = m / (127 sqrt(mean h^2 + eps)).  A row whose m is below 1e-36
+ * (ties to even; computed as t times 127 (1 / m) in float32) and
+ * scale = m / (127 sqrt(mean h^2 + eps)).  A row whose m is below 1e-36
  * has q = 0 and scale 0; one that holds NaN or an infinity q = 0 and scale NaN.  q is 16-byte
  * aligned, its rows q_stride = C rounded up to a multiple of 16 bytes apart, the bytes
  * between zero. */
