@@ -1,0 +1,999 @@
+// Selective state space scan over (B, T, C) with N states a channel:
+//   d = softplus(dt + dt_bias)   (or dt + dt_bias as it is)
+//   h_t[c,n] = e^{d_t[c] A[c,n]} h_{t-1}[c,n] + d_t[c] x_t[c] B_t[n]
+//   y_t[c] = sum_n C_t[n] h_t[c,n] + D[c] x_t[c],   out_t = y_t silu(z_t),
+// its backward pass and its step for one token.  B and C are shared by the C / G channels of a
+// group.  A token marked in `starts` begins a sequence: the state before it is dropped, not
+// multiplied by zero.
+//
+// A run of tokens maps the state entering it to the one leaving it by h -> e^{A S} h + H with S
+// the sum of its d: one number a channel beside H.  The axis is cut into chunks: a first kernel
+// composes every chunk (S and H), a second walks over the chunks, a third walks each chunk's
+// tokens again from the state that enters it.  What bounds this is not memory but the
+// exponentials, N for each token and channel, and the four or five operations around each: a
+// wave of 64 lanes has a channel a lane, all its states in registers, and B and C, the same for
+// all lanes, in scalar registers, from float32 rows that a small kernel lays out.
+//
+// Backward: the gradients that enter chunks from the right come the same way.  The forward
+// keeps the state before every 16th token; from it a workgroup forms 16 tokens' states again,
+// keeps them and their decays in registers, and walks back.  Here a lane has four states of a
+// channel, and sums over states and over channels are formed by lane exchanges.
+// Sums over workgroups are written as partial sums and added in a fixed order.
+// Everything is float32 between the inputs' and the outputs' types.
+#include <limits.h>
+
+#include "gdn2.h"
+#include "gdn2_common.h"
+
+namespace gdn2 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kKeep = 16;      // tokens between kept states
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kNegInf = -__builtin_inff();
+
+// Strides are in elements; channels are contiguous.
+struct Rows {
+  const void* p;
+  long long sb, st;
+};
+struct SsmArgs {
+  Rows x, dt, z, bm, cm, dout;
+  const float *A, *D, *dt_bias, *h0, *dh_final;   // (C,N) (C) (C) (B,C,N) (B,C,N); or null but A
+  const unsigned char* starts;                     // (B,T) or null
+  void *out, *dx, *ddt, *dz, *dbm, *dcm;           // dense
+  float *h_final, *dh0, *dA, *dD, *dbias;
+  float* kept;                                     // (B, ceil(T / kKeep), C, NP) or null
+  // workspace
+  float* bc;      // (B, T, G, 2, NP): B and C in float32, the states past N zero
+  float* part_bc; // (tiles, B, T, 2, NP)
+  float* part_a;  // (B chunks, C, NP)
+  float* part_c;  // (B chunks, 2, C)
+  float* slot;    // (B, chunks, C, NP): state or gradient that enters a chunk
+  float* sum;     // (B, chunks, C): S of a chunk, -inf where a sequence starts in it
+  int B, T, C, G, N;
+  int Cg, tiles;  // channels of a group, tiles of a group
+  int L, chunks;  // tokens of a chunk
+  int softplus;
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// log(1 + e^v) = max(v, 0) + log1p(e^-|v|), log1p(u) = 2 artanh(s) with s = u / (2 + u) <= 1/3, and
+// artanh(s) = s (1 + s^2/3 + s^4/5 + ...), whose terms from s^16/17 on are below 2^-29.
+__device__ __forceinline__ float softplus(float v) {
+  const float u = exp2_(-fabsf(v) * kLog2e), s = u * rcp_(2.f + u), q = s * s;
+  float p = 1.f / 15.f;
+  p = fmaf(p, q, 1.f / 13.f);
+  p = fmaf(p, q, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  return fmaf(2.f * s, p, v != v ? v : fmaxf(v, 0.f));
+}
+__device__ __forceinline__ float sigmoid(float v) { return rcp_(1.f + exp2_(-v * kLog2e)); }
+
+// Float32 values that are the same for all lanes of a wave: read through the scalar cache.
+typedef const __attribute__((address_space(4))) float* uniform_ptr;
+__device__ __forceinline__ uniform_ptr uniform(const float* p) { return (uniform_ptr)(uintptr_t)p; }
+
+template <typename T>
+__device__ __forceinline__ float element(const Rows& r, int b, int t, int c) {
+  return (float)((const T*)r.p)[b * r.sb + t * r.st + c];
+}
+
+// B and C in float32, NP states each.
+template <typename TX>
+__global__ void __launch_bounds__(kThreads) ssm_rows(SsmArgs a, int NP) {
+  const long long n = (long long)a.B * a.T * a.G * 2 * NP;
+  for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < n;
+       e += (long long)gridDim.x * kThreads) {
+    const int s = (int)(e % NP);
+    const long long row = e / NP;          // ((b T + t) G + g) 2 + which
+    const long long bt = row / 2 / a.G;
+    const int g = (int)(row / 2 - bt * a.G), t = (int)(bt % a.T), b = (int)(bt / a.T);
+    a.bc[e] = s < a.N ? element<TX>(row & 1 ? a.cm : a.bm, b, t, g * a.N + s) : 0.f;
+  }
+}
+
+// Where a wave of a channel a lane works.
+struct WavePlace {
+  int b, chunk, g, c, t0, t1;
+  bool on, idle;
+  __device__ WavePlace(const SsmArgs& a, int first_chunk, int chunks) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int nt = a.G * a.tiles;
+    const int unit = blockIdx.x * (kThreads / 64) + wave;
+    idle = unit >= a.B * chunks * nt;
+    const int tile = unit % nt, rest = unit / nt;
+    chunk = first_chunk + rest % chunks;
+    b = rest / chunks;
+    g = tile / a.tiles;
+    const int cg = (tile - g * a.tiles) * 64 + lane;
+    on = cg < a.Cg;
+    c = g * a.Cg + (on ? cg : 0);          // loads stay in bounds, nothing is stored
+    t0 = chunk * a.L;
+    t1 = a.T - t0 < a.L ? a.T : t0 + a.L;
+  }
+};
+
+constexpr int kAhead = 4;   // tokens loaded at a time
+
+// NP states of (row, c) at p (rows of C channels), from and to float32.
+template <int NP>
+__device__ __forceinline__ void load_states(const float* p, float (&h)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; n += 4) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[n + e] = v[e];
+  }
+}
+template <int NP>
+__device__ __forceinline__ void store_states(float* p, const float (&h)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; n += 4)
+    *reinterpret_cast<f32x4*>(p + n) = f32x4{h[n], h[n + 1], h[n + 2], h[n + 3]};
+}
+template <int NP>
+__device__ __forceinline__ void load_user(const float* p, int N, float (&h)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; ++n) h[n] = p && n < N ? p[n] : 0.f;
+}
+
+// Forward.  OUT: the tokens from the entering state, outputs and kept states; else the
+// composition of chunks 0 .. chunks - 2, H of chunk k into slot k + 1.
+template <typename TX, typename TD, int NP, bool OUT>
+__global__ void __launch_bounds__(kThreads) ssm_fwd(SsmArgs a) {
+  const WavePlace w(a, 0, OUT ? a.chunks : a.chunks - 1);
+  if (w.idle) return;
+  const int nch = a.chunks;
+  float A2[NP], h[NP];
+  load_user<NP>(a.A + (long long)w.c * a.N, a.N, A2);
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    A2[n] *= kLog2e;
+    h[n] = 0.f;
+  }
+  const float bias = a.dt_bias ? a.dt_bias[w.c] : 0.f, D = OUT && a.D ? a.D[w.c] : 0.f;
+  if (OUT) {
+    if (w.chunk == 0)
+      load_user<NP>(a.h0 ? a.h0 + ((long long)w.b * a.C + w.c) * a.N : nullptr, a.N, h);
+    else
+      load_states<NP>(a.slot + (((long long)w.b * nch + w.chunk) * a.C + w.c) * NP, h);
+  }
+  const int nb = (a.T + kKeep - 1) / kKeep;
+  const TX* px = (const TX*)a.x.p + w.b * a.x.sb + w.c;
+  const TD* pd = (const TD*)a.dt.p + w.b * a.dt.sb + w.c;
+  const TX* pz = (const TX*)a.z.p + w.b * a.z.sb + w.c;
+  const bool gate = OUT && a.z.p;
+  TX rx[kAhead], rz[kAhead];
+  TD rd[kAhead];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const long long ti = t + i < w.t1 ? t + i : w.t1 - 1;
+      rx[i] = px[ti * a.x.st];
+      rd[i] = pd[ti * a.dt.st];
+      if (gate) rz[i] = pz[ti * a.z.st];
+    }
+  };
+  load(w.t0);
+  float S = 0.f;
+  bool fresh = false;
+  TX* out = (TX*)a.out + ((long long)w.b * a.T) * a.C + w.c;
+  for (int t = w.t0; t < w.t1; t += kAhead) {
+    if (OUT && a.kept && t % kKeep == 0 && w.on)
+      store_states<NP>(a.kept + (((long long)w.b * nb + t / kKeep) * a.C + w.c) * NP, h);
+    float x[kAhead], d[kAhead], z[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      x[i] = (float)rx[i];
+      d[i] = (float)rd[i] + bias;
+      if (gate) z[i] = (float)rz[i];
+    }
+    if (a.softplus) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
+    }
+    if (t + kAhead < w.t1) load(t + kAhead);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t + i >= w.t1) break;
+      const long long bt = (long long)w.b * a.T + t + i;
+      if (a.starts && a.starts[bt]) {
+        fresh = true;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) h[n] = 0.f;
+      }
+      const uniform_ptr row = uniform(a.bc) + (bt * a.G + w.g) * 2 * NP;
+      const float u = d[i] * x[i];
+      float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        h[n] = fmaf(exp2_(d[i] * A2[n]), h[n], u * row[n]);
+        if (OUT) (n & 1 ? y1 : y0) = fmaf(h[n], row[NP + n], n & 1 ? y1 : y0);
+      }
+      S += d[i];
+      if (OUT) {
+        float y = fmaf(D, x[i], y0 + y1);
+        if (gate) y *= z[i] * sigmoid(z[i]);
+        if (w.on) out[(long long)(t + i) * a.C] = (TX)y;
+      }
+    }
+  }
+  if (!w.on) return;
+  if (!OUT) {
+    store_states<NP>(a.slot + (((long long)w.b * nch + w.chunk + 1) * a.C + w.c) * NP, h);
+    a.sum[((long long)w.b * nch + w.chunk) * a.C + w.c] = fresh ? kNegInf : S;
+  } else if (w.chunk == nch - 1) {
+    float* p = a.h_final + ((long long)w.b * a.C + w.c) * a.N;
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+      if (n < a.N) p[n] = h[n];
+  }
+}
+
+// The gradient that leaves chunks 1 .. chunks - 1 at their beginning with none entering, into the
+// slot of the chunk before, and S.
+template <typename TX, typename TD, int NP>
+__global__ void __launch_bounds__(kThreads) ssm_rev(SsmArgs a) {
+  const WavePlace w(a, 1, a.chunks - 1);
+  if (w.idle) return;
+  const int nch = a.chunks;
+  float A2[NP], e[NP];
+  load_user<NP>(a.A + (long long)w.c * a.N, a.N, A2);
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    A2[n] *= kLog2e;
+    e[n] = 0.f;
+  }
+  const float bias = a.dt_bias ? a.dt_bias[w.c] : 0.f;
+  const TX* po = (const TX*)a.dout.p + w.b * a.dout.sb + w.c;
+  const TD* pd = (const TD*)a.dt.p + w.b * a.dt.sb + w.c;
+  const TX* pz = (const TX*)a.z.p + w.b * a.z.sb + w.c;
+  const bool gate = a.z.p, has = a.dout.p;
+  TX ro[kAhead], rz[kAhead];
+  TD rd[kAhead];
+  auto load = [&](int t) {   // tokens t, t - 1, ...
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const long long ti = t - i > w.t0 ? t - i : w.t0;
+      if (has) ro[i] = po[ti * a.dout.st];
+      rd[i] = pd[ti * a.dt.st];
+      if (gate) rz[i] = pz[ti * a.z.st];
+    }
+  };
+  load(w.t1 - 1);
+  float S = 0.f;
+  bool fresh = false;
+  for (int t = w.t1 - 1; t >= w.t0; t -= kAhead) {
+    float g[kAhead], d[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      g[i] = has ? (float)ro[i] : 0.f;
+      d[i] = (float)rd[i] + bias;
+      if (gate) {
+        const float z = (float)rz[i];
+        g[i] *= z * sigmoid(z);
+      }
+    }
+    if (a.softplus) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
+    }
+    if (t - kAhead >= w.t0) load(t - kAhead);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t - i < w.t0) break;
+      const long long bt = (long long)w.b * a.T + t - i;
+      const uniform_ptr row = uniform(a.bc) + ((bt * a.G + w.g) * 2 + 1) * NP;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) e[n] = exp2_(d[i] * A2[n]) * fmaf(g[i], row[n], e[n]);
+      S += d[i];
+      if (a.starts && a.starts[bt]) {
+        fresh = true;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) e[n] = 0.f;
+      }
+    }
+  }
+  if (!w.on) return;
+  store_states<NP>(a.slot + (((long long)w.b * nch + w.chunk - 1) * a.C + w.c) * NP, e);
+  a.sum[((long long)w.b * nch + w.chunk) * a.C + w.c] = fresh ? kNegInf : S;
+}
+
+// What enters each chunk, from the compositions: a thread a state of a channel, the chunks in
+// order (REV: from the last).
+template <int NP, bool REV>
+__global__ void __launch_bounds__(kThreads) ssm_join(SsmArgs a) {
+  const long long e = (long long)blockIdx.x * kThreads + threadIdx.x;
+  const int n = (int)(e % NP);
+  const long long bc = e / NP;
+  const int b = (int)(bc / a.C), c = (int)(bc - (long long)b * a.C);
+  if (b >= a.B) return;
+  const float A2 = n < a.N ? a.A[(long long)c * a.N + n] * kLog2e : 0.f;
+  const float* first = REV ? a.dh_final : a.h0;
+  float h = first && n < a.N ? first[bc * a.N + n] : 0.f;
+  const int nch = a.chunks;
+  const long long step = (REV ? -1ll : 1ll) * a.C;
+  const long long at = ((long long)b * nch + (REV ? nch - 1 : 0)) * a.C + c;
+  float* slot = a.slot + at * NP + n;
+  const float* sum = a.sum + at;
+  if (REV) *slot = h;    // the forward's first chunk reads h0 itself
+  // the composition of one chunk is read while the one before is applied
+  constexpr int U = 8;
+  for (int k0 = 1; k0 < nch; k0 += U) {
+    float H[U], S[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const long long k = k0 + i < nch ? k0 + i : nch - 1;
+      H[i] = slot[k * step * NP];
+      S[i] = sum[(k - 1) * step];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (k0 + i >= nch) break;
+      h = S[i] == kNegInf ? H[i] : fmaf(exp2_(A2 * S[i]), h, H[i]);
+      slot[(k0 + i) * step * NP] = h;
+    }
+  }
+}
+
+// ---- Backward ----------------------------------------------------------------------
+
+// The value of the lane whose number differs in bit BIT, where lanes that differ in lower bits
+// alone may be exchanged for one another beforehand (all that is needed to sum over lanes).
+template <int BIT>
+__device__ __forceinline__ float partner(float v) {
+  const int i = __builtin_bit_cast(int, v);
+  if constexpr (BIT == 0)
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0xB1, 0xF, 0xF, true));
+  else if constexpr (BIT == 1)
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x4E, 0xF, 0xF, true));
+  else if constexpr (BIT == 2)   // row_half_mirror: lane 7 - l of eight
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x141, 0xF, 0xF, true));
+  else if constexpr (BIT == 3)   // row_mirror: lane 15 - l of sixteen
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x140, 0xF, 0xF, true));
+  else
+    return __shfl_xor(v, 1 << BIT);
+}
+// v0 (v1) summed over lane pairs that differ in bit BIT, in the lanes where the bit is 0 (1).
+template <int BIT>
+__device__ __forceinline__ float fold(float v0, float v1, int lane) {
+  const bool high = lane >> BIT & 1;
+  return (high ? v1 : v0) + partner<BIT>(high ? v0 : v1);
+}
+template <int BIT>
+__device__ __forceinline__ float whole(float v) { return v + partner<BIT>(v); }
+
+// Eight sums over the lanes' low LG bits: from the highest bit down, three folds deal the values out
+// to the lanes, the rest is summed whole.  On return the lane holds the value whose number
+// has as its bits the lane's bits LG - 1, LG - 2, LG - 3 (as many as there are; v[0], or v[0..1]
+// ... where there are fewer).
+template <int LG>
+__device__ __forceinline__ void sum_lanes8(float (&v)[8], int lane) {
+  static_assert(LG >= 2 && LG <= 5, "4 to 32 lanes");
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = fold<LG - 1>(v[k], v[k + 4], lane);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) v[k] = fold<LG - 2>(v[k], v[k + 2], lane);
+  if constexpr (LG >= 3) v[0] = fold<LG - 3>(v[0], v[1], lane);
+  if constexpr (LG >= 4) v[0] = whole<LG - 4>(v[0]);
+  if constexpr (LG >= 5) v[0] = whole<LG - 5>(v[0]);
+}
+
+// Sum over the lane bits FROM .. 5.
+template <int FROM>
+__device__ __forceinline__ float sum_high(float v) {
+  if constexpr (FROM <= 2) v = v + __shfl_xor(v, 4);
+  if constexpr (FROM <= 3) v = v + __shfl_xor(v, 8);
+  if constexpr (FROM <= 4) v = v + __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// A workgroup walks a chunk of CT channels backwards, 16 tokens at a time.
+template <typename TX, typename TD, int NP>
+struct Bwd {
+  static constexpr int NG = NP / 4;          // lane groups, four states each
+  static constexpr int CH = 64 / NG;         // channels of a wave
+  static constexpr int LG = CH == 32 ? 5 : CH == 16 ? 4 : CH == 8 ? 3 : 2;
+  static constexpr int CT = 4 * CH;          // and of a workgroup
+  static constexpr int PER = kKeep * CT / kThreads;   // (token, channel) values of a thread
+  static constexpr int STEP = kThreads / CT;          // tokens that the threads cover at a time
+  struct Shared {
+    float d[kKeep][CT], x[kKeep][CT], dy[kKeep][CT];
+    float sb[kKeep][CT], sa[kKeep][CT], y[kKeep][CT];   // sums over the states
+    float bc[kKeep][2][NP];
+    float red[4][kKeep][2][NP];                         // sums over a wave's channels
+    unsigned fresh;                                     // bit i: token i starts a sequence
+  };
+};
+
+template <typename TX, typename TD, int NP>
+__global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
+  using P = Bwd<TX, TD, NP>;
+  constexpr int CH = P::CH, CT = P::CT, PER = P::PER, STEP = P::STEP, LG = P::LG;
+  __shared__ __attribute__((aligned(16))) typename P::Shared s;
+  const int nt = a.G * a.tiles;
+  const int tile = blockIdx.x % nt, rest = blockIdx.x / nt;
+  const int chunk = rest % a.chunks, b = rest / a.chunks;
+  const int g = tile / a.tiles, first = (tile - g * a.tiles) * CT;   // first channel of the group's
+  const int t0 = chunk * a.L, t1 = a.T - t0 < a.L ? a.T : t0 + a.L;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int nb = (a.T + kKeep - 1) / kKeep;
+
+  // this thread's channel of the rows that are read and written, and its first token
+  const int rc = tid % CT, ri = tid / CT;
+  const bool r_on = first + rc < a.Cg;
+  const int r_c = g * a.Cg + (r_on ? first + rc : 0);
+  const float bias = a.dt_bias ? a.dt_bias[r_c] : 0.f, D = a.D ? a.D[r_c] : 0.f;
+  float sum_D = 0.f, sum_bias = 0.f;
+  const bool gate = a.z.p, has = a.dout.p;
+
+  // this lane's channel and states
+  const int ci = wave * CH + lane % CH, q = lane / CH;
+  const bool on = first + ci < a.Cg;
+  const int c = g * a.Cg + (on ? first + ci : 0);
+  float A[4], A2[4], e[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
+  const long long bc_c = (long long)b * a.C + c;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int n = 4 * q + k;
+    A[k] = n < a.N ? a.A[(long long)c * a.N + n] : 0.f;
+    A2[k] = A[k] * kLog2e;
+    e[k] = 0.f;
+    if (chunk == a.chunks - 1 && a.dh_final && n < a.N) e[k] = a.dh_final[bc_c * a.N + n];
+  }
+  if (chunk < a.chunks - 1) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(
+        a.slot + (((long long)b * a.chunks + chunk) * a.C + c) * NP + 4 * q);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e[k] = v[k];
+  }
+
+  TX rx[PER], ro[PER], rz[PER];
+  TD rd[PER];
+  auto load = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int ti = t + ri + i * STEP < t1 ? t + ri + i * STEP : t1 - 1;
+      rx[i] = ((const TX*)a.x.p)[b * a.x.sb + ti * a.x.st + r_c];
+      rd[i] = ((const TD*)a.dt.p)[b * a.dt.sb + ti * a.dt.st + r_c];
+      if (has) ro[i] = ((const TX*)a.dout.p)[b * a.dout.sb + ti * a.dout.st + r_c];
+      if (gate) rz[i] = ((const TX*)a.z.p)[b * a.z.sb + ti * a.z.st + r_c];
+    }
+  };
+  const int last = (t1 - t0 - 1) / kKeep * kKeep + t0;
+  load(last);
+  for (int t = last; t >= t0; t -= kKeep) {
+    // stage: tokens past the end are neutral (d = x = dy = 0)
+    float raw[PER], xv[PER], zv[PER], ov[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = ri + i * STEP;
+      const bool real = r_on && t + k < t1;
+      xv[i] = real ? (float)rx[i] : 0.f;
+      ov[i] = real && has ? (float)ro[i] : 0.f;
+      zv[i] = real && gate ? (float)rz[i] : 0.f;
+      raw[i] = (float)rd[i] + bias;
+      const float d = a.softplus ? softplus(raw[i]) : raw[i];
+      s.d[k][rc] = real ? d : 0.f;
+      s.x[k][rc] = xv[i];
+      s.dy[k][rc] = gate ? ov[i] * zv[i] * sigmoid(zv[i]) : ov[i];
+    }
+    for (int k = tid; k < kKeep * 2 * NP; k += kThreads) {
+      const int i = k / (2 * NP);
+      const long long bt = (long long)b * a.T + (t + i < t1 ? t + i : t1 - 1);
+      (&s.bc[0][0][0])[k] = a.bc[(bt * a.G + g) * 2 * NP + k % (2 * NP)];
+    }
+    if (wave == 0) {
+      const bool f = a.starts && lane < kKeep && t + lane < t1 &&
+                     a.starts[(long long)b * a.T + t + lane];
+      const unsigned long long m = __ballot(f);
+      if (lane == 0) s.fresh = (unsigned)m;
+    }
+    const f32x4 hv = *reinterpret_cast<const f32x4*>(
+        a.kept + (((long long)b * nb + t / kKeep) * a.C + c) * NP + 4 * q);
+    __syncthreads();
+    if (t > t0) load(t - kKeep);
+    const unsigned fresh = __builtin_amdgcn_readfirstlane(s.fresh);
+
+    float h[kKeep][4], dec[kKeep][4], h_in[4], now[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h_in[k] = now[k] = hv[k];
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+      const float d = s.d[i][ci], u = d * s.x[i][ci];
+      const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s.bc[i][0][4 * q]);
+      const bool f = fresh >> i & 1;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float r = exp2_(d * A2[k]);
+        dec[i][k] = f ? 0.f : r;
+        now[k] = f ? u * Bv[k] : fmaf(r, now[k], u * Bv[k]);
+        h[i][k] = now[k];
+      }
+    }
+#pragma unroll
+    for (int i = kKeep - 1; i >= 0; --i) {
+      const float d = s.d[i][ci], u = d * s.x[i][ci], dy = s.dy[i][ci];
+      const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s.bc[i][0][4 * q]);
+      const f32x4 Cv = *reinterpret_cast<const f32x4*>(&s.bc[i][1][4 * q]);
+      const bool f = fresh >> i & 1;
+      float v[8], sb = 0.f, sa = 0.f, y = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float dh = fmaf(dy, Cv[k], e[k]);
+        v[k] = dh * u;             // of B
+        v[4 + k] = dy * h[i][k];   // of C
+        sb = fmaf(dh, Bv[k], sb);
+        const float back = f ? 0.f : dh * dec[i][k];
+        const float through = f ? 0.f : back * (i ? h[i - 1][k] : h_in[k]);
+        sa = fmaf(through, A[k], sa);
+        dA[k] = fmaf(through, d, dA[k]);
+        y = fmaf(Cv[k], h[i][k], y);
+        e[k] = back;
+      }
+      sb = sum_high<LG>(sb);
+      sa = sum_high<LG>(sa);
+      if (gate) y = sum_high<LG>(y);
+      if (q == 0) {
+        s.sb[i][ci] = sb;
+        s.sa[i][ci] = sa;
+        if (gate) s.y[i][ci] = y;
+      }
+      sum_lanes8<LG>(v, lane);
+      // the lanes with the values: v[0] of number (bits LG - 1, LG - 2, LG - 3)
+      if constexpr (LG >= 3) {
+        if ((lane & ((1 << (LG - 3)) - 1)) == 0) {
+          const int k = lane >> (LG - 1) & 1, k2 = lane >> (LG - 2) & 1, k3 = lane >> (LG - 3) & 1;
+          s.red[wave][i][k][4 * q + 2 * k2 + k3] = v[0];
+        }
+      } else {
+        const int k = lane >> 1 & 1, k2 = lane & 1;
+        s.red[wave][i][k][4 * q + 2 * k2] = v[0];
+        s.red[wave][i][k][4 * q + 2 * k2 + 1] = v[1];
+      }
+    }
+    __syncthreads();
+    // sums over the states to gradients of x, dt and z; sums over the waves' channels
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int k = ri + i * STEP;
+      if (!r_on || t + k >= t1) continue;
+      const float d = s.d[k][rc], dy = s.dy[k][rc], sb = s.sb[k][rc];
+      const long long at = ((long long)b * a.T + t + k) * a.C + r_c;
+      ((TX*)a.dx)[at] = (TX)fmaf(d, sb, D * dy);
+      float dd = fmaf(xv[i], sb, s.sa[k][rc]);
+      if (a.softplus) dd *= sigmoid(raw[i]);
+      ((TD*)a.ddt)[at] = (TD)dd;
+      sum_bias += dd;
+      sum_D = fmaf(dy, xv[i], sum_D);
+      if (gate) {
+        const float sg = sigmoid(zv[i]), y = fmaf(D, xv[i], s.y[k][rc]);
+        ((TX*)a.dz)[at] = (TX)(ov[i] * y * sg * fmaf(zv[i], 1.f - sg, 1.f));
+      }
+    }
+    for (int k = tid; k < kKeep * 2 * NP; k += kThreads) {
+      const int i = k / (2 * NP);
+      if (t + i >= t1) continue;
+      const float* r = &s.red[0][0][0][0] + k;
+      const float v = (r[0] + r[kKeep * 2 * NP]) + (r[2 * kKeep * 2 * NP] + r[3 * kKeep * 2 * NP]);
+      a.part_bc[(((long long)tile * a.B + b) * a.T + t + i) * 2 * NP + k % (2 * NP)] = v;
+    }
+    __syncthreads();   // the next tokens are staged over what was read here
+  }
+
+  const long long row = (long long)b * a.chunks + chunk;
+  if (on) {
+    *reinterpret_cast<f32x4*>(a.part_a + (row * a.C + c) * NP + 4 * q) =
+        f32x4{dA[0], dA[1], dA[2], dA[3]};
+    if (chunk == 0 && a.dh0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (4 * q + k < a.N) a.dh0[bc_c * a.N + 4 * q + k] = e[k];
+    }
+  }
+  s.sb[ri][rc] = sum_D;
+  s.sa[ri][rc] = sum_bias;
+  __syncthreads();
+  if (tid < CT && r_on) {
+    float u = 0.f, v = 0.f;
+#pragma unroll
+    for (int k = 0; k < STEP; ++k) {
+      u += s.sb[k][rc];
+      v += s.sa[k][rc];
+    }
+    a.part_c[row * 2 * a.C + r_c] = u;
+    a.part_c[(row * 2 + 1) * a.C + r_c] = v;
+  }
+}
+
+// Gradients of A, D and dt_bias: partial sums over the rows added in their order, 64 columns a
+// workgroup, 16 rows at a time.  Columns: C NP of part_a, then 2 C of part_c.
+__global__ void __launch_bounds__(1024) ssm_sums(SsmArgs a, int NP) {
+  __shared__ float sum[16][64];
+  const int col = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const long long wa = (long long)a.C * NP, wc = 2ll * a.C, rows = (long long)a.B * a.chunks;
+  const long long at = (long long)blockIdx.x * 64 + col;
+  float v = 0.f;
+  if (at < wa) {
+    for (long long k = r; k < rows; k += 16) v += a.part_a[k * wa + at];
+  } else if (at < wa + wc) {
+    for (long long k = r; k < rows; k += 16) v += a.part_c[k * wc + at - wa];
+  }
+  sum[r][col] = v;
+  __syncthreads();
+  if (r) return;
+  v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v += sum[k][col];
+  if (at < wa) {
+    const long long c = at / NP;
+    const int n = (int)(at - c * NP);
+    if (n < a.N) a.dA[c * a.N + n] = v;
+  } else if (at < wa + a.C) {
+    if (a.dD) a.dD[at - wa] = v;
+  } else if (at < wa + wc) {
+    if (a.dbias) a.dbias[at - wa - a.C] = v;
+  }
+}
+
+// Gradients of B and C: the tiles of a group added in their order.
+template <typename TX>
+__global__ void __launch_bounds__(kThreads) ssm_sums_bc(SsmArgs a, int NP) {
+  const long long bt = (long long)a.B * a.T, n = bt * a.G * 2 * NP;
+  for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < n;
+       e += (long long)gridDim.x * kThreads) {
+    const long long row = e / (2 * NP);    // bt G + g
+    const int k = (int)(e - row * 2 * NP), g = (int)(row % a.G);
+    const int s = k % NP;
+    if (s >= a.N) continue;
+    const float* p = a.part_bc + ((long long)g * a.tiles * bt + row / a.G) * 2 * NP + k;
+    float v = 0.f;
+    for (int i = 0; i < a.tiles; ++i) v += p[i * bt * 2 * NP];
+    ((TX*)(k < NP ? a.dbm : a.dcm))[row * a.N + s] = (TX)v;
+  }
+}
+
+// One token: NG lanes a channel, four states each.
+struct StepArgs {
+  const void *x, *dt, *bm, *cm, *z;
+  const float *A, *D, *dt_bias, *h_in;
+  float* h_out;
+  void* out;
+  int B, C, G, N, Cg, softplus;
+};
+template <typename TX, typename TD, int NP>
+__global__ void __launch_bounds__(kThreads) ssm_step(StepArgs a) {
+  constexpr int NG = NP / 4;
+  const int q = threadIdx.x % NG;
+  const long long n = (long long)a.B * a.C;
+  // every lane group of a wave walks the same number of times: its exchanges need all lanes
+  const long long per = kThreads / NG, rounds = (n + per * gridDim.x - 1) / (per * gridDim.x);
+  for (long long r = 0; r < rounds; ++r) {
+    const long long e = (r * gridDim.x + blockIdx.x) * per + threadIdx.x / NG;
+    const bool on = e < n;
+    const long long bc = on ? e : n - 1;
+    const int b = (int)(bc / a.C), c = (int)(bc - (long long)b * a.C);
+    const long long g = (long long)b * a.G + c / a.Cg;
+    const float x = (float)((const TX*)a.x)[bc];
+    float d = (float)((const TD*)a.dt)[bc] + (a.dt_bias ? a.dt_bias[c] : 0.f);
+    if (a.softplus) d = softplus(d);
+    const float u = d * x;
+    float y = 0.f, h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = 4 * q + k;
+      h[k] = 0.f;
+      if (s < a.N) {
+        const float was = a.h_in ? a.h_in[bc * a.N + s] : 0.f;
+        const float in = u * (float)((const TX*)a.bm)[g * a.N + s];
+        h[k] = fmaf(exp2_(d * (a.A[(long long)c * a.N + s] * kLog2e)), was, in);
+        y = fmaf(h[k], (float)((const TX*)a.cm)[g * a.N + s], y);
+      }
+    }
+#pragma unroll
+    for (int m = 1; m < NG; m *= 2) y += __shfl_xor(y, m);
+    if (!on) continue;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (4 * q + k < a.N) a.h_out[bc * a.N + 4 * q + k] = h[k];
+    if (q == 0) {
+      if (a.D) y = fmaf(a.D[c], x, y);
+      if (a.z) {
+        const float z = (float)((const TX*)a.z)[bc];
+        y *= z * sigmoid(z);
+      }
+      ((TX*)a.out)[bc] = (TX)y;
+    }
+  }
+}
+
+// ---- Host ----------------------------------------------------------------------------
+
+int padded(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+
+// Channels of a workgroup of the backward.
+int bwd_tile(int NP) { return 4 * (64 / (NP / 4)); }
+
+struct Split {
+  int np, L, chunks;
+  int tiles, btiles;            // of a group: waves' (64 channels) and the backward's
+  size_t bc, slot, sum, part_bc, part_a, part_c;   // bytes, multiples of 16
+  size_t fwd() const { return bc + slot + sum; }
+  size_t bwd() const { return bc + slot + sum + part_bc + part_a + part_c; }
+};
+size_t round16(double n) { return ((size_t)n + 15) / 16 * 16; }
+
+// Chunks by sizes alone: the forward and the backward cut the axis alike.
+Split split(int B, int T, int C, int G, int N) {
+  Split s;
+  s.np = padded(N);
+  const int Cg = C / G;
+  s.tiles = (Cg + 63) / 64;
+  s.btiles = (Cg + bwd_tile(s.np) - 1) / bwd_tile(s.np);
+  // chunks of 128 tokens where they make some waves a SIMD, else of 64 or 32
+  s.L = 128;
+  while (s.L > 32 && (double)B * G * s.tiles * ((T + s.L - 1) / s.L) < 4096) s.L /= 2;
+  s.chunks = T ? (T + s.L - 1) / s.L : 1;
+  const double bt = (double)B * T, rows = (double)B * s.chunks;
+  s.bc = round16(bt * G * 2 * s.np * 4);
+  s.slot = s.chunks > 1 ? round16(rows * C * s.np * 4) : 0;
+  s.sum = s.chunks > 1 ? round16(rows * C * 4) : 0;
+  s.part_bc = round16((double)s.btiles * G * bt * 2 * s.np * 4);
+  s.part_a = round16(rows * C * s.np * 4);
+  s.part_c = round16(rows * 2 * C * 4);
+  return s;
+}
+
+int validate(int B, int T, int C, int G, int N, int in_dtype, int dt_dtype) {
+  if (B < 1 || T < 0 || C < 1 || G < 1 || G > C || C % G || N < 1 || N > 64) return GDN2_ERR_SHAPE;
+  if (T > INT_MAX - 1024 || C > (1 << 24)) return GDN2_ERR_SHAPE;
+  if (in_dtype != GDN2_F32 && in_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
+  if (dt_dtype != GDN2_F32 && dt_dtype != in_dtype) return GDN2_ERR_DTYPE;
+  // a launch's threads stay within 32 bits and its waves' numbers within 31: one wave for at
+  // least 32 tokens of at most 64 channels, one thread for a state
+  const Split s = split(B, T, C, G, N);
+  if ((double)B * G * s.tiles * s.chunks > (double)(1 << 25) ||
+      (double)B * G * s.btiles * s.chunks > (double)(1 << 23) ||
+      (double)B * C * s.np > (double)(1ll << 30))
+    return GDN2_ERR_SHAPE;
+  return GDN2_OK;
+}
+
+int check_rows(const Rows& r, int dtype, bool optional) {
+  if (!r.p) return optional ? GDN2_OK : GDN2_ERR_NULL;
+  return (uintptr_t)r.p % (dtype == GDN2_F32 ? 4 : 2) ? GDN2_ERR_ALIGN : GDN2_OK;
+}
+int check_f32(const void* p, bool optional) {
+  if (!p) return optional ? GDN2_OK : GDN2_ERR_NULL;
+  return (uintptr_t)p % 4 ? GDN2_ERR_ALIGN : GDN2_OK;
+}
+int check_ws(const void* p, size_t need, size_t have) {
+  if (!need) return GDN2_OK;
+  return !p ? GDN2_ERR_NULL : (uintptr_t)p % 16 ? GDN2_ERR_ALIGN
+         : have < need ? GDN2_ERR_WORKSPACE : GDN2_OK;
+}
+
+unsigned groups_of(double n, double per, double most = 65536) {
+  const double w = (n + per - 1) / per;
+  return (unsigned)(w < most ? w : most);
+}
+
+template <typename TX>
+void launch_rows(hipStream_t st, const SsmArgs& a, int NP) {
+  hipLaunchKernelGGL((ssm_rows<TX>), dim3(groups_of((double)a.B * a.T * a.G * 2 * NP, kThreads)),
+                     dim3(kThreads), 0, st, a, NP);
+}
+
+template <typename TX, typename TD, int NP>
+void launch_fwd(hipStream_t st, const SsmArgs& a) {
+  const long long waves = (long long)a.B * a.G * a.tiles;
+  launch_rows<TX>(st, a, NP);
+  if (a.chunks > 1) {
+    hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, false>),
+                       dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((ssm_join<NP, false>),
+                       dim3((unsigned)(((long long)a.B * a.C * NP + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, st, a);
+  }
+  hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, true>), dim3((unsigned)((waves * a.chunks + 3) / 4)),
+                     dim3(kThreads), 0, st, a);
+}
+
+template <typename TX, typename TD, int NP>
+void launch_bwd(hipStream_t st, SsmArgs a) {
+  const long long waves = (long long)a.B * a.G * a.tiles;
+  launch_rows<TX>(st, a, NP);
+  if (a.chunks > 1) {
+    hipLaunchKernelGGL((ssm_rev<TX, TD, NP>), dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)),
+                       dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((ssm_join<NP, true>),
+                       dim3((unsigned)(((long long)a.B * a.C * NP + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, st, a);
+  }
+  a.tiles = (a.Cg + bwd_tile(NP) - 1) / bwd_tile(NP);
+  hipLaunchKernelGGL((ssm_bwd<TX, TD, NP>),
+                     dim3((unsigned)((long long)a.B * a.G * a.tiles * a.chunks)), dim3(kThreads), 0,
+                     st, a);
+  hipLaunchKernelGGL((ssm_sums), dim3((unsigned)(((long long)a.C * (NP + 2) + 63) / 64)), dim3(1024),
+                     0, st, a, NP);
+  hipLaunchKernelGGL((ssm_sums_bc<TX>),
+                     dim3(groups_of((double)a.B * a.T * a.G * 2 * NP, kThreads)), dim3(kThreads), 0,
+                     st, a, NP);
+}
+
+template <typename TX, typename TD>
+hipError_t launch_types(hipStream_t st, const SsmArgs& a, bool bwd) {
+  switch (padded(a.N)) {
+#define GDN2_CASE(NP)                                                              \
+  case NP:                                                                         \
+    bwd ? launch_bwd<TX, TD, NP>(st, a) : launch_fwd<TX, TD, NP>(st, a);           \
+    break
+    GDN2_CASE(8);
+    GDN2_CASE(16);
+    GDN2_CASE(32);
+    GDN2_CASE(64);
+#undef GDN2_CASE
+  }
+  return hipGetLastError();
+}
+int launch(hipStream_t st, const SsmArgs& a, int in_dtype, int dt_dtype, bool bwd) {
+  const hipError_t e = in_dtype == GDN2_F32    ? launch_types<float, float>(st, a, bwd)
+                       : dt_dtype == GDN2_F32 ? launch_types<bf16_t, float>(st, a, bwd)
+                                              : launch_types<bf16_t, bf16_t>(st, a, bwd);
+  return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+template <typename TX, typename TD>
+hipError_t launch_step(hipStream_t st, const StepArgs& a) {
+  const int NP = padded(a.N);
+  const dim3 grid(groups_of((double)a.B * a.C, kThreads / (NP / 4))), block(kThreads);
+  switch (NP) {
+    case 8: hipLaunchKernelGGL((ssm_step<TX, TD, 8>), grid, block, 0, st, a); break;
+    case 16: hipLaunchKernelGGL((ssm_step<TX, TD, 16>), grid, block, 0, st, a); break;
+    case 32: hipLaunchKernelGGL((ssm_step<TX, TD, 32>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((ssm_step<TX, TD, 64>), grid, block, 0, st, a);
+  }
+  return hipGetLastError();
+}
+
+// The inputs that the forward and the backward share.
+int set_inputs(SsmArgs& a, int B, int T, int C, int G, int N, int in_dtype, int dt_dtype,
+               int softplus, const void* const* ins, const long long* strides, const float* A,
+               const float* D, const float* dt_bias, const unsigned char* starts) {
+  if (softplus != 0 && softplus != 1) return GDN2_ERR_FLAGS;
+  if (!ins) return GDN2_ERR_NULL;
+  const long long widths[5] = {C, C, C, (long long)G * N, (long long)G * N};
+  Rows* rows[5] = {&a.x, &a.dt, &a.z, &a.bm, &a.cm};
+  int rc;
+  for (int i = 0; i < 5; ++i) {
+    *rows[i] = Rows{ins[i], strides ? strides[2 * i] : T * widths[i],
+                    strides ? strides[2 * i + 1] : widths[i]};
+    if ((rc = check_rows(*rows[i], i == 1 ? dt_dtype : in_dtype, i == 2))) return rc;
+  }
+  if ((rc = check_f32(A, false)) || (rc = check_f32(D, true)) || (rc = check_f32(dt_bias, true)))
+    return rc;
+  a.A = A, a.D = D, a.dt_bias = dt_bias, a.starts = starts, a.softplus = softplus;
+  a.B = B, a.T = T, a.C = C, a.G = G, a.N = N, a.Cg = C / G;
+  return GDN2_OK;
+}
+void set_workspace(SsmArgs& a, const Split& s, void* ws) {
+  char* p = (char*)ws;
+  a.bc = (float*)p;
+  a.slot = (float*)(p += s.bc);
+  a.sum = (float*)(p += s.slot);
+  a.part_bc = (float*)(p += s.sum);
+  a.part_a = (float*)(p += s.part_bc);
+  a.part_c = (float*)(p += s.part_a);
+  a.tiles = s.tiles, a.L = s.L, a.chunks = s.chunks;
+}
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+size_t gdn2_selective_scan_kept_bytes(int B, int T, int C, int G, int N) {
+  if (validate(B, T, C, G, N, GDN2_F32, GDN2_F32) != GDN2_OK) return 0;
+  return (size_t)B * ((T + kKeep - 1) / kKeep) * C * padded(N) * sizeof(float);
+}
+
+size_t gdn2_selective_scan_workspace_bytes(int B, int T, int C, int G, int N, int backward) {
+  if (validate(B, T, C, G, N, GDN2_F32, GDN2_F32) != GDN2_OK || T == 0) return 0;
+  const Split s = split(B, T, C, G, N);
+  return backward ? s.bwd() : s.fwd();
+}
+
+int gdn2_selective_scan_fwd(void* stream, int B, int T, int C, int G, int N, int in_dtype,
+                            int dt_dtype, int softplus, const void* const* ins,
+                            const long long* strides, const float* A, const float* D,
+                            const float* dt_bias, const float* h0, const unsigned char* starts,
+                            void* out, float* h_final, float* kept, void* ws, size_t ws_bytes) {
+  int rc = validate(B, T, C, G, N, in_dtype, dt_dtype);
+  if (rc) return rc;
+  if (T == 0) return GDN2_ERR_SEQ_LEN;
+  SsmArgs a = {};
+  if ((rc = set_inputs(a, B, T, C, G, N, in_dtype, dt_dtype, softplus, ins, strides, A, D, dt_bias,
+                       starts)))
+    return rc;
+  if ((rc = check_rows({out, 0, 0}, in_dtype, false)) || (rc = check_f32(h_final, false)) ||
+      (rc = check_f32(h0, true)))
+    return rc;
+  if ((uintptr_t)kept % 16) return GDN2_ERR_ALIGN;
+  if (h0 == h_final) return GDN2_ERR_FLAGS;    // read by other workgroups
+  const Split s = split(B, T, C, G, N);
+  if ((rc = check_ws(ws, s.fwd(), ws_bytes))) return rc;
+  set_workspace(a, s, ws);
+  a.h0 = h0, a.out = out, a.h_final = h_final, a.kept = kept;
+  return launch((hipStream_t)stream, a, in_dtype, dt_dtype, false);
+}
+
+int gdn2_selective_scan_bwd(void* stream, int B, int T, int C, int G, int N, int in_dtype,
+                            int dt_dtype, int softplus, const void* const* ins,
+                            const long long* strides, const float* A, const float* D,
+                            const float* dt_bias, const unsigned char* starts, const void* dout,
+                            const long long* dout_strides, const float* dh_final,
+                            const float* kept, void* const* outs, float* dA, float* dD,
+                            float* ddt_bias, float* dh0, void* ws, size_t ws_bytes) {
+  int rc = validate(B, T, C, G, N, in_dtype, dt_dtype);
+  if (rc) return rc;
+  if (T == 0) return GDN2_ERR_SEQ_LEN;
+  SsmArgs a = {};
+  if ((rc = set_inputs(a, B, T, C, G, N, in_dtype, dt_dtype, softplus, ins, strides, A, D, dt_bias,
+                       starts)))
+    return rc;
+  if (!outs) return GDN2_ERR_NULL;
+  for (int i = 0; i < 5; ++i)
+    if ((rc = check_rows({outs[i], 0, 0}, i == 1 ? dt_dtype : in_dtype, i == 2 && !a.z.p)))
+      return rc;
+  a.dout = Rows{dout, dout_strides ? dout_strides[0] : (long long)T * C,
+                dout_strides ? dout_strides[1] : C};
+  if ((rc = check_rows(a.dout, in_dtype, true)) || (rc = check_f32(dh_final, true)) ||
+      (rc = check_f32(kept, false)) || (rc = check_f32(dA, false)) || (rc = check_f32(dD, true)) ||
+      (rc = check_f32(ddt_bias, true)) || (rc = check_f32(dh0, true)))
+    return rc;
+  if ((uintptr_t)kept % 16) return GDN2_ERR_ALIGN;
+  const Split s = split(B, T, C, G, N);
+  if ((rc = check_ws(ws, s.bwd(), ws_bytes))) return rc;
+  set_workspace(a, s, ws);
+  a.dx = outs[0], a.ddt = outs[1], a.dz = outs[2], a.dbm = outs[3], a.dcm = outs[4];
+  a.dh_final = dh_final, a.kept = const_cast<float*>(kept);
+  a.dA = dA, a.dD = dD, a.dbias = ddt_bias, a.dh0 = dh0;
+  return launch((hipStream_t)stream, a, in_dtype, dt_dtype, true);
+}
+
+int gdn2_selective_scan_step(void* stream, int B, int C, int G, int N, int in_dtype, int dt_dtype,
+                             int softplus, const void* x, const void* dt, const float* A,
+                             const void* Bm, const void* Cm, const float* D, const void* z,
+                             const float* dt_bias, const float* h_in, float* h_out, void* out) {
+  if (B < 0) return GDN2_ERR_SHAPE;
+  int rc = validate(1, 1, C, G, N, in_dtype, dt_dtype);
+  if (rc) return rc;
+  if (softplus != 0 && softplus != 1) return GDN2_ERR_FLAGS;
+  if (B == 0) return GDN2_OK;
+  for (const void* p : {x, Bm, Cm, (const void*)out})
+    if ((rc = check_rows({p, 0, 0}, in_dtype, false))) return rc;
+  if ((rc = check_rows({dt, 0, 0}, dt_dtype, false)) ||
+      (rc = check_rows({z, 0, 0}, in_dtype, true)))
+    return rc;
+  if ((rc = check_f32(A, false)) || (rc = check_f32(D, true)) || (rc = check_f32(dt_bias, true)) ||
+      (rc = check_f32(h_in, true)) || (rc = check_f32(h_out, false)))
+    return rc;
+  StepArgs a = {x, dt, Bm, Cm, z, A, D, dt_bias, h_in, h_out, out, B, C, G, N, C / G, softplus};
+  const hipError_t e =
+      in_dtype == GDN2_F32   ? launch_step<float, float>((hipStream_t)stream, a)
+      : dt_dtype == GDN2_F32 ? launch_step<bf16_t, float>((hipStream_t)stream, a)
+                             : launch_step<bf16_t, bf16_t>((hipStream_t)stream, a);
+  return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -105,6 +105,15 @@ SIGNATURES = {
     "gdn2_dequantize_int8": (_c_int, [_vp] + [_c_int] * 3 + [_vp, _c_ll, _vp, _vp]),
     "gdn2_int8_matmul": (_c_int, [_vp] + [_c_int] * 4 + [_vp, _c_ll, _vp, _vp, _c_ll]
                          + [_vp] * 3),
+    "gdn2_short_conv_fwd": (_c_int, [_vp] + [_c_int] * 6 + [_vp] * 8),
+    "gdn2_short_conv_bwd_workspace_bytes": (_c_size, [_c_int] * 4),
+    "gdn2_short_conv_bwd": (_c_int, [_vp] + [_c_int] * 6 + [_vp] * 14 + [_c_size]),
+    "gdn2_short_conv_step": (_c_int, [_vp] + [_c_int] * 5 + [_vp] * 6),
+    "gdn2_selective_scan_kept_bytes": (_c_size, [_c_int] * 5),
+    "gdn2_selective_scan_workspace_bytes": (_c_size, [_c_int] * 6),
+    "gdn2_selective_scan_fwd": (_c_int, [_vp] + [_c_int] * 8 + [_vp] * 11 + [_c_size]),
+    "gdn2_selective_scan_bwd": (_c_int, [_vp] + [_c_int] * 8 + [_vp] * 16 + [_c_size]),
+    "gdn2_selective_scan_step": (_c_int, [_vp] + [_c_int] * 7 + [_vp] * 11),
 }
 
 

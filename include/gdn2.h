@@ -441,6 +441,81 @@ int gdn2_int8_matmul(void* stream, int M, int N, int K, int out_dtype, const voi
                      long long x_stride, const float* x_scale, const void* w,
                      long long w_stride, const float* w_scale, const float* bias, void* out);
 
+/* ---- Short causal convolution --------------------------------------------------
+ * Over each channel of (B,T,C) tensors (no counterpart in the reference):
+ *   y_t = act(bias + sum_{k < W} w[k] x_{t - W + 1 + k}),   2 <= W <= 4,
+ * act the identity (silu = 0) or v / (1 + e^{-v}) (silu = 1).  state (B,W-1,C) holds the
+ * inputs before the first token, oldest first (NULL: zeros), last the W - 1 inputs up to the
+ * last token; w (C,W) and bias (C, or NULL) are float32, all else is of dtype (GDN2_F32,
+ * GDN2_BF16).  starts (B,T) bytes, or NULL: a token whose byte is not zero begins a sequence,
+ * nothing from before it enters, and the entries of `last` before the last such token are zero.
+ * x and dy may be strided as for the gated recurrence; all else is dense.  Pointers are
+ * aligned to their elements (faster: to four, with strides and C % 4 == 0).  T >= 1;
+ * float32 sums. */
+int gdn2_short_conv_fwd(void* stream, int B, int T, int C, int W, int dtype, int silu,
+                        const void* x, const long long* x_strides, const float* w,
+                        const float* bias, const void* state, const unsigned char* starts,
+                        void* y, void* last /* not state */);
+
+/* Gradients from those of y and last (dy, dlast: either may be NULL, zero): dx, dw (C,W),
+ * dbias (C, or NULL) and dstate (B,W-1,C, or NULL). */
+size_t gdn2_short_conv_bwd_workspace_bytes(int B, int T, int C, int W);
+int gdn2_short_conv_bwd(void* stream, int B, int T, int C, int W, int dtype, int silu,
+                        const void* x, const long long* x_strides, const float* w,
+                        const float* bias, const void* state, const unsigned char* starts,
+                        const void* dy, const long long* dy_strides, const void* dlast, void* dx,
+                        float* dw, float* dbias, void* dstate, void* ws, size_t ws_bytes);
+
+/* One token, x and y (B,C); state_in may be NULL (zeros) and equal to state_out. */
+int gdn2_short_conv_step(void* stream, int B, int C, int W, int dtype, int silu, const void* x,
+                         const float* w, const float* bias, const void* state_in,
+                         void* state_out, void* y);
+
+/* ---- Selective state space scan --------------------------------------------------
+ * Over (B,T,C) tensors with N <= 64 states a channel (no counterpart in the reference):
+ *   d = dt + dt_bias, with softplus = 1 log(1 + e^d);
+ *   h_t[c,n] = e^{d_t[c] A[c,n]} h_{t-1}[c,n] + d_t[c] x_t[c] Bm_t[n];
+ *   y_t[c] = sum_n Cm_t[n] h_t[c,n] + D[c] x_t[c];   out_t = y_t z_t / (1 + e^{-z_t}).
+ * Bm and Cm (B,T,G,N) are shared by the C / G channels of a group.  A (C,N), D (C, or NULL: 0),
+ * dt_bias (C, or NULL: 0), h0, h_final and their gradients (B,C,N) are float32; x, Bm, Cm, z
+ * (NULL: no gate), out, dout and their gradients are of in_dtype (GDN2_F32, GDN2_BF16), dt and
+ * ddt of dt_dtype (GDN2_F32, or in_dtype).  Float32 arithmetic; the sums of d A over any run
+ * of tokens must stay below 88 (d >= 0 and A <= 0 in use).  starts: as for the convolution, the
+ * state before such a token is dropped and no gradient passes it.
+ * ins: host array of x, dt, z, Bm, Cm; strides: NULL (dense) or ten host integers, for each of
+ * them the elements from one batch entry and one token to the next; the rest of a row is
+ * contiguous.  Pointers are aligned to their elements, kept and ws to 16 bytes.  T >= 1. */
+
+/* Bytes of the states kept for the backward (float32, one for every 16 tokens, N padded to 8,
+ * 16, 32 or 64) and of the workspace of the forward or the backward. */
+size_t gdn2_selective_scan_kept_bytes(int B, int T, int C, int G, int N);
+size_t gdn2_selective_scan_workspace_bytes(int B, int T, int C, int G, int N, int backward);
+
+/* h0 may be NULL (zero; not h_final); kept may be NULL (inference). */
+int gdn2_selective_scan_fwd(void* stream, int B, int T, int C, int G, int N, int in_dtype,
+                            int dt_dtype, int softplus, const void* const* ins,
+                            const long long* strides, const float* A, const float* D,
+                            const float* dt_bias, const float* h0, const unsigned char* starts,
+                            void* out, float* h_final, float* kept, void* ws, size_t ws_bytes);
+
+/* Gradients from those of out and h_final (either may be NULL: zero), the forward's inputs
+ * and its kept states.  outs: host array of dx, ddt, dz (NULL without z), dBm, dCm, all dense;
+ * dD, ddt_bias and dh0 are written where they are not NULL. */
+int gdn2_selective_scan_bwd(void* stream, int B, int T, int C, int G, int N, int in_dtype,
+                            int dt_dtype, int softplus, const void* const* ins,
+                            const long long* strides, const float* A, const float* D,
+                            const float* dt_bias, const unsigned char* starts, const void* dout,
+                            const long long* dout_strides, const float* dh_final,
+                            const float* kept, void* const* outs, float* dA, float* dD,
+                            float* ddt_bias, float* dh0, void* ws, size_t ws_bytes);
+
+/* One token: x, dt, z, out (B,C), Bm, Cm (B,G,N), all dense; h_in may be NULL (zero) and
+ * equal to h_out. */
+int gdn2_selective_scan_step(void* stream, int B, int C, int G, int N, int in_dtype, int dt_dtype,
+                             int softplus, const void* x, const void* dt, const float* A,
+                             const void* Bm, const void* Cm, const float* D, const void* z,
+                             const float* dt_bias, const float* h_in, float* h_out, void* out);
+
 #ifdef __cplusplus
 }
 #endif
