@@ -32,6 +32,7 @@ constexpr int kThreads = 256;
 constexpr int kKeep = 16;      // tokens between kept states
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_inff();
+constexpr long long kMaxStride = 1 << 25;   // elements from one token to the next
 
 // Strides are in elements; channels are contiguous.
 struct Rows {
@@ -77,13 +78,20 @@ __device__ __forceinline__ float softplus(float v) {
 }
 __device__ __forceinline__ float sigmoid(float v) { return rcp_(1.f + exp2_(-v * kLog2e)); }
 
-// Float32 values that are the same for all lanes of a wave: read through the scalar cache.
-typedef const __attribute__((address_space(4))) float* uniform_ptr;
-__device__ __forceinline__ uniform_ptr uniform(const float* p) { return (uniform_ptr)(uintptr_t)p; }
-
 template <typename T>
 __device__ __forceinline__ float element(const Rows& r, int b, int t, int c) {
   return (float)((const T*)r.p)[b * r.sb + t * r.st + c];
+}
+
+// A value at a distance in bytes from a place that is the same for all lanes: one address in
+// scalar registers, 32 bits a lane.
+template <typename T>
+__device__ __forceinline__ T at(const T* p, unsigned off) {
+  return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + off);
+}
+template <typename T>
+__device__ __forceinline__ void put(T* p, unsigned off, T v) {
+  *reinterpret_cast<T*>(reinterpret_cast<char*>(p) + off) = v;
 }
 
 // B and C in float32, NP states each.
@@ -139,16 +147,50 @@ __device__ __forceinline__ void store_states(float* p, const float (&h)[NP]) {
   for (int n = 0; n < NP; n += 4)
     *reinterpret_cast<f32x4*>(p + n) = f32x4{h[n], h[n + 1], h[n + 2], h[n + 3]};
 }
+// N values at p, the others zero (all of them without p); no branches, so one wait for all.
 template <int NP>
 __device__ __forceinline__ void load_user(const float* p, int N, float (&h)[NP]) {
 #pragma unroll
-  for (int n = 0; n < NP; ++n) h[n] = p && n < N ? p[n] : 0.f;
+  for (int n = 0; n < NP; ++n) h[n] = 0.f;
+  if (!p) return;
+  float v[NP];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) v[n] = p[n < N ? n : N - 1];
+#pragma unroll
+  for (int n = 0; n < NP; ++n) h[n] = n < N ? v[n] : 0.f;
 }
 
+// Rows of B and C (W floats from `from` on of each row of bc) of 16 tokens in LDS, a part for each
+// wave: a token's row is then the same 16-byte reads for all lanes.  (In scalar registers, read
+// token by token, every token waited for its row: 1 x 4001 x 1536 x 16 composed in 38 us, so 30.)
+template <int W>
+struct WaveRows {
+  static constexpr int PIECES = kKeep * W / 4, PER = (PIECES + 63) / 64;
+  f32x4 r[PER];
+  __device__ __forceinline__ void load(const float* rows, long long stride, int t, int t1) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int p = i * 64 + (threadIdx.x & 63), k = p / (W / 4);
+      const int ti = t + k < t1 ? t + k : t1 - 1;
+      r[i] = *reinterpret_cast<const f32x4*>(rows + ti * stride + p % (W / 4) * 4);
+    }
+  }
+  __device__ __forceinline__ void store(float* lds) const {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int p = i * 64 + (threadIdx.x & 63);
+      if (PIECES % 64 == 0 || p < PIECES) *reinterpret_cast<f32x4*>(lds + 4 * p) = r[i];
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
 // Forward.  OUT: the tokens from the entering state, outputs and kept states; else the
-// composition of chunks 0 .. chunks - 2, H of chunk k into slot k + 1.
-template <typename TX, typename TD, int NP, bool OUT>
-__global__ void __launch_bounds__(kThreads) ssm_fwd(SsmArgs a) {
+// composition of chunks 0 .. chunks - 2, H of chunk k into slot k + 1.  STARTS apart: a branch in
+// every token costs a copy of all states (8 x 8192 x 768 x 16 composed in 201 us, without 178).
+template <typename TX, typename TD, int NP, bool STARTS, bool OUT>
+__global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a) {
   const WavePlace w(a, 0, OUT ? a.chunks : a.chunks - 1);
   if (w.idle) return;
   const int nch = a.chunks;
@@ -167,9 +209,10 @@ __global__ void __launch_bounds__(kThreads) ssm_fwd(SsmArgs a) {
       load_states<NP>(a.slot + (((long long)w.b * nch + w.chunk) * a.C + w.c) * NP, h);
   }
   const int nb = (a.T + kKeep - 1) / kKeep;
-  const TX* px = (const TX*)a.x.p + w.b * a.x.sb + w.c;
-  const TD* pd = (const TD*)a.dt.p + w.b * a.dt.sb + w.c;
-  const TX* pz = (const TX*)a.z.p + w.b * a.z.sb + w.c;
+  const TX* px = (const TX*)a.x.p + w.b * a.x.sb;
+  const TD* pd = (const TD*)a.dt.p + w.b * a.dt.sb;
+  const TX* pz = (const TX*)a.z.p + w.b * a.z.sb;
+  const unsigned ox = (unsigned)w.c * sizeof(TX), od = (unsigned)w.c * sizeof(TD);
   const bool gate = OUT && a.z.p;
   TX rx[kAhead], rz[kAhead];
   TD rd[kAhead];
@@ -177,53 +220,75 @@ __global__ void __launch_bounds__(kThreads) ssm_fwd(SsmArgs a) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const long long ti = t + i < w.t1 ? t + i : w.t1 - 1;
-      rx[i] = px[ti * a.x.st];
-      rd[i] = pd[ti * a.dt.st];
-      if (gate) rz[i] = pz[ti * a.z.st];
+      rx[i] = at(px + ti * a.x.st, ox);
+      rd[i] = at(pd + ti * a.dt.st, od);
+      if (gate) rz[i] = at(pz + ti * a.z.st, ox);
     }
   };
   load(w.t0);
   float S = 0.f;
   bool fresh = false;
-  TX* out = (TX*)a.out + ((long long)w.b * a.T) * a.C + w.c;
+  TX* out = (TX*)a.out + (long long)w.b * a.T * a.C;
+  constexpr int RW = OUT ? 2 * NP : NP;
+  __shared__ __attribute__((aligned(16))) float lds[kThreads / 64][kKeep * RW];
+  float* own = lds[threadIdx.x >> 6];
+  const long long stride = (long long)a.G * 2 * NP;
+  const float* bc = a.bc + (long long)w.b * a.T * stride + w.g * 2 * NP;
+  WaveRows<RW> rows;
+  rows.load(bc, stride, w.t0, w.t1);
+  auto token = [&](int t, float x, float d, float z) {
+    if (STARTS && a.starts[(long long)w.b * a.T + t]) {
+      fresh = true;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) h[n] = 0.f;
+    }
+    const float* row = own + t % kKeep * RW;
+    const float u = d * x;
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NP; n += 4) {
+      const f32x4 Bv = *reinterpret_cast<const f32x4*>(row + n);
+      f32x4 Cv;
+      if (OUT) Cv = *reinterpret_cast<const f32x4*>(row + NP + n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        h[n + k] = fmaf(exp2_(d * A2[n + k]), h[n + k], u * Bv[k]);
+        if (OUT) y[k] = fmaf(h[n + k], Cv[k], y[k]);
+      }
+    }
+    S += d;
+    if (OUT) {
+      float o = fmaf(D, x, (y[0] + y[1]) + (y[2] + y[3]));
+      if (gate) o *= z * sigmoid(z);
+      if (w.on) put(out + (long long)t * a.C, ox, (TX)o);
+    }
+  };
   for (int t = w.t0; t < w.t1; t += kAhead) {
-    if (OUT && a.kept && t % kKeep == 0 && w.on)
-      store_states<NP>(a.kept + (((long long)w.b * nb + t / kKeep) * a.C + w.c) * NP, h);
+    if (t % kKeep == 0) {
+      rows.store(own);
+      if (t + kKeep < w.t1) rows.load(bc, stride, t + kKeep, w.t1);
+      if (OUT && a.kept && w.on)
+        store_states<NP>(a.kept + (((long long)w.b * nb + t / kKeep) * a.C + w.c) * NP, h);
+    }
     float x[kAhead], d[kAhead], z[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       x[i] = (float)rx[i];
       d[i] = (float)rd[i] + bias;
-      if (gate) z[i] = (float)rz[i];
+      z[i] = gate ? (float)rz[i] : 0.f;
     }
     if (a.softplus) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
     }
     if (t + kAhead < w.t1) load(t + kAhead);
+    if (t + kAhead <= w.t1) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (t + i >= w.t1) break;
-      const long long bt = (long long)w.b * a.T + t + i;
-      if (a.starts && a.starts[bt]) {
-        fresh = true;
+      for (int i = 0; i < kAhead; ++i) token(t + i, x[i], d[i], z[i]);
+    } else {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) h[n] = 0.f;
-      }
-      const uniform_ptr row = uniform(a.bc) + (bt * a.G + w.g) * 2 * NP;
-      const float u = d[i] * x[i];
-      float y0 = 0.f, y1 = 0.f;
-#pragma unroll
-      for (int n = 0; n < NP; ++n) {
-        h[n] = fmaf(exp2_(d[i] * A2[n]), h[n], u * row[n]);
-        if (OUT) (n & 1 ? y1 : y0) = fmaf(h[n], row[NP + n], n & 1 ? y1 : y0);
-      }
-      S += d[i];
-      if (OUT) {
-        float y = fmaf(D, x[i], y0 + y1);
-        if (gate) y *= z[i] * sigmoid(z[i]);
-        if (w.on) out[(long long)(t + i) * a.C] = (TX)y;
-      }
+      for (int i = 0; i < kAhead - 1; ++i)
+        if (t + i < w.t1) token(t + i, x[i], d[i], z[i]);
     }
   }
   if (!w.on) return;
@@ -240,8 +305,8 @@ __global__ void __launch_bounds__(kThreads) ssm_fwd(SsmArgs a) {
 
 // The gradient that leaves chunks 1 .. chunks - 1 at their beginning with none entering, into the
 // slot of the chunk before, and S.
-template <typename TX, typename TD, int NP>
-__global__ void __launch_bounds__(kThreads) ssm_rev(SsmArgs a) {
+template <typename TX, typename TD, int NP, bool STARTS>
+__global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a) {
   const WavePlace w(a, 1, a.chunks - 1);
   if (w.idle) return;
   const int nch = a.chunks;
@@ -253,9 +318,10 @@ __global__ void __launch_bounds__(kThreads) ssm_rev(SsmArgs a) {
     e[n] = 0.f;
   }
   const float bias = a.dt_bias ? a.dt_bias[w.c] : 0.f;
-  const TX* po = (const TX*)a.dout.p + w.b * a.dout.sb + w.c;
-  const TD* pd = (const TD*)a.dt.p + w.b * a.dt.sb + w.c;
-  const TX* pz = (const TX*)a.z.p + w.b * a.z.sb + w.c;
+  const TX* po = (const TX*)a.dout.p + w.b * a.dout.sb;
+  const TD* pd = (const TD*)a.dt.p + w.b * a.dt.sb;
+  const TX* pz = (const TX*)a.z.p + w.b * a.z.sb;
+  const unsigned ox = (unsigned)w.c * sizeof(TX), od = (unsigned)w.c * sizeof(TD);
   const bool gate = a.z.p, has = a.dout.p;
   TX ro[kAhead], rz[kAhead];
   TD rd[kAhead];
@@ -263,14 +329,43 @@ __global__ void __launch_bounds__(kThreads) ssm_rev(SsmArgs a) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const long long ti = t - i > w.t0 ? t - i : w.t0;
-      if (has) ro[i] = po[ti * a.dout.st];
-      rd[i] = pd[ti * a.dt.st];
-      if (gate) rz[i] = pz[ti * a.z.st];
+      if (has) ro[i] = at(po + ti * a.dout.st, ox);
+      rd[i] = at(pd + ti * a.dt.st, od);
+      if (gate) rz[i] = at(pz + ti * a.z.st, ox);
     }
   };
   load(w.t1 - 1);
   float S = 0.f;
   bool fresh = false;
+  __shared__ __attribute__((aligned(16))) float lds[kThreads / 64][kKeep * NP];
+  float* own = lds[threadIdx.x >> 6];
+  const long long stride = (long long)a.G * 2 * NP;
+  const float* bc = a.bc + (long long)w.b * a.T * stride + (w.g * 2 + 1) * NP;
+  WaveRows<NP> rows;
+  const int block = (w.t1 - 1) / kKeep * kKeep;
+  rows.load(bc, stride, block, w.t1);
+  rows.store(own);
+  if (block > w.t0) rows.load(bc, stride, block - kKeep, w.t1);
+  auto token = [&](int t, float g, float d) {
+    const float* row = own + t % kKeep * NP;
+#pragma unroll
+    for (int n = 0; n < NP; n += 4) {
+      const f32x4 Cv = *reinterpret_cast<const f32x4*>(row + n);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        e[n + k] = exp2_(d * A2[n + k]) * fmaf(g, Cv[k], e[n + k]);
+    }
+    if (t % kKeep == 0 && t > w.t0) {   // the sixteen tokens before this one are next
+      rows.store(own);
+      if (t - kKeep > w.t0) rows.load(bc, stride, t - 2 * kKeep, w.t1);
+    }
+    S += d;
+    if (STARTS && a.starts[(long long)w.b * a.T + t]) {
+      fresh = true;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) e[n] = 0.f;
+    }
+  };
   for (int t = w.t1 - 1; t >= w.t0; t -= kAhead) {
     float g[kAhead], d[kAhead];
 #pragma unroll
@@ -287,19 +382,13 @@ __global__ void __launch_bounds__(kThreads) ssm_rev(SsmArgs a) {
       for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
     }
     if (t - kAhead >= w.t0) load(t - kAhead);
+    if (t - kAhead + 1 >= w.t0) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (t - i < w.t0) break;
-      const long long bt = (long long)w.b * a.T + t - i;
-      const uniform_ptr row = uniform(a.bc) + ((bt * a.G + w.g) * 2 + 1) * NP;
+      for (int i = 0; i < kAhead; ++i) token(t - i, g[i], d[i]);
+    } else {
 #pragma unroll
-      for (int n = 0; n < NP; ++n) e[n] = exp2_(d[i] * A2[n]) * fmaf(g[i], row[n], e[n]);
-      S += d[i];
-      if (a.starts && a.starts[bt]) {
-        fresh = true;
-#pragma unroll
-        for (int n = 0; n < NP; ++n) e[n] = 0.f;
-      }
+      for (int i = 0; i < kAhead - 1; ++i)
+        if (t - i >= w.t0) token(t - i, g[i], d[i]);
     }
   }
   if (!w.on) return;
@@ -346,67 +435,67 @@ __global__ void __launch_bounds__(kThreads) ssm_join(SsmArgs a) {
 
 // ---- Backward ----------------------------------------------------------------------
 
-// The value of the lane whose number differs in bit BIT, where lanes that differ in lower bits
-// alone may be exchanged for one another beforehand (all that is needed to sum over lanes).
+// v + the value of the lane whose number differs in bit BIT, for sums over the low bits from bit 0
+// on: lanes that differ in lower bits alone hold the same by then, so a mirror will do.
 template <int BIT>
-__device__ __forceinline__ float partner(float v) {
-  const int i = __builtin_bit_cast(int, v);
-  if constexpr (BIT == 0)
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0xB1, 0xF, 0xF, true));
-  else if constexpr (BIT == 1)
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x4E, 0xF, 0xF, true));
-  else if constexpr (BIT == 2)   // row_half_mirror: lane 7 - l of eight
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x141, 0xF, 0xF, true));
-  else if constexpr (BIT == 3)   // row_mirror: lane 15 - l of sixteen
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, i, 0x140, 0xF, 0xF, true));
-  else
-    return __shfl_xor(v, 1 << BIT);
+__device__ __forceinline__ float add_low(float v) {
+  constexpr int ctrl = BIT == 0 ? 0xB1 : BIT == 1 ? 0x4E : BIT == 2 ? 0x141 : 0x140;
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                 0, __builtin_bit_cast(int, v), ctrl, 0xF, 0xF, true));
 }
-// v0 (v1) summed over lane pairs that differ in bit BIT, in the lanes where the bit is 0 (1).
-template <int BIT>
-__device__ __forceinline__ float fold(float v0, float v1, int lane) {
-  const bool high = lane >> BIT & 1;
-  return (high ? v1 : v0) + partner<BIT>(high ? v0 : v1);
+// Sum over the low LN bits of the lane's number.
+template <int LN>
+__device__ __forceinline__ float sum_low(float v) {
+  v = add_low<0>(v);
+  if constexpr (LN > 1) v = add_low<1>(v);
+  if constexpr (LN > 2) v = add_low<2>(v);
+  if constexpr (LN > 3) v = add_low<3>(v);
+  return v;
 }
-template <int BIT>
-__device__ __forceinline__ float whole(float v) { return v + partner<BIT>(v); }
-
-// Eight sums over the lanes' low LG bits: from the highest bit down, three folds deal the values out
-// to the lanes, the rest is summed whole.  On return the lane holds the value whose number
-// has as its bits the lane's bits LG - 1, LG - 2, LG - 3 (as many as there are; v[0], or v[0..1]
-// ... where there are fewer).
-template <int LG>
-__device__ __forceinline__ void sum_lanes8(float (&v)[8], int lane) {
-  static_assert(LG >= 2 && LG <= 5, "4 to 32 lanes");
+// v0 and v1 summed over lane pairs that differ in bit 5 (4): v0's sum where the bit is 0, v1's
+// where it is 1.
+__device__ __forceinline__ float fold5(float v0, float v1) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v0), __float_as_uint(v1), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float fold4(float v0, float v1) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v0), __float_as_uint(v1), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int N>
+__device__ __forceinline__ float add_rotated(float v) {   // within 16 lanes
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                 0, __builtin_bit_cast(int, v), 0x120 + N, 0xF, 0xF, true));
+}
+// Eight sums over all bits of the lane's number from LN on.  On return v[0] and v[1] are those of
+// numbers 4 (bit 5) + 2 (bit 4) + 0 and 1.
+template <int LN>
+__device__ __forceinline__ void sum_high8(float (&v)[8]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = fold<LG - 1>(v[k], v[k + 4], lane);
+  for (int k = 0; k < 4; ++k) v[k] = fold5(v[k], v[k + 4]);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) v[k] = fold<LG - 2>(v[k], v[k + 2], lane);
-  if constexpr (LG >= 3) v[0] = fold<LG - 3>(v[0], v[1], lane);
-  if constexpr (LG >= 4) v[0] = whole<LG - 4>(v[0]);
-  if constexpr (LG >= 5) v[0] = whole<LG - 5>(v[0]);
-}
-
-// Sum over the lane bits FROM .. 5.
-template <int FROM>
-__device__ __forceinline__ float sum_high(float v) {
-  if constexpr (FROM <= 2) v = v + __shfl_xor(v, 4);
-  if constexpr (FROM <= 3) v = v + __shfl_xor(v, 8);
-  if constexpr (FROM <= 4) v = v + __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  for (int k = 0; k < 2; ++k) {
+    v[k] = fold4(v[k], v[k + 2]);
+    if constexpr (LN <= 3) v[k] = add_rotated<8>(v[k]);
+    if constexpr (LN <= 2) v[k] = add_rotated<4>(v[k]);
+    if constexpr (LN <= 1) v[k] = add_rotated<2>(v[k]);
+  }
 }
 
 // A workgroup walks a chunk of CT channels backwards, 16 tokens at a time.
-template <typename TX, typename TD, int NP>
+template <int NP>
 struct Bwd {
-  static constexpr int NG = NP / 4;          // lane groups, four states each
+  static constexpr int NG = NP / 4;          // lanes of a channel, four states each
+  static constexpr int LN = NG == 2 ? 1 : NG == 4 ? 2 : NG == 8 ? 3 : 4;
   static constexpr int CH = 64 / NG;         // channels of a wave
-  static constexpr int LG = CH == 32 ? 5 : CH == 16 ? 4 : CH == 8 ? 3 : 2;
   static constexpr int CT = 4 * CH;          // and of a workgroup
   static constexpr int PER = kKeep * CT / kThreads;   // (token, channel) values of a thread
   static constexpr int STEP = kThreads / CT;          // tokens that the threads cover at a time
   struct Shared {
     float d[kKeep][CT], x[kKeep][CT], dy[kKeep][CT];
+    float raw[kKeep][CT], dout[kKeep][CT], z[kKeep][CT];
     float sb[kKeep][CT], sa[kKeep][CT], y[kKeep][CT];   // sums over the states
     float bc[kKeep][2][NP];
     float red[4][kKeep][2][NP];                         // sums over a wave's channels
@@ -414,10 +503,10 @@ struct Bwd {
   };
 };
 
-template <typename TX, typename TD, int NP>
+template <typename TX, typename TD, int NP, bool STARTS>
 __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
-  using P = Bwd<TX, TD, NP>;
-  constexpr int CH = P::CH, CT = P::CT, PER = P::PER, STEP = P::STEP, LG = P::LG;
+  using P = Bwd<NP>;
+  constexpr int NG = P::NG, CH = P::CH, CT = P::CT, PER = P::PER, STEP = P::STEP, LN = P::LN;
   __shared__ __attribute__((aligned(16))) typename P::Shared s;
   const int nt = a.G * a.tiles;
   const int tile = blockIdx.x % nt, rest = blockIdx.x / nt;
@@ -436,16 +525,15 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
   const bool gate = a.z.p, has = a.dout.p;
 
   // this lane's channel and states
-  const int ci = wave * CH + lane % CH, q = lane / CH;
+  const int ci = wave * CH + lane / NG, q = lane % NG;
   const bool on = first + ci < a.Cg;
   const int c = g * a.Cg + (on ? first + ci : 0);
-  float A[4], A2[4], e[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
+  float A[4], e[4], dA[4] = {0.f, 0.f, 0.f, 0.f};
   const long long bc_c = (long long)b * a.C + c;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int n = 4 * q + k;
     A[k] = n < a.N ? a.A[(long long)c * a.N + n] : 0.f;
-    A2[k] = A[k] * kLog2e;
     e[k] = 0.f;
     if (chunk == a.chunks - 1 && a.dh_final && n < a.N) e[k] = a.dh_final[bc_c * a.N + n];
   }
@@ -456,109 +544,165 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
     for (int k = 0; k < 4; ++k) e[k] = v[k];
   }
 
+  // What sixteen tokens need is loaded while the sixteen after them are worked on.  Rows: tokens ri,
+  // ri + STEP, ... of this thread's channel; every sixteen tokens but the last lie in the chunk.
+  constexpr int ROW = 2 * NP, BC = kKeep * ROW / kThreads;   // values of a thread of B's and C's rows
+  const int last = (t1 - t0 - 1) / kKeep * kKeep + t0;
+  const int c0 = g * a.Cg;
+  const long long bt = (long long)b * a.T + last;
+  const TX* px = (const TX*)a.x.p + b * a.x.sb + last * a.x.st + c0;
+  const TD* pd = (const TD*)a.dt.p + b * a.dt.sb + last * a.dt.st + c0;
+  const TX* po = (const TX*)a.dout.p + b * a.dout.sb + last * a.dout.st + c0;
+  const TX* pz = (const TX*)a.z.p + b * a.z.sb + last * a.z.st + c0;
+  const float* pbc = a.bc + (bt * a.G + g) * ROW;
+  const float* pk = a.kept + (((long long)b * nb + last / kKeep) * a.C + c0) * NP;
+  const unsigned char* ps = a.starts + bt;
+  const unsigned cc = r_c - c0, ok = ((c - c0) * NP + 4 * q) * 4;
   TX rx[PER], ro[PER], rz[PER];
   TD rd[PER];
-  auto load = [&](int t) {
+  float rbc[BC];
+  f32x4 rk;
+  bool rs = false;
+  // first: the tokens at the chunk's end, of which not all need exist (the last one instead)
+  auto load = [&](auto first) {
+    constexpr bool FIRST = decltype(first)::value;
+    const int most = t1 - last - 1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int ti = t + ri + i * STEP < t1 ? t + ri + i * STEP : t1 - 1;
-      rx[i] = ((const TX*)a.x.p)[b * a.x.sb + ti * a.x.st + r_c];
-      rd[i] = ((const TD*)a.dt.p)[b * a.dt.sb + ti * a.dt.st + r_c];
-      if (has) ro[i] = ((const TX*)a.dout.p)[b * a.dout.sb + ti * a.dout.st + r_c];
-      if (gate) rz[i] = ((const TX*)a.z.p)[b * a.z.sb + ti * a.z.st + r_c];
+      const unsigned k = FIRST && ri + i * STEP > most ? most : ri + (FIRST ? i * STEP : 0);
+      const long long m = FIRST ? 0 : i * STEP;
+      rx[i] = at(px + m * a.x.st, (k * (unsigned)a.x.st + cc) * (unsigned)sizeof(TX));
+      rd[i] = at(pd + m * a.dt.st, (k * (unsigned)a.dt.st + cc) * (unsigned)sizeof(TD));
+      if (has) ro[i] = at(po + m * a.dout.st, (k * (unsigned)a.dout.st + cc) * (unsigned)sizeof(TX));
+      if (gate) rz[i] = at(pz + m * a.z.st, (k * (unsigned)a.z.st + cc) * (unsigned)sizeof(TX));
     }
+#pragma unroll
+    for (int i = 0; i < BC; ++i) {
+      constexpr int S = kThreads / ROW;
+      const unsigned j = tid / ROW, k = FIRST && (int)j + i * S > most ? most
+                                                                     : j + (FIRST ? i * S : 0);
+      const long long m = FIRST ? 0 : i * S;
+      rbc[i] = at(pbc + m * a.G * ROW, (k * (unsigned)a.G * ROW + tid % ROW) * 4u);
+    }
+    rk = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(pk) + ok);
+    if (STARTS) rs = lane < kKeep && (!FIRST || lane <= most) && at(ps, (unsigned)lane);
   };
-  const int last = (t1 - t0 - 1) / kKeep * kKeep + t0;
-  load(last);
+  load(std::true_type{});
+  const unsigned oo = ri * (unsigned)a.C + cc;      // of the rows that are written
+  const long long o0 = bt * a.C + c0;
+  TX *pdx = (TX*)a.dx + o0, *pdz = (TX*)a.dz + o0;
+  TD* pdd = (TD*)a.ddt + o0;
+  float* pp = a.part_bc + (((long long)tile * a.B + b) * a.T + last) * ROW;
   for (int t = last; t >= t0; t -= kKeep) {
     // stage: tokens past the end are neutral (d = x = dy = 0)
-    float raw[PER], xv[PER], zv[PER], ov[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int k = ri + i * STEP;
       const bool real = r_on && t + k < t1;
-      xv[i] = real ? (float)rx[i] : 0.f;
-      ov[i] = real && has ? (float)ro[i] : 0.f;
-      zv[i] = real && gate ? (float)rz[i] : 0.f;
-      raw[i] = (float)rd[i] + bias;
-      const float d = a.softplus ? softplus(raw[i]) : raw[i];
+      const float o = real && has ? (float)ro[i] : 0.f, raw = (float)rd[i] + bias;
+      const float d = a.softplus ? softplus(raw) : raw;
       s.d[k][rc] = real ? d : 0.f;
-      s.x[k][rc] = xv[i];
-      s.dy[k][rc] = gate ? ov[i] * zv[i] * sigmoid(zv[i]) : ov[i];
+      s.x[k][rc] = real ? (float)rx[i] : 0.f;
+      s.raw[k][rc] = raw;
+      s.dout[k][rc] = o;
+      float dy = o;
+      if (gate) {
+        const float z = real ? (float)rz[i] : 0.f;
+        s.z[k][rc] = z;
+        dy *= z * sigmoid(z);
+      }
+      s.dy[k][rc] = dy;
     }
-    for (int k = tid; k < kKeep * 2 * NP; k += kThreads) {
-      const int i = k / (2 * NP);
-      const long long bt = (long long)b * a.T + (t + i < t1 ? t + i : t1 - 1);
-      (&s.bc[0][0][0])[k] = a.bc[(bt * a.G + g) * 2 * NP + k % (2 * NP)];
-    }
-    if (wave == 0) {
-      const bool f = a.starts && lane < kKeep && t + lane < t1 &&
-                     a.starts[(long long)b * a.T + t + lane];
-      const unsigned long long m = __ballot(f);
+#pragma unroll
+    for (int i = 0; i < BC; ++i) (&s.bc[0][0][0])[tid + i * kThreads] = rbc[i];
+    if (STARTS && wave == 0) {
+      const unsigned long long m = __ballot(rs);
       if (lane == 0) s.fresh = (unsigned)m;
     }
-    const f32x4 hv = *reinterpret_cast<const f32x4*>(
-        a.kept + (((long long)b * nb + t / kKeep) * a.C + c) * NP + 4 * q);
+    const f32x4 hv = rk;
     __syncthreads();
-    if (t > t0) load(t - kKeep);
-    const unsigned fresh = __builtin_amdgcn_readfirstlane(s.fresh);
+    if (t > t0) {
+      px -= kKeep * a.x.st;
+      pd -= kKeep * a.dt.st;
+      po -= kKeep * a.dout.st;
+      pz -= kKeep * a.z.st;
+      pbc -= (long long)kKeep * a.G * ROW;
+      pk -= (long long)a.C * NP;
+      ps -= kKeep;
+      load(std::false_type{});
+    }
+    const unsigned fresh = STARTS ? __builtin_amdgcn_readfirstlane(s.fresh) : 0u;
 
-    float h[kKeep][4], dec[kKeep][4], h_in[4], now[4];
+    // One token's values are read while the one before is worked on, and no further ahead: all of
+    // them would not leave registers for the states.
+    struct Token {
+      float d, x, dy;
+      f32x4 B, C;
+    };
+    auto read = [&](int i, bool back) {
+      Token k;
+      k.d = s.d[i][ci];
+      k.x = s.x[i][ci];
+      k.B = *reinterpret_cast<const f32x4*>(&s.bc[i][0][4 * q]);
+      if (back) {
+        k.dy = s.dy[i][ci];
+        k.C = *reinterpret_cast<const f32x4*>(&s.bc[i][1][4 * q]);
+      }
+      return k;
+    };
+    float h[kKeep][4], dec[kKeep][4], now[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) h_in[k] = now[k] = hv[k];
+    for (int k = 0; k < 4; ++k) now[k] = hv[k];
+    Token next = read(0, false);
 #pragma unroll
     for (int i = 0; i < kKeep; ++i) {
-      const float d = s.d[i][ci], u = d * s.x[i][ci];
-      const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s.bc[i][0][4 * q]);
-      const bool f = fresh >> i & 1;
+      const Token m = next;
+      next = i + 1 < kKeep ? read(i + 1, false) : read(i, true);
+      const float u = m.d * m.x, d2 = m.d * kLog2e;
+      const bool f = STARTS && (fresh >> i & 1);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float r = exp2_(d * A2[k]);
-        dec[i][k] = f ? 0.f : r;
-        now[k] = f ? u * Bv[k] : fmaf(r, now[k], u * Bv[k]);
+        dec[i][k] = exp2_(d2 * A[k]);
+        now[k] = fmaf(dec[i][k], f ? 0.f : now[k], u * m.B[k]);
         h[i][k] = now[k];
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int i = kKeep - 1; i >= 0; --i) {
-      const float d = s.d[i][ci], u = d * s.x[i][ci], dy = s.dy[i][ci];
-      const f32x4 Bv = *reinterpret_cast<const f32x4*>(&s.bc[i][0][4 * q]);
-      const f32x4 Cv = *reinterpret_cast<const f32x4*>(&s.bc[i][1][4 * q]);
-      const bool f = fresh >> i & 1;
+      const Token m = next;
+      if (i) next = read(i - 1, true);
+      const float u = m.d * m.x;
+      const bool f = STARTS && (fresh >> i & 1);
       float v[8], sb = 0.f, sa = 0.f, y = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float dh = fmaf(dy, Cv[k], e[k]);
-        v[k] = dh * u;             // of B
-        v[4 + k] = dy * h[i][k];   // of C
-        sb = fmaf(dh, Bv[k], sb);
+        const float dh = fmaf(m.dy, m.C[k], e[k]);
+        v[k] = dh * u;               // of B
+        v[4 + k] = m.dy * h[i][k];   // of C
+        sb = fmaf(dh, m.B[k], sb);
         const float back = f ? 0.f : dh * dec[i][k];
-        const float through = f ? 0.f : back * (i ? h[i - 1][k] : h_in[k]);
+        const float through = f ? 0.f : back * (i ? h[i - 1][k] : hv[k]);
         sa = fmaf(through, A[k], sa);
-        dA[k] = fmaf(through, d, dA[k]);
-        y = fmaf(Cv[k], h[i][k], y);
+        dA[k] = fmaf(through, m.d, dA[k]);
+        y = fmaf(m.C[k], h[i][k], y);
         e[k] = back;
       }
-      sb = sum_high<LG>(sb);
-      sa = sum_high<LG>(sa);
-      if (gate) y = sum_high<LG>(y);
+      sb = sum_low<LN>(sb);
+      sa = sum_low<LN>(sa);
+      if (gate) y = sum_low<LN>(y);
       if (q == 0) {
         s.sb[i][ci] = sb;
         s.sa[i][ci] = sa;
         if (gate) s.y[i][ci] = y;
       }
-      sum_lanes8<LG>(v, lane);
-      // the lanes with the values: v[0] of number (bits LG - 1, LG - 2, LG - 3)
-      if constexpr (LG >= 3) {
-        if ((lane & ((1 << (LG - 3)) - 1)) == 0) {
-          const int k = lane >> (LG - 1) & 1, k2 = lane >> (LG - 2) & 1, k3 = lane >> (LG - 3) & 1;
-          s.red[wave][i][k][4 * q + 2 * k2 + k3] = v[0];
-        }
-      } else {
-        const int k = lane >> 1 & 1, k2 = lane & 1;
-        s.red[wave][i][k][4 * q + 2 * k2] = v[0];
-        s.red[wave][i][k][4 * q + 2 * k2 + 1] = v[1];
+      sum_high8<LN>(v);
+      if ((lane & 15) < NG) {
+        float* r = &s.red[wave][i][lane >> 5][4 * q + 2 * (lane >> 4 & 1)];
+        r[0] = v[0];
+        r[1] = v[1];
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     // sums over the states to gradients of x, dt and z; sums over the waves' channels
@@ -566,26 +710,31 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
     for (int i = 0; i < PER; ++i) {
       const int k = ri + i * STEP;
       if (!r_on || t + k >= t1) continue;
-      const float d = s.d[k][rc], dy = s.dy[k][rc], sb = s.sb[k][rc];
-      const long long at = ((long long)b * a.T + t + k) * a.C + r_c;
-      ((TX*)a.dx)[at] = (TX)fmaf(d, sb, D * dy);
-      float dd = fmaf(xv[i], sb, s.sa[k][rc]);
-      if (a.softplus) dd *= sigmoid(raw[i]);
-      ((TD*)a.ddt)[at] = (TD)dd;
+      const float d = s.d[k][rc], x = s.x[k][rc], dy = s.dy[k][rc], sb = s.sb[k][rc];
+      const long long m = (long long)i * STEP * a.C;
+      put(pdx + m, oo * (unsigned)sizeof(TX), (TX)fmaf(d, sb, D * dy));
+      float dd = fmaf(x, sb, s.sa[k][rc]);
+      if (a.softplus) dd *= sigmoid(s.raw[k][rc]);
+      put(pdd + m, oo * (unsigned)sizeof(TD), (TD)dd);
       sum_bias += dd;
-      sum_D = fmaf(dy, xv[i], sum_D);
+      sum_D = fmaf(dy, x, sum_D);
       if (gate) {
-        const float sg = sigmoid(zv[i]), y = fmaf(D, xv[i], s.y[k][rc]);
-        ((TX*)a.dz)[at] = (TX)(ov[i] * y * sg * fmaf(zv[i], 1.f - sg, 1.f));
+        const float z = s.z[k][rc], sg = sigmoid(z), y = fmaf(D, x, s.y[k][rc]);
+        put(pdz + m, oo * (unsigned)sizeof(TX),
+            (TX)(s.dout[k][rc] * y * sg * fmaf(z, 1.f - sg, 1.f)));
       }
     }
-    for (int k = tid; k < kKeep * 2 * NP; k += kThreads) {
-      const int i = k / (2 * NP);
-      if (t + i >= t1) continue;
+#pragma unroll
+    for (int i = 0; i < BC; ++i) {
+      const int k = tid + i * kThreads;
       const float* r = &s.red[0][0][0][0] + k;
-      const float v = (r[0] + r[kKeep * 2 * NP]) + (r[2 * kKeep * 2 * NP] + r[3 * kKeep * 2 * NP]);
-      a.part_bc[(((long long)tile * a.B + b) * a.T + t + i) * 2 * NP + k % (2 * NP)] = v;
+      if (k / ROW < t1 - t)
+        put(pp, k * 4u, (r[0] + r[kKeep * ROW]) + (r[2 * kKeep * ROW] + r[3 * kKeep * ROW]));
     }
+    pdx -= (long long)kKeep * a.C;
+    pdd -= (long long)kKeep * a.C;
+    pdz -= (long long)kKeep * a.C;
+    pp -= kKeep * ROW;
     __syncthreads();   // the next tokens are staged over what was read here
   }
 
@@ -754,7 +903,8 @@ Split split(int B, int T, int C, int G, int N) {
 
 int validate(int B, int T, int C, int G, int N, int in_dtype, int dt_dtype) {
   if (B < 1 || T < 0 || C < 1 || G < 1 || G > C || C % G || N < 1 || N > 64) return GDN2_ERR_SHAPE;
-  if (T > INT_MAX - 1024 || C > (1 << 24)) return GDN2_ERR_SHAPE;
+  // channels and sixteen tokens' rows are reached in 32 bits (of bytes)
+  if (T > INT_MAX - 1024 || C > (1 << 24) || G > (1 << 18)) return GDN2_ERR_SHAPE;
   if (in_dtype != GDN2_F32 && in_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
   if (dt_dtype != GDN2_F32 && dt_dtype != in_dtype) return GDN2_ERR_DTYPE;
   // a launch's threads stay within 32 bits and its waves' numbers within 31: one wave for at
@@ -792,34 +942,34 @@ void launch_rows(hipStream_t st, const SsmArgs& a, int NP) {
                      dim3(kThreads), 0, st, a, NP);
 }
 
-template <typename TX, typename TD, int NP>
+template <typename TX, typename TD, int NP, bool STARTS>
 void launch_fwd(hipStream_t st, const SsmArgs& a) {
   const long long waves = (long long)a.B * a.G * a.tiles;
   launch_rows<TX>(st, a, NP);
   if (a.chunks > 1) {
-    hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, false>),
+    hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, STARTS, false>),
                        dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)), dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((ssm_join<NP, false>),
                        dim3((unsigned)(((long long)a.B * a.C * NP + kThreads - 1) / kThreads)),
                        dim3(kThreads), 0, st, a);
   }
-  hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, true>), dim3((unsigned)((waves * a.chunks + 3) / 4)),
+  hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, STARTS, true>), dim3((unsigned)((waves * a.chunks + 3) / 4)),
                      dim3(kThreads), 0, st, a);
 }
 
-template <typename TX, typename TD, int NP>
+template <typename TX, typename TD, int NP, bool STARTS>
 void launch_bwd(hipStream_t st, SsmArgs a) {
   const long long waves = (long long)a.B * a.G * a.tiles;
   launch_rows<TX>(st, a, NP);
   if (a.chunks > 1) {
-    hipLaunchKernelGGL((ssm_rev<TX, TD, NP>), dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)),
+    hipLaunchKernelGGL((ssm_rev<TX, TD, NP, STARTS>), dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)),
                        dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((ssm_join<NP, true>),
                        dim3((unsigned)(((long long)a.B * a.C * NP + kThreads - 1) / kThreads)),
                        dim3(kThreads), 0, st, a);
   }
   a.tiles = (a.Cg + bwd_tile(NP) - 1) / bwd_tile(NP);
-  hipLaunchKernelGGL((ssm_bwd<TX, TD, NP>),
+  hipLaunchKernelGGL((ssm_bwd<TX, TD, NP, STARTS>),
                      dim3((unsigned)((long long)a.B * a.G * a.tiles * a.chunks)), dim3(kThreads), 0,
                      st, a);
   hipLaunchKernelGGL((ssm_sums), dim3((unsigned)(((long long)a.C * (NP + 2) + 63) / 64)), dim3(1024),
@@ -834,7 +984,10 @@ hipError_t launch_types(hipStream_t st, const SsmArgs& a, bool bwd) {
   switch (padded(a.N)) {
 #define GDN2_CASE(NP)                                                              \
   case NP:                                                                         \
-    bwd ? launch_bwd<TX, TD, NP>(st, a) : launch_fwd<TX, TD, NP>(st, a);           \
+    if (a.starts)                                                                  \
+      bwd ? launch_bwd<TX, TD, NP, true>(st, a) : launch_fwd<TX, TD, NP, true>(st, a);   \
+    else                                                                           \
+      bwd ? launch_bwd<TX, TD, NP, false>(st, a) : launch_fwd<TX, TD, NP, false>(st, a); \
     break
     GDN2_CASE(8);
     GDN2_CASE(16);
@@ -877,6 +1030,7 @@ int set_inputs(SsmArgs& a, int B, int T, int C, int G, int N, int in_dtype, int 
     *rows[i] = Rows{ins[i], strides ? strides[2 * i] : T * widths[i],
                     strides ? strides[2 * i + 1] : widths[i]};
     if ((rc = check_rows(*rows[i], i == 1 ? dt_dtype : in_dtype, i == 2))) return rc;
+    if (rows[i]->p && (rows[i]->st < 0 || rows[i]->st > kMaxStride)) return GDN2_ERR_SHAPE;
   }
   if ((rc = check_f32(A, false)) || (rc = check_f32(D, true)) || (rc = check_f32(dt_bias, true)))
     return rc;
@@ -957,6 +1111,7 @@ int gdn2_selective_scan_bwd(void* stream, int B, int T, int C, int G, int N, int
       return rc;
   a.dout = Rows{dout, dout_strides ? dout_strides[0] : (long long)T * C,
                 dout_strides ? dout_strides[1] : C};
+  if (dout && (a.dout.st < 0 || a.dout.st > kMaxStride)) return GDN2_ERR_SHAPE;
   if ((rc = check_rows(a.dout, in_dtype, true)) || (rc = check_f32(dh_final, true)) ||
       (rc = check_f32(kept, false)) || (rc = check_f32(dA, false)) || (rc = check_f32(dD, true)) ||
       (rc = check_f32(ddt_bias, true)) || (rc = check_f32(dh0, true)))

@@ -33,6 +33,7 @@ from .gdn2_scan import _as
 _Ptrs5 = ctypes.c_void_p * 5
 _Strides5 = ctypes.c_longlong * 10
 _MAX_STATES = 64
+_MAX_STRIDE = 2 ** 25   # elements from one token to the next that are read in place
 
 
 def _prepare(x, dt, A, B, C, D, z, dt_bias, state, lead, what):
@@ -87,7 +88,7 @@ def _row_operand(t):
     """t with a token's values contiguous, and the elements from one batch entry and one token
     to the next.  Strides of axes of one element say nothing."""
     width = t.shape[2:].numel()
-    if t[0, 0].is_contiguous():
+    if t[0, 0].is_contiguous() and (t.shape[1] == 1 or t.stride(1) <= _MAX_STRIDE):
         return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * width,
                    t.stride(1) if t.shape[1] > 1 else width)
     t = t.contiguous()

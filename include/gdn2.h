@@ -483,8 +483,8 @@ int gdn2_short_conv_step(void* stream, int B, int C, int W, int dtype, int silu,
  * of tokens must stay below 88 (d >= 0 and A <= 0 in use).  starts: as for the convolution, the
  * state before such a token is dropped and no gradient passes it.
  * ins: host array of x, dt, z, Bm, Cm; strides: NULL (dense) or ten host integers, for each of
- * them the elements from one batch entry and one token to the next; the rest of a row is
- * contiguous.  Pointers are aligned to their elements, kept and ws to 16 bytes.  T >= 1. */
+ * them the elements from one batch entry and one token (at most 2^25) to the next; the rest of a
+ * row is contiguous.  C <= 2^24, G <= 2^18.  Pointers are aligned to their elements, kept and ws to 16 bytes.  T >= 1. */
 
 /* Bytes of the states kept for the backward (float32, one for every 16 tokens, N padded to 8,
  * 16, 32 or 64) and of the workspace of the forward or the backward. */
