@@ -21,7 +21,7 @@ BUILD = HERE / "_build"
 OUT = HERE / "gdn2_package" / "libgdn2_hip.so"
 SOURCES = ["gdn2_api.cpp", "gdn2_fwd.hip", "gdn2_bwd.hip", "gdn2_decode.hip", "gdn2_noalloc.hip",
            "gdn2_stage.hip", "gdn2_gscan.hip", "gdn2_norm.hip", "gdn2_int8.hip",
-           "gdn2_conv.hip", "gdn2_ssm.hip"]
+           "gdn2_conv.hip", "gdn2_ssm.hip", "gdn2_fp8.hip"]
 ARCH = "gfx950"
 
 # Packed-fp32 VALU forms are kept out of the generated code on purpose.

@@ -1,0 +1,819 @@
+// Values in 8-bit floating point (OCP e4m3) with a scale for each block of 128, and their matrix
+// product:
+//   out[m][n] = sum_b sx[m][b] sw[n or n / 128][b] sum_{k in block b} x[m][k] w[n][k]  (+ bias[n]),
+// x (M,K), w (N,K), both with contiguous k in blocks of 128.
+//
+// A block's scale is the smallest power of two s with max|t| <= 448 s, so that t / s is exact and
+// a value is rounded once, to e4m3 (three bits below its leading one): a larger scale would not
+// hold more of it, as it would with integers.  The product takes any float32 scales.
+//
+// Quantisation: a workgroup holds 128 x 128 values in registers, 8 x 8 a thread, and writes them
+// with scales for its rows (1 x 128), its columns (transposed: the operands of a gradient of a
+// weight, summed over the tokens) or all of them (128 x 128, and transposed), so that what needs
+// two forms of the same values reads them once.  Memory bounds it.
+//
+// Product: one v_mfma_f32_16x16x128_f8f6f4 is one block of k of 16 x 16 outputs.  Its result is scaled
+// and added in float32 by the vector units while the next ones run: four multiply-adds a lane (sx
+// sw is one number a lane and block of w) against 32 cycles of the matrix core.  Slices of 128
+// bytes of k are staged through LDS by global_load_lds in a ring, the 16-byte pieces of a row
+// permuted within it by the row number so that the eight lanes that LDS serves together read
+// different banks; as the DMA writes LDS in lane order, the lanes' global addresses are permuted
+// instead.  The weight is the left operand, its rows dealt to the fragments so that a lane ends up
+// with eight neighbouring columns of one output row.
+//
+// Few rows: the weight's traffic is all that counts.  A workgroup takes 16 weight rows and its
+// eight waves the slices of k in turn, straight from memory to registers; their sums meet in LDS.
+//
+// k past K: rows are readable up to a multiple of 16 bytes, loads are clamped there, and the
+// bytes of both operands from K on are zeroed in the last slice (what is there may be NaN).
+#include <limits.h>
+
+#include "gdn2.h"
+#include "gdn2_common.h"
+
+namespace gdn2 {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+// 16 bytes at any value of TO: rows of results start where N puts them
+template <typename TO>
+struct __attribute__((packed, aligned(sizeof(TO)))) Piece {
+  i32x4 v;
+};
+
+constexpr int kBlock = 128;   // values that share a scale; bytes of k of a slice
+constexpr int kBK = kBlock;
+
+// ---- Quantisation ----------------------------------------------------------------------
+
+struct QuantArgs {
+  const void* x;
+  long long ldx;             // elements between rows
+  unsigned char *q, *qt;     // (M, ldq), (C, ldt): rows, and columns as rows
+  long long ldq, ldt;
+  float *s, *st;             // (C / 128, M), (M / 128, C); blocks: (M / 128, C / 128) and transposed
+  float* part;               // (M / 128, C) sums of each 128 rows, or null
+  int M, C, kb, mb;          // blocks along the columns, the rows
+  int vec;
+};
+
+// The scale and its inverse of values whose largest magnitude has these bits: 0, 0 where all are
+// zero, NaN, 0 where one is NaN or infinite.
+__device__ __forceinline__ void scales(unsigned top, float& s, float& inv) {
+  // top = 1.f 2^(E - 127) <= 1.75 2^(8 + e)
+  int e = (int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u);
+  e = e < -126 ? -126 : e;
+  s = __uint_as_float((unsigned)(e + 127) << 23);
+  inv = __uint_as_float((unsigned)(127 - e) << 23);
+  if (top == 0) s = inv = 0.f;
+  if (top >= 0x7f800000u) {
+    s = __builtin_nanf("");
+    inv = 0.f;
+  }
+}
+__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+template <int CTRL>
+__device__ __forceinline__ unsigned larger_dpp(unsigned v) {
+  return larger(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
+}
+// v * inv in e4m3, four values; where inv is 0 so is every one of them (an infinity would not be).
+__device__ __forceinline__ int pack4(float a, float b, float c, float d, float ia, float ib, float ic,
+                                     float id) {
+  a = ia == 0.f ? 0.f : a * ia;
+  b = ib == 0.f ? 0.f : b * ib;
+  c = ic == 0.f ? 0.f : c * ic;
+  d = id == 0.f ? 0.f : d * id;
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// ROWS: q with a scale for each row and 128 columns.  COLS: qt with one for each column and 128
+// rows.  BLOCK: q, and where it is given qt, with one for each 128 x 128.
+enum { kRows = 1, kCols = 2, kBlocks = 4 };
+template <typename TX, int MODE>
+__global__ void __launch_bounds__(256) fp8_quantize(QuantArgs a) {
+  // thread: rows m + 0..7, columns c + 0..7 of the tile
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int tc = blockIdx.x % a.kb, tm = blockIdx.x / a.kb;
+  const int m = tm * kBlock + (tid >> 4) * 8, c = tc * kBlock + (tid & 15) * 8;
+  __shared__ unsigned top[16][kBlock];
+  float v[8][8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    // rows past the end count as zeros, read from the last one
+    const TX* p = (const TX*)a.x + (m + r < a.M ? m + r : a.M - 1) * a.ldx;
+    const bool row = m + r < a.M;
+    if (a.vec) {
+      load_f<8>(p + (c < a.C ? c : 0), v[r]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[r][k] = row && c < a.C ? v[r][k] : 0.f;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = to_f(p[c + k < a.C ? c + k : a.C - 1]);
+        v[r][k] = row && c + k < a.C ? f : 0.f;
+      }
+    }
+  }
+  if (a.part) {
+    float* sum = reinterpret_cast<float*>(&top[0][0]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float t = v[0][k];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) t += v[r][k];
+      sum[(tid >> 4) * kBlock + (tid & 15) * 8 + k] = t;
+    }
+    __syncthreads();
+    if (tid < kBlock && tc * kBlock + tid < a.C) {
+      float t = 0.f;
+#pragma unroll
+      for (int g = 0; g < 16; ++g) t += sum[g * kBlock + tid];
+      a.part[(long long)tm * a.C + tc * kBlock + tid] = t;
+    }
+    __syncthreads();
+  }
+  unsigned char* q = a.q + m * a.ldq + c;
+  if constexpr ((MODE & kRows) != 0) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      unsigned t = magnitude(v[r][0]);
+#pragma unroll
+      for (int k = 1; k < 8; ++k) t = larger(t, magnitude(v[r][k]));
+      // over the 16 lanes of the row
+      t = larger_dpp<0xB1>(t);
+      t = larger_dpp<0x4E>(t);
+      t = larger_dpp<0x141>(t);
+      t = larger_dpp<0x140>(t);
+      float s, i;
+      scales(t, s, i);
+      if (m + r < a.M) {
+        if (c < a.ldq)
+          *reinterpret_cast<i32x2*>(q + r * a.ldq) =
+              i32x2{pack4(v[r][0], v[r][1], v[r][2], v[r][3], i, i, i, i),
+                    pack4(v[r][4], v[r][5], v[r][6], v[r][7], i, i, i, i)};
+        if ((tid & 15) == 0) a.s[(long long)tc * a.M + m + r] = s;
+      }
+    }
+  }
+  if constexpr ((MODE & (kCols | kBlocks)) != 0) {
+    unsigned t[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      t[k] = magnitude(v[0][k]);
+#pragma unroll
+      for (int r = 1; r < 8; ++r) t[k] = larger(t[k], magnitude(v[r][k]));
+    }
+    if constexpr ((MODE & kBlocks) != 0) {
+      unsigned all = t[0];
+#pragma unroll
+      for (int k = 1; k < 8; ++k) all = larger(all, t[k]);
+#pragma unroll
+      for (int b = 1; b < 64; b *= 2) all = larger(all, __shfl_xor(all, b));
+      if ((tid & 63) == 0) top[0][wave] = all;
+      __syncthreads();
+      all = larger(larger(top[0][0], top[0][1]), larger(top[0][2], top[0][3]));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[k] = all;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top[tid >> 4][(tid & 15) * 8 + k] = t[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        t[k] = 0;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) t[k] = larger(t[k], top[g][(tid & 15) * 8 + k]);
+      }
+    }
+    float s[8], i[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) scales(t[k], s[k], i[k]);
+    if constexpr ((MODE & kBlocks) != 0) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (m + r < a.M && c < a.ldq)
+          *reinterpret_cast<i32x2*>(q + r * a.ldq) =
+              i32x2{pack4(v[r][0], v[r][1], v[r][2], v[r][3], i[0], i[0], i[0], i[0]),
+                    pack4(v[r][4], v[r][5], v[r][6], v[r][7], i[0], i[0], i[0], i[0])};
+      if (tid == 0) {
+        a.s[(long long)tm * a.kb + tc] = s[0];
+        if (a.st) a.st[(long long)tc * a.mb + tm] = s[0];
+      }
+    } else if ((tid >> 4) == 0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k < a.C) a.st[(long long)tm * a.C + c + k] = s[k];
+    }
+    if (a.qt && m < a.ldt) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k < a.C)
+          *reinterpret_cast<i32x2*>(a.qt + (c + k) * a.ldt + m) =
+              i32x2{pack4(v[0][k], v[1][k], v[2][k], v[3][k], i[k], i[k], i[k], i[k]),
+                    pack4(v[4][k], v[5][k], v[6][k], v[7][k], i[k], i[k], i[k], i[k])};
+    }
+  }
+}
+
+// Partial sums added in their order: 64 columns a workgroup, 16 rows at a time.
+__global__ void __launch_bounds__(1024) fp8_sums(const float* part, int rows, int C, float* out) {
+  __shared__ float s[16][64];
+  const int col = threadIdx.x & 63, r = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + col;
+  float v = 0.f;
+  if (c < C)
+    for (int k = r; k < rows; k += 16) v += part[(long long)k * C + c];
+  s[r][col] = v;
+  __syncthreads();
+  if (r || c >= C) return;
+  v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v += s[k][col];
+  out[c] = v;
+}
+
+// The values that q stands for: s at (row / rb) sm + (column / 128) sk.
+template <typename TO>
+__global__ void __launch_bounds__(256) fp8_dequantize(const unsigned char* q, long long ldq,
+                                                      const float* s, long long sm, long long sk,
+                                                      int rb, int M, int C, TO* out) {
+  const int per = (C + 15) / 16;
+  const long long n = (long long)M * per;
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < n; e += (long long)gridDim.x * 256) {
+    const int m = (int)(e / per), c = (int)(e - (long long)m * per) * 16;
+    const float f = s[m / rb * sm + c / kBlock * sk];
+    const unsigned char* p = q + m * ldq + c;
+    TO* o = out + (long long)m * C + c;
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (c + k < C) o[k] = from_f<TO>(__builtin_amdgcn_cvt_f32_fp8(p[k], 0) * f);
+  }
+}
+
+// ---- Product ---------------------------------------------------------------------------
+
+struct MmArgs {
+  const unsigned char *x, *w;
+  long long ldx, ldw;          // bytes between rows
+  const float *sx, *sw;        // (blocks, M); (blocks, N) or, for blocks of 128 rows, (N / 128, blocks)
+  const float* bias;           // (N) or null
+  long long ldsx, ldsw;        // elements between rows of sx and sw
+  void* out;                   // (M, N) dense
+  int M, N, K;
+  int tm, tn, chunk;           // tiles; tiles of one XCD
+};
+
+// The products of one block of 128, summed; 32 values of a row a lane.  The 8-bit matrix instruction
+// aligns eight products at a time (neighbours of one lane) to the largest of them and drops what
+// lies below 2^-13 of it, towards zero; between these groups it adds in float32.  Of normally
+// distributed values that is 1.4e-5 of a result's rms, nothing beside a bfloat16 result's
+// 2^-9 and too much for a float32 one: there the values go through the bfloat16 matrix
+// instruction, whose products are exact and whose sums are float32's, at half the rate.
+template <typename TO>
+__device__ __forceinline__ f32x4 mma8(const i32x8& x, const i32x8& y) {
+  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(TO) == 2) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+  } else {
+    auto wide = [](const i32x8& v, int k) {
+      bf16x8 r;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * k + h], 1.f, false);
+        const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * k + h], 1.f, true);
+        r[4 * h] = lo[0], r[4 * h + 1] = lo[1], r[4 * h + 2] = hi[0], r[4 * h + 3] = hi[1];
+      }
+      return r;
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide(x, k), wide(y, k), c, 0, 0, 0);
+    return c;
+  }
+}
+
+// Zero the bytes from byte n on of a 16-byte piece (n may be <= 0 or >= 16): the four values of v
+// from `at` on.
+__device__ __forceinline__ void keep_bytes(i32x8& v, int at, int n) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int k = n - 4 * d;
+    const unsigned mask = k >= 4 ? 0xffffffffu : k <= 0 ? 0u : (1u << (8 * k)) - 1u;
+    v[at + d] = (int)((unsigned)v[at + d] & mask);
+  }
+}
+// A lane's fragment of a row is the pieces lg and lg + 4 of a slice; `left` bytes of it count.
+__device__ __forceinline__ void keep_row(i32x8& v, int lg, int left) {
+  keep_bytes(v, 0, left - 16 * lg);
+  keep_bytes(v, 4, left - 64 - 16 * lg);
+}
+__device__ __forceinline__ i32x8 both(const i32x4& a, const i32x4& b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Place of 16-byte piece c of row r within its slice: piece c ^ swz(r).  Activations'
+// fragments read rows i = 0..15, the weight's rows 8 (i / 4) + i % 4 (+ 4).
+__device__ __forceinline__ int swz_x(int r) { return r & 7; }
+__device__ __forceinline__ int swz_w(int r) { return (r & 3) | ((r >> 1) & 4); }
+
+// The 16-byte pieces of two halves of a row's columns, as lanes 16 lg + li hold them for rows
+// li = 0..15 (t0: the first half, t1: the second), dealt so that t0 holds both halves of the
+// rows 0..7 and t1 those of the rows 8..15: lanes li and li ^ 8 exchange a piece.  Each of
+// the two stores that follow then writes 128 bytes of eight rows, not 64 of sixteen.
+__device__ __forceinline__ void whole_lines(i32x4& t0, i32x4& t1) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    // row_ror:8, written to the lanes 8..15 of a row alone, and to 0..7
+    const int first = t0[d];
+    t0[d] = __builtin_amdgcn_update_dpp(first, t1[d], 0x128, 0xF, 0xC, false);
+    t1[d] = __builtin_amdgcn_update_dpp(t1[d], first, 0x128, 0xF, 0x3, false);
+  }
+}
+
+// Eight values from column n on of a vector of N, those past the end repeating the last.
+__device__ __forceinline__ void load_columns(const float* v, int n, int N, float (&f)[8]) {
+  if (n + 8 <= N) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const i32x4 r = reinterpret_cast<const Piece<float>*>(v + n)[h].v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * h + e] = __int_as_float(r[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = v[n + e < N ? n + e : N - 1];
+  }
+}
+
+// Add the bias to a wave's part, convert and store it: the fragment pair 2 j, 2 j + 1 of tile i
+// holds row li, columns 32 j + 8 lg + e.  m, n: its first row and column.
+template <typename TO, int NI, int MI>
+__device__ __forceinline__ void store_part(const MmArgs& a, const f32x4 (&acc)[NI][MI], int m,
+                                           int n, int li, int lg) {
+  // before the first store, which could alias it for all the compiler knows
+  float bi[NI / 2][8];
+#pragma unroll
+  for (int j = 0; j < NI / 2; ++j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bi[j][e] = 0.f;
+    if (a.bias) load_columns(a.bias, n + 32 * j + 8 * lg, a.N, bi[j]);
+  }
+  auto result = [&](int i, int j, float (&y)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = acc[2 * j + e / 4][i][e % 4] + bi[j][e];
+  };
+  auto piece = [](const float (&y)[8], int half) {   // float32: the half of it
+    i32x4 r;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      if constexpr (sizeof(TO) == 4)
+        r[d] = __float_as_int(y[4 * half + d]);
+      else
+        r[d] = __builtin_bit_cast(int, bf16x2{(bf16_t)y[2 * d], (bf16_t)y[2 * d + 1]});
+    }
+    return r;
+  };
+  TO* out = (TO*)a.out + (long long)m * a.N + n;
+  if ((sizeof(TO) == 4 || NI % 4 == 0) && n + 16 * NI <= a.N && m + 16 * MI <= a.M) {
+    // two halves of 128 bytes: float32 the two pieces of 8 values, bfloat16 two fragment pairs
+    const bool high = li >= 8;
+    constexpr int STEP = sizeof(TO) == 4 ? 1 : 2;
+    TO* p = out + (long long)(li & 7) * a.N + 8 * lg + (sizeof(TO) == 4 ? 4 : 32) * high;
+#pragma unroll
+    for (int i = 0; i < MI; ++i, p += 16ll * a.N)
+#pragma unroll
+      for (int j = 0; j + STEP <= NI / 2; j += STEP) {
+        float y0[8], y1[8];
+        result(i, j, y0);
+        if constexpr (STEP == 2) result(i, j + 1, y1);
+        i32x4 t0 = piece(y0, 0), t1 = piece(STEP == 2 ? y1 : y0, STEP == 2 ? 0 : 1);
+        whole_lines(t0, t1);
+        reinterpret_cast<Piece<TO>*>(p + 32 * j)->v = t0;
+        reinterpret_cast<Piece<TO>*>(p + 8ll * a.N + 32 * j)->v = t1;
+      }
+    return;
+  }
+  TO* p = out + (long long)li * a.N + 8 * lg;
+#pragma unroll
+  for (int i = 0; i < MI; ++i, p += 16ll * a.N)
+    if (m + 16 * i + li < a.M) {
+#pragma unroll
+      for (int j = 0; j < NI / 2; ++j) {
+        float y[8];
+        result(i, j, y);
+        const int left = a.N - (n + 32 * j + 8 * lg);
+        if (left >= 8) {
+          Piece<TO>* q = reinterpret_cast<Piece<TO>*>(p + 32 * j);
+          q[0].v = piece(y, 0);
+          if constexpr (sizeof(TO) == 4) q[1].v = piece(y, 1);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < left) p[32 * j + e] = from_f<TO>(y[e]);
+        }
+      }
+    }
+}
+
+// BM x BN outputs; WR x WC waves; ST slices of k in LDS; PER_CU workgroups on a CU.
+template <int BM_, int BN_, int WR_, int WC_, int ST_, int PER_CU_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, ST = ST_, PER_CU = PER_CU_;
+  static constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC;   // waves, and a wave's part
+  static constexpr int MI = WM / 16, NI = WN / 16;
+  static constexpr int STAGE = (BM + BN) * kBK;
+  static constexpr int NL = STAGE / 1024 / NW;                     // DMA instructions of a wave
+  static_assert(STAGE % (1024 * NW) == 0 && NI % 2 == 0 && BM % 16 == 0, "tile");
+  static_assert(kBlock % BN == 0, "a tile lies within one block of the weight's rows");
+};
+
+// WROW: the weight has a scale for each row, else for each 128 rows.
+template <typename C, bool WROW, typename TO>
+__global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmArgs a) {
+  constexpr int BM = C::BM, BN = C::BN, NW = C::NW, MI = C::MI, NI = C::NI, NL = C::NL;
+  constexpr int ST = C::ST;
+  __shared__ __attribute__((aligned(16))) char lds[ST * C::STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int li = lane & 15, lg = lane >> 4;
+
+  // Tiles: neighbours on one XCD, eight rows of tiles before the next column, so that what runs
+  // together on an XCD shares rows and columns in its L2.
+  constexpr int GROUP = 8;
+  const int item = (blockIdx.x & 7) * a.chunk + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= a.chunk || item >= a.tm * a.tn) return;
+  const int group = item / (GROUP * a.tn), in_group = item - group * GROUP * a.tn;
+  const int rows = a.tm - GROUP * group < GROUP ? a.tm - GROUP * group : GROUP;
+  const int m0 = (GROUP * group + in_group % rows) * BM, n0 = (in_group / rows) * BN;
+
+  // the source of each DMA: eight rows of one operand from a wave's address on, this lane's
+  // row and piece of the slice in 32 bits
+  const char* base[NL];
+  unsigned off[NL];
+  int at[NL];
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const bool act = (wave * NL + i) * 8 < BM;
+    const int r = (wave * NL + i) * 8 + lane / 8 - (act ? 0 : BM);
+    const int most = act ? a.M - 1 - m0 : a.N - 1 - n0;
+    at[i] = 16 * (lane % 8 ^ (act ? swz_x(r) : swz_w(r)));
+    base[i] = (const char*)(act ? a.x + m0 * a.ldx : a.w + n0 * a.ldw);
+    off[i] = (unsigned)(r < most ? r : most) * (unsigned)(act ? a.ldx : a.ldw) + at[i];
+  }
+  const int last = (a.K + 15) / 16 * 16 - 16;   // the last readable piece of a row
+  auto load = [&](int kb, int buf) {
+    char* dst = lds + buf * C::STAGE + wave * NL * 1024;
+    if ((kb + 1) * kBK <= last + 16) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) lds_dma16(base[i] + kb * kBK + (size_t)off[i], dst + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int past = kb * kBK + at[i] - last;
+        lds_dma16(base[i] + kb * kBK + (long long)off[i] - (past > 0 ? past : 0), dst + i * 1024);
+      }
+    }
+  };
+
+  // this lane's fragments in a slice; the slice's second half is 64 bytes on (^ 64)
+  const int wm = (wave / C::WC) * C::WM, wn = (wave % C::WC) * C::WN;
+  int rw[NI], rx[MI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int r = wn + (j / 2) * 32 + (li / 4) * 8 + (j & 1) * 4 + li % 4;
+    rw[j] = (BM + r) * kBK + 16 * (lg ^ swz_w(r));
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r = wm + i * 16 + li;
+    rx[i] = r * kBK + 16 * (lg ^ swz_x(r));
+  }
+  auto row = [&](int buf, int at) {
+    const char* s = lds + buf * C::STAGE;
+    return both(*reinterpret_cast<const i32x4*>(s + at), *reinterpret_cast<const i32x4*>(s + (at ^ 64)));
+  };
+  // scales of one slice: rows 16 i + li of x; of w one, or columns 32 j + 8 lg + e
+  struct Scales {
+    float row[MI], col[WROW ? NI / 2 : 1][8];
+  };
+  const int nk = (a.K + kBK - 1) / kBK;
+  int sm[MI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int r = m0 + wm + 16 * i + li;
+    sm[i] = r < a.M ? r : a.M - 1;
+  }
+  auto load_scales = [&](Scales& s, int kb) {
+    kb = kb < nk ? kb : nk - 1;
+    const float* p = a.sx + kb * a.ldsx;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) s.row[i] = p[sm[i]];
+    if constexpr (WROW) {
+#pragma unroll
+      for (int j = 0; j < NI / 2; ++j)
+        load_columns(a.sw + kb * a.ldsw, n0 + wn + 32 * j + 8 * lg, a.N, s.col[j]);
+    } else {
+      s.col[0][0] = a.sw[n0 / kBlock * a.ldsw + kb];
+    }
+  };
+
+  f32x4 acc[NI][MI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j)
+#pragma unroll
+    for (int i = 0; i < MI; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the outputs of half of the weight's fragments
+  constexpr int NH = NI / 2;
+  auto multiply = [&](const i32x8 (&w)[NH], const i32x8 (&x)[MI], const Scales& s, int j0) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const float f = WROW ? s.row[i] : s.row[i] * s.col[0][0];
+#pragma unroll
+      for (int j = 0; j < NH; ++j) {
+        const f32x4 p = mma8<TO>(w[j], x[i]);
+        f32x4& c = acc[j0 + j][i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (WROW)
+            c[e] = fmaf(p[e] * f, s.col[(j0 + j) / 2][(j0 + j) % 2 * 4 + e], c[e]);
+          else
+            c[e] = fmaf(p[e], f, c[e]);
+        }
+      }
+    }
+  };
+
+  Scales sc[2];
+  load_scales(sc[0], 0);
+#pragma unroll
+  for (int s = 0; s < ST; ++s)
+    if (s < nk) load(s, s);
+  if (nk >= ST)
+    wait_vmcnt<(ST - 1) * NL>();
+  else
+    wait_vmcnt<0>();
+  lds_barrier();
+  // half of the weight's fragments are multiplied while the other half, or the next slice's, are read
+  i32x8 x[2][MI], w0[2][NH], w1[NH];
+  auto read = [&](int p, int buf) {
+#pragma unroll
+    for (int j = 0; j < NH; ++j) w0[p][j] = row(buf, rw[j]);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) x[p][i] = row(buf, rx[i]);
+  };
+  read(0, 0);
+  constexpr int UN = ST % 2 ? 2 * ST : ST;   // slices of one round: the registers alternate
+  for (int k0 = 0; k0 < nk; k0 += UN) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int kb = k0 + u, buf = u % ST;
+      if (kb >= nk) break;
+      auto& xs = x[u & 1];
+      auto& ws = w0[u & 1];
+#pragma unroll
+      for (int j = 0; j < NH; ++j) w1[j] = row(buf, rw[NH + j]);
+      load_scales(sc[(u + 1) & 1], kb + 1);
+      const int left = a.K - kb * kBK;
+      if (left < kBK) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) keep_row(xs[i], lg, left);
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+          keep_row(ws[j], lg, left);
+          keep_row(w1[j], lg, left);
+        }
+      }
+      multiply(ws, xs, sc[u & 1], 0);
+      // slice kb + 1 has arrived once only the ST - 2 later ones are in flight; every wave has
+      // read slice kb, whose buffer is free
+      if (kb + ST <= nk)
+        wait_vmcnt<(ST - 2) * NL>();
+      else
+        wait_vmcnt<0>();
+      lds_barrier();
+      if (kb + ST < nk) load(kb + ST, buf);
+      read((u + 1) & 1, (u + 1) % ST);   // after the last slice: stale data that nothing uses
+      multiply(w1, xs, sc[u & 1], NH);
+    }
+  }
+  store_part<TO>(a, acc, m0 + wm, n0 + wn, li, lg);
+}
+
+// 16 weight rows and all of x's (up to 16 MT) a workgroup; wave w takes the slices of 128
+// bytes w, w + 8, ... of k.
+template <int MT, bool WROW, typename TO>
+__global__ void __launch_bounds__(512) fp8_mm_rows(MmArgs a) {
+  constexpr int NW = 8;
+  __shared__ float sum[NW][MT][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int li = lane & 15, lg = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const int n = n0 + li < a.N ? n0 + li : a.N - 1;
+  const unsigned char* w = a.w + n * a.ldw;
+  const unsigned char* x[MT];
+  int m[MT], c[4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    m[i] = m0 + i * 16 + li < a.M ? m0 + i * 16 + li : a.M - 1;
+    x[i] = a.x + m[i] * a.ldx;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) c[r] = n0 + 4 * lg + r < a.N ? n0 + 4 * lg + r : a.N - 1;
+  const int last = (a.K + 15) / 16 * 16 - 16;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wave * kBK; k0 < a.K; k0 += NW * kBK) {
+    const int ka = k0 + 16 * lg, kc = ka + 64;
+    const int p0 = ka < last ? ka : last, p1 = kc < last ? kc : last, kb = k0 / kBK;
+    auto row = [&](const unsigned char* p) {
+      i32x8 v = both(*reinterpret_cast<const i32x4*>(p + p0), *reinterpret_cast<const i32x4*>(p + p1));
+      if (k0 + kBK > a.K) keep_row(v, lg, a.K - k0);
+      return v;
+    };
+    float sw[4], sx[MT];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      sw[r] = WROW ? a.sw[kb * a.ldsw + c[r]] : a.sw[n0 / kBlock * a.ldsw + kb];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sx[i] = a.sx[kb * a.ldsx + m[i]];
+    const i32x8 fw = row(w);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const f32x4 p = mma8<TO>(fw, row(x[i]));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(p[r] * sx[i], sw[r], acc[i][r]);
+    }
+  }
+  // lane: columns 4 lg + r, row li
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[wave][i][li][4 * lg + r] = acc[i][r];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MT * 256; e += 64 * NW) {
+    const int ml = e / 16, col = e % 16, mm = m0 + ml;
+    if (mm < a.M && n0 + col < a.N) {
+      float s = a.bias ? a.bias[n0 + col] : 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) s += sum[k][ml / 16][ml % 16][col];
+      ((TO*)a.out)[(long long)mm * a.N + n0 + col] = from_f<TO>(s);
+    }
+  }
+}
+
+template <typename C, bool WROW, typename TO>
+void launch_tiles(hipStream_t st, MmArgs a) {
+  a.tm = (a.M + C::BM - 1) / C::BM;
+  a.tn = (a.N + C::BN - 1) / C::BN;
+  a.chunk = (a.tm * a.tn + 7) / 8;
+  hipLaunchKernelGGL((fp8_mm<C, WROW, TO>), dim3(8u * (unsigned)a.chunk), dim3(64 * C::NW), 0, st, a);
+}
+template <int MT, bool WROW, typename TO>
+void launch_rows(hipStream_t st, const MmArgs& a) {
+  hipLaunchKernelGGL((fp8_mm_rows<MT, WROW, TO>),
+                     dim3((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+                     dim3(512), 0, st, a);
+}
+
+template <bool WROW, typename TO>
+hipError_t launch_mm(hipStream_t st, const MmArgs& a) {
+  const int cus = num_cus();
+  auto tiles = [&](int bm, int bn) {
+    return (((long long)a.M + bm - 1) / bm) * (((long long)a.N + bn - 1) / bn);
+  };
+  if (a.M <= 16)
+    launch_rows<1, WROW, TO>(st, a);
+  else if (a.M <= 32 || tiles(32, 16) <= cus)
+    launch_rows<2, WROW, TO>(st, a);
+  else if (sizeof(TO) == 4 || tiles(64, 64) <= 3 * cus)   // float32: registers for no more
+    launch_tiles<Tile<64, 64, 2, 2, 3, 3>, WROW, TO>(st, a);
+  else if constexpr (sizeof(TO) == 2)
+    launch_tiles<Tile<128, 128, 2, 2, 2, 2>, WROW, TO>(st, a);
+  return hipGetLastError();
+}
+
+template <typename TX>
+hipError_t launch_quantize(hipStream_t st, const QuantArgs& a, int mode) {
+  const dim3 grid((unsigned)((long long)a.kb * a.mb)), block(256);
+  switch (mode) {
+    case kRows: hipLaunchKernelGGL((fp8_quantize<TX, kRows>), grid, block, 0, st, a); break;
+    case kCols: hipLaunchKernelGGL((fp8_quantize<TX, kCols>), grid, block, 0, st, a); break;
+    case kRows | kCols:
+      hipLaunchKernelGGL((fp8_quantize<TX, kRows | kCols>), grid, block, 0, st, a);
+      break;
+    default: hipLaunchKernelGGL((fp8_quantize<TX, kBlocks>), grid, block, 0, st, a);
+  }
+  return hipGetLastError();
+}
+
+long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+int gdn2_quantize_fp8(void* stream, int M, int C, int x_dtype, const void* x, long long x_stride,
+                      int blocks, void* q, long long q_stride, float* scale, void* qt,
+                      long long qt_stride, float* scale_t, float* part, float* sums) {
+  if (M < 0 || C < 1 || C > INT_MAX - 256 || M > INT_MAX - 256) return GDN2_ERR_SHAPE;
+  if (x_dtype != GDN2_F32 && x_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
+  if (blocks != 0 && blocks != 1) return GDN2_ERR_FLAGS;
+  if (M == 0) return GDN2_OK;
+  if (!q && (!qt || blocks)) return GDN2_ERR_NULL;
+  if ((q && q_stride != round_up(C, 16)) || (qt && qt_stride != round_up(M, 16)))
+    return GDN2_ERR_SHAPE;
+  QuantArgs a = {};
+  a.kb = (C + kBlock - 1) / kBlock, a.mb = (M + kBlock - 1) / kBlock;
+  // a launch's threads stay within 32 bits
+  if ((long long)a.kb * a.mb > (1ll << 23) || C > (1 << 27)) return GDN2_ERR_SHAPE;
+  if (!x || (q && !scale) || (qt && !scale_t) || !part != !sums) return GDN2_ERR_NULL;
+  const uintptr_t es = x_dtype == GDN2_F32 ? 4 : 2;
+  if ((uintptr_t)x % es || (uintptr_t)q % 16 || (uintptr_t)qt % 16 || (uintptr_t)scale % 4 ||
+      (uintptr_t)scale_t % 4 || (uintptr_t)part % 4 || (uintptr_t)sums % 4)
+    return GDN2_ERR_ALIGN;
+  a.part = part;
+  a.x = x, a.ldx = x_stride, a.M = M, a.C = C;
+  a.q = (unsigned char*)q, a.ldq = q_stride, a.s = scale;
+  a.qt = (unsigned char*)qt, a.ldt = qt_stride, a.st = qt ? scale_t : nullptr;
+  // eight values at a time
+  a.vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0;
+  const int mode = blocks ? kBlocks : (q ? kRows : 0) | (qt ? kCols : 0);
+  const hipError_t e = x_dtype == GDN2_F32 ? launch_quantize<float>((hipStream_t)stream, a, mode)
+                                           : launch_quantize<bf16_t>((hipStream_t)stream, a, mode);
+  if (e != hipSuccess) return GDN2_ERR_LAUNCH;
+  if (!part) return GDN2_OK;
+  hipLaunchKernelGGL(fp8_sums, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream,
+                     part, a.mb, C, sums);
+  return hipGetLastError() == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+int gdn2_dequantize_fp8(void* stream, int M, int C, int out_dtype, const void* q,
+                        long long q_stride, int row_block, const float* scale,
+                        const long long* scale_strides, void* out) {
+  if (M < 0 || C < 1 || C > INT_MAX - 256 || (row_block != 1 && row_block != kBlock))
+    return GDN2_ERR_SHAPE;
+  if (out_dtype != GDN2_F32 && out_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
+  if (M == 0) return GDN2_OK;
+  if (!q || !scale || !scale_strides || !out) return GDN2_ERR_NULL;
+  if ((uintptr_t)scale % 4 || (uintptr_t)out % (out_dtype == GDN2_F32 ? 4 : 2))
+    return GDN2_ERR_ALIGN;
+  const long long n = (long long)M * ((C + 15) / 16), wgs = (n + 255) / 256;
+  const dim3 grid((unsigned)(wgs < 65536 ? wgs : 65536)), block(256);
+  if (out_dtype == GDN2_F32)
+    hipLaunchKernelGGL((fp8_dequantize<float>), grid, block, 0, (hipStream_t)stream,
+                       (const unsigned char*)q, q_stride, scale, scale_strides[0],
+                       scale_strides[1], row_block, M, C, (float*)out);
+  else
+    hipLaunchKernelGGL((fp8_dequantize<bf16_t>), grid, block, 0, (hipStream_t)stream,
+                       (const unsigned char*)q, q_stride, scale, scale_strides[0],
+                       scale_strides[1], row_block, M, C, (bf16_t*)out);
+  return hipGetLastError() == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+int gdn2_fp8_matmul(void* stream, int M, int N, int K, int out_dtype, const void* x,
+                    long long x_stride, const float* x_scale, long long x_scale_stride,
+                    const void* w, long long w_stride, int w_row_block, const float* w_scale,
+                    long long w_scale_stride, const float* bias, void* out) {
+  if (M < 0 || N < 1 || K < 1 || K > INT_MAX - 256) return GDN2_ERR_SHAPE;
+  if (w_row_block != 1 && w_row_block != kBlock) return GDN2_ERR_SHAPE;
+  if (out_dtype != GDN2_F32 && out_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
+  const long long row = round_up(K, 16), kb = (K + kBlock - 1) / kBlock;
+  if (x_stride < row || w_stride < row) return GDN2_ERR_SHAPE;
+  if (x_scale_stride < M || w_scale_stride < (w_row_block == 1 ? N : kb)) return GDN2_ERR_SHAPE;
+  // rows of a tile are reached in 32 bits
+  if (x_stride > (1 << 24) || w_stride > (1 << 24)) return GDN2_ERR_SHAPE;
+  // a launch's threads stay within 32 bits (128 x 128 tiles of 256, 16 columns of 512), and a
+  // tile's row numbers, which may pass the end by 255, within 31
+  if (M > INT_MAX - 256 || N > (1 << 26) || ((M + 127ll) / 128) * ((N + 127ll) / 128) > (1ll << 23))
+    return GDN2_ERR_SHAPE;
+  if (M == 0) return GDN2_OK;
+  const size_t es = out_dtype == GDN2_F32 ? 4 : 2;
+  for (const void* p : {x, (const void*)x_scale, w, (const void*)w_scale, (const void*)out})
+    if (!p) return GDN2_ERR_NULL;
+  if ((uintptr_t)x % 16 || (uintptr_t)w % 16 || x_stride % 16 || w_stride % 16)
+    return GDN2_ERR_ALIGN;
+  if ((uintptr_t)x_scale % 4 || (uintptr_t)w_scale % 4 || (uintptr_t)bias % 4 ||
+      (uintptr_t)out % es)
+    return GDN2_ERR_ALIGN;
+  MmArgs a = {};
+  a.x = (const unsigned char*)x, a.w = (const unsigned char*)w, a.ldx = x_stride, a.ldw = w_stride;
+  a.sx = x_scale, a.sw = w_scale, a.ldsx = x_scale_stride, a.ldsw = w_scale_stride;
+  a.bias = bias, a.out = out, a.M = M, a.N = N, a.K = K;
+  const hipStream_t st = (hipStream_t)stream;
+  hipError_t e;
+  if (w_row_block == 1)
+    e = out_dtype == GDN2_F32 ? launch_mm<true, float>(st, a) : launch_mm<true, bf16_t>(st, a);
+  else
+    e = out_dtype == GDN2_F32 ? launch_mm<false, float>(st, a) : launch_mm<false, bf16_t>(st, a);
+  return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+}  // extern "C"

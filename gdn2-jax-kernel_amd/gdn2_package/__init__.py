@@ -17,7 +17,10 @@ for each row), ``gdn2_int8_matmul`` with ``gdn2_quantize_int8`` /
 ``gdn2_dequantize_int8``, and ``gdn2_gated_scan`` (a gated linear recurrence,
 trainable) with ``gdn2_gated_scan_step``; ``gdn2_short_conv`` (a short causal
 convolution over each channel) and ``gdn2_selective_scan`` (a selective state space
-scan), both trainable, with ``gdn2_short_conv_step`` and ``gdn2_selective_scan_step``.
+scan), both trainable, with ``gdn2_short_conv_step`` and ``gdn2_selective_scan_step``;
+``gdn2_fp8_matmul`` (a matrix product in 8-bit floating point with a scale for each
+block of 128), ``gdn2_quantize_fp8`` / ``gdn2_dequantize_fp8`` and ``gdn2_fp8_linear``
+(a linear layer trained that way).
 Compute runs in libgdn2_hip.so (hand-written gfx950 HIP kernels, C ABI in
 include/gdn2.h); torch supplies device memory and streams.
 """
@@ -25,6 +28,8 @@ from . import gdn2_bwd, gdn2_decode, gdn2_fwd, gdn2_pipeline
 from ._lib import GDN2LibraryError
 from .gdn2_conv import gdn2_short_conv, gdn2_short_conv_step
 from .gdn2_decode import gdn2_decode_step
+from .gdn2_fp8 import (gdn2_dequantize_fp8, gdn2_fp8_linear, gdn2_fp8_matmul,
+                       gdn2_quantize_fp8)
 from .gdn2_fwd import (GDN2Error, GDN2ShapeError, gdn2_pallas_forward,
                        gdn2_pallas_forward_raw, gdn2_pallas_forward_varlen,
                        gdn2_pallas_forward_with_residuals)
@@ -45,6 +50,7 @@ __all__ = [
     "gdn2_gated_scan", "gdn2_gated_scan_step", "gdn2_rms_norm", "gdn2_rms_norm_int8",
     "gdn2_quantize_int8", "gdn2_dequantize_int8", "gdn2_int8_matmul",
     "gdn2_short_conv", "gdn2_short_conv_step", "gdn2_selective_scan", "gdn2_selective_scan_step",
+    "gdn2_quantize_fp8", "gdn2_dequantize_fp8", "gdn2_fp8_matmul", "gdn2_fp8_linear",
     "GDN2Error", "GDN2ShapeError",
     "GDN2LibraryError", "gdn2_fwd", "gdn2_bwd", "gdn2_pipeline", "__version__",
 ]

@@ -114,6 +114,11 @@ SIGNATURES = {
     "gdn2_selective_scan_fwd": (_c_int, [_vp] + [_c_int] * 8 + [_vp] * 11 + [_c_size]),
     "gdn2_selective_scan_bwd": (_c_int, [_vp] + [_c_int] * 8 + [_vp] * 16 + [_c_size]),
     "gdn2_selective_scan_step": (_c_int, [_vp] + [_c_int] * 7 + [_vp] * 11),
+    "gdn2_quantize_fp8": (_c_int, [_vp] + [_c_int] * 3 + [_vp, _c_ll, _c_int, _vp, _c_ll, _vp, _vp,
+                                                          _c_ll] + [_vp] * 3),
+    "gdn2_dequantize_fp8": (_c_int, [_vp] + [_c_int] * 3 + [_vp, _c_ll, _c_int] + [_vp] * 3),
+    "gdn2_fp8_matmul": (_c_int, [_vp] + [_c_int] * 4 + [_vp, _c_ll] * 3 + [_c_int, _vp, _c_ll]
+                        + [_vp] * 2),
 }
 
 

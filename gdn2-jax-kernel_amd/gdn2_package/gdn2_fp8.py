@@ -1,0 +1,269 @@
+"""Values in 8-bit floating point with a scale for each block of 128, and products of them:
+
+    q, scale = gdn2_quantize_fp8(x)                    # rows, blocks of 1 x 128
+    q, scale = gdn2_quantize_fp8(w, blocks=True)       # a weight, blocks of 128 x 128
+    x = gdn2_dequantize_fp8(q, scale, dtype=torch.bfloat16)
+    y = gdn2_fp8_matmul(q, scale, w, w_scale, bias=None, out_dtype=torch.bfloat16)
+    y = gdn2_fp8_linear(x, w, bias=None)               # autograd
+
+A block's scale is the smallest power of two s with max|t| <= 448 s, and its values are held as
+e4m3(t / s) (torch.float8_e4m3fn, ties to even): the one rounding there is.  A block of zeros has
+scale 0; one that holds NaN or an infinity has scale NaN and q = 0, so that all that is computed
+from it is NaN.  The product takes any float32 scales, so a weight may come from a checkpoint
+that was quantised otherwise.
+
+Rows of q start at multiples of 16 bytes: where the width is none, q is a view of a wider
+tensor; the scales of rows are laid out block by block (a transposed view).  The product takes both
+as they are and copies others.  Quantisation and gdn2_fp8_matmul are inference only: as with
+the decode step, their results carry no gradient, whatever the inputs require.  No counterpart
+in the reference.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .gdn2_conv import _floating, _ptr
+from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
+from .gdn2_norm import _as, _as_rows, _forward_mode, _gradients, _row_stride, _tensor
+
+_BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+
+
+def _count(n):
+    """Blocks of n values."""
+    return (n + _BLOCK - 1) // _BLOCK
+
+
+def _empty_q(M, C, dev):
+    """e4m3 (M, C), rows at multiples of 16 bytes: the tensor and its row stride."""
+    ld = (C + 15) // 16 * 16
+    q = torch.empty((M, ld), dtype=_E4M3, device=dev)
+    return (q if ld == C else q[:, :C]), ld
+
+
+def _quantize(rows, mode, sums=None):
+    """Rows (M, C) of a supported type in 8 bits.  mode "rows": (q, scale); "columns": those of
+    the transposed matrix; "both": (q, scale, qt, scale_t); "blocks": (q, scale); "blocks both":
+    (q, scale, qt, scale_t).  Scales of rows and columns are (blocks, rows).  sums (C): takes the
+    sums of the columns."""
+    M, C = rows.shape
+    dev, kb, mb = rows.device, _count(C), _count(M)
+    blocks = mode.startswith("blocks")
+    q = s = qt = st = None
+    ldq = ldt = 0
+    if mode != "columns":
+        q, ldq = _empty_q(M, C, dev)
+        s = torch.empty((mb, kb) if blocks else (kb, M), dtype=torch.float32, device=dev)
+    if mode in ("columns", "both", "blocks both"):
+        qt, ldt = _empty_q(C, M, dev)
+        st = torch.empty((kb, mb) if blocks else (mb, C), dtype=torch.float32, device=dev)
+    part = None if sums is None else torch.empty((mb, C), dtype=torch.float32, device=dev)
+    rc = _lib.launch("gdn2_quantize_fp8", dev, M, C, _dtype_code(rows.dtype), rows.data_ptr(),
+                     _row_stride(rows), int(blocks), _ptr(q), ldq, _ptr(s), _ptr(qt), ldt, _ptr(st),
+                     _ptr(part), _ptr(sums))
+    if rc:
+        _raise(rc, f"gdn2_quantize_fp8 (M,C)=({M},{C})")
+    return tuple(t for t in (q, s, qt, st) if t is not None)
+
+
+def gdn2_quantize_fp8(x, blocks=False):
+    """x (..., C) in 8 bits: q (float8_e4m3fn of x's shape) and scale (float32), (..., ceil(C / 128))
+    for rows, or with blocks=True for a matrix (N, C) (ceil(N / 128), ceil(C / 128))."""
+    what = "gdn2_quantize_fp8"
+    _tensor(x, "x", what)
+    if x.dim() < 1 or (blocks and x.dim() != 2):
+        raise GDN2ShapeError(f"{what}: expected {'a matrix' if blocks else 'rows'}; got "
+                             f"{tuple(x.shape)}")
+    if x.shape[-1] < 1:
+        raise GDN2ShapeError(f"{what}: no columns in {tuple(x.shape)}")
+    if not x.is_floating_point():
+        raise GDN2Error(f"{what}: x must be floating point; got {x.dtype}")
+    if x.dtype not in _SUPPORTED_IN:
+        x = x.float()
+    q, s = _quantize(_as_rows(x), "blocks" if blocks else "rows")
+    if blocks:
+        return q, s
+    lead = x.shape[:-1]
+    return q.unflatten(0, lead) if x.dim() > 2 else q.view(x.shape), \
+        s.view(s.shape[0], *lead).movedim(0, -1)
+
+
+def _scaled_rows(q, scale, names, what, device, blocks):
+    """(q, its rows (M, C), the scale, whether it is one for blocks of 128 x 128), checked.
+    blocks: that such scales are allowed."""
+    _tensor(q, names[0], what)
+    _tensor(scale, names[1], what)
+    if q.dtype != _E4M3 or scale.dtype != torch.float32:
+        raise GDN2Error(f"{what}: {names[0]} must be float8_e4m3fn and {names[1]} float32; got "
+                        f"{q.dtype}, {scale.dtype}")
+    if q.device != device or scale.device != device:
+        raise GDN2Error(f"{what}: all tensors must live on {device}")
+    if q.dim() < 1 or q.shape[-1] < 1:
+        raise GDN2ShapeError(f"{what}: no columns in {names[0]} {tuple(q.shape)}")
+    per_row = (*q.shape[:-1], _count(q.shape[-1]))
+    per_block = (_count(q.shape[0]), per_row[-1]) if blocks and q.dim() == 2 else None
+    if scale.shape not in (per_row, per_block):
+        more = f" or {per_block}" if per_block else ""
+        raise GDN2ShapeError(f"{what}: {names[1]} must have shape {per_row}{more} for "
+                             f"{names[0]} {tuple(q.shape)}; got {tuple(scale.shape)}")
+    # one row has a scale of its own and is a block of rows: the same
+    return _as_rows(q), scale, scale.shape != per_row
+
+
+def gdn2_dequantize_fp8(q, scale, dtype=torch.bfloat16):
+    """The values that q stands for with the scales of its rows, or of its blocks of 128 x 128, in
+    float32 or bfloat16."""
+    what = "gdn2_dequantize_fp8"
+    if dtype not in _SUPPORTED_IN:
+        raise GDN2Error(f"{what}: dtype must be float32 or bfloat16; got {dtype}")
+    rows, s, blocks = _scaled_rows(q, scale, ("q", "scale"), what, getattr(q, "device", None), True)
+    M, C = rows.shape
+    s = s if blocks else _by_block(s, M).t()
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    rc = _lib.launch(
+        "gdn2_dequantize_fp8", q.device, M, C, _dtype_code(dtype), rows.data_ptr(),
+        _row_stride(rows), _BLOCK if blocks else 1, s.data_ptr(),
+        (_lib.ctypes.c_longlong * 2)(*s.stride()), out.data_ptr())
+    if rc:
+        _raise(rc, f"{what} (M,C)=({M},{C})")
+    return out
+
+
+def _wide_rows(q):
+    """(q, row stride) with rows at multiples of 16 bytes, at most 16 MiB apart, that are
+    readable up to the next multiple of 16; q itself where it is laid out so."""
+    M, K = q.shape
+    ld = q.stride(0) if M > 1 else (K + 15) // 16 * 16
+    end = (K + 15) // 16 * 16
+    if ld % 16 == 0 and end <= ld <= 1 << 24 and q.data_ptr() % 16 == 0 and (
+            K == end or M == 0 or
+            q.untyped_storage().nbytes() >= q.storage_offset() + (M - 1) * ld + end):
+        return q, ld
+    wide = torch.empty((M, end), dtype=q.dtype, device=q.device)
+    wide[:, :K] = q
+    return wide, end
+
+
+def _by_block(scale, M):
+    """Scales (..., blocks) of M rows as (blocks, M), dense; a copy only where they are not laid
+    out so."""
+    return scale.movedim(-1, 0).reshape(scale.shape[-1], M).contiguous()
+
+
+def _matmul(x, sx, w, sw, blocks, bias, out_dtype, what):
+    """x (M, K) with sx (blocks, M) times w (N, K)^T with sw (blocks, N) or, for blocks of 128
+    rows, (N / 128, blocks)."""
+    (M, K), N = x.shape, w.shape[0]
+    x, ldx = _wide_rows(x)
+    w, ldw = _wide_rows(w)
+    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    rc = _lib.launch(
+        "gdn2_fp8_matmul", x.device, M, N, K, _dtype_code(out_dtype), x.data_ptr(), ldx,
+        sx.data_ptr(), M, w.data_ptr(), ldw, _BLOCK if blocks else 1, sw.data_ptr(),
+        _count(K) if blocks else N, _ptr(bias), out.data_ptr())
+    if rc:
+        _raise(rc, f"{what} (M,N,K)=({M},{N},{K})")
+    return out
+
+
+def gdn2_fp8_matmul(q, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
+    """What q stands for times what the weight stands for, transposed, plus bias.
+
+    q (..., K) float8_e4m3fn with scale (..., ceil(K / 128)); weight (N, K) with weight_scale
+    (ceil(N / 128), ceil(K / 128)) or, a scale for each row, (N, ceil(K / 128)); bias (N,) or
+    None.  Returns (..., N) in out_dtype (float32 or bfloat16): float32 sums of a block's
+    products, scaled and added in float32 and rounded once.  Inference only."""
+    what = "gdn2_fp8_matmul"
+    if out_dtype not in _SUPPORTED_IN:
+        raise GDN2Error(f"{what}: out_dtype must be float32 or bfloat16; got {out_dtype}")
+    dev = getattr(q, "device", None)
+    x, sx, _ = _scaled_rows(q, scale, ("q", "scale"), what, dev, False)
+    w, sw, blocks = _scaled_rows(weight, weight_scale, ("weight", "weight_scale"), what, dev, True)
+    if weight.dim() != 2 or w.shape[1] != x.shape[1]:
+        raise GDN2ShapeError(f"{what}: weight must be (N, {x.shape[1]}); got "
+                             f"{tuple(weight.shape)}")
+    if bias is not None:
+        bias = _as(_floating(bias, "bias", (w.shape[0],), dev, what), torch.float32).contiguous()
+    sw = sw.contiguous() if blocks else _by_block(sw, w.shape[0])
+    out = _matmul(x, _by_block(sx, x.shape[0]), w, sw, blocks, bias, out_dtype, what)
+    return out.view(*q.shape[:-1], w.shape[0])
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, keep):
+        # the gradients' operands are made with the forward's: their inputs are read once
+        rows = _as_rows(x)
+        need_x, need_w = keep
+        q, sx, *xt = _quantize(rows, "both" if need_w else "rows")
+        w, sw, *wt = _quantize(weight, "blocks both" if need_x else "blocks")
+        ctx.save_for_backward(*xt, *wt)
+        ctx.need, ctx.shape, ctx.dtype, ctx.bias_dtype = keep, x.shape, x.dtype, \
+            None if bias is None else bias.dtype
+        b = None if bias is None else _as(bias, torch.float32).contiguous()
+        return _matmul(q, sx, w, sw, True, b, x.dtype, "gdn2_fp8_linear").view(
+            *x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _gradients(_Fp8Linear._grads, ctx, dy)
+
+    @staticmethod
+    def _grads(ctx, dy):
+        saved, (need_x, need_w) = list(ctx.saved_tensors), ctx.need
+        rows = _as_rows(_as(dy, ctx.dtype))
+        dx = dw = db = None
+        if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
+            db = torch.empty(rows.shape[1], dtype=torch.float32, device=rows.device)
+        mode = "both" if need_x and need_w else "columns" if need_w else "rows"
+        parts = _quantize(rows, mode, db)
+        xt = saved[:2] if need_w else None
+        wt = saved[2 * need_w:] if need_x else None
+        if need_x:
+            dx = _matmul(*parts[:2], *wt, True, None, ctx.dtype, "gdn2_fp8_linear").view(ctx.shape)
+        if need_w:
+            dw = _matmul(*parts[-2:], *xt, False, None, ctx.dtype, "gdn2_fp8_linear")
+        return dx, dw, None if db is None else _as(db, ctx.bias_dtype), None
+
+
+def gdn2_fp8_linear(x, weight, bias=None):
+    """x weight^T + bias as a linear layer that multiplies in 8 bits, for training.
+
+    x (..., K), weight (N, K), bias (N,); x and weight float32 or bfloat16 (mixed or other types
+    are widened to float32).  Returns (..., N) in x's type.  Forward: x in rows of 1 x 128, the
+    weight in blocks of 128 x 128.  Backward: the gradient of x from the output's in rows and the
+    weight's blocks, that of the weight from the output's gradient and x in blocks of 128 tokens;
+    the bias's is the sum of the output's gradient as it comes.  Between the passes x and the
+    weight are kept in 8 bits.  Differentiable in x, weight and bias in reverse mode (tangents of
+    forward mode raise NotImplementedError): gradients pass through the roundings as if they were
+    none.  To serve, quantise the weight once and call gdn2_fp8_matmul."""
+    what = "gdn2_fp8_linear"
+    _tensor(x, "x", what)
+    if not isinstance(weight, torch.Tensor):
+        raise TypeError(f"{what}: weight must be a torch tensor")
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
+        raise GDN2ShapeError(f"{what}: weight must be (N, K) for x (..., K); got "
+                             f"{tuple(weight.shape)} for x {tuple(x.shape)}")
+    if not x.is_floating_point():
+        raise GDN2Error(f"{what}: x must be floating point; got {x.dtype}")
+    weight = _floating(weight, "weight", weight.shape, x.device, what)
+    if bias is not None:
+        bias = _floating(bias, "bias", weight.shape[:1], x.device, what)
+    t = x.dtype if x.dtype in _SUPPORTED_IN and weight.dtype == x.dtype else torch.float32
+    xs, w = _as(x, t), _as(weight, t)
+    if x.numel() == 0:   # no values, and gradients of zero
+        y = xs @ w.t()
+        return _as(y if bias is None else y + bias, x.dtype)
+    # tangents go to the autograd function too, which refuses them
+    grad = torch.is_grad_enabled()
+    keep = (grad and xs.requires_grad, grad and w.requires_grad)
+    if _forward_mode() or any(keep) or (grad and bias is not None and bias.requires_grad):
+        y = _Fp8Linear.apply(xs, w, bias, keep)
+    else:
+        q, sx = _quantize(_as_rows(xs), "rows")
+        wq, sw = _quantize(_as_rows(w), "blocks")
+        b = None if bias is None else _as(bias, torch.float32).contiguous()
+        y = _matmul(q, sx, wq, sw, True, b, t, what).view(*x.shape[:-1], w.shape[0])
+    return _as(y, x.dtype)

@@ -516,6 +516,39 @@ int gdn2_selective_scan_step(void* stream, int B, int C, int G, int N, int in_dt
                              const void* Bm, const void* Cm, const float* D, const void* z,
                              const float* dt_bias, const float* h_in, float* h_out, void* out);
 
+/* ---- 8-bit floating point with a scale for each block of 128 -----------------------
+ * Values are OCP e4m3 (no counterpart in the reference).  A block's scale is the smallest power
+ * of two s >= 2^-126 with max|t| <= 448 s, q = e4m3(t / s), ties to even.  A block of zeros has scale
+ * 0, one that holds NaN or an infinity scale NaN and q = 0. */
+
+/* x (M,C), rows x_stride elements apart.  blocks = 0: q (M,C) with scale (ceil(C/128), M), a scale
+ * for each 1 x 128 values of a row, and / or qt (C,M), x transposed, with scale_t
+ * (ceil(M/128), C), one for each 128 values of a column.  blocks = 1: q with scale (ceil(M/128),
+ * ceil(C/128)), one for each 128 x 128 values, and where it is given qt with the same transposed.
+ * q or qt may be NULL (q not with blocks).  Rows of q and qt are C and M rounded up to 16 bytes
+ * apart, the bytes between zero, both 16-byte aligned.  part (ceil(M/128), C), a workspace, and
+ * sums (C), or both NULL: the sums of x's columns (of its values, not of what q stands for; the
+ * gradient of a bias).  C <= 2^27, at most 2^23 blocks of 128 x 128. */
+int gdn2_quantize_fp8(void* stream, int M, int C, int x_dtype, const void* x, long long x_stride,
+                      int blocks, void* q, long long q_stride, float* scale, void* qt,
+                      long long qt_stride, float* scale_t, float* part, float* sums);
+
+/* out = q scale, (M,C) dense; the scale of row m and block k at scale[(m / row_block) *
+ * scale_strides[0] + k * scale_strides[1]] (a host array), row_block 1 or 128. */
+int gdn2_dequantize_fp8(void* stream, int M, int C, int out_dtype, const void* q,
+                        long long q_stride, int row_block, const float* scale,
+                        const long long* scale_strides, void* out);
+
+/* out[m][n] = sum_b x_scale[b][m] s[n][b] sum_{k in block b} x[m][k] w[n][k] + bias[n] (bias float32
+ * or NULL), out (M,N) dense of out_dtype; x (M,K) and w (N,K).  s[n][b] is w_scale[b][n] with
+ * w_row_block 1, w_scale[n / 128][b] with 128; *_scale_stride are the elements between rows of
+ * the scales (at least M; N or ceil(K/128)); they may have any values.  Products of a block are
+ * summed by the matrix cores in float32, blocks in float32 too.  Otherwise as gdn2_int8_matmul. */
+int gdn2_fp8_matmul(void* stream, int M, int N, int K, int out_dtype, const void* x,
+                    long long x_stride, const float* x_scale, long long x_scale_stride,
+                    const void* w, long long w_stride, int w_row_block, const float* w_scale,
+                    long long w_scale_stride, const float* bias, void* out);
+
 #ifdef __cplusplus
 }
 #endif
