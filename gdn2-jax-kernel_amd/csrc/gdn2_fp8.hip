@@ -711,24 +711,19 @@ hipError_t launch_quantize(hipStream_t st, const QuantArgs& a, int mode) {
   return hipGetLastError();
 }
 
-long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
+size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-}  // namespace
-}  // namespace gdn2
-
-using namespace gdn2;
-
-extern "C" {
-
-int gdn2_quantize_fp8(void* stream, int M, int C, int x_dtype, const void* x, long long x_stride,
-                      int blocks, void* q, long long q_stride, float* scale, void* qt,
-                      long long qt_stride, float* scale_t, float* part, float* sums) {
+// What gdn2_quantize_fp8 takes, checked; the launches.
+int quantize(hipStream_t st, int M, int C, int x_dtype, const void* x, long long x_stride,
+             int blocks, void* q, long long q_stride, float* scale, void* qt, long long qt_stride,
+             float* scale_t, float* part, float* sums) {
   if (M < 0 || C < 1 || C > INT_MAX - 256 || M > INT_MAX - 256) return GDN2_ERR_SHAPE;
   if (x_dtype != GDN2_F32 && x_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
   if (blocks != 0 && blocks != 1) return GDN2_ERR_FLAGS;
   if (M == 0) return GDN2_OK;
   if (!q && (!qt || blocks)) return GDN2_ERR_NULL;
-  if ((q && q_stride != round_up(C, 16)) || (qt && qt_stride != round_up(M, 16)))
+  if ((q && q_stride != (long long)round_up(C, 16)) ||
+      (qt && qt_stride != (long long)round_up(M, 16)))
     return GDN2_ERR_SHAPE;
   QuantArgs a = {};
   a.kb = (C + kBlock - 1) / kBlock, a.mb = (M + kBlock - 1) / kBlock;
@@ -746,13 +741,89 @@ int gdn2_quantize_fp8(void* stream, int M, int C, int x_dtype, const void* x, lo
   // eight values at a time
   a.vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0;
   const int mode = blocks ? kBlocks : (q ? kRows : 0) | (qt ? kCols : 0);
-  const hipError_t e = x_dtype == GDN2_F32 ? launch_quantize<float>((hipStream_t)stream, a, mode)
-                                           : launch_quantize<bf16_t>((hipStream_t)stream, a, mode);
+  const hipError_t e = x_dtype == GDN2_F32 ? launch_quantize<float>(st, a, mode)
+                                           : launch_quantize<bf16_t>(st, a, mode);
   if (e != hipSuccess) return GDN2_ERR_LAUNCH;
   if (!part) return GDN2_OK;
-  hipLaunchKernelGGL(fp8_sums, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, (hipStream_t)stream,
-                     part, a.mb, C, sums);
+  hipLaunchKernelGGL(fp8_sums, dim3((unsigned)((C + 63) / 64)), dim3(1024), 0, st, part, a.mb, C,
+                     sums);
   return hipGetLastError() == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+int matmul(hipStream_t st, int M, int N, int K, int out_dtype, const void* x, long long x_stride,
+           const float* x_scale, long long x_scale_stride, const void* w, long long w_stride,
+           int w_row_block, const float* w_scale, long long w_scale_stride, const float* bias,
+           void* out) {
+  if (M < 0 || N < 1 || K < 1 || K > INT_MAX - 256) return GDN2_ERR_SHAPE;
+  if (w_row_block != 1 && w_row_block != kBlock) return GDN2_ERR_SHAPE;
+  if (out_dtype != GDN2_F32 && out_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
+  const long long row = (K + 15ll) / 16 * 16, kb = (K + kBlock - 1) / kBlock;
+  if (x_stride < row || w_stride < row) return GDN2_ERR_SHAPE;
+  if (x_scale_stride < M || w_scale_stride < (w_row_block == 1 ? N : kb)) return GDN2_ERR_SHAPE;
+  // rows of a tile are reached in 32 bits
+  if (x_stride > (1 << 24) || w_stride > (1 << 24)) return GDN2_ERR_SHAPE;
+  // a launch's threads stay within 32 bits (64 x 64 tiles of 256, 16 columns of 512), and a
+  // tile's row numbers, which may pass the end by 255, within 31
+  if (M > INT_MAX - 256 || N > (1 << 26) || ((M + 63ll) / 64) * ((N + 63ll) / 64) > (1ll << 23))
+    return GDN2_ERR_SHAPE;
+  if (M == 0) return GDN2_OK;
+  const size_t es = out_dtype == GDN2_F32 ? 4 : 2;
+  for (const void* p : {x, (const void*)x_scale, w, (const void*)w_scale, (const void*)out})
+    if (!p) return GDN2_ERR_NULL;
+  if ((uintptr_t)x % 16 || (uintptr_t)w % 16 || x_stride % 16 || w_stride % 16)
+    return GDN2_ERR_ALIGN;
+  if ((uintptr_t)x_scale % 4 || (uintptr_t)w_scale % 4 || (uintptr_t)bias % 4 ||
+      (uintptr_t)out % es)
+    return GDN2_ERR_ALIGN;
+  MmArgs a = {};
+  a.x = (const unsigned char*)x, a.w = (const unsigned char*)w, a.ldx = x_stride, a.ldw = w_stride;
+  a.sx = x_scale, a.sw = w_scale, a.ldsx = x_scale_stride, a.ldsw = w_scale_stride;
+  a.bias = bias, a.out = out, a.M = M, a.N = N, a.K = K;
+  hipError_t e;
+  if (w_row_block == 1)
+    e = out_dtype == GDN2_F32 ? launch_mm<true, float>(st, a) : launch_mm<true, bf16_t>(st, a);
+  else
+    e = out_dtype == GDN2_F32 ? launch_mm<false, float>(st, a) : launch_mm<false, bf16_t>(st, a);
+  return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+}
+
+// A matrix (rows, along) in 8 bits and its scales within a buffer.
+struct Held {
+  char* q;
+  float* s;
+  long long ld;     // bytes between rows
+  // blocks: of 128 x 128, else of 1 x 128
+  static size_t bytes(int rows, int along, bool blocks) {
+    const size_t nb = (along + 127) / 128, n = blocks ? (rows + 127) / 128 : rows;
+    return round_up((size_t)rows * round_up(along, 16), 16) + round_up(n * nb * 4, 16);
+  }
+  // at p, which moves past it
+  Held(char*& p, int rows, int along, bool blocks) : q(p), ld((long long)round_up(along, 16)) {
+    s = (float*)(p + (size_t)rows * ld);
+    p += bytes(rows, along, blocks);
+  }
+};
+// Sizes of the linear layer that every one of its calls can be made with.
+int validate_linear(int M, int N, int K, int dtype) {
+  if (M < 0 || N < 1 || K < 1 || N > (1 << 24) || K > (1 << 24) || M > (1 << 24))
+    return GDN2_ERR_SHAPE;
+  const long long m = (M + 63ll) / 64, n = (N + 63ll) / 64, k = (K + 63ll) / 64;
+  if (m * n > (1ll << 23) || m * k > (1ll << 23) || n * k > (1ll << 23)) return GDN2_ERR_SHAPE;
+  return dtype == GDN2_F32 || dtype == GDN2_BF16 ? GDN2_OK : GDN2_ERR_DTYPE;
+}
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" {
+
+int gdn2_quantize_fp8(void* stream, int M, int C, int x_dtype, const void* x, long long x_stride,
+                      int blocks, void* q, long long q_stride, float* scale, void* qt,
+                      long long qt_stride, float* scale_t, float* part, float* sums) {
+  return quantize((hipStream_t)stream, M, C, x_dtype, x, x_stride, blocks, q, q_stride, scale, qt,
+                  qt_stride, scale_t, part, sums);
 }
 
 int gdn2_dequantize_fp8(void* stream, int M, int C, int out_dtype, const void* q,
@@ -782,38 +853,75 @@ int gdn2_fp8_matmul(void* stream, int M, int N, int K, int out_dtype, const void
                     long long x_stride, const float* x_scale, long long x_scale_stride,
                     const void* w, long long w_stride, int w_row_block, const float* w_scale,
                     long long w_scale_stride, const float* bias, void* out) {
-  if (M < 0 || N < 1 || K < 1 || K > INT_MAX - 256) return GDN2_ERR_SHAPE;
-  if (w_row_block != 1 && w_row_block != kBlock) return GDN2_ERR_SHAPE;
-  if (out_dtype != GDN2_F32 && out_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
-  const long long row = round_up(K, 16), kb = (K + kBlock - 1) / kBlock;
-  if (x_stride < row || w_stride < row) return GDN2_ERR_SHAPE;
-  if (x_scale_stride < M || w_scale_stride < (w_row_block == 1 ? N : kb)) return GDN2_ERR_SHAPE;
-  // rows of a tile are reached in 32 bits
-  if (x_stride > (1 << 24) || w_stride > (1 << 24)) return GDN2_ERR_SHAPE;
-  // a launch's threads stay within 32 bits (128 x 128 tiles of 256, 16 columns of 512), and a
-  // tile's row numbers, which may pass the end by 255, within 31
-  if (M > INT_MAX - 256 || N > (1 << 26) || ((M + 127ll) / 128) * ((N + 127ll) / 128) > (1ll << 23))
-    return GDN2_ERR_SHAPE;
+  return matmul((hipStream_t)stream, M, N, K, out_dtype, x, x_stride, x_scale, x_scale_stride, w,
+                w_stride, w_row_block, w_scale, w_scale_stride, bias, out);
+}
+
+size_t gdn2_fp8_linear_kept_bytes(int M, int N, int K, int need_dx, int need_dw) {
+  if (validate_linear(M, N, K, GDN2_F32) != GDN2_OK || M == 0) return 0;
+  return (need_dw ? Held::bytes(K, M, false) : 0) + (need_dx ? Held::bytes(K, N, true) : 0);
+}
+
+size_t gdn2_fp8_linear_workspace_bytes(int M, int N, int K, int backward) {
+  if (validate_linear(M, N, K, GDN2_F32) != GDN2_OK || M == 0) return 0;
+  if (!backward) return Held::bytes(M, K, false) + Held::bytes(N, K, true);
+  return Held::bytes(M, N, false) + Held::bytes(N, M, false) +
+         round_up((size_t)((M + 127) / 128) * N * 4, 16);
+}
+
+int gdn2_fp8_linear_fwd(void* stream, int M, int N, int K, int dtype, const void* x,
+                        long long x_stride, const void* w, long long w_stride, const float* bias,
+                        int need_dx, int need_dw, void* y, void* kept, void* ws,
+                        size_t ws_bytes) {
+  int rc = validate_linear(M, N, K, dtype);
+  if (rc) return rc;
   if (M == 0) return GDN2_OK;
-  const size_t es = out_dtype == GDN2_F32 ? 4 : 2;
-  for (const void* p : {x, (const void*)x_scale, w, (const void*)w_scale, (const void*)out})
-    if (!p) return GDN2_ERR_NULL;
-  if ((uintptr_t)x % 16 || (uintptr_t)w % 16 || x_stride % 16 || w_stride % 16)
-    return GDN2_ERR_ALIGN;
-  if ((uintptr_t)x_scale % 4 || (uintptr_t)w_scale % 4 || (uintptr_t)bias % 4 ||
-      (uintptr_t)out % es)
-    return GDN2_ERR_ALIGN;
-  MmArgs a = {};
-  a.x = (const unsigned char*)x, a.w = (const unsigned char*)w, a.ldx = x_stride, a.ldw = w_stride;
-  a.sx = x_scale, a.sw = w_scale, a.ldsx = x_scale_stride, a.ldsw = w_scale_stride;
-  a.bias = bias, a.out = out, a.M = M, a.N = N, a.K = K;
   const hipStream_t st = (hipStream_t)stream;
-  hipError_t e;
-  if (w_row_block == 1)
-    e = out_dtype == GDN2_F32 ? launch_mm<true, float>(st, a) : launch_mm<true, bf16_t>(st, a);
-  else
-    e = out_dtype == GDN2_F32 ? launch_mm<false, float>(st, a) : launch_mm<false, bf16_t>(st, a);
-  return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
+  if (!ws || !w || !y || ((need_dx || need_dw) && !kept)) return GDN2_ERR_NULL;
+  if ((uintptr_t)ws % 16 || (uintptr_t)kept % 16) return GDN2_ERR_ALIGN;
+  if (ws_bytes < gdn2_fp8_linear_workspace_bytes(M, N, K, 0)) return GDN2_ERR_WORKSPACE;
+  const long long kb = (K + 127) / 128;
+  char *p = (char*)ws, *k = (char*)kept;
+  const Held qx(p, M, K, false), qw(p, N, K, true);
+  Held xt = qx, wt = qw;
+  if (need_dw) xt = Held(k, K, M, false);
+  if (need_dx) wt = Held(k, K, N, true);
+  if ((rc = quantize(st, M, K, dtype, x, x_stride, 0, qx.q, qx.ld, qx.s, need_dw ? xt.q : nullptr,
+                     xt.ld, xt.s, nullptr, nullptr)) ||
+      (rc = quantize(st, N, K, dtype, w, w_stride, 1, qw.q, qw.ld, qw.s, need_dx ? wt.q : nullptr,
+                     wt.ld, wt.s, nullptr, nullptr)))
+    return rc;
+  return matmul(st, M, N, K, dtype, qx.q, qx.ld, qx.s, M, qw.q, qw.ld, kBlock, qw.s, kb, bias, y);
+}
+
+int gdn2_fp8_linear_bwd(void* stream, int M, int N, int K, int dtype, const void* dy,
+                        long long dy_stride, const void* kept, int kept_dx, int kept_dw, void* dx,
+                        void* dw, float* dbias, void* ws, size_t ws_bytes) {
+  int rc = validate_linear(M, N, K, dtype);
+  if (rc) return rc;
+  if (M == 0) return GDN2_ERR_SHAPE;
+  if ((dx && !kept_dx) || (dw && !kept_dw)) return GDN2_ERR_FLAGS;
+  const hipStream_t st = (hipStream_t)stream;
+  if (!ws || !dy || ((dx || dw) && !kept)) return GDN2_ERR_NULL;
+  if ((uintptr_t)ws % 16 || (uintptr_t)kept % 16) return GDN2_ERR_ALIGN;
+  if (ws_bytes < gdn2_fp8_linear_workspace_bytes(M, N, K, 1)) return GDN2_ERR_WORKSPACE;
+  char *p = (char*)ws, *k = (char*)kept;
+  const Held rows(p, M, N, false), cols(p, N, M, false);
+  const bool need_rows = dx || !dw;   // the sums alone come with either
+  if ((rc = quantize(st, M, N, dtype, dy, dy_stride, 0, need_rows ? rows.q : nullptr, rows.ld,
+                     rows.s, dw ? cols.q : nullptr, cols.ld, cols.s, dbias ? (float*)p : nullptr,
+                     dbias)))
+    return rc;
+  const Held xt = kept_dw ? Held(k, K, M, false) : rows;
+  if (dw) {
+    if ((rc = matmul(st, N, K, M, dtype, cols.q, cols.ld, cols.s, N, xt.q, xt.ld, 1, xt.s, K,
+                     nullptr, dw)))
+      return rc;
+  }
+  if (!dx) return GDN2_OK;
+  const Held wt(k, K, N, true);
+  return matmul(st, M, K, N, dtype, rows.q, rows.ld, rows.s, M, wt.q, wt.ld, kBlock, wt.s,
+                (N + 127) / 128, nullptr, dx);
 }
 
 }  // extern "C"

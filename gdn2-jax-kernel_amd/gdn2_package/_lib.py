@@ -119,6 +119,12 @@ SIGNATURES = {
     "gdn2_dequantize_fp8": (_c_int, [_vp] + [_c_int] * 3 + [_vp, _c_ll, _c_int] + [_vp] * 3),
     "gdn2_fp8_matmul": (_c_int, [_vp] + [_c_int] * 4 + [_vp, _c_ll] * 3 + [_c_int, _vp, _c_ll]
                         + [_vp] * 2),
+    "gdn2_fp8_linear_kept_bytes": (_c_size, [_c_int] * 5),
+    "gdn2_fp8_linear_workspace_bytes": (_c_size, [_c_int] * 4),
+    "gdn2_fp8_linear_fwd": (_c_int, [_vp] + [_c_int] * 4 + [_vp, _c_ll, _vp, _c_ll, _vp, _c_int,
+                                                            _c_int] + [_vp] * 3 + [_c_size]),
+    "gdn2_fp8_linear_bwd": (_c_int, [_vp] + [_c_int] * 4 + [_vp, _c_ll, _vp, _c_int, _c_int]
+                            + [_vp] * 4 + [_c_size]),
 }
 
 

@@ -43,31 +43,6 @@ def _empty_q(M, C, dev):
     return (q if ld == C else q[:, :C]), ld
 
 
-def _quantize(rows, mode, sums=None):
-    """Rows (M, C) of a supported type in 8 bits.  mode "rows": (q, scale); "columns": those of
-    the transposed matrix; "both": (q, scale, qt, scale_t); "blocks": (q, scale); "blocks both":
-    (q, scale, qt, scale_t).  Scales of rows and columns are (blocks, rows).  sums (C): takes the
-    sums of the columns."""
-    M, C = rows.shape
-    dev, kb, mb = rows.device, _count(C), _count(M)
-    blocks = mode.startswith("blocks")
-    q = s = qt = st = None
-    ldq = ldt = 0
-    if mode != "columns":
-        q, ldq = _empty_q(M, C, dev)
-        s = torch.empty((mb, kb) if blocks else (kb, M), dtype=torch.float32, device=dev)
-    if mode in ("columns", "both", "blocks both"):
-        qt, ldt = _empty_q(C, M, dev)
-        st = torch.empty((kb, mb) if blocks else (mb, C), dtype=torch.float32, device=dev)
-    part = None if sums is None else torch.empty((mb, C), dtype=torch.float32, device=dev)
-    rc = _lib.launch("gdn2_quantize_fp8", dev, M, C, _dtype_code(rows.dtype), rows.data_ptr(),
-                     _row_stride(rows), int(blocks), _ptr(q), ldq, _ptr(s), _ptr(qt), ldt, _ptr(st),
-                     _ptr(part), _ptr(sums))
-    if rc:
-        _raise(rc, f"gdn2_quantize_fp8 (M,C)=({M},{C})")
-    return tuple(t for t in (q, s, qt, st) if t is not None)
-
-
 def gdn2_quantize_fp8(x, blocks=False):
     """x (..., C) in 8 bits: q (float8_e4m3fn of x's shape) and scale (float32), (..., ceil(C / 128))
     for rows, or with blocks=True for a matrix (N, C) (ceil(N / 128), ceil(C / 128))."""
@@ -82,7 +57,16 @@ def gdn2_quantize_fp8(x, blocks=False):
         raise GDN2Error(f"{what}: x must be floating point; got {x.dtype}")
     if x.dtype not in _SUPPORTED_IN:
         x = x.float()
-    q, s = _quantize(_as_rows(x), "blocks" if blocks else "rows")
+    rows = _as_rows(x)
+    M, C = rows.shape
+    q, ld = _empty_q(M, C, x.device)
+    kb = _count(C)
+    s = torch.empty((_count(M), kb) if blocks else (kb, M), dtype=torch.float32, device=x.device)
+    rc = _lib.launch("gdn2_quantize_fp8", x.device, M, C, _dtype_code(rows.dtype), rows.data_ptr(),
+                     _row_stride(rows), int(blocks), q.data_ptr(), ld, s.data_ptr(), None, 0, None,
+                     None, None)
+    if rc:
+        _raise(rc, f"{what} (M,C)=({M},{C})")
     if blocks:
         return q, s
     lead = x.shape[:-1]
@@ -152,22 +136,6 @@ def _by_block(scale, M):
     return scale.movedim(-1, 0).reshape(scale.shape[-1], M).contiguous()
 
 
-def _matmul(x, sx, w, sw, blocks, bias, out_dtype, what):
-    """x (M, K) with sx (blocks, M) times w (N, K)^T with sw (blocks, N) or, for blocks of 128
-    rows, (N / 128, blocks)."""
-    (M, K), N = x.shape, w.shape[0]
-    x, ldx = _wide_rows(x)
-    w, ldw = _wide_rows(w)
-    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-    rc = _lib.launch(
-        "gdn2_fp8_matmul", x.device, M, N, K, _dtype_code(out_dtype), x.data_ptr(), ldx,
-        sx.data_ptr(), M, w.data_ptr(), ldw, _BLOCK if blocks else 1, sw.data_ptr(),
-        _count(K) if blocks else N, _ptr(bias), out.data_ptr())
-    if rc:
-        _raise(rc, f"{what} (M,N,K)=({M},{N},{K})")
-    return out
-
-
 def gdn2_fp8_matmul(q, scale, weight, weight_scale, bias=None, out_dtype=torch.bfloat16):
     """What q stands for times what the weight stands for, transposed, plus bias.
 
@@ -186,25 +154,52 @@ def gdn2_fp8_matmul(q, scale, weight, weight_scale, bias=None, out_dtype=torch.b
                              f"{tuple(weight.shape)}")
     if bias is not None:
         bias = _as(_floating(bias, "bias", (w.shape[0],), dev, what), torch.float32).contiguous()
-    sw = sw.contiguous() if blocks else _by_block(sw, w.shape[0])
-    out = _matmul(x, _by_block(sx, x.shape[0]), w, sw, blocks, bias, out_dtype, what)
-    return out.view(*q.shape[:-1], w.shape[0])
+    (M, K), N = x.shape, w.shape[0]
+    sx = _by_block(sx, M)
+    sw = sw.contiguous() if blocks else _by_block(sw, N)
+    x, ldx = _wide_rows(x)
+    w, ldw = _wide_rows(w)
+    out = torch.empty((*q.shape[:-1], N), dtype=out_dtype, device=dev)
+    rc = _lib.launch(
+        "gdn2_fp8_matmul", dev, M, N, K, _dtype_code(out_dtype), x.data_ptr(), ldx,
+        sx.data_ptr(), M, w.data_ptr(), ldw, _BLOCK if blocks else 1, sw.data_ptr(),
+        _count(K) if blocks else N, _ptr(bias), out.data_ptr())
+    if rc:
+        _raise(rc, f"{what} (M,N,K)=({M},{N},{K})")
+    return out
+
+
+def _launch_linear(x, weight, bias, need_x, need_w):
+    """(y, what the backward needs of x and the weight)"""
+    rows, shape, dev, L = _as_rows(x), x.shape, x.device, _lib.lib()
+    if weight.stride(1) != 1 and weight.shape[1] != 1:
+        weight = weight.contiguous()
+    (M, K), N = rows.shape, weight.shape[0]
+    bias = None if bias is None else _as(bias, torch.float32).contiguous()
+    y = torch.empty((*shape[:-1], N), dtype=x.dtype, device=dev)
+    kept = torch.empty(L.gdn2_fp8_linear_kept_bytes(M, N, K, need_x, need_w), dtype=torch.uint8,
+                       device=dev) if need_x or need_w else None
+    nbytes = L.gdn2_fp8_linear_workspace_bytes(M, N, K, 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    rc = _lib.launch(
+        "gdn2_fp8_linear_fwd", dev, M, N, K, _dtype_code(x.dtype), rows.data_ptr(),
+        _row_stride(rows), weight.data_ptr(), _row_stride(weight), _ptr(bias), need_x, need_w,
+        y.data_ptr(), _ptr(kept), ws.data_ptr(), nbytes)
+    if rc:
+        _raise(rc, f"gdn2_fp8_linear (M,N,K)=({M},{N},{K})")
+    return y, kept
 
 
 class _Fp8Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, keep):
+    def forward(ctx, x, weight, bias):
         # the gradients' operands are made with the forward's: their inputs are read once
-        rows = _as_rows(x)
-        need_x, need_w = keep
-        q, sx, *xt = _quantize(rows, "both" if need_w else "rows")
-        w, sw, *wt = _quantize(weight, "blocks both" if need_x else "blocks")
-        ctx.save_for_backward(*xt, *wt)
-        ctx.need, ctx.shape, ctx.dtype, ctx.bias_dtype = keep, x.shape, x.dtype, \
-            None if bias is None else bias.dtype
-        b = None if bias is None else _as(bias, torch.float32).contiguous()
-        return _matmul(q, sx, w, sw, True, b, x.dtype, "gdn2_fp8_linear").view(
-            *x.shape[:-1], w.shape[0])
+        need_x, need_w = ctx.needs_input_grad[:2]
+        y, kept = _launch_linear(x, weight, bias, need_x, need_w)
+        ctx.save_for_backward(kept)
+        ctx.kept, ctx.shape, ctx.dtype = (need_x, need_w), x.shape, x.dtype
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
 
     @staticmethod
     def backward(ctx, dy):
@@ -212,20 +207,22 @@ class _Fp8Linear(torch.autograd.Function):
 
     @staticmethod
     def _grads(ctx, dy):
-        saved, (need_x, need_w) = list(ctx.saved_tensors), ctx.need
-        rows = _as_rows(_as(dy, ctx.dtype))
-        dx = dw = db = None
-        if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
-            db = torch.empty(rows.shape[1], dtype=torch.float32, device=rows.device)
-        mode = "both" if need_x and need_w else "columns" if need_w else "rows"
-        parts = _quantize(rows, mode, db)
-        xt = saved[:2] if need_w else None
-        wt = saved[2 * need_w:] if need_x else None
-        if need_x:
-            dx = _matmul(*parts[:2], *wt, True, None, ctx.dtype, "gdn2_fp8_linear").view(ctx.shape)
-        if need_w:
-            dw = _matmul(*parts[-2:], *xt, False, None, ctx.dtype, "gdn2_fp8_linear")
-        return dx, dw, None if db is None else _as(db, ctx.bias_dtype), None
+        kept, = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        rows, dev, L = _as_rows(_as(dy, ctx.dtype)), dy.device, _lib.lib()
+        (M, N), K = rows.shape, ctx.shape[-1]
+        dx = torch.empty(ctx.shape, dtype=ctx.dtype, device=dev) if need_x else None
+        dw = torch.empty((N, K), dtype=ctx.dtype, device=dev) if need_w else None
+        db = torch.empty(N, dtype=torch.float32, device=dev) if need_b else None
+        nbytes = L.gdn2_fp8_linear_workspace_bytes(M, N, K, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        rc = _lib.launch(
+            "gdn2_fp8_linear_bwd", dev, M, N, K, _dtype_code(ctx.dtype), rows.data_ptr(),
+            _row_stride(rows), _ptr(kept), *ctx.kept, _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(),
+            nbytes)
+        if rc:
+            _raise(rc, f"gdn2_fp8_linear_bwd (M,N,K)=({M},{N},{K})")
+        return dx, dw, db if db is None else _as(db, ctx.bias_dtype)
 
 
 def gdn2_fp8_linear(x, weight, bias=None):
@@ -257,13 +254,9 @@ def gdn2_fp8_linear(x, weight, bias=None):
         y = xs @ w.t()
         return _as(y if bias is None else y + bias, x.dtype)
     # tangents go to the autograd function too, which refuses them
-    grad = torch.is_grad_enabled()
-    keep = (grad and xs.requires_grad, grad and w.requires_grad)
-    if _forward_mode() or any(keep) or (grad and bias is not None and bias.requires_grad):
-        y = _Fp8Linear.apply(xs, w, bias, keep)
+    if _forward_mode() or torch.is_grad_enabled() and (
+            xs.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)):
+        y = _Fp8Linear.apply(xs, w, bias)
     else:
-        q, sx = _quantize(_as_rows(xs), "rows")
-        wq, sw = _quantize(_as_rows(w), "blocks")
-        b = None if bias is None else _as(bias, torch.float32).contiguous()
-        y = _matmul(q, sx, wq, sw, True, b, t, what).view(*x.shape[:-1], w.shape[0])
+        y, _ = _launch_linear(xs, w, bias, False, False)
     return _as(y, x.dtype)

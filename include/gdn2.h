@@ -549,6 +549,22 @@ int gdn2_fp8_matmul(void* stream, int M, int N, int K, int out_dtype, const void
                     const void* w, long long w_stride, int w_row_block, const float* w_scale,
                     long long w_scale_stride, const float* bias, void* out);
 
+/* A linear layer multiplied in 8 bits, y = x w^T + bias over x (M,K), w (N,K), y (M,N) dense, all
+ * of dtype, bias float32 or NULL; rows of x, w and dy are *_stride elements apart.  Forward: x in
+ * blocks of 1 x 128, w of 128 x 128.  Backward: dx from dy in blocks of 1 x 128 and w's, dw from dy
+ * and x in blocks of 128 tokens, dbias (float32) the sums of dy's columns.  kept holds the
+ * operands of the gradients that need_dx and need_dw name (NULL for neither), for the backward,
+ * which is told the same (kept_dx, kept_dw) and writes those of dx, dw and dbias that are not NULL.
+ * M, N, K <= 2^24; kept and ws 16-byte aligned. */
+size_t gdn2_fp8_linear_kept_bytes(int M, int N, int K, int need_dx, int need_dw);
+size_t gdn2_fp8_linear_workspace_bytes(int M, int N, int K, int backward);
+int gdn2_fp8_linear_fwd(void* stream, int M, int N, int K, int dtype, const void* x,
+                        long long x_stride, const void* w, long long w_stride, const float* bias,
+                        int need_dx, int need_dw, void* y, void* kept, void* ws, size_t ws_bytes);
+int gdn2_fp8_linear_bwd(void* stream, int M, int N, int K, int dtype, const void* dy,
+                        long long dy_stride, const void* kept, int kept_dx, int kept_dw, void* dx,
+                        void* dw, float* dbias, void* ws, size_t ws_bytes);
+
 #ifdef __cplusplus
 }
 #endif

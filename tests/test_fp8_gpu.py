@@ -86,25 +86,42 @@ def test_quantize_and_back(dev, C, M, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("M,C", [(1, 5), (130, 100), (300, 257), (128, 128)])
 def test_both_directions(dev, M, C, dtype):
-    """What the linear layer quantises at once: rows, columns, their sums, blocks transposed."""
-    from gdn2_package import gdn2_fp8
+    """gdn2_quantize_fp8 of the C ABI with rows and columns at once, the columns' sums, columns
+    alone, and blocks both ways."""
+    from gdn2_package import _lib
+    L, code = _lib.lib(), _lib.GDN2_F32 if dtype == F32 else _lib.GDN2_BF16
     x = values(M, C, dtype, dev, 3)
-    sums = torch.empty(C, device=dev)
-    q, s, qt, st = gdn2_fp8._quantize(x, "both", sums)
-    for got, scale, t in ((q, s, x), (qt, st, x.t())):
-        _, qv, sv = held(t.double(), 1, 128)
-        assert torch.equal(got.double(), qv) and torch.equal(scale.t().double(), sv)
+    kb, mb, up = -(-C // 128), -(-M // 128), lambda n: (n + 15) // 16 * 16
+    f32 = lambda *s: torch.full(s, torch.nan, device=dev)
+    u8 = lambda *s: torch.full(s, 0x7F, dtype=torch.uint8, device=dev)
+    q, qt, part, sums = u8(M, up(C)), u8(C, up(M)), f32(mb, C), f32(C)
+
+    def call(blocks, q, s, qt, st, part=None, sums=None):
+        ptr = lambda t: None if t is None else t.data_ptr()
+        assert L.gdn2_quantize_fp8(torch.cuda.current_stream().cuda_stream, M, C, code,
+                                   x.data_ptr(), C, blocks, ptr(q), up(C), ptr(s), ptr(qt), up(M),
+                                   ptr(st), ptr(part), ptr(sums)) == 0
+
+    def same(q, s, t, down):
+        _, qv, sv = held(t.double(), down, 128)
+        width = t.shape[1]
+        assert torch.equal(q.view(E4M3)[:, :width].double(), qv) and (q[:, width:] == 0).all()
+        assert torch.equal(s.double(), sv)
+    s, st = f32(kb, M), f32(mb, C)
+    call(0, q, s, qt, st, part, sums)
+    same(q, s.t(), x, 1)
+    same(qt, st.t(), x.t(), 1)
+    # eight rows, sixteen of those, and the rows of partial sums in turn
     mag = x.double().abs().sum(0)
-    assert ((sums.double() - x.double().sum(0)).abs() <= (24 + M / 128 / 16 + 16) * ULP * mag).all()
-    qc, sc = gdn2_fp8._quantize(x, "columns")
-    assert torch.equal(qc.double(), qt.double()) and torch.equal(sc, st)
-    q, s, qt, st = gdn2_fp8._quantize(x, "blocks both")
-    _, qv, sv = held(x.double(), 128, 128)
-    assert torch.equal(q.double(), qv) and torch.equal(qt.double(), qv.t())
-    assert torch.equal(s.double(), sv) and torch.equal(st, s.t())
-    ld = (M + 15) // 16 * 16
-    rows = torch.as_strided(qt.view(torch.uint8), (C, ld), (ld, 1))
-    assert (rows[:, M:] == 0).all()
+    assert ((sums.double() - x.double().sum(0)).abs() <= (8 + 16 + mb + 16) * ULP * mag).all()
+    qt.fill_(0x7F), st.fill_(torch.nan)
+    call(0, None, None, qt, st)
+    same(qt, st.t(), x.t(), 1)
+    q.fill_(0x7F), qt.fill_(0x7F)
+    s, st = f32(mb, kb), f32(kb, mb)
+    call(1, q, s, qt, st)
+    same(q, s, x, 128)
+    same(qt, st, x.t(), 128)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
