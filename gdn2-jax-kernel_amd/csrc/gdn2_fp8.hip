@@ -28,6 +28,8 @@
 // bytes of both operands from K on are zeroed in the last slice (what is there may be NaN).
 #include <limits.h>
 
+#include <utility>
+
 #include "gdn2.h"
 #include "gdn2_common.h"
 
@@ -55,6 +57,10 @@ struct QuantArgs {
   unsigned char *q, *qt;     // (M, ldq), (C, ldt): rows, and columns as rows
   long long ldq, ldt;
   float *s, *st;             // (C / 128, M), (M / 128, C); blocks: (M / 128, C / 128) and transposed
+  // instead of s and st, the scales' exponents for each row of q and qt, block after block:
+  // (M, lds8), (C, ldt8), biased as the matrix instruction takes them
+  unsigned char *s8, *st8;
+  int lds8, ldt8;
   float* part;               // (M / 128, C) sums of each 128 rows, or null
   int M, C, kb, mb;          // blocks along the columns, the rows
   int vec;
@@ -73,6 +79,10 @@ __device__ __forceinline__ void scales(unsigned top, float& s, float& inv) {
     s = __builtin_nanf("");
     inv = 0.f;
   }
+}
+// The biased exponent of a scale; 255 stands for NaN, and of zeros any scale is one.
+__device__ __forceinline__ unsigned char exponent(float s) {
+  return (unsigned char)(__float_as_uint(s) >> 23 & 0xffu);
 }
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
@@ -156,7 +166,12 @@ __global__ void __launch_bounds__(256) fp8_quantize(QuantArgs a) {
           *reinterpret_cast<i32x2*>(q + r * a.ldq) =
               i32x2{pack4(v[r][0], v[r][1], v[r][2], v[r][3], i, i, i, i),
                     pack4(v[r][4], v[r][5], v[r][6], v[r][7], i, i, i, i)};
-        if ((tid & 15) == 0) a.s[(long long)tc * a.M + m + r] = s;
+        if ((tid & 15) == 0) {
+          if (a.s8)
+            a.s8[(long long)(m + r) * a.lds8 + tc] = exponent(s);
+          else
+            a.s[(long long)tc * a.M + m + r] = s;
+        }
       }
     }
   }
@@ -200,14 +215,23 @@ __global__ void __launch_bounds__(256) fp8_quantize(QuantArgs a) {
           *reinterpret_cast<i32x2*>(q + r * a.ldq) =
               i32x2{pack4(v[r][0], v[r][1], v[r][2], v[r][3], i[0], i[0], i[0], i[0]),
                     pack4(v[r][4], v[r][5], v[r][6], v[r][7], i[0], i[0], i[0], i[0])};
-      if (tid == 0) {
+      const int row = tm * kBlock + tid, col = tc * kBlock + tid;
+      if (a.s8) {
+        if (tid < kBlock && row < a.M) a.s8[(long long)row * a.lds8 + tc] = exponent(s[0]);
+        if (a.st8 && tid < kBlock && col < a.C) a.st8[(long long)col * a.ldt8 + tm] = exponent(s[0]);
+      } else if (tid == 0) {
         a.s[(long long)tm * a.kb + tc] = s[0];
         if (a.st) a.st[(long long)tc * a.mb + tm] = s[0];
       }
     } else if ((tid >> 4) == 0) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (c + k < a.C) a.st[(long long)tm * a.C + c + k] = s[k];
+        if (c + k < a.C) {
+          if (a.st8)
+            a.st8[(long long)(c + k) * a.ldt8 + tm] = exponent(s[k]);
+          else
+            a.st[(long long)tm * a.C + c + k] = s[k];
+        }
     }
     if (a.qt && m < a.ldt) {
 #pragma unroll
@@ -257,9 +281,14 @@ __global__ void __launch_bounds__(256) fp8_dequantize(const unsigned char* q, lo
 
 // ---- Product ---------------------------------------------------------------------------
 
+// Scales of the weight: one for each 128 rows, for each row, or (kExponents) those of both
+// operands as exponents for each row, applied by the matrix instruction itself.
+enum Scaling { kOfBlocks, kOfRows, kExponents };
 struct MmArgs {
   const unsigned char *x, *w;
   long long ldx, ldw;          // bytes between rows
+  const unsigned char *ex, *ew;  // exponents (M, lde), (N, lde), lde a multiple of 4
+  int lde;
   const float *sx, *sw;        // (blocks, M); (blocks, N) or, for blocks of 128 rows, (N / 128, blocks)
   const float* bias;           // (N) or null
   long long ldsx, ldsw;        // elements between rows of sx and sw
@@ -429,14 +458,15 @@ struct Tile {
   static constexpr int STAGE = (BM + BN) * kBK;
   static constexpr int NL = STAGE / 1024 / NW;                     // DMA instructions of a wave
   static_assert(STAGE % (1024 * NW) == 0 && NI % 2 == 0 && BM % 16 == 0, "tile");
-  static_assert(kBlock % BN == 0, "a tile lies within one block of the weight's rows");
+  static_assert(kBlock % BN == 0 || BN % kBlock == 0, "a tile lies within one block of the weight's rows");
 };
 
-// WROW: the weight has a scale for each row, else for each 128 rows.
-template <typename C, bool WROW, typename TO>
+template <typename C, Scaling SC, typename TO>
 __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmArgs a) {
   constexpr int BM = C::BM, BN = C::BN, NW = C::NW, MI = C::MI, NI = C::NI, NL = C::NL;
   constexpr int ST = C::ST;
+  constexpr bool WROW = SC == kOfRows, MX = SC == kExponents;
+  static_assert(!MX || (ST % 2 == 0 && sizeof(TO) == 2), "four exponents are read at a time");
   __shared__ __attribute__((aligned(16))) char lds[ST * C::STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, lg = lane >> 4;
@@ -496,28 +526,45 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     const char* s = lds + buf * C::STAGE;
     return both(*reinterpret_cast<const i32x4*>(s + at), *reinterpret_cast<const i32x4*>(s + (at ^ 64)));
   };
-  // scales of one slice: rows 16 i + li of x; of w one, or columns 32 j + 8 lg + e
+  // scales of one slice: rows 16 i + li of x; of w one, or columns 32 j + 8 lg + e.  Exponents: of
+  // four slices, a byte each, for the rows of the fragments.
   struct Scales {
     float row[MI], col[WROW ? NI / 2 : 1][8];
   };
+  struct Exponents {
+    int row[MI], col[NI];
+  };
   const int nk = (a.K + kBK - 1) / kBK;
-  int sm[MI];
+  int sm[MI], sn[NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int r = m0 + wm + 16 * i + li;
-    sm[i] = r < a.M ? r : a.M - 1;
+    sm[i] = (r < a.M ? r : a.M - 1) * (MX ? a.lde : 1);
   }
-  auto load_scales = [&](Scales& s, int kb) {
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int r = n0 + wn + (j / 2) * 32 + (li / 4) * 8 + (j & 1) * 4 + li % 4;
+    sn[j] = (r < a.N ? r : a.N - 1) * a.lde;
+  }
+  using Factors = std::conditional_t<MX, Exponents, Scales>;
+  auto load_scales = [&](Factors& s, int kb) {
     kb = kb < nk ? kb : nk - 1;
-    const float* p = a.sx + kb * a.ldsx;
+    if constexpr (MX) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) s.row[i] = p[sm[i]];
-    if constexpr (WROW) {
+      for (int i = 0; i < MI; ++i) s.row[i] = *reinterpret_cast<const int*>(a.ex + sm[i] + kb);
 #pragma unroll
-      for (int j = 0; j < NI / 2; ++j)
-        load_columns(a.sw + kb * a.ldsw, n0 + wn + 32 * j + 8 * lg, a.N, s.col[j]);
+      for (int j = 0; j < NI; ++j) s.col[j] = *reinterpret_cast<const int*>(a.ew + sn[j] + kb);
     } else {
-      s.col[0][0] = a.sw[n0 / kBlock * a.ldsw + kb];
+      const float* p = a.sx + kb * a.ldsx;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) s.row[i] = p[sm[i]];
+      if constexpr (WROW) {
+#pragma unroll
+        for (int j = 0; j < NI / 2; ++j)
+          load_columns(a.sw + kb * a.ldsw, n0 + wn + 32 * j + 8 * lg, a.N, s.col[j]);
+      } else {
+        s.col[0][0] = a.sw[n0 / kBlock * a.ldsw + kb];
+      }
     }
   };
 
@@ -528,26 +575,37 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     for (int i = 0; i < MI; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   // the outputs of half of the weight's fragments
   constexpr int NH = NI / 2;
-  auto multiply = [&](const i32x8 (&w)[NH], const i32x8 (&x)[MI], const Scales& s, int j0) {
+  auto multiply = [&](const i32x8 (&w)[NH], const i32x8 (&x)[MI], const Factors& s, int j0,
+                      auto byte) {
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const float f = WROW ? s.row[i] : s.row[i] * s.col[0][0];
+      if constexpr (MX) {
 #pragma unroll
-      for (int j = 0; j < NH; ++j) {
-        const f32x4 p = mma8<TO>(w[j], x[i]);
-        f32x4& c = acc[j0 + j][i];
+        for (int j = 0; j < NH; ++j) {
+          f32x4& c = acc[j0 + j][i];
+          c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              w[j], x[i], c, 0, 0, decltype(byte)::value, s.col[j0 + j], decltype(byte)::value,
+              s.row[i]);
+        }
+      } else {
+        const float f = WROW ? s.row[i] : s.row[i] * s.col[0][0];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (WROW)
-            c[e] = fmaf(p[e] * f, s.col[(j0 + j) / 2][(j0 + j) % 2 * 4 + e], c[e]);
-          else
-            c[e] = fmaf(p[e], f, c[e]);
+        for (int j = 0; j < NH; ++j) {
+          const f32x4 p = mma8<TO>(w[j], x[i]);
+          f32x4& c = acc[j0 + j][i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (WROW)
+              c[e] = fmaf(p[e] * f, s.col[(j0 + j) / 2][(j0 + j) % 2 * 4 + e], c[e]);
+            else
+              c[e] = fmaf(p[e], f, c[e]);
+          }
         }
       }
     }
   };
 
-  Scales sc[2];
+  Factors sc[2];   // of slices in turn, or of four slices
   load_scales(sc[0], 0);
 #pragma unroll
   for (int s = 0; s < ST; ++s)
@@ -566,17 +624,23 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     for (int i = 0; i < MI; ++i) x[p][i] = row(buf, rx[i]);
   };
   read(0, 0);
-  constexpr int UN = ST % 2 ? 2 * ST : ST;   // slices of one round: the registers alternate
+  // slices of one round: the registers alternate (with exponents, every four slices)
+  constexpr int UN = MX ? 8 : ST % 2 ? 2 * ST : ST;
+  static_assert(UN % ST == 0, "a slice's place in LDS is known");
   for (int k0 = 0; k0 < nk; k0 += UN) {
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int kb = k0 + u, buf = u % ST;
-      if (kb >= nk) break;
+    auto slice = [&](auto number) {
+      constexpr int u = decltype(number)::value, buf = u % ST;
+      constexpr int now = MX ? u / 4 % 2 : u & 1;
+      const std::integral_constant<int, MX ? u & 3 : 0> byte;
+      const int kb = k0 + u;
       auto& xs = x[u & 1];
       auto& ws = w0[u & 1];
 #pragma unroll
       for (int j = 0; j < NH; ++j) w1[j] = row(buf, rw[NH + j]);
-      load_scales(sc[(u + 1) & 1], kb + 1);
+      if constexpr (!MX)
+        load_scales(sc[1 - now], kb + 1);
+      else if constexpr (u % 4 == 0)
+        load_scales(sc[1 - now], kb + 4 < nk ? kb + 4 : kb);
       const int left = a.K - kb * kBK;
       if (left < kBK) {
 #pragma unroll
@@ -587,7 +651,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
           keep_row(w1[j], lg, left);
         }
       }
-      multiply(ws, xs, sc[u & 1], 0);
+      multiply(ws, xs, sc[now], 0, byte);
       // slice kb + 1 has arrived once only the ST - 2 later ones are in flight; every wave has
       // read slice kb, whose buffer is free
       if (kb + ST <= nk)
@@ -597,17 +661,22 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
       lds_barrier();
       if (kb + ST < nk) load(kb + ST, buf);
       read((u + 1) & 1, (u + 1) % ST);   // after the last slice: stale data that nothing uses
-      multiply(w1, xs, sc[u & 1], NH);
-    }
+      multiply(w1, xs, sc[now], NH, byte);
+    };
+    [&]<int... U>(std::integer_sequence<int, U...>) {
+      // stops at the last slice
+      ((k0 + U < nk ? (slice(std::integral_constant<int, U>{}), true) : false) && ...);
+    }(std::make_integer_sequence<int, UN>{});
   }
   store_part<TO>(a, acc, m0 + wm, n0 + wn, li, lg);
 }
 
 // 16 weight rows and all of x's (up to 16 MT) a workgroup; wave w takes the slices of 128
 // bytes w, w + 8, ... of k.
-template <int MT, bool WROW, typename TO>
+template <int MT, Scaling SC, typename TO>
 __global__ void __launch_bounds__(512) fp8_mm_rows(MmArgs a) {
   constexpr int NW = 8;
+  constexpr bool WROW = SC == kOfRows, MX = SC == kExponents;
   __shared__ float sum[NW][MT][16][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int li = lane & 15, lg = lane >> 4;
@@ -635,13 +704,21 @@ __global__ void __launch_bounds__(512) fp8_mm_rows(MmArgs a) {
       if (k0 + kBK > a.K) keep_row(v, lg, a.K - k0);
       return v;
     };
+    const i32x8 fw = row(w);
+    if constexpr (MX) {
+      const int ew = a.ew[(long long)n * a.lde + kb];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+            fw, row(x[i]), acc[i], 0, 0, 0, ew, 0, (int)a.ex[(long long)m[i] * a.lde + kb]);
+      continue;
+    }
     float sw[4], sx[MT];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       sw[r] = WROW ? a.sw[kb * a.ldsw + c[r]] : a.sw[n0 / kBlock * a.ldsw + kb];
 #pragma unroll
     for (int i = 0; i < MT; ++i) sx[i] = a.sx[kb * a.ldsx + m[i]];
-    const i32x8 fw = row(w);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const f32x4 p = mma8<TO>(fw, row(x[i]));
@@ -666,34 +743,34 @@ __global__ void __launch_bounds__(512) fp8_mm_rows(MmArgs a) {
   }
 }
 
-template <typename C, bool WROW, typename TO>
+template <typename C, Scaling SC, typename TO>
 void launch_tiles(hipStream_t st, MmArgs a) {
   a.tm = (a.M + C::BM - 1) / C::BM;
   a.tn = (a.N + C::BN - 1) / C::BN;
   a.chunk = (a.tm * a.tn + 7) / 8;
-  hipLaunchKernelGGL((fp8_mm<C, WROW, TO>), dim3(8u * (unsigned)a.chunk), dim3(64 * C::NW), 0, st, a);
+  hipLaunchKernelGGL((fp8_mm<C, SC, TO>), dim3(8u * (unsigned)a.chunk), dim3(64 * C::NW), 0, st, a);
 }
-template <int MT, bool WROW, typename TO>
+template <int MT, Scaling SC, typename TO>
 void launch_rows(hipStream_t st, const MmArgs& a) {
-  hipLaunchKernelGGL((fp8_mm_rows<MT, WROW, TO>),
+  hipLaunchKernelGGL((fp8_mm_rows<MT, SC, TO>),
                      dim3((unsigned)((a.N + 15) / 16), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
                      dim3(512), 0, st, a);
 }
 
-template <bool WROW, typename TO>
+template <Scaling SC, typename TO>
 hipError_t launch_mm(hipStream_t st, const MmArgs& a) {
   const int cus = num_cus();
   auto tiles = [&](int bm, int bn) {
     return (((long long)a.M + bm - 1) / bm) * (((long long)a.N + bn - 1) / bn);
   };
   if (a.M <= 16)
-    launch_rows<1, WROW, TO>(st, a);
+    launch_rows<1, SC, TO>(st, a);
   else if (a.M <= 32 || tiles(32, 16) <= cus)
-    launch_rows<2, WROW, TO>(st, a);
+    launch_rows<2, SC, TO>(st, a);
   else if (sizeof(TO) == 4 || tiles(64, 64) <= 3 * cus)   // float32: registers for no more
-    launch_tiles<Tile<64, 64, 2, 2, 3, 3>, WROW, TO>(st, a);
+    launch_tiles<Tile<64, 64, 2, 2, SC == kExponents ? 4 : 3, SC == kExponents ? 2 : 3>, SC, TO>(st, a);
   else if constexpr (sizeof(TO) == 2)
-    launch_tiles<Tile<128, 128, 2, 2, 2, 2>, WROW, TO>(st, a);
+    launch_tiles<Tile<128, 128, 2, 2, 2, 2>, SC, TO>(st, a);
   return hipGetLastError();
 }
 
@@ -713,10 +790,13 @@ hipError_t launch_quantize(hipStream_t st, const QuantArgs& a, int mode) {
 
 size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-// What gdn2_quantize_fp8 takes, checked; the launches.
+// Bytes between rows of exponents of nb blocks.
+int exponents_of(int nb) { return (nb + 3) / 4 * 4; }
+
+// What gdn2_quantize_fp8 takes, checked; the launches.  exponents: scales come as those, for each row.
 int quantize(hipStream_t st, int M, int C, int x_dtype, const void* x, long long x_stride,
              int blocks, void* q, long long q_stride, float* scale, void* qt, long long qt_stride,
-             float* scale_t, float* part, float* sums) {
+             float* scale_t, float* part, float* sums, bool exponents = false) {
   if (M < 0 || C < 1 || C > INT_MAX - 256 || M > INT_MAX - 256) return GDN2_ERR_SHAPE;
   if (x_dtype != GDN2_F32 && x_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
   if (blocks != 0 && blocks != 1) return GDN2_ERR_FLAGS;
@@ -738,6 +818,10 @@ int quantize(hipStream_t st, int M, int C, int x_dtype, const void* x, long long
   a.x = x, a.ldx = x_stride, a.M = M, a.C = C;
   a.q = (unsigned char*)q, a.ldq = q_stride, a.s = scale;
   a.qt = (unsigned char*)qt, a.ldt = qt_stride, a.st = qt ? scale_t : nullptr;
+  if (exponents) {
+    a.s8 = (unsigned char*)scale, a.lds8 = exponents_of(a.kb);
+    a.st8 = (unsigned char*)a.st, a.ldt8 = exponents_of(a.mb);
+  }
   // eight values at a time
   a.vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0;
   const int mode = blocks ? kBlocks : (q ? kRows : 0) | (qt ? kCols : 0);
@@ -753,7 +837,7 @@ int quantize(hipStream_t st, int M, int C, int x_dtype, const void* x, long long
 int matmul(hipStream_t st, int M, int N, int K, int out_dtype, const void* x, long long x_stride,
            const float* x_scale, long long x_scale_stride, const void* w, long long w_stride,
            int w_row_block, const float* w_scale, long long w_scale_stride, const float* bias,
-           void* out) {
+           void* out, bool exponents = false) {
   if (M < 0 || N < 1 || K < 1 || K > INT_MAX - 256) return GDN2_ERR_SHAPE;
   if (w_row_block != 1 && w_row_block != kBlock) return GDN2_ERR_SHAPE;
   if (out_dtype != GDN2_F32 && out_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
@@ -780,10 +864,18 @@ int matmul(hipStream_t st, int M, int N, int K, int out_dtype, const void* x, lo
   a.sx = x_scale, a.sw = w_scale, a.ldsx = x_scale_stride, a.ldsw = w_scale_stride;
   a.bias = bias, a.out = out, a.M = M, a.N = N, a.K = K;
   hipError_t e;
-  if (w_row_block == 1)
-    e = out_dtype == GDN2_F32 ? launch_mm<true, float>(st, a) : launch_mm<true, bf16_t>(st, a);
-  else
-    e = out_dtype == GDN2_F32 ? launch_mm<false, float>(st, a) : launch_mm<false, bf16_t>(st, a);
+  if (exponents) {   // bfloat16 results alone
+    a.ex = (const unsigned char*)x_scale, a.ew = (const unsigned char*)w_scale;
+    a.lde = exponents_of((int)kb);
+    // rows of exponents are reached in 32 bits
+    if ((double)a.lde * (M > N ? M : N) > (double)INT_MAX) return GDN2_ERR_SHAPE;
+    e = launch_mm<kExponents, bf16_t>(st, a);
+  } else if (w_row_block == 1) {
+    e = out_dtype == GDN2_F32 ? launch_mm<kOfRows, float>(st, a) : launch_mm<kOfRows, bf16_t>(st, a);
+  } else {
+    e = out_dtype == GDN2_F32 ? launch_mm<kOfBlocks, float>(st, a)
+                              : launch_mm<kOfBlocks, bf16_t>(st, a);
+  }
   return e == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
 }
 
@@ -794,8 +886,10 @@ struct Held {
   long long ld;     // bytes between rows
   // blocks: of 128 x 128, else of 1 x 128
   static size_t bytes(int rows, int along, bool blocks) {
+    // room for either form of the scales
     const size_t nb = (along + 127) / 128, n = blocks ? (rows + 127) / 128 : rows;
-    return round_up((size_t)rows * round_up(along, 16), 16) + round_up(n * nb * 4, 16);
+    const size_t f = n * nb * 4, e = (size_t)rows * exponents_of((int)nb);
+    return round_up((size_t)rows * round_up(along, 16), 16) + round_up(f > e ? f : e, 16);
   }
   // at p, which moves past it
   Held(char*& p, int rows, int along, bool blocks) : q(p), ld((long long)round_up(along, 16)) {
@@ -808,6 +902,7 @@ int validate_linear(int M, int N, int K, int dtype) {
   if (M < 0 || N < 1 || K < 1 || N > (1 << 24) || K > (1 << 24) || M > (1 << 24))
     return GDN2_ERR_SHAPE;
   const long long m = (M + 63ll) / 64, n = (N + 63ll) / 64, k = (K + 63ll) / 64;
+  // (m n <= 2^23 and the like also keep rows of exponents, at most (m + 1) (k / 2 + 4) 64, in 32 bits)
   if (m * n > (1ll << 23) || m * k > (1ll << 23) || n * k > (1ll << 23)) return GDN2_ERR_SHAPE;
   return dtype == GDN2_F32 || dtype == GDN2_BF16 ? GDN2_OK : GDN2_ERR_DTYPE;
 }
@@ -883,15 +978,16 @@ int gdn2_fp8_linear_fwd(void* stream, int M, int N, int K, int dtype, const void
   const long long kb = (K + 127) / 128;
   char *p = (char*)ws, *k = (char*)kept;
   const Held qx(p, M, K, false), qw(p, N, K, true);
+  const bool mx = dtype == GDN2_BF16;   // float32 results: see mma8
   Held xt = qx, wt = qw;
   if (need_dw) xt = Held(k, K, M, false);
   if (need_dx) wt = Held(k, K, N, true);
   if ((rc = quantize(st, M, K, dtype, x, x_stride, 0, qx.q, qx.ld, qx.s, need_dw ? xt.q : nullptr,
-                     xt.ld, xt.s, nullptr, nullptr)) ||
+                     xt.ld, xt.s, nullptr, nullptr, mx)) ||
       (rc = quantize(st, N, K, dtype, w, w_stride, 1, qw.q, qw.ld, qw.s, need_dx ? wt.q : nullptr,
-                     wt.ld, wt.s, nullptr, nullptr)))
+                     wt.ld, wt.s, nullptr, nullptr, mx)))
     return rc;
-  return matmul(st, M, N, K, dtype, qx.q, qx.ld, qx.s, M, qw.q, qw.ld, kBlock, qw.s, kb, bias, y);
+  return matmul(st, M, N, K, dtype, qx.q, qx.ld, qx.s, M, qw.q, qw.ld, kBlock, qw.s, kb, bias, y, mx);
 }
 
 int gdn2_fp8_linear_bwd(void* stream, int M, int N, int K, int dtype, const void* dy,
@@ -908,20 +1004,21 @@ int gdn2_fp8_linear_bwd(void* stream, int M, int N, int K, int dtype, const void
   char *p = (char*)ws, *k = (char*)kept;
   const Held rows(p, M, N, false), cols(p, N, M, false);
   const bool need_rows = dx || !dw;   // the sums alone come with either
+  const bool mx = dtype == GDN2_BF16;
   if ((rc = quantize(st, M, N, dtype, dy, dy_stride, 0, need_rows ? rows.q : nullptr, rows.ld,
                      rows.s, dw ? cols.q : nullptr, cols.ld, cols.s, dbias ? (float*)p : nullptr,
-                     dbias)))
+                     dbias, mx)))
     return rc;
   const Held xt = kept_dw ? Held(k, K, M, false) : rows;
   if (dw) {
     if ((rc = matmul(st, N, K, M, dtype, cols.q, cols.ld, cols.s, N, xt.q, xt.ld, 1, xt.s, K,
-                     nullptr, dw)))
+                     nullptr, dw, mx)))
       return rc;
   }
   if (!dx) return GDN2_OK;
   const Held wt(k, K, N, true);
   return matmul(st, M, K, N, dtype, rows.q, rows.ld, rows.s, M, wt.q, wt.ld, kBlock, wt.s,
-                (N + 127) / 128, nullptr, dx);
+                (N + 127) / 128, nullptr, dx, mx);
 }
 
 }  // extern "C"
