@@ -467,7 +467,10 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   constexpr int ST = C::ST;
   constexpr bool WROW = SC == kOfRows, MX = SC == kExponents;
   static_assert(!MX || (ST % 2 == 0 && sizeof(TO) == 2), "four exponents are read at a time");
+  // with a scale for each row of both operands, those of a slice come with it
+  constexpr int SCALES = WROW ? BM + BN : 0, NV = NL + (WROW ? 1 : 0);
   __shared__ __attribute__((aligned(16))) char lds[ST * C::STAGE];
+  __shared__ __attribute__((aligned(16))) float lds_scales[WROW ? ST * SCALES : 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, lg = lane >> 4;
 
@@ -494,10 +497,25 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     base[i] = (const char*)(act ? a.x + m0 * a.ldx : a.w + n0 * a.ldw);
     off[i] = (unsigned)(r < most ? r : most) * (unsigned)(act ? a.ldx : a.ldw) + at[i];
   }
+  // 64 of the scales a wave (some waves the same as others, where there are fewer)
+  const int part = WROW ? wave % (SCALES / 64) : 0;
+  const float* scale = a.sx;
+  long long scale_stride = a.ldsx;
+  unsigned scale_off = 0;
+  if constexpr (WROW) {
+    static_assert(BM % 64 == 0 && BN % 64 == 0, "a wave's scales are of one operand");
+    const int e = part * 64 + lane, r = e < BM ? m0 + e : n0 + e - BM;
+    const int most = (part * 64 < BM ? a.M : a.N) - 1;
+    if (part * 64 >= BM) scale = a.sw, scale_stride = a.ldsw;
+    scale_off = 4u * (unsigned)(r < most ? r : most);
+  }
   const int last = (a.K + 15) / 16 * 16 - 16;   // the last readable piece of a row
-  auto load = [&](int kb, int buf) {
+  auto load = [&](int kb, int buf, auto whole) {
+    if constexpr (WROW)
+      lds_dma4((const char*)(scale + kb * scale_stride) + (size_t)scale_off,
+               lds_scales + buf * SCALES + part * 64);
     char* dst = lds + buf * C::STAGE + wave * NL * 1024;
-    if ((kb + 1) * kBK <= last + 16) {
+    if (decltype(whole)::value || (kb + 1) * kBK <= last + 16) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) lds_dma16(base[i] + kb * kBK + (size_t)off[i], dst + i * 1024);
     } else {
@@ -558,13 +576,22 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
       const float* p = a.sx + kb * a.ldsx;
 #pragma unroll
       for (int i = 0; i < MI; ++i) s.row[i] = p[sm[i]];
-      if constexpr (WROW) {
+      s.col[0][0] = a.sw[n0 / kBlock * a.ldsw + kb];
+    }
+  };
+  auto read_scales = [&](Factors& s, int buf) {   // from LDS
+    if constexpr (WROW) {
+      const float* p = lds_scales + buf * SCALES;
 #pragma unroll
-        for (int j = 0; j < NI / 2; ++j)
-          load_columns(a.sw + kb * a.ldsw, n0 + wn + 32 * j + 8 * lg, a.N, s.col[j]);
-      } else {
-        s.col[0][0] = a.sw[n0 / kBlock * a.ldsw + kb];
-      }
+      for (int i = 0; i < MI; ++i) s.row[i] = p[wm + 16 * i + li];
+#pragma unroll
+      for (int j = 0; j < NI / 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 v = *reinterpret_cast<const f32x4*>(p + BM + wn + 32 * j + 8 * lg + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s.col[j][4 * h + e] = v[e];
+        }
     }
   };
 
@@ -605,13 +632,13 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     }
   };
 
-  Factors sc[2];   // of slices in turn, or of four slices
-  load_scales(sc[0], 0);
+  Factors sc[2];   // of slices in turn; exponents: of four slices and the four after them
+  if constexpr (!WROW) load_scales(sc[0], 0);
 #pragma unroll
   for (int s = 0; s < ST; ++s)
-    if (s < nk) load(s, s);
+    if (s < nk) load(s, s, std::false_type{});
   if (nk >= ST)
-    wait_vmcnt<(ST - 1) * NL>();
+    wait_vmcnt<(ST - 1) * NV>();
   else
     wait_vmcnt<0>();
   lds_barrier();
@@ -624,23 +651,25 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     for (int i = 0; i < MI; ++i) x[p][i] = row(buf, rx[i]);
   };
   read(0, 0);
-  // slices of one round: the registers alternate (with exponents, every four slices)
-  constexpr int UN = MX ? 8 : ST % 2 ? 2 * ST : ST;
-  static_assert(UN % ST == 0, "a slice's place in LDS is known");
-  for (int k0 = 0; k0 < nk; k0 += UN) {
-    auto slice = [&](auto number) {
-      constexpr int u = decltype(number)::value, buf = u % ST;
-      constexpr int now = MX ? u / 4 % 2 : u & 1;
-      const std::integral_constant<int, MX ? u & 3 : 0> byte;
-      const int kb = k0 + u;
-      auto& xs = x[u & 1];
-      auto& ws = w0[u & 1];
+  // A slice.  INNER: a whole one with ST more behind it; no branches, so that its products stay where
+  // they are written, between the reads (moved behind the branches by the compiler, the products
+  // of a slice ran in one piece after the barrier and its reads in another: AAA).
+  auto slice = [&](auto number, auto inner, int kb) {
+    constexpr bool INNER = decltype(inner)::value;
+    constexpr int u = decltype(number)::value, buf = u % ST;
+    constexpr int now = MX || WROW ? 0 : u & 1;
+    const std::integral_constant<int, MX ? u & 3 : 0> byte;
+    auto& xs = x[u & 1];
+    auto& ws = w0[u & 1];
 #pragma unroll
-      for (int j = 0; j < NH; ++j) w1[j] = row(buf, rw[NH + j]);
-      if constexpr (!MX)
-        load_scales(sc[1 - now], kb + 1);
-      else if constexpr (u % 4 == 0)
-        load_scales(sc[1 - now], kb + 4 < nk ? kb + 4 : kb);
+    for (int j = 0; j < NH; ++j) w1[j] = row(buf, rw[NH + j]);
+    if constexpr (WROW)
+      read_scales(sc[0], buf);
+    else if constexpr (!MX)
+      load_scales(sc[1 - now], kb + 1);
+    else if constexpr (u % 4 == 0)
+      load_scales(sc[1], kb + 4 < nk ? kb + 4 : kb);
+    if constexpr (!INNER) {
       const int left = a.K - kb * kBK;
       if (left < kBK) {
 #pragma unroll
@@ -651,23 +680,43 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
           keep_row(w1[j], lg, left);
         }
       }
-      multiply(ws, xs, sc[now], 0, byte);
-      // slice kb + 1 has arrived once only the ST - 2 later ones are in flight; every wave has
-      // read slice kb, whose buffer is free
-      if (kb + ST <= nk)
-        wait_vmcnt<(ST - 2) * NL>();
-      else
-        wait_vmcnt<0>();
-      lds_barrier();
-      if (kb + ST < nk) load(kb + ST, buf);
-      read((u + 1) & 1, (u + 1) % ST);   // after the last slice: stale data that nothing uses
-      multiply(w1, xs, sc[now], NH, byte);
-    };
-    [&]<int... U>(std::integer_sequence<int, U...>) {
-      // stops at the last slice
-      ((k0 + U < nk ? (slice(std::integral_constant<int, U>{}), true) : false) && ...);
-    }(std::make_integer_sequence<int, UN>{});
-  }
+    }
+    multiply(ws, xs, sc[now], 0, byte);
+    // slice kb + 1 has arrived once only the ST - 2 later ones are in flight; every wave has
+    // read slice kb, whose buffer is free
+    if (INNER) __builtin_amdgcn_sched_barrier(0);
+    if (INNER || kb + ST <= nk)
+      wait_vmcnt<(ST - 2) * NV>();
+    else
+      wait_vmcnt<0>();
+    if constexpr (MX && u % 4 == 2) {
+      // the exponents have come long since; said here, where the compiler counts what was loaded after
+      // them (at the end of the round it would wait for all of it)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(sc[1].row[i]));
+#pragma unroll
+      for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(sc[1].col[j]));
+    }
+    lds_barrier();
+    if (INNER || kb + ST < nk) load(kb + ST, buf, inner);
+    read((u + 1) & 1, (u + 1) % ST);   // after the last slice: stale data that nothing uses
+    multiply(w1, xs, sc[now], NH, byte);
+    if constexpr (MX && u % 4 == 3) sc[0] = sc[1];
+    if (INNER) __builtin_amdgcn_sched_barrier(0);
+  };
+  // slices of one round: the registers alternate (with exponents, every four slices)
+  constexpr int UN = MX ? (ST < 4 ? 4 : ST) : ST % 2 ? 2 * ST : ST;
+  static_assert(UN % ST == 0 && UN % 2 == 0, "a slice's place in LDS and registers is known");
+  auto round = [&]<int... U>(std::integer_sequence<int, U...>, auto inner, int k0) {
+    // not inner: stops at the last slice
+    ((decltype(inner)::value || k0 + U < nk
+          ? (slice(std::integral_constant<int, U>{}, inner, k0 + U), true)
+          : false) && ...);
+  };
+  const std::make_integer_sequence<int, UN> all;
+  int k0 = 0;
+  for (; (k0 + UN + ST) * kBK <= a.K; k0 += UN) round(all, std::true_type{}, k0);
+  for (; k0 < nk; k0 += UN) round(all, std::false_type{}, k0);
   store_part<TO>(a, acc, m0 + wm, n0 + wn, li, lg);
 }
 
