@@ -467,10 +467,11 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   constexpr int ST = C::ST;
   constexpr bool WROW = SC == kOfRows, MX = SC == kExponents;
   static_assert(!MX || (ST % 2 == 0 && sizeof(TO) == 2), "four exponents are read at a time");
-  // with a scale for each row of both operands, those of a slice come with it
-  constexpr int SCALES = WROW ? BM + BN : 0, NV = NL + (WROW ? 1 : 0);
+  // scales that are no exponents come with their slice: those of x's rows, and of the weight's, or 64
+  // times the one of its block
+  constexpr int SCALES = MX ? 64 : BM + (WROW ? BN : 64), NV = NL + (MX ? 0 : 1);
   __shared__ __attribute__((aligned(16))) char lds[ST * C::STAGE];
-  __shared__ __attribute__((aligned(16))) float lds_scales[WROW ? ST * SCALES : 4];
+  __shared__ __attribute__((aligned(16))) float lds_scales[MX ? 4 : ST * SCALES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, lg = lane >> 4;
 
@@ -498,20 +499,23 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     off[i] = (unsigned)(r < most ? r : most) * (unsigned)(act ? a.ldx : a.ldw) + at[i];
   }
   // 64 of the scales a wave (some waves the same as others, where there are fewer)
-  const int part = WROW ? wave % (SCALES / 64) : 0;
+  const int part = wave % (SCALES / 64);
   const float* scale = a.sx;
   long long scale_stride = a.ldsx;
   unsigned scale_off = 0;
-  if constexpr (WROW) {
+  if constexpr (!MX) {
     static_assert(BM % 64 == 0 && BN % 64 == 0, "a wave's scales are of one operand");
     const int e = part * 64 + lane, r = e < BM ? m0 + e : n0 + e - BM;
     const int most = (part * 64 < BM ? a.M : a.N) - 1;
-    if (part * 64 >= BM) scale = a.sw, scale_stride = a.ldsw;
     scale_off = 4u * (unsigned)(r < most ? r : most);
+    if (part * 64 >= BM) {
+      scale = a.sw, scale_stride = a.ldsw;
+      if (!WROW) scale += n0 / kBlock * a.ldsw, scale_stride = 1, scale_off = 0;
+    }
   }
   const int last = (a.K + 15) / 16 * 16 - 16;   // the last readable piece of a row
   auto load = [&](int kb, int buf, auto whole) {
-    if constexpr (WROW)
+    if constexpr (!MX)
       lds_dma4((const char*)(scale + kb * scale_stride) + (size_t)scale_off,
                lds_scales + buf * SCALES + part * 64);
     char* dst = lds + buf * C::STAGE + wave * NL * 1024;
@@ -544,8 +548,8 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     const char* s = lds + buf * C::STAGE;
     return both(*reinterpret_cast<const i32x4*>(s + at), *reinterpret_cast<const i32x4*>(s + (at ^ 64)));
   };
-  // scales of one slice: rows 16 i + li of x; of w one, or columns 32 j + 8 lg + e.  Exponents: of
-  // four slices, a byte each, for the rows of the fragments.
+  // scales of one slice: rows 16 i + li of x (times the one of w's block), columns 32 j + 8 lg + e.
+  // Exponents: of four slices, a byte each, for the rows of the fragments.
   struct Scales {
     float row[MI], col[WROW ? NI / 2 : 1][8];
   };
@@ -553,11 +557,11 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     int row[MI], col[NI];
   };
   const int nk = (a.K + kBK - 1) / kBK;
-  int sm[MI], sn[NI];
+  int sm[MI], sn[NI];   // the exponents' rows
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int r = m0 + wm + 16 * i + li;
-    sm[i] = (r < a.M ? r : a.M - 1) * (MX ? a.lde : 1);
+    sm[i] = (r < a.M ? r : a.M - 1) * a.lde;
   }
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
@@ -565,33 +569,32 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     sn[j] = (r < a.N ? r : a.N - 1) * a.lde;
   }
   using Factors = std::conditional_t<MX, Exponents, Scales>;
-  auto load_scales = [&](Factors& s, int kb) {
-    kb = kb < nk ? kb : nk - 1;
+  auto load_exponents = [&](Factors& s, int kb) {
     if constexpr (MX) {
 #pragma unroll
       for (int i = 0; i < MI; ++i) s.row[i] = *reinterpret_cast<const int*>(a.ex + sm[i] + kb);
 #pragma unroll
       for (int j = 0; j < NI; ++j) s.col[j] = *reinterpret_cast<const int*>(a.ew + sn[j] + kb);
-    } else {
-      const float* p = a.sx + kb * a.ldsx;
-#pragma unroll
-      for (int i = 0; i < MI; ++i) s.row[i] = p[sm[i]];
-      s.col[0][0] = a.sw[n0 / kBlock * a.ldsw + kb];
     }
   };
   auto read_scales = [&](Factors& s, int buf) {   // from LDS
-    if constexpr (WROW) {
+    if constexpr (!MX) {
       const float* p = lds_scales + buf * SCALES;
 #pragma unroll
       for (int i = 0; i < MI; ++i) s.row[i] = p[wm + 16 * i + li];
+      if constexpr (!WROW) {
 #pragma unroll
-      for (int j = 0; j < NI / 2; ++j)
+        for (int i = 0; i < MI; ++i) s.row[i] *= p[BM];
+      } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(p + BM + wn + 32 * j + 8 * lg + 4 * h);
+        for (int j = 0; j < NI / 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s.col[j][4 * h + e] = v[e];
-        }
+          for (int h = 0; h < 2; ++h) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + BM + wn + 32 * j + 8 * lg + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s.col[j][4 * h + e] = v[e];
+          }
+      }
     }
   };
 
@@ -615,7 +618,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
               s.row[i]);
         }
       } else {
-        const float f = WROW ? s.row[i] : s.row[i] * s.col[0][0];
+        const float f = s.row[i];
 #pragma unroll
         for (int j = 0; j < NH; ++j) {
           const f32x4 p = mma8<TO>(w[j], x[i]);
@@ -632,8 +635,8 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     }
   };
 
-  Factors sc[2];   // of slices in turn; exponents: of four slices and the four after them
-  if constexpr (!WROW) load_scales(sc[0], 0);
+  Factors sc[2];   // of a slice; exponents: of four slices and the four after them
+  load_exponents(sc[0], 0);
 #pragma unroll
   for (int s = 0; s < ST; ++s)
     if (s < nk) load(s, s, std::false_type{});
@@ -642,6 +645,12 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   else
     wait_vmcnt<0>();
   lds_barrier();
+  if constexpr (MX) {   // waited for here, not at the head of the loop in every round
+#pragma unroll
+    for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(sc[0].row[i]));
+#pragma unroll
+    for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(sc[0].col[j]));
+  }
   // half of the weight's fragments are multiplied while the other half, or the next slice's, are read
   i32x8 x[2][MI], w0[2][NH], w1[NH];
   auto read = [&](int p, int buf) {
@@ -657,18 +666,13 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   auto slice = [&](auto number, auto inner, int kb) {
     constexpr bool INNER = decltype(inner)::value;
     constexpr int u = decltype(number)::value, buf = u % ST;
-    constexpr int now = MX || WROW ? 0 : u & 1;
     const std::integral_constant<int, MX ? u & 3 : 0> byte;
     auto& xs = x[u & 1];
     auto& ws = w0[u & 1];
 #pragma unroll
     for (int j = 0; j < NH; ++j) w1[j] = row(buf, rw[NH + j]);
-    if constexpr (WROW)
-      read_scales(sc[0], buf);
-    else if constexpr (!MX)
-      load_scales(sc[1 - now], kb + 1);
-    else if constexpr (u % 4 == 0)
-      load_scales(sc[1], kb + 4 < nk ? kb + 4 : kb);
+    read_scales(sc[0], buf);
+    if constexpr (MX && u % 4 == 0) load_exponents(sc[1], kb + 4 < nk ? kb + 4 : kb);
     if constexpr (!INNER) {
       const int left = a.K - kb * kBK;
       if (left < kBK) {
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
         }
       }
     }
-    multiply(ws, xs, sc[now], 0, byte);
+    multiply(ws, xs, sc[0], 0, byte);
     // slice kb + 1 has arrived once only the ST - 2 later ones are in flight; every wave has
     // read slice kb, whose buffer is free
     if (INNER) __builtin_amdgcn_sched_barrier(0);
@@ -700,7 +704,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     lds_barrier();
     if (INNER || kb + ST < nk) load(kb + ST, buf, inner);
     read((u + 1) & 1, (u + 1) % ST);   // after the last slice: stale data that nothing uses
-    multiply(w1, xs, sc[now], NH, byte);
+    multiply(w1, xs, sc[0], NH, byte);
     if constexpr (MX && u % 4 == 3) sc[0] = sc[1];
     if (INNER) __builtin_amdgcn_sched_barrier(0);
   };
