@@ -38,6 +38,8 @@ struct ConvArgs {
 template <typename T, int V> struct Raw;
 template <> struct Raw<float, 4> { using type = f32x4; };
 template <> struct Raw<bf16_t, 4> { using type = bf16x4; };
+template <> struct Raw<float, 2> { using type = float __attribute__((ext_vector_type(2))); };
+template <> struct Raw<bf16_t, 2> { using type = bf16_t __attribute__((ext_vector_type(2))); };
 template <> struct Raw<float, 1> { using type = float; };
 template <> struct Raw<bf16_t, 1> { using type = bf16_t; };
 template <typename T, int V> using raw_t = typename Raw<T, V>::type;
@@ -64,7 +66,7 @@ __device__ __forceinline__ void put(T* p, const float (&f)[V]) {
 }
 
 __device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + __expf(-v));
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-v * 1.44269504088896340736f));
 }
 
 // Where a thread works: CT lanes across the channels, kThreads / CT runs of a workgroup.
@@ -174,13 +176,14 @@ __global__ void __launch_bounds__(kThreads) conv_fwd(ConvArgs a) {
   m.load(a, p.c);
   const int end = a.T - p.first < a.run ? a.T : p.first + a.run;
   raw_t<TX, V> raw[kAhead];
-  bool fresh[kAhead];
+  bool fresh[kAhead] = {};
+  const TX* px = (const TX*)a.x + p.b * a.xb + p.c;
   auto load = [&](int t) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int ti = t + i < end ? t + i : end - 1;
-      raw[i] = input<TX, V, W>(a, p.b, p.c, ti);
-      fresh[i] = starts_at(a, p.b, ti);
+      raw[i] = *reinterpret_cast<const raw_t<TX, V>*>(px + ti * a.xt);
+      if (a.starts) fresh[i] = a.starts[(long long)p.b * a.T + ti];
     }
   };
   load(p.first);
@@ -221,8 +224,8 @@ __global__ void __launch_bounds__(kThreads) conv_fwd(ConvArgs a) {
 // dx_t = sum_d w[W - 1 - d] dp_{t + d} over the tokens t + d < t + W of its sequence, dw[k] =
 // sum_t dp_t x_{t - W + 1 + k}, dbias = sum_t dp_t; the last inputs' gradients come in addition.
 // A run walks on W - 1 tokens past its end for the sums that begin in it.
-template <typename TX, int V, int W, int CT>
-__global__ void __launch_bounds__(kThreads) conv_bwd(ConvArgs a) {
+template <typename TX, int V, int W, int CT, bool STARTS>
+__global__ void __launch_bounds__(kThreads, V == 2 ? 4 : 1) conv_bwd(ConvArgs a) {
   using P = Place<V, CT>;
   using R = raw_t<TX, V>;
   const P p(a);
@@ -240,15 +243,18 @@ __global__ void __launch_bounds__(kThreads) conv_bwd(ConvArgs a) {
     const int own = a.T - p.first < a.run ? a.T : p.first + a.run;   // end of the run
     const int end = a.T - own < W - 1 ? a.T : own + W - 1;           // and of the walk
     R rx[kAhead], rd[kAhead];
-    bool fresh[kAhead];
+    bool fresh[kAhead] = {};
+    const TX* px = (const TX*)a.x + p.b * a.xb + p.c;
+    const bool has = a.dy;   // without it, x's values in its place, not used
+    const TX* pd = has ? (const TX*)a.dy + p.b * a.db + p.c : px;
+    const long long dt = has ? a.dt : a.xt;
     auto load = [&](int t) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int ti = t + i < end ? t + i : end - 1;
-        rx[i] = input<TX, V, W>(a, p.b, p.c, ti);
-        if (a.dy)
-          rd[i] = *reinterpret_cast<const R*>((const TX*)a.dy + p.b * a.db + ti * a.dt + p.c);
-        fresh[i] = starts_at(a, p.b, ti);
+        rx[i] = *reinterpret_cast<const R*>(px + ti * a.xt);
+        rd[i] = *reinterpret_cast<const R*>(pd + ti * dt);
+        if (STARTS) fresh[i] = a.starts[(long long)p.b * a.T + ti];
       }
     };
     load(p.first);
@@ -273,21 +279,71 @@ __global__ void __launch_bounds__(kThreads) conv_bwd(ConvArgs a) {
       else if (t < 0 && p.first == 0 && a.dstate)
         put<TX, V>(ds + (long long)(W - 1 + t) * a.C, f);
     };
-    for (int t = p.first; t < end; t += kAhead) {
-      float now[kAhead][V], d[kAhead][V];
-      bool anew[kAhead];
+    // A group of tokens, taken out of the registers that the next one is then loaded into.
+    float now[kAhead][V], d[kAhead][V];
+    bool anew[kAhead];
+    auto take = [&](int t) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         widen<TX, V>(rx[i], now[i]);
         anew[i] = fresh[i];
-        if (a.dy) {
-          widen<TX, V>(rd[i], d[i]);
-        } else {
+        widen<TX, V>(rd[i], d[i]);
 #pragma unroll
-          for (int v = 0; v < V; ++v) d[i][v] = 0.f;
+        for (int v = 0; v < V; ++v) d[i][v] = has ? d[i][v] : 0.f;
+      }
+      load(t + kAhead < end ? t + kAhead : end - 1);
+    };
+    // Whether the next group is of the run, not its first and far from a start, in all lanes, as
+    // nearly always: then there is nothing to choose, and the windows move once.
+    auto plain = [&](int t) {
+      bool yes = t > p.first && t + kAhead <= own && age >= W - 1;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) yes &= !fresh[i];
+      return __all(yes);
+    };
+    auto quick = [&](int t) {
+      constexpr int H = W - 1, N = H + kAhead;
+      float x[N][V], s[N][V];   // tokens t - H ..
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          x[k][v] = taps.x[k][v];
+          s[k][v] = sum[H - k][v];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          x[H + i][v] = now[i][v];
+          s[H + i][v] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          float dp = d[i][v];
+          if (a.silu) {
+            float pre = m.bias[v];
+#pragma unroll
+            for (int k = 0; k < W; ++k) pre = fmaf(m.w[k][v], x[i + k][v], pre);
+            const float g = sigmoid(pre);
+            dp *= g * fmaf(pre, 1.f - g, 1.f);
+          }
+          dbias[v] += dp;
+#pragma unroll
+          for (int k = 0; k < W; ++k) {
+            s[i + k][v] = fmaf(m.w[k][v], dp, s[i + k][v]);
+            dw[k][v] = fmaf(dp, x[i + k][v], dw[k][v]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          taps.x[k][v] = x[kAhead + k][v];
+          sum[H - k][v] = s[kAhead + k][v];
         }
       }
-      if (t + kAhead < end) load(t + kAhead);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) put<TX, V>(dx + (long long)(t + i - H) * a.C, s[i]);
+      age += kAhead;
+    };
+    auto slow = [&](int t) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         if (t + i >= end) break;
@@ -311,9 +367,9 @@ __global__ void __launch_bounds__(kThreads) conv_bwd(ConvArgs a) {
           if (mine) {
             dbias[v] += d[i][v];
             dw[W - 1][v] = fmaf(d[i][v], now[i][v], dw[W - 1][v]);
+            // taps before a start are zero
 #pragma unroll
-            for (int k = 0; k < W - 1; ++k)
-              if (W - 1 - k <= age) dw[k][v] = fmaf(d[i][v], taps.x[k][v], dw[k][v]);
+            for (int k = 0; k < W - 1; ++k) dw[k][v] = fmaf(d[i][v], taps.x[k][v], dw[k][v]);
           }
         }
         finish(t + i - (W - 1), sum[W - 1]);
@@ -325,6 +381,25 @@ __global__ void __launch_bounds__(kThreads) conv_bwd(ConvArgs a) {
         }
         taps.push(now[i]);
       }
+    };
+    // The loop of plain groups has one path, so that the stores behind a group's loads can be counted
+    // when these are waited for; stores that a lane may leave out could not, and every group
+    // waited for all stores before it (8 x 8192 x 768 bfloat16, W = 4, 129 us, so 81).  Loads from before
+    // it are waited for ahead of it.
+    for (int t = p.first; t < end; t += kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        asm volatile("" : "+v"(rx[i]));
+        asm volatile("" : "+v"(rd[i]));
+      }
+      while (plain(t)) {
+        take(t);
+        quick(t);
+        t += kAhead;
+      }
+      if (t >= end) break;
+      take(t);
+      slow(t);
     }
     // sum[q] is token end - q's: at the end of the axis the last inputs' gradients join it
     if (end == a.T) {
@@ -359,22 +434,22 @@ __global__ void __launch_bounds__(kThreads) conv_bwd(ConvArgs a) {
   }
 }
 
-// The partial sums of dw and dbias added in their order: 64 columns a workgroup, 16 rows at a
+// The partial sums of dw and dbias added in their order: 16 columns a workgroup, 64 rows at a
 // time.
 __global__ void __launch_bounds__(1024) conv_sums(const float* part, long long rows, int C, int W,
                                                   float* dw, float* dbias) {
-  __shared__ float s[16][64];
-  const int col = threadIdx.x & 63, r = threadIdx.x >> 6;
-  const long long at = (long long)blockIdx.x * 64 + col, width = (long long)C * (W + 1);
+  __shared__ float s[64][16];
+  const int col = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const long long at = (long long)blockIdx.x * 16 + col, width = (long long)C * (W + 1);
   float v = 0.f;
   if (at < width)
-    for (long long k = r; k < rows; k += 16) v += part[k * width + at];
+    for (long long k = r; k < rows; k += 64) v += part[k * width + at];
   s[r][col] = v;
   __syncthreads();
   if (r || at >= width) return;
   v = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) v += s[k][col];
+  for (int k = 0; k < 64; ++k) v += s[k][col];
   const long long c = at / (W + 1);
   const int k = (int)(at - c * (W + 1));
   if (k < W)
@@ -418,7 +493,7 @@ struct Split {
   int ct, run, runs, nct;       // runs: workgroups along the tokens of a batch entry
 };
 // Lanes across the channels and tokens of a run, by sizes alone: the backward's workspace is
-// sized for one channel a thread or four, whichever needs more.
+// sized for one channel a thread or two, whichever needs more.
 Split split(int B, int T, int C, int V) {
   Split s;
   const int groups = (C + V - 1) / V;
@@ -437,7 +512,7 @@ int validate(int B, int T, int C, int W, int dtype) {
   if (B < 1 || T < 0 || C < 1 || W < 2 || W > 4) return GDN2_ERR_SHAPE;
   // token numbers of a run and its halo stay within 31 bits, a launch's threads within 32
   if (T > INT_MAX - 1024 || C > (1 << 24)) return GDN2_ERR_SHAPE;
-  for (int V : {1, 4}) {
+  for (int V : {1, 2, 4}) {
     const Split s = split(B, T, C, V);
     if ((double)B * s.nct * (s.runs < 1 ? 1 : s.runs) > (double)(1 << 23)) return GDN2_ERR_SHAPE;
   }
@@ -460,6 +535,11 @@ int check_f32(const void* p, bool optional) {
 
 enum Mode { kForward, kBackward, kStep };
 
+// Channels of a thread of the backward, where four fit: their sums and windows would leave room for two
+// waves a SIMD, those of two for four (8 x 8192 x 768 bfloat16, W = 4, 137 and 129 us, both before
+// the loop of plain groups).
+template <int V> constexpr int kBwd = V == 4 ? 2 : V;
+
 template <typename TX, int V, int W>
 void launch_width(hipStream_t st, ConvArgs& a, Mode mode) {
   if (mode == kStep) {
@@ -468,14 +548,16 @@ void launch_width(hipStream_t st, ConvArgs& a, Mode mode) {
                        dim3(kThreads), 0, st, a);
     return;
   }
-  const Split s = split(a.B, a.T, a.C, V);
+  const Split s = split(a.B, a.T, a.C, mode == kBackward ? kBwd<V> : V);
   a.run = s.run, a.runs = s.runs, a.nct = s.nct;
   const dim3 grid((unsigned)((long long)a.B * s.runs * s.nct)), block(kThreads);
 #define GDN2_CONV(CT)                                                             \
   if (mode == kForward)                                                           \
     hipLaunchKernelGGL((conv_fwd<TX, V, W, CT>), grid, block, 0, st, a);          \
+  else if (a.starts)                                                              \
+    hipLaunchKernelGGL((conv_bwd<TX, kBwd<V>, W, CT, true>), grid, block, 0, st, a); \
   else                                                                            \
-    hipLaunchKernelGGL((conv_bwd<TX, V, W, CT>), grid, block, 0, st, a)
+    hipLaunchKernelGGL((conv_bwd<TX, kBwd<V>, W, CT, false>), grid, block, 0, st, a)
   if (s.ct == 16) {
     GDN2_CONV(16);
   } else {
@@ -505,8 +587,8 @@ extern "C" {
 
 size_t gdn2_short_conv_bwd_workspace_bytes(int B, int T, int C, int W) {
   if (validate(B, T, C, W, GDN2_F32) != GDN2_OK || T == 0) return 0;
-  const int r1 = split(B, T, C, 1).runs, r4 = split(B, T, C, 4).runs;
-  return (size_t)B * (r1 > r4 ? r1 : r4) * C * (W + 1) * sizeof(float);
+  const int r1 = split(B, T, C, 1).runs, r2 = split(B, T, C, 2).runs;
+  return (size_t)B * (r1 > r2 ? r1 : r2) * C * (W + 1) * sizeof(float);
 }
 
 int gdn2_short_conv_fwd(void* stream, int B, int T, int C, int W, int dtype, int silu,
@@ -558,7 +640,7 @@ int gdn2_short_conv_bwd(void* stream, int B, int T, int C, int W, int dtype, int
   a.dy = dy, a.db = d[0], a.dt = d[1], a.dlast = dlast, a.dx = dx, a.dstate = dstate;
   a.part = (float*)ws, a.B = B, a.T = T, a.C = C, a.silu = silu;
   if ((rc = launch((hipStream_t)stream, a, W, dtype, vec, kBackward))) return rc;
-  const unsigned wgs = (unsigned)(((long long)C * (W + 1) + 63) / 64);
+  const unsigned wgs = (unsigned)(((long long)C * (W + 1) + 15) / 16);
   hipLaunchKernelGGL(conv_sums, dim3(wgs), dim3(1024), 0, (hipStream_t)stream, a.part,
                      (long long)B * a.runs, C, W, dw, dbias);
   return hipGetLastError() == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;

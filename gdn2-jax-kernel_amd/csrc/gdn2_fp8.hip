@@ -63,7 +63,6 @@ struct QuantArgs {
   int lds8, ldt8;
   float* part;               // (M / 128, C) sums of each 128 rows, or null
   int M, C, kb, mb;          // blocks along the columns, the rows
-  int vec;
 };
 
 // The scale and its inverse of values whose largest magnitude has these bits: 0, 0 where all are
@@ -101,6 +100,30 @@ __device__ __forceinline__ int pack4(float a, float b, float c, float d, float i
   return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
+// Eight values at any alignment of theirs.
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const i32x4 r = reinterpret_cast<const Piece<float>*>(p)[h].v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[4 * h + e] = __int_as_float(r[e]);
+  }
+}
+__device__ __forceinline__ void load8(const bf16_t* p, float (&f)[8]) {
+  const bf16x8 r = __builtin_bit_cast(bf16x8, reinterpret_cast<const Piece<bf16_t>*>(p)->v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = (float)r[e];
+}
+// The values from number n on, zeros behind them (all zeros for n >= 8).
+__device__ __forceinline__ void shift8(float (&v)[8], int n) {
+#pragma unroll
+  for (int b = 1; b <= 8; b *= 2)
+    if (n & b || (b == 8 && n >= 8)) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = k + b < 8 ? v[k + b < 8 ? k + b : 0] : 0.f;
+    }
+}
+
 // ROWS: q with a scale for each row and 128 columns.  COLS: qt with one for each column and 128
 // rows.  BLOCK: q, and where it is given qt, with one for each 128 x 128.
 enum { kRows = 1, kCols = 2, kBlocks = 4 };
@@ -110,17 +133,22 @@ __global__ void __launch_bounds__(256) fp8_quantize(QuantArgs a) {
   const int tid = threadIdx.x, wave = tid >> 6;
   const int tc = blockIdx.x % a.kb, tm = blockIdx.x / a.kb;
   const int m = tm * kBlock + (tid >> 4) * 8, c = tc * kBlock + (tid & 15) * 8;
-  __shared__ unsigned top[16][kBlock];
+  __shared__ __attribute__((aligned(16))) unsigned char tile[(MODE & kRows) != MODE ? kBlock * kBlock : 8192];
+  unsigned(&top)[16][kBlock] = *reinterpret_cast<unsigned(*)[16][kBlock]>(tile);
   float v[8][8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
     // rows past the end count as zeros, read from the last one
     const TX* p = (const TX*)a.x + (m + r < a.M ? m + r : a.M - 1) * a.ldx;
     const bool row = m + r < a.M;
-    if (a.vec) {
-      load_f<8>(p + (c < a.C ? c : 0), v[r]);
+    if (a.C >= 8) {
+      // eight values at any alignment, those that end the row where they would pass it
+      const int from = c + 8 <= a.C ? c : a.C - 8, past = c - from;   // past > 0: from column c - past on
+      float f[8];
+      load8(p + from, f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[r][k] = row && c < a.C ? v[r][k] : 0.f;
+      for (int k = 0; k < 8; ++k) v[r][k] = row ? f[k] : 0.f;
+      if (past > 0) shift8(v[r], past);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -233,13 +261,28 @@ __global__ void __launch_bounds__(256) fp8_quantize(QuantArgs a) {
             a.st[(long long)tm * a.C + c + k] = s[k];
         }
     }
-    if (a.qt && m < a.ldt) {
+    if (!a.qt) return;
+    // Columns through LDS, so that 128 bytes of one are written at a time (8192 x 4096 bfloat16, rows
+    // and columns, stored from registers 39.7 us, so AAA): piece j of eight rows of column k
+    // at place j ^ (k / 8), which spreads what a wave writes, and what it reads, over the banks.
+    __syncthreads();   // top is read no more
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c + k < a.C)
-          *reinterpret_cast<i32x2*>(a.qt + (c + k) * a.ldt + m) =
-              i32x2{pack4(v[0][k], v[1][k], v[2][k], v[3][k], i[k], i[k], i[k], i[k]),
-                    pack4(v[4][k], v[5][k], v[6][k], v[7][k], i[k], i[k], i[k], i[k])};
+    for (int k = 0; k < 8; ++k) {
+      const int col = (tid & 15) * 8 + k, j = (tid >> 4) ^ (tid & 15);
+      *reinterpret_cast<i32x2*>(&tile[col * kBlock + j * 8]) =
+          i32x2{pack4(v[0][k], v[1][k], v[2][k], v[3][k], i[k], i[k], i[k], i[k]),
+                pack4(v[4][k], v[5][k], v[6][k], v[7][k], i[k], i[k], i[k], i[k])};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int col = r * 32 + (tid >> 3), p = tid & 7, x = col >> 3;   // 16 bytes: pieces 2 p, 2 p + 1
+      const i32x4 t = *reinterpret_cast<const i32x4*>(&tile[col * kBlock + ((2 * p) ^ (x & ~1)) * 8]);
+      const bool swap = x & 1;
+      const long long at = tm * kBlock + 16 * p;
+      if (tc * kBlock + col < a.C && at < a.ldt)
+        *reinterpret_cast<i32x4*>(a.qt + (long long)(tc * kBlock + col) * a.ldt + at) =
+            swap ? i32x4{t[2], t[3], t[0], t[1]} : t;
     }
   }
 }
@@ -875,8 +918,6 @@ int quantize(hipStream_t st, int M, int C, int x_dtype, const void* x, long long
     a.s8 = (unsigned char*)scale, a.lds8 = exponents_of(a.kb);
     a.st8 = (unsigned char*)a.st, a.ldt8 = exponents_of(a.mb);
   }
-  // eight values at a time
-  a.vec = C % 8 == 0 && (uintptr_t)x % 16 == 0 && x_stride * es % 16 == 0;
   const int mode = blocks ? kBlocks : (q ? kRows : 0) | (qt ? kCols : 0);
   const hipError_t e = x_dtype == GDN2_F32 ? launch_quantize<float>(st, a, mode)
                                            : launch_quantize<bf16_t>(st, a, mode);
