@@ -46,8 +46,8 @@ struct SsmArgs {
   void *out, *dx, *ddt, *dz, *dbm, *dcm;           // dense
   float *h_final, *dh0, *dA, *dD, *dbias;
   float* kept;                                     // (B, ceil(T / kKeep), C, NP) or null
-  // workspace
   float* bc;      // (B, T, G, 2, NP): B and C in float32, the states past N zero
+  // workspace
   float* part_bc; // (tiles, B, T, 2, NP)
   float* part_a;  // (B chunks, C, NP)
   float* part_c;  // (B chunks, 2, C)
@@ -763,9 +763,26 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
   }
 }
 
-// Gradients of A, D and dt_bias: partial sums over the rows added in their order, 64 columns a
-// workgroup, 16 rows at a time.  Columns: C NP of part_a, then 2 C of part_c.
-__global__ void __launch_bounds__(1024) ssm_sums(SsmArgs a, int NP) {
+// Partial sums added in their order.  The first workgroups: the gradients of A, D and dt_bias, 64
+// columns each (C NP of part_a, then 2 C of part_c), 16 rows at a time.  The others: those of B and
+// C, the tiles of a group for each value.
+template <typename TX>
+__global__ void __launch_bounds__(1024) ssm_sums(SsmArgs a, int NP, int first) {
+  if ((int)blockIdx.x >= first) {
+    const long long bt = (long long)a.B * a.T, n = bt * a.G * 2 * NP;
+    for (long long e = (long long)(blockIdx.x - first) * 1024 + threadIdx.x; e < n;
+         e += (long long)(gridDim.x - first) * 1024) {
+      const long long row = e / (2 * NP);    // bt G + g
+      const int k = (int)(e - row * 2 * NP), g = (int)(row % a.G);
+      const int s = k % NP;
+      if (s >= a.N) continue;
+      const float* p = a.part_bc + ((long long)g * a.tiles * bt + row / a.G) * 2 * NP + k;
+      float v = 0.f;
+      for (int i = 0; i < a.tiles; ++i) v += p[i * bt * 2 * NP];
+      ((TX*)(k < NP ? a.dbm : a.dcm))[row * a.N + s] = (TX)v;
+    }
+    return;
+  }
   __shared__ float sum[16][64];
   const int col = threadIdx.x & 63, r = threadIdx.x >> 6;
   const long long wa = (long long)a.C * NP, wc = 2ll * a.C, rows = (long long)a.B * a.chunks;
@@ -790,23 +807,6 @@ __global__ void __launch_bounds__(1024) ssm_sums(SsmArgs a, int NP) {
     if (a.dD) a.dD[at - wa] = v;
   } else if (at < wa + wc) {
     if (a.dbias) a.dbias[at - wa - a.C] = v;
-  }
-}
-
-// Gradients of B and C: the tiles of a group added in their order.
-template <typename TX>
-__global__ void __launch_bounds__(kThreads) ssm_sums_bc(SsmArgs a, int NP) {
-  const long long bt = (long long)a.B * a.T, n = bt * a.G * 2 * NP;
-  for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < n;
-       e += (long long)gridDim.x * kThreads) {
-    const long long row = e / (2 * NP);    // bt G + g
-    const int k = (int)(e - row * 2 * NP), g = (int)(row % a.G);
-    const int s = k % NP;
-    if (s >= a.N) continue;
-    const float* p = a.part_bc + ((long long)g * a.tiles * bt + row / a.G) * 2 * NP + k;
-    float v = 0.f;
-    for (int i = 0; i < a.tiles; ++i) v += p[i * bt * 2 * NP];
-    ((TX*)(k < NP ? a.dbm : a.dcm))[row * a.N + s] = (TX)v;
   }
 }
 
@@ -875,8 +875,9 @@ struct Split {
   int np, L, chunks;
   int tiles, btiles;            // of a group: waves' (64 channels) and the backward's
   size_t bc, slot, sum, part_bc, part_a, part_c;   // bytes, multiples of 16
-  size_t fwd() const { return bc + slot + sum; }
-  size_t bwd() const { return bc + slot + sum + part_bc + part_a + part_c; }
+  // the forward's rows of B and C are in its workspace or, kept for the backward, behind the states
+  size_t fwd() const { return slot + sum + bc; }
+  size_t bwd() const { return slot + sum + part_bc + part_a + part_c; }
 };
 size_t round16(double n) { return ((size_t)n + 15) / 16 * 16; }
 
@@ -887,9 +888,12 @@ Split split(int B, int T, int C, int G, int N) {
   const int Cg = C / G;
   s.tiles = (Cg + 63) / 64;
   s.btiles = (Cg + bwd_tile(s.np) - 1) / bwd_tile(s.np);
-  // chunks of 128 tokens where they make some waves a SIMD, else of 64 or 32
+  // chunks of 128 tokens where they make some waves a SIMD, else of 64 or 32, and of 16 where those
+  // would not give every SIMD one (2 x 1003 x 500 x 21 float32: 32 tokens 27, 33, 27 and 41 us, 16
+  // 17, 21, 18 and 42, and two joins 4 more each)
   s.L = 128;
-  while (s.L > 32 && (double)B * G * s.tiles * ((T + s.L - 1) / s.L) < 4096) s.L /= 2;
+  auto waves = [&] { return (double)B * G * s.tiles * ((T + s.L - 1) / s.L); };
+  while ((s.L > 32 && waves() < 4096) || (s.L > 16 && waves() < 1024)) s.L /= 2;
   s.chunks = T ? (T + s.L - 1) / s.L : 1;
   const double bt = (double)B * T, rows = (double)B * s.chunks;
   s.bc = round16(bt * G * 2 * s.np * 4);
@@ -908,7 +912,7 @@ int validate(int B, int T, int C, int G, int N, int in_dtype, int dt_dtype) {
   if (in_dtype != GDN2_F32 && in_dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
   if (dt_dtype != GDN2_F32 && dt_dtype != in_dtype) return GDN2_ERR_DTYPE;
   // a launch's threads stay within 32 bits and its waves' numbers within 31: one wave for at
-  // least 32 tokens of at most 64 channels, one thread for a state
+  // least 16 tokens of at most 64 channels, one thread for a state
   const Split s = split(B, T, C, G, N);
   if ((double)B * G * s.tiles * s.chunks > (double)(1 << 25) ||
       (double)B * G * s.btiles * s.chunks > (double)(1 << 23) ||
@@ -960,7 +964,6 @@ void launch_fwd(hipStream_t st, const SsmArgs& a) {
 template <typename TX, typename TD, int NP, bool STARTS>
 void launch_bwd(hipStream_t st, SsmArgs a) {
   const long long waves = (long long)a.B * a.G * a.tiles;
-  launch_rows<TX>(st, a, NP);
   if (a.chunks > 1) {
     hipLaunchKernelGGL((ssm_rev<TX, TD, NP, STARTS>), dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)),
                        dim3(kThreads), 0, st, a);
@@ -972,11 +975,10 @@ void launch_bwd(hipStream_t st, SsmArgs a) {
   hipLaunchKernelGGL((ssm_bwd<TX, TD, NP, STARTS>),
                      dim3((unsigned)((long long)a.B * a.G * a.tiles * a.chunks)), dim3(kThreads), 0,
                      st, a);
-  hipLaunchKernelGGL((ssm_sums), dim3((unsigned)(((long long)a.C * (NP + 2) + 63) / 64)), dim3(1024),
-                     0, st, a, NP);
-  hipLaunchKernelGGL((ssm_sums_bc<TX>),
-                     dim3(groups_of((double)a.B * a.T * a.G * 2 * NP, kThreads)), dim3(kThreads), 0,
-                     st, a, NP);
+  const int first = (int)(((long long)a.C * (NP + 2) + 63) / 64);
+  hipLaunchKernelGGL((ssm_sums<TX>),
+                     dim3(first + groups_of((double)a.B * a.T * a.G * 2 * NP, 1024, 16384)), dim3(1024),
+                     0, st, a, NP, first);
 }
 
 template <typename TX, typename TD>
@@ -1038,14 +1040,19 @@ int set_inputs(SsmArgs& a, int B, int T, int C, int G, int N, int in_dtype, int 
   a.B = B, a.T = T, a.C = C, a.G = G, a.N = N, a.Cg = C / G;
   return GDN2_OK;
 }
-void set_workspace(SsmArgs& a, const Split& s, void* ws) {
+// Bytes of the kept states, without the rows of B and C behind them.
+size_t kept_states(int B, int T, int C, int N) {
+  return (size_t)B * ((T + kKeep - 1) / kKeep) * C * padded(N) * sizeof(float);
+}
+void set_workspace(SsmArgs& a, const Split& s, void* ws, void* kept) {
   char* p = (char*)ws;
-  a.bc = (float*)p;
-  a.slot = (float*)(p += s.bc);
+  a.slot = (float*)p;
   a.sum = (float*)(p += s.slot);
-  a.part_bc = (float*)(p += s.sum);
+  a.bc = a.part_bc = (float*)(p += s.sum);
   a.part_a = (float*)(p += s.part_bc);
   a.part_c = (float*)(p += s.part_a);
+  if (kept) a.bc = (float*)((char*)kept + kept_states(a.B, a.T, a.C, a.N));
+  a.kept = (float*)kept;
   a.tiles = s.tiles, a.L = s.L, a.chunks = s.chunks;
 }
 
@@ -1058,7 +1065,7 @@ extern "C" {
 
 size_t gdn2_selective_scan_kept_bytes(int B, int T, int C, int G, int N) {
   if (validate(B, T, C, G, N, GDN2_F32, GDN2_F32) != GDN2_OK) return 0;
-  return (size_t)B * ((T + kKeep - 1) / kKeep) * C * padded(N) * sizeof(float);
+  return kept_states(B, T, C, N) + split(B, T, C, G, N).bc;
 }
 
 size_t gdn2_selective_scan_workspace_bytes(int B, int T, int C, int G, int N, int backward) {
@@ -1086,8 +1093,8 @@ int gdn2_selective_scan_fwd(void* stream, int B, int T, int C, int G, int N, int
   if (h0 == h_final) return GDN2_ERR_FLAGS;    // read by other workgroups
   const Split s = split(B, T, C, G, N);
   if ((rc = check_ws(ws, s.fwd(), ws_bytes))) return rc;
-  set_workspace(a, s, ws);
-  a.h0 = h0, a.out = out, a.h_final = h_final, a.kept = kept;
+  set_workspace(a, s, ws, kept);
+  a.h0 = h0, a.out = out, a.h_final = h_final;
   return launch((hipStream_t)stream, a, in_dtype, dt_dtype, false);
 }
 
@@ -1119,9 +1126,9 @@ int gdn2_selective_scan_bwd(void* stream, int B, int T, int C, int G, int N, int
   if ((uintptr_t)kept % 16) return GDN2_ERR_ALIGN;
   const Split s = split(B, T, C, G, N);
   if ((rc = check_ws(ws, s.bwd(), ws_bytes))) return rc;
-  set_workspace(a, s, ws);
+  set_workspace(a, s, ws, const_cast<float*>(kept));
   a.dx = outs[0], a.ddt = outs[1], a.dz = outs[2], a.dbm = outs[3], a.dcm = outs[4];
-  a.dh_final = dh_final, a.kept = const_cast<float*>(kept);
+  a.dh_final = dh_final;
   a.dA = dA, a.dD = dD, a.dbias = ddt_bias, a.dh0 = dh0;
   return launch((hipStream_t)stream, a, in_dtype, dt_dtype, true);
 }

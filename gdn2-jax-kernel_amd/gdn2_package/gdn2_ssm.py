@@ -76,7 +76,7 @@ def _prepare(x, dt, A, B, C, D, z, dt_bias, state, lead, what):
     if state is not None:
         state = _floating(state, "the state", (x.shape[0], Ch, N), dev, what)
     t = x.dtype
-    if t not in _SUPPORTED_IN or any(o is not None and o.dtype != t for o in (B, C, z)):
+    if t not in _SUPPORTED_IN or B.dtype != t or C.dtype != t or (z is not None and z.dtype != t):
         t = torch.float32
     f32 = lambda o: None if o is None else _as(o, torch.float32).contiguous()
     dt = dt if dt.dtype == t else _as(dt, torch.float32)
@@ -87,24 +87,28 @@ def _prepare(x, dt, A, B, C, D, z, dt_bias, state, lead, what):
 def _row_operand(t):
     """t with a token's values contiguous, and the elements from one batch entry and one token
     to the next.  Strides of axes of one element say nothing."""
-    width = t.shape[2:].numel()
-    if t[0, 0].is_contiguous() and (t.shape[1] == 1 or t.stride(1) <= _MAX_STRIDE):
-        return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * width,
-                   t.stride(1) if t.shape[1] > 1 else width)
-    t = t.contiguous()
-    return t, (t.shape[1] * width, width)
+    shape = t.shape
+    width = shape[2] if len(shape) == 3 else shape[2] * shape[3]
+    if t.is_contiguous():
+        return t, (shape[1] * width, width)
+    s = t.stride()
+    inner = s[-1] == 1 or shape[-1] == 1
+    if len(shape) == 4:
+        inner = inner and (s[2] == shape[3] or shape[2] == 1)
+    if inner and (shape[1] == 1 or s[1] <= _MAX_STRIDE):
+        return t, (s[0], s[1] if shape[1] > 1 else width)
+    return t.contiguous(), (shape[1] * width, width)
 
 
 def _operands(x, dt, z, B, C):
     """(the tensors, which must outlive the launch; pointers; strides)"""
-    kept, strides = [], []
-    for t in (x, dt, z, B, C):
-        s = (0, 0)
+    kept, ptrs, strides = [], _Ptrs5(), _Strides5()
+    for i, t in enumerate((x, dt, z, B, C)):
         if t is not None:
-            t, s = _row_operand(t)
-        kept.append(t)
-        strides += s
-    return kept, _Ptrs5(*(_ptr(t) for t in kept)), _Strides5(*strides)
+            t, (strides[2 * i], strides[2 * i + 1]) = _row_operand(t)
+            ptrs[i] = t.data_ptr()
+            kept.append(t)
+    return kept, ptrs, strides
 
 
 def _sizes(x, B):

@@ -486,8 +486,8 @@ int gdn2_short_conv_step(void* stream, int B, int C, int W, int dtype, int silu,
  * them the elements from one batch entry and one token (at most 2^25) to the next; the rest of a
  * row is contiguous.  C <= 2^24, G <= 2^18.  Pointers are aligned to their elements, kept and ws to 16 bytes.  T >= 1. */
 
-/* Bytes of the states kept for the backward (float32, one for every 16 tokens, N padded to 8,
- * 16, 32 or 64) and of the workspace of the forward or the backward. */
+/* Bytes of what is kept for the backward (float32: the states before every 16th token, N padded to
+ * 8, 16, 32 or 64, and the rows of Bm and Cm) and of the workspace of the forward or the backward. */
 size_t gdn2_selective_scan_kept_bytes(int B, int T, int C, int G, int N);
 size_t gdn2_selective_scan_workspace_bytes(int B, int T, int C, int G, int N, int backward);
 
@@ -499,7 +499,7 @@ int gdn2_selective_scan_fwd(void* stream, int B, int T, int C, int G, int N, int
                             void* out, float* h_final, float* kept, void* ws, size_t ws_bytes);
 
 /* Gradients from those of out and h_final (either may be NULL: zero), the forward's inputs
- * and its kept states.  outs: host array of dx, ddt, dz (NULL without z), dBm, dCm, all dense;
+ * and what it kept.  outs: host array of dx, ddt, dz (NULL without z), dBm, dCm, all dense;
  * dD, ddt_bias and dh0 are written where they are not NULL. */
 int gdn2_selective_scan_bwd(void* stream, int B, int T, int C, int G, int N, int in_dtype,
                             int dt_dtype, int softplus, const void* const* ins,
