@@ -502,7 +502,7 @@ Split split(int B, int T, int C, int V) {
   const int per = kThreads / s.ct;
   // runs of 32 tokens where they make two workgroups a CU, else of 16 or 8
   s.run = 32;
-  while (s.run > 8 && (long long)B * s.nct * ((T + per * s.run - 1ll) / (per * s.run)) < 512)
+  while (s.run > 8 && (double)B * s.nct * ((T + per * s.run - 1ll) / (per * s.run)) < 512)
     s.run /= 2;
   s.runs = (int)((T + (long long)per * s.run - 1) / ((long long)per * s.run));
   return s;

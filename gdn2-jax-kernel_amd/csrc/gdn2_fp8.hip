@@ -504,6 +504,12 @@ struct Tile {
   static_assert(kBlock % BN == 0 || BN % kBlock == 0, "a tile lies within one block of the weight's rows");
 };
 
+// f(0), f(1), ... as constants, as long as it returns true.
+template <int... U, typename F>
+__device__ __forceinline__ void while_each(std::integer_sequence<int, U...>, F&& f) {
+  (void)(f(std::integral_constant<int, U>{}) && ...);
+}
+
 template <typename C, Scaling SC, typename TO>
 __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmArgs a) {
   constexpr int BM = C::BM, BN = C::BN, NW = C::NW, MI = C::MI, NI = C::NI, NL = C::NL;
@@ -755,16 +761,19 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   // slices of one round: the registers alternate (with exponents, every four slices)
   constexpr int UN = MX ? (ST < 4 ? 4 : ST) : ST % 2 ? 2 * ST : ST;
   static_assert(UN % ST == 0 && UN % 2 == 0, "a slice's place in LDS and registers is known");
-  auto round = [&]<int... U>(std::integer_sequence<int, U...>, auto inner, int k0) {
-    // not inner: stops at the last slice
-    ((decltype(inner)::value || k0 + U < nk
-          ? (slice(std::integral_constant<int, U>{}, inner, k0 + U), true)
-          : false) && ...);
-  };
   const std::make_integer_sequence<int, UN> all;
   int k0 = 0;
-  for (; (k0 + UN + ST) * kBK <= a.K; k0 += UN) round(all, std::true_type{}, k0);
-  for (; k0 < nk; k0 += UN) round(all, std::false_type{}, k0);
+  for (; (k0 + UN + ST) * kBK <= a.K; k0 += UN)
+    while_each(all, [&](auto u) {
+      slice(u, std::true_type{}, k0 + decltype(u)::value);
+      return true;
+    });
+  for (; k0 < nk; k0 += UN)
+    while_each(all, [&](auto u) {   // stops at the last slice
+      const int kb = k0 + decltype(u)::value;
+      if (kb < nk) slice(u, std::false_type{}, kb);
+      return kb < nk;
+    });
   store_part<TO>(a, acc, m0 + wm, n0 + wn, li, lg);
 }
 

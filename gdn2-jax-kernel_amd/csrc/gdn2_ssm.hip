@@ -879,7 +879,8 @@ struct Split {
   size_t fwd() const { return slot + sum + bc; }
   size_t bwd() const { return slot + sum + part_bc + part_a + part_c; }
 };
-size_t round16(double n) { return ((size_t)n + 15) / 16 * 16; }
+// (sizes that are refused need only come out large)
+size_t round16(double n) { return n > 1e17 ? (size_t)1 << 58 : ((size_t)n + 15) / 16 * 16; }
 
 // Chunks by sizes alone: the forward and the backward cut the axis alike.
 Split split(int B, int T, int C, int G, int N) {

@@ -25,7 +25,7 @@ import torch
 from . import _lib
 from .gdn2_conv import _floating, _ptr
 from .gdn2_fwd import _SUPPORTED_IN, GDN2Error, GDN2ShapeError, _dtype_code, _raise
-from .gdn2_norm import _as, _as_rows, _forward_mode, _gradients, _row_stride, _tensor
+from .gdn2_norm import _INT_MAX, _as, _as_rows, _forward_mode, _gradients, _row_stride, _tensor
 
 _BLOCK = 128
 _E4M3 = torch.float8_e4m3fn
@@ -243,6 +243,8 @@ def gdn2_fp8_linear(x, weight, bias=None):
     if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise GDN2ShapeError(f"{what}: weight must be (N, K) for x (..., K); got "
                              f"{tuple(weight.shape)} for x {tuple(x.shape)}")
+    if max(weight.shape) > _INT_MAX:   # ctypes would cut it to 32 bits
+        raise GDN2ShapeError(f"{what}: sizes past 2^31 - 1 in {tuple(weight.shape)}")
     if not x.is_floating_point():
         raise GDN2Error(f"{what}: x must be floating point; got {x.dtype}")
     weight = _floating(weight, "weight", weight.shape, x.device, what)

@@ -310,6 +310,28 @@ def test_linear_partial_and_types(dev):
     assert (torch.autograd.grad(y.sum(), full[1])[0] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N", [(8, 40), (200, 300), (2100, 2100)])
+def test_linear_with_nan(dev, M, N, dtype):
+    """NaN and infinities in a block reach every output that it enters, and no other."""
+    import gdn2_package as gp
+    K = 300
+    x, w, dy = (values(*s, dtype, dev, i) for i, s in enumerate(((M, K), (N, K), (M, N))))
+    x[:, :] = x.clamp(-100, 100)
+    x[2, 140], x[5, 299], dy[3, 7] = torch.nan, torch.inf, -torch.inf
+    x[4], dy[:128, 9] = 0.0, 0.0
+    leaf = [x.requires_grad_(), w.requires_grad_()]
+    y = gp.gdn2_fp8_linear(*leaf)
+    bad = torch.zeros(M, dtype=torch.bool, device=dev)
+    bad[2] = bad[5] = True
+    assert torch.isnan(y[bad]).all() and torch.isfinite(y[~bad]).all() and (y[4] == 0).all()
+    dx, dw = torch.autograd.grad(y, leaf, dy)
+    assert torch.isnan(dx[3]).all() and torch.isfinite(dx[torch.arange(M, device=dev) != 3]).all()
+    lost = torch.zeros((N, K), dtype=torch.bool, device=dev)
+    lost[7], lost[:, 140], lost[:, 299] = True, True, True
+    assert torch.equal(torch.isnan(dw), lost)
+
+
 def test_graph(dev):
     """A captured training step of the layer and a captured product replay as the eager ones."""
     import gdn2_package as gp
