@@ -34,7 +34,7 @@ def _floating(t, name, shape, device, what):
     """t, checked to be a floating point tensor of that shape there."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: {name} must be a torch tensor")
-    if t.shape != torch.Size(shape):
+    if t.shape != shape:
         raise GDN2ShapeError(f"{what}: {name} must have shape {tuple(shape)}; got "
                              f"{tuple(t.shape)}")
     if t.device != device:

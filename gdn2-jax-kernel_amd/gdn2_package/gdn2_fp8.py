@@ -69,9 +69,10 @@ def gdn2_quantize_fp8(x, blocks=False):
         _raise(rc, f"{what} (M,C)=({M},{C})")
     if blocks:
         return q, s
+    if x.dim() == 2:
+        return q, s.t()
     lead = x.shape[:-1]
-    return q.unflatten(0, lead) if x.dim() > 2 else q.view(x.shape), \
-        s.view(s.shape[0], *lead).movedim(0, -1)
+    return q.unflatten(0, lead) if lead else q.view(x.shape), s.view(kb, *lead).movedim(0, -1)
 
 
 def _scaled_rows(q, scale, names, what, device, blocks):
@@ -133,6 +134,8 @@ def _wide_rows(q):
 def _by_block(scale, M):
     """Scales (..., blocks) of M rows as (blocks, M), dense; a copy only where they are not laid
     out so."""
+    if scale.dim() == 2 and scale.stride() == (1, M):
+        return scale.t()
     return scale.movedim(-1, 0).reshape(scale.shape[-1], M).contiguous()
 
 

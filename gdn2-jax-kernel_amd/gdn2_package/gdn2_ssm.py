@@ -36,6 +36,12 @@ _MAX_STATES = 64
 _MAX_STRIDE = 2 ** 25   # elements from one token to the next that are read in place
 
 
+def _f32(t):
+    if t is None or t.dtype == torch.float32 and t.is_contiguous():
+        return t
+    return t.to(torch.float32).contiguous()
+
+
 def _prepare(x, dt, A, B, C, D, z, dt_bias, state, lead, what):
     """The inputs in the types that the kernels take, checked: x, dt, z (*lead, Ch), B, C
     (*lead, G, N).  x has `lead` axes before its channels."""
@@ -78,10 +84,9 @@ def _prepare(x, dt, A, B, C, D, z, dt_bias, state, lead, what):
     t = x.dtype
     if t not in _SUPPORTED_IN or B.dtype != t or C.dtype != t or (z is not None and z.dtype != t):
         t = torch.float32
-    f32 = lambda o: None if o is None else _as(o, torch.float32).contiguous()
     dt = dt if dt.dtype == t else _as(dt, torch.float32)
-    return (_as(x, t), dt, f32(A), _as(B, t), _as(C, t), f32(D),
-            None if z is None else _as(z, t), f32(dt_bias), f32(state))
+    return (_as(x, t), dt, _f32(A), _as(B, t), _as(C, t), _f32(D),
+            None if z is None else _as(z, t), _f32(dt_bias), _f32(state))
 
 
 def _row_operand(t):
@@ -219,7 +224,7 @@ def gdn2_selective_scan_step(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_so
                     not state.is_contiguous()):
         raise GDN2Error(f"{what}: inplace needs a contiguous float32 state")
     xs, ds, A, B, C, D, zs, dt_bias, h = _prepare(x, dt, A, B, C, D, z, dt_bias, state, 1, what)
-    xs, ds, B, C = (t.contiguous() for t in (xs, ds, B, C))
+    xs, ds, B, C = xs.contiguous(), ds.contiguous(), B.contiguous(), C.contiguous()
     zs = None if zs is None else zs.contiguous()
     Bt, Ch = xs.shape
     G, N = B.shape[1:]
