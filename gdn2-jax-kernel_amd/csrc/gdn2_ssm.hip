@@ -121,15 +121,16 @@ struct WavePlace {
     chunk = first_chunk + rest % chunks;
     b = rest / chunks;
     g = tile / a.tiles;
-    const int cg = (tile - g * a.tiles) * 64 + lane;
+    const int first = (tile - g * a.tiles) * 64, cg = first + lane;
     on = cg < a.Cg;
-    c = g * a.Cg + (on ? cg : 0);          // loads stay in bounds, nothing is stored
+    c = g * a.Cg + (on ? cg : first);      // lanes without a channel repeat the wave's first
     t0 = chunk * a.L;
     t1 = a.T - t0 < a.L ? a.T : t0 + a.L;
   }
 };
 
-constexpr int kAhead = 4;   // tokens loaded at a time
+// Tokens loaded at a time: fewer where the states fill the registers.
+constexpr int ahead(int NP) { return NP <= 32 ? 4 : 2; }
 
 // NP states of (row, c) at p (rows of C channels), from and to float32.
 template <int NP>
@@ -191,6 +192,7 @@ struct WaveRows {
 // every token costs a copy of all states (8 x 8192 x 768 x 16 composed in 201 us, without 178).
 template <typename TX, typename TD, int NP, bool STARTS, bool OUT>
 __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a) {
+  constexpr int kAhead = ahead(NP);
   const WavePlace w(a, 0, OUT ? a.chunks : a.chunks - 1);
   if (w.idle) return;
   const int nch = a.chunks;
@@ -260,17 +262,19 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a)
     if (OUT) {
       float o = fmaf(D, x, (y[0] + y[1]) + (y[2] + y[3]));
       if (gate) o *= z * sigmoid(z);
-      if (w.on) put(out + (long long)t * a.C, ox, (TX)o);
+      // by all lanes, the same value where one repeats another's channel: stores that a lane may leave
+      // out cannot be counted, and loads behind them wait for all (8 x 2048 x 1536 x 16 135 us, so 133)
+      put(out + (long long)t * a.C, ox, (TX)o);
     }
   };
-  for (int t = w.t0; t < w.t1; t += kAhead) {
+  float x[kAhead], d[kAhead], z[kAhead];
+  auto take = [&](int t) {
     if (t % kKeep == 0) {
       rows.store(own);
       if (t + kKeep < w.t1) rows.load(bc, stride, t + kKeep, w.t1);
       if (OUT && a.kept && w.on)
         store_states<NP>(a.kept + (((long long)w.b * nb + t / kKeep) * a.C + w.c) * NP, h);
     }
-    float x[kAhead], d[kAhead], z[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       x[i] = (float)rx[i];
@@ -281,15 +285,20 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a)
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
     }
-    if (t + kAhead < w.t1) load(t + kAhead);
-    if (t + kAhead <= w.t1) {
+  };
+  // the odd ones last, apart: within the loop they would cost a copy of all states
+  int t = w.t0;
+  for (; t + kAhead <= w.t1; t += kAhead) {
+    take(t);
+    load(t + kAhead);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) token(t + i, x[i], d[i], z[i]);
-    } else {
+    for (int i = 0; i < kAhead; ++i) token(t + i, x[i], d[i], z[i]);
+  }
+  if (t < w.t1) {
+    take(t);
 #pragma unroll
-      for (int i = 0; i < kAhead - 1; ++i)
-        if (t + i < w.t1) token(t + i, x[i], d[i], z[i]);
-    }
+    for (int i = 0; i < kAhead - 1; ++i)
+      if (t + i < w.t1) token(t + i, x[i], d[i], z[i]);
   }
   if (!w.on) return;
   if (!OUT) {
@@ -307,6 +316,7 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a)
 // slot of the chunk before, and S.
 template <typename TX, typename TD, int NP, bool STARTS>
 __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a) {
+  constexpr int kAhead = ahead(NP);
   const WavePlace w(a, 1, a.chunks - 1);
   if (w.idle) return;
   const int nch = a.chunks;
@@ -334,7 +344,6 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a)
       if (gate) rz[i] = at(pz + ti * a.z.st, ox);
     }
   };
-  load(w.t1 - 1);
   float S = 0.f;
   bool fresh = false;
   __shared__ __attribute__((aligned(16))) float lds[kThreads / 64][kKeep * NP];
@@ -354,10 +363,9 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         e[n + k] = exp2_(d * A2[n + k]) * fmaf(g, Cv[k], e[n + k]);
-    }
-    if (t % kKeep == 0 && t > w.t0) {   // the sixteen tokens before this one are next
-      rows.store(own);
-      if (t - kKeep > w.t0) rows.load(bc, stride, t - 2 * kKeep, w.t1);
+      // whole before the loop turns, or both factors are carried over
+#pragma unroll
+      for (int k = 0; k < 4; ++k) asm("" : "+v"(e[n + k]));
     }
     S += d;
     if (STARTS && a.starts[(long long)w.b * a.T + t]) {
@@ -366,8 +374,8 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a)
       for (int n = 0; n < NP; ++n) e[n] = 0.f;
     }
   };
-  for (int t = w.t1 - 1; t >= w.t0; t -= kAhead) {
-    float g[kAhead], d[kAhead];
+  float g[kAhead], d[kAhead];
+  auto take = [&] {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       g[i] = has ? (float)ro[i] : 0.f;
@@ -381,15 +389,32 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a)
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) d[i] = softplus(d[i]);
     }
-    if (t - kAhead >= w.t0) load(t - kAhead);
-    if (t - kAhead + 1 >= w.t0) {
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) token(t - i, g[i], d[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kAhead - 1; ++i)
-        if (t - i >= w.t0) token(t - i, g[i], d[i]);
+  };
+  auto turn = [&](int t) {   // once token t is done: the sixteen tokens before it are next
+    if (t % kKeep == 0 && t > w.t0) {
+      rows.store(own);
+      if (t - kKeep > w.t0) rows.load(bc, stride, t - 2 * kKeep, w.t1);
     }
+  };
+  // the odd ones first, apart: within the loop they would cost a copy of all states
+  int t = w.t1 - 1;
+  load(t);
+  const int odd = (w.t1 - w.t0) % kAhead;
+  if (odd) {
+    take();
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i)
+      if (i < odd) token(t - i, g[i], d[i]);
+    t -= odd;
+    turn(t + 1);
+    load(t);
+  }
+  for (; t >= w.t0; t -= kAhead) {
+    take();
+    load(t - kAhead);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) token(t - i, g[i], d[i]);
+    turn(t - kAhead + 1);
   }
   if (!w.on) return;
   store_states<NP>(a.slot + (((long long)w.b * nch + w.chunk - 1) * a.C + w.c) * NP, e);
@@ -668,6 +693,12 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    // Every lane of a channel holds the sums over its states, and several lanes the same sums over the
+    // channels: each keeps those of its tokens in turn, and all write together, without a branch
+    // in every token (8 x 2048 x 1536 x 16 411 us, so 373).
+    constexpr int CP = 16 / NG;              // lanes with the same sums over channels
+    const int cp = (lane & 15) / NG;
+    float keep_b = 0.f, keep_a = 0.f, keep_y = 0.f, keep0 = 0.f, keep1 = 0.f;
 #pragma unroll
     for (int i = kKeep - 1; i >= 0; --i) {
       const Token m = next;
@@ -690,17 +721,24 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
       }
       sb = sum_low<LN>(sb);
       sa = sum_low<LN>(sa);
-      if (gate) y = sum_low<LN>(y);
-      if (q == 0) {
-        s.sb[i][ci] = sb;
-        s.sa[i][ci] = sa;
-        if (gate) s.y[i][ci] = y;
+      y = sum_low<LN>(y);
+      const bool mine = q == i % NG;
+      keep_b = mine ? sb : keep_b;
+      keep_a = mine ? sa : keep_a;
+      keep_y = mine ? y : keep_y;
+      if (i % NG == 0) {
+        s.sb[i + q][ci] = keep_b;
+        s.sa[i + q][ci] = keep_a;
+        s.y[i + q][ci] = keep_y;
       }
       sum_high8<LN>(v);
-      if ((lane & 15) < NG) {
-        float* r = &s.red[wave][i][lane >> 5][4 * q + 2 * (lane >> 4 & 1)];
-        r[0] = v[0];
-        r[1] = v[1];
+      const bool held = CP == 1 || cp == i % CP;
+      keep0 = held ? v[0] : keep0;
+      keep1 = held ? v[1] : keep1;
+      if (i % CP == 0) {
+        float* r = &s.red[wave][i + cp][lane >> 5][4 * q + 2 * (lane >> 4 & 1)];
+        r[0] = keep0;
+        r[1] = keep1;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
