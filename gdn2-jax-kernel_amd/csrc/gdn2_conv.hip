@@ -9,6 +9,9 @@
 // of tokens for its V channels (8- or 16-byte accesses) with the taps in registers, the
 // next tokens' loads in flight.  The halo of a run, W - 1 tokens (twice that in the backward,
 // which forms the pre-activation values again), is read from cache.  Sums are float32.
+// 8 x 8192 x 768 in bfloat16: forward 35 to 41 us (5.8 to 4.9 TB/s), backward 81 (3.7 TB/s; its
+// operations bound it: the pre-activation again, its sigmoid, 2 W multiply-adds a value) and 4.5 for
+// its sums over runs.
 #include <limits.h>
 
 #include "gdn2.h"
@@ -497,10 +500,14 @@ struct Split {
 Split split(int B, int T, int C, int V) {
   Split s;
   const int groups = (C + V - 1) / V;
-  s.ct = groups <= 16 ? 16 : 64;
+  // 16 lanes across the channels where 64 would leave over a third of the lanes without any (8 x 8192 x
+  // 288 in bfloat16 with 64 lanes 27 us, with 16 21; 3 x 1001 x 1003, one channel a lane, 7.5 and 11.5)
+  const int lanes16 = (groups + 15) / 16 * 16, lanes64 = (groups + 63) / 64 * 64;
+  s.ct = 2ll * lanes64 > 3ll * lanes16 ? 16 : 64;
   s.nct = (groups + s.ct - 1) / s.ct;
   const int per = kThreads / s.ct;
-  // runs of 32 tokens where they make two workgroups a CU, else of 16 or 8
+  // runs of 32 tokens where they make two workgroups a CU, else of 16 or 8 (runs of 32, 16 and 8: 8 x
+  // 8192 x 768 in bfloat16 34, 35 and 36 us, 1 x 4096 x 768 10, 7.0 and 6.3, 8 x 2048 x 64 9.9, 6.5 and 4.8)
   s.run = 32;
   while (s.run > 8 && (double)B * s.nct * ((T + per * s.run - 1ll) / (per * s.run)) < 512)
     s.run /= 2;

@@ -10,14 +10,21 @@
 // the sum of its d: one number a channel beside H.  The axis is cut into chunks: a first kernel
 // composes every chunk (S and H), a second walks over the chunks, a third walks each chunk's
 // tokens again from the state that enters it.  What bounds this is not memory but the
-// exponentials, N for each token and channel, and the four or five operations around each: a
-// wave of 64 lanes has a channel a lane, all its states in registers, and B and C, the same for
-// all lanes, in scalar registers, from float32 rows that a small kernel lays out.
+// exponentials, N for each token and channel, of which a SIMD starts a wave's every 16 cycles, and
+// the three to five operations around each at 4: a wave of 64 lanes has a channel a lane and all
+// its states in registers, so that nothing else is left to do but for B and C.  Those, the same for
+// all lanes, a small kernel lays out as float32 rows, which each wave brings to its part of LDS,
+// sixteen tokens at a time.  8 x 8192 x 768 x 16 in bfloat16, gated: rows 10 us, compositions 162,
+// join 13, outputs 215, where the exponentials, multiplies and additions for the states alone need
+// 28 and 32 cycles for 64 states, 143 and 164 us at 2.4 GHz; softplus and the gate, once for each
+// token and channel, are most of the rest.
 //
 // Backward: the gradients that enter chunks from the right come the same way.  The forward
 // keeps the state before every 16th token; from it a workgroup forms 16 tokens' states again,
 // keeps them and their decays in registers, and walks back.  Here a lane has four states of a
-// channel, and sums over states and over channels are formed by lane exchanges.
+// channel, and sums over states and over channels are formed by lane exchanges.  A state takes one
+// exponential and about 20 operations, half of them for those sums, which bound it: 8 x 2048 x
+// 1536 x 16 in 375 us (forward 89, 11 and 127, reverse 97 and 12, sums over workgroups 23).
 // Sums over workgroups are written as partial sums and added in a fixed order.
 // Everything is float32 between the inputs' and the outputs' types.
 #include <limits.h>
@@ -129,8 +136,7 @@ struct WavePlace {
   }
 };
 
-// Tokens loaded at a time: fewer where the states fill the registers.
-constexpr int ahead(int NP) { return NP <= 32 ? 4 : 2; }
+constexpr int kAhead = 4;   // tokens loaded at a time
 
 // NP states of (row, c) at p (rows of C channels), from and to float32.
 template <int NP>
@@ -189,10 +195,9 @@ struct WaveRows {
 
 // Forward.  OUT: the tokens from the entering state, outputs and kept states; else the
 // composition of chunks 0 .. chunks - 2, H of chunk k into slot k + 1.  STARTS apart: a branch in
-// every token costs a copy of all states (8 x 8192 x 768 x 16 composed in 201 us, without 178).
+// every token costs a copy of all states (8 x 8192 x 768 x 16 composed in 201 us, without 178 then).
 template <typename TX, typename TD, int NP, bool STARTS, bool OUT>
-__global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a) {
-  constexpr int kAhead = ahead(NP);
+__global__ void __launch_bounds__(kThreads, NP <= 16 ? 4 : 2) ssm_fwd(SsmArgs a) {
   const WavePlace w(a, 0, OUT ? a.chunks : a.chunks - 1);
   if (w.idle) return;
   const int nch = a.chunks;
@@ -315,8 +320,7 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_fwd(SsmArgs a)
 // The gradient that leaves chunks 1 .. chunks - 1 at their beginning with none entering, into the
 // slot of the chunk before, and S.
 template <typename TX, typename TD, int NP, bool STARTS>
-__global__ void __launch_bounds__(kThreads, NP <= 16 ? 3 : 2) ssm_rev(SsmArgs a) {
-  constexpr int kAhead = ahead(NP);
+__global__ void __launch_bounds__(kThreads, NP <= 16 ? 4 : 2) ssm_rev(SsmArgs a) {
   const WavePlace w(a, 1, a.chunks - 1);
   if (w.idle) return;
   const int nch = a.chunks;
@@ -927,9 +931,13 @@ Split split(int B, int T, int C, int G, int N) {
   const int Cg = C / G;
   s.tiles = (Cg + 63) / 64;
   s.btiles = (Cg + bwd_tile(s.np) - 1) / bwd_tile(s.np);
-  // chunks of 128 tokens where they make some waves a SIMD, else of 64 or 32, and of 16 where those
-  // would not give every SIMD one (2 x 1003 x 500 x 21 float32: 32 tokens 27, 33, 27 and 41 us, 16
-  // 17, 21, 18 and 42, and two joins 4 more each)
+  // chunks of 128 tokens where they make four waves a SIMD, else of 64 or 32, and of 16 where those
+  // would not give every SIMD one.  Forward in us, chunks of 16, 32, 64 and 128 tokens:
+  //   1 x 500 x 768 x 16     30   39   60  103     (waves: 384 of 16 tokens)
+  //   1 x 4001 x 1536 x 16  104   88   96  119     (3000 of 32)
+  //   4 x 2048 x 768 x 64   283  238  249  302     (3072 of 32)
+  //   8 x 2048 x 1536 x 16  259  222  212  215     (6144 of 64)
+  //   8 x 8192 x 768 x 16   522  425  396  394     (6144 of 128)
   s.L = 128;
   auto waves = [&] { return (double)B * G * s.tiles * ((T + s.L - 1) / s.L); };
   while ((s.L > 32 && waves() < 4096) || (s.L > 16 && waves() < 1024)) s.L /= 2;
