@@ -21,9 +21,11 @@
 // different banks; as the DMA writes LDS in lane order, the lanes' global addresses are permuted
 // instead.  The weight is the left operand, its rows dealt to the fragments so that a lane ends up
 // with eight neighbouring columns of one output row.  8192 x 8192 x 8192 into bfloat16 650 us (1.69
-// P/s), 4096 x 4096 x 4096 73 (1.88), 16384 x 4096 x 4096 298 (1.85); the matrix instruction alone,
+// P/s), 4096 x 4096 x 4096 73 (1.88), 16384 x 4096 x 4096 293 (1.87; with
+// operands and results not in the last-level cache 340); the matrix instruction alone,
 // on random data in registers, ran at 3.5, with the multiply-adds at 3.1.  Beside it LDS is as busy:
-// a wave's 64 x 64 outputs read 16 KB a slice, 128 bytes a cycle for the four of a CU.
+// a wave's 64 x 64 outputs read 16 KB a slice, 128 bytes a cycle for the four of a CU (37 % of
+// all cycles each, the vector units 31 %).
 //
 // Few rows: the weight's traffic is all that counts.  A workgroup takes 16 weight rows and its
 // eight waves the slices of k in turn, straight from memory to registers; their sums meet in LDS.
