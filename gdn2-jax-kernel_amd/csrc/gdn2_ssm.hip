@@ -14,8 +14,8 @@
 // the three to five operations around each at 4: a wave of 64 lanes has a channel a lane and all
 // its states in registers, so that nothing else is left to do but for B and C.  Those, the same for
 // all lanes, a small kernel lays out as float32 rows, which each wave brings to its part of LDS,
-// sixteen tokens at a time.  8 x 8192 x 768 x 16 in bfloat16, gated: rows 10 us, compositions 162,
-// join 13, outputs 215, where the exponentials, multiplies and additions for the states alone need
+// sixteen tokens at a time.  8 x 8192 x 768 x 16 in bfloat16, gated: rows 6 us, compositions 162,
+// join 12, outputs 215, where the exponentials, multiplies and additions for the states alone need
 // 28 and 32 cycles for 64 states, 143 and 164 us at 2.4 GHz; softplus and the gate, once for each
 // token and channel, are most of the rest.
 //
@@ -101,17 +101,23 @@ __device__ __forceinline__ void put(T* p, unsigned off, T v) {
   *reinterpret_cast<T*>(reinterpret_cast<char*>(p) + off) = v;
 }
 
-// B and C in float32, NP states each.
+// B and C in float32, NP states each, four a thread.
 template <typename TX>
 __global__ void __launch_bounds__(kThreads) ssm_rows(SsmArgs a, int NP) {
-  const long long n = (long long)a.B * a.T * a.G * 2 * NP;
+  const int quads = NP / 4, shift = __builtin_ctz(quads);
+  const long long n = (long long)a.B * a.T * a.G * 2 << shift;
   for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < n;
        e += (long long)gridDim.x * kThreads) {
-    const int s = (int)(e % NP);
-    const long long row = e / NP;          // ((b T + t) G + g) 2 + which
-    const long long bt = row / 2 / a.G;
-    const int g = (int)(row / 2 - bt * a.G), t = (int)(bt % a.T), b = (int)(bt / a.T);
-    a.bc[e] = s < a.N ? element<TX>(row & 1 ? a.cm : a.bm, b, t, g * a.N + s) : 0.f;
+    const int s = (int)(e & (quads - 1)) * 4;
+    const long long row = e >> shift;          // ((b T + t) G + g) 2 + which
+    const long long bt = a.G == 1 ? row >> 1 : (row >> 1) / a.G;
+    const int g = (int)((row >> 1) - bt * a.G), b = (int)(bt / a.T), t = (int)(bt - (long long)b * a.T);
+    const Rows& r = row & 1 ? a.cm : a.bm;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (s + k < a.N) v[k] = element<TX>(r, b, t, g * a.N + s + k);
+    *reinterpret_cast<f32x4*>(a.bc + 4 * e) = v;
   }
 }
 
@@ -427,9 +433,10 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 4 : 2) ssm_rev(SsmArgs a)
 
 // What enters each chunk, from the compositions: a thread a state of a channel, the chunks in
 // order (REV: from the last).
+constexpr int kJoin = 64;   // threads: few states are to reach all CUs
 template <int NP, bool REV>
-__global__ void __launch_bounds__(kThreads) ssm_join(SsmArgs a) {
-  const long long e = (long long)blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kJoin) ssm_join(SsmArgs a) {
+  const long long e = (long long)blockIdx.x * kJoin + threadIdx.x;
   const int n = (int)(e % NP);
   const long long bc = e / NP;
   const int b = (int)(bc / a.C), c = (int)(bc - (long long)b * a.C);
@@ -443,22 +450,36 @@ __global__ void __launch_bounds__(kThreads) ssm_join(SsmArgs a) {
   float* slot = a.slot + at * NP + n;
   const float* sum = a.sum + at;
   if (REV) *slot = h;    // the forward's first chunk reads h0 itself
-  // the composition of one chunk is read while the one before is applied
-  constexpr int U = 8;
-  for (int k0 = 1; k0 < nch; k0 += U) {
-    float H[U], S[U];
+  // compositions are read sixteen at a time, the next while these are applied (1 x 4001 x 1536 x 16, 126
+  // chunks: 13 us; eight at a time, each waited for, 17)
+  constexpr int U = 16;
+  float H[U], S[U];
+  auto load = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const long long k = k0 + i < nch ? k0 + i : nch - 1;
       H[i] = slot[k * step * NP];
       S[i] = sum[(k - 1) * step];
     }
+  };
+  auto apply = [&](int k, float Hk, float Sk) {
+    h = Sk == kNegInf ? Hk : fmaf(exp2_(A2 * Sk), h, Hk);
+    slot[k * step * NP] = h;
+  };
+  int k0 = 1;
+  load(k0);
+  for (; k0 + U <= nch; k0 += U) {
+    float now[U], sums[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (k0 + i >= nch) break;
-      h = S[i] == kNegInf ? H[i] : fmaf(exp2_(A2 * S[i]), h, H[i]);
-      slot[(k0 + i) * step * NP] = h;
-    }
+    for (int i = 0; i < U; ++i) now[i] = H[i], sums[i] = S[i];
+    load(k0 + U);   // past the last chunk: its, read again and not used
+#pragma unroll
+    for (int i = 0; i < U; ++i) apply(k0 + i, now[i], sums[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < U - 1; ++i) {
+    if (k0 + i >= nch) break;
+    apply(k0 + i, H[i], S[i]);
   }
 }
 
@@ -989,7 +1010,7 @@ unsigned groups_of(double n, double per, double most = 65536) {
 
 template <typename TX>
 void launch_rows(hipStream_t st, const SsmArgs& a, int NP) {
-  hipLaunchKernelGGL((ssm_rows<TX>), dim3(groups_of((double)a.B * a.T * a.G * 2 * NP, kThreads)),
+  hipLaunchKernelGGL((ssm_rows<TX>), dim3(groups_of((double)a.B * a.T * a.G * 2 * (NP / 4), kThreads)),
                      dim3(kThreads), 0, st, a, NP);
 }
 
@@ -1001,8 +1022,8 @@ void launch_fwd(hipStream_t st, const SsmArgs& a) {
     hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, STARTS, false>),
                        dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)), dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((ssm_join<NP, false>),
-                       dim3((unsigned)(((long long)a.B * a.C * NP + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, st, a);
+                       dim3((unsigned)(((long long)a.B * a.C * NP + kJoin - 1) / kJoin)),
+                       dim3(kJoin), 0, st, a);
   }
   hipLaunchKernelGGL((ssm_fwd<TX, TD, NP, STARTS, true>), dim3((unsigned)((waves * a.chunks + 3) / 4)),
                      dim3(kThreads), 0, st, a);
@@ -1015,8 +1036,8 @@ void launch_bwd(hipStream_t st, SsmArgs a) {
     hipLaunchKernelGGL((ssm_rev<TX, TD, NP, STARTS>), dim3((unsigned)((waves * (a.chunks - 1) + 3) / 4)),
                        dim3(kThreads), 0, st, a);
     hipLaunchKernelGGL((ssm_join<NP, true>),
-                       dim3((unsigned)(((long long)a.B * a.C * NP + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, st, a);
+                       dim3((unsigned)(((long long)a.B * a.C * NP + kJoin - 1) / kJoin)),
+                       dim3(kJoin), 0, st, a);
   }
   a.tiles = (a.Cg + bwd_tile(NP) - 1) / bwd_tile(NP);
   hipLaunchKernelGGL((ssm_bwd<TX, TD, NP, STARTS>),
