@@ -27,6 +27,9 @@
 // a wave's 64 x 64 outputs read 16 KB a slice, 128 bytes a cycle for the four of a CU (37 % of
 // all cycles each, the vector units 31 %).
 //
+// At most a tile for a CU: a slice's chain of reads, products and barrier is what takes the time (0.4
+// us), so eight waves share a tile, four to each half of k, and join their sums in LDS.
+//
 // Few rows: the weight's traffic is all that counts.  A workgroup takes 16 weight rows and its
 // eight waves the slices of k in turn, straight from memory to registers; their sums meet in LDS.
 //
@@ -498,10 +501,11 @@ __device__ __forceinline__ void store_part(const MmArgs& a, const f32x4 (&acc)[N
     }
 }
 
-// BM x BN outputs; WR x WC waves; ST slices of k in LDS; PER_CU workgroups on a CU.
-template <int BM_, int BN_, int WR_, int WC_, int ST_, int PER_CU_>
+// BM x BN outputs; WR x WC waves for each of the KS parts of k; ST slices of a part in LDS; PER_CU
+// workgroups on a CU.
+template <int BM_, int BN_, int WR_, int WC_, int ST_, int PER_CU_, int KS_ = 1>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, ST = ST_, PER_CU = PER_CU_;
+  static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, ST = ST_, PER_CU = PER_CU_, KS = KS_;
   static constexpr int NW = WR * WC, WM = BM / WR, WN = BN / WC;   // waves, and a wave's part
   static constexpr int MI = WM / 16, NI = WN / 16;
   static constexpr int STAGE = (BM + BN) * kBK;
@@ -517,18 +521,30 @@ __device__ __forceinline__ void while_each(std::integer_sequence<int, U...>, F&&
 }
 
 template <typename C, Scaling SC, typename TO>
-__global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmArgs a) {
+__global__ void __launch_bounds__(64 * C::NW * C::KS, C::NW * C::KS * C::PER_CU / 4)
+fp8_mm(MmArgs a) {
   constexpr int BM = C::BM, BN = C::BN, NW = C::NW, MI = C::MI, NI = C::NI, NL = C::NL;
-  constexpr int ST = C::ST;
+  constexpr int ST = C::ST, KS = C::KS;
   constexpr bool WROW = SC == kOfRows, MX = SC == kExponents;
   static_assert(!MX || (ST % 2 == 0 && sizeof(TO) == 2), "four exponents are read at a time");
   // scales that are no exponents come with their slice: those of x's rows, and of the weight's, or 64
   // times the one of its block
   constexpr int SCALES = MX ? 64 : BM + (WROW ? BN : 64), NV = NL + (MX ? 0 : 1);
-  __shared__ __attribute__((aligned(16))) char lds[ST * C::STAGE];
-  __shared__ __attribute__((aligned(16))) float lds_scales[MX ? 4 : ST * SCALES];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) char lds_all[KS * ST * C::STAGE];
+  __shared__ __attribute__((aligned(16))) float lds_scales_all[MX ? 4 : KS * ST * SCALES];
+  const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = wave_all % NW, part_k = wave_all / NW;
   const int li = lane & 15, lg = lane >> 4;
+  // KS = 2: the first waves take the first half of the slices, the others the rest, each half with a
+  // ring of its own; the launch has seen to it that neither is empty
+  static_assert(KS == 1 || KS == 2, "two halves");
+  char* lds = lds_all + (KS == 1 ? 0 : part_k * ST * C::STAGE);
+  float* lds_scales = lds_scales_all + (KS == 1 || MX ? 0 : part_k * ST * SCALES);
+  const int slices = (a.K + kBK - 1) / kBK;
+  const int half = KS == 1 ? slices : MX ? ((slices + 1) / 2 + 3) / 4 * 4 : (slices + 1) / 2;
+  const int first = KS == 1 ? 0 : part_k * half;                  // slices before this wave's
+  const int nk = KS == 1 || part_k == 0 ? half : slices - half;   // its own
+  const int K = KS == 1 ? a.K : part_k == 0 ? half * kBK : a.K - half * kBK;
 
   // Tiles: neighbours on one XCD, eight rows of tiles before the next column, so that what runs
   // together on an XCD shares rows and columns in its L2.
@@ -551,6 +567,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     const int most = act ? a.M - 1 - m0 : a.N - 1 - n0;
     at[i] = 16 * (lane % 8 ^ (act ? swz_x(r) : swz_w(r)));
     base[i] = (const char*)(act ? a.x + m0 * a.ldx : a.w + n0 * a.ldw);
+    base[i] += (size_t)first * kBK;
     off[i] = (unsigned)(r < most ? r : most) * (unsigned)(act ? a.ldx : a.ldw) + at[i];
   }
   // 64 of the scales a wave (some waves the same as others, where there are fewer)
@@ -567,8 +584,9 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
       scale = a.sw, scale_stride = a.ldsw;
       if (!WROW) scale += n0 / kBlock * a.ldsw, scale_stride = 1, scale_off = 0;
     }
+    scale += first * scale_stride;
   }
-  const int last = (a.K + 15) / 16 * 16 - 16;   // the last readable piece of a row
+  const int last = (a.K + 15) / 16 * 16 - 16 - first * kBK;   // the last readable piece of a row
   auto load = [&](int kb, int buf, auto whole) {
     if constexpr (!MX)
       lds_dma4((const char*)(scale + kb * scale_stride) + (size_t)scale_off,
@@ -611,17 +629,16 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   struct Exponents {
     int row[MI], col[NI];
   };
-  const int nk = (a.K + kBK - 1) / kBK;
   int sm[MI], sn[NI];   // the exponents' rows
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int r = m0 + wm + 16 * i + li;
-    sm[i] = (r < a.M ? r : a.M - 1) * a.lde;
+    sm[i] = (r < a.M ? r : a.M - 1) * a.lde + first;
   }
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     const int r = n0 + wn + (j / 2) * 32 + (li / 4) * 8 + (j & 1) * 4 + li % 4;
-    sn[j] = (r < a.N ? r : a.N - 1) * a.lde;
+    sn[j] = (r < a.N ? r : a.N - 1) * a.lde + first;
   }
   using Factors = std::conditional_t<MX, Exponents, Scales>;
   auto load_exponents = [&](Factors& s, int kb) {
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
     read_scales(sc[0], buf);
     if constexpr (MX && u % 4 == 0) load_exponents(sc[1], kb + 4 < nk ? kb + 4 : kb);
     if constexpr (!INNER) {
-      const int left = a.K - kb * kBK;
+      const int left = K - kb * kBK;
       if (left < kBK) {
 #pragma unroll
         for (int i = 0; i < MI; ++i) keep_row(xs[i], lg, left);
@@ -769,7 +786,7 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
   static_assert(UN % ST == 0 && UN % 2 == 0, "a slice's place in LDS and registers is known");
   const std::make_integer_sequence<int, UN> all;
   int k0 = 0;
-  for (; (k0 + UN + ST) * kBK <= a.K; k0 += UN)
+  for (; (k0 + UN + ST) * kBK <= K; k0 += UN)
     while_each(all, [&](auto u) {
       slice(u, std::true_type{}, k0 + decltype(u)::value);
       return true;
@@ -780,6 +797,29 @@ __global__ void __launch_bounds__(64 * C::NW, C::NW * C::PER_CU / 4) fp8_mm(MmAr
       if (kb < nk) slice(u, std::false_type{}, kb);
       return kb < nk;
     });
+  if constexpr (KS == 2) {
+    // the second half's sums to the first's waves, over the second ring once nobody reads it
+    for (int i = nk; i < half; ++i) lds_barrier();   // a barrier a slice
+    lds_barrier();
+    f32x4* sums = reinterpret_cast<f32x4*>(lds_all + ST * C::STAGE) + wave * 64 + lane;
+    static_assert(NI * MI * NW * 64 * 16 <= ST * C::STAGE, "room");
+    if (part_k) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int i = 0; i < MI; ++i) sums[(j * MI + i) * NW * 64] = acc[j][i];
+    }
+    lds_barrier();
+    if (part_k) return;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const f32x4 v = sums[(j * MI + i) * NW * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][i][e] += v[e];
+      }
+  }
   store_part<TO>(a, acc, m0 + wm, n0 + wn, li, lg);
 }
 
@@ -860,7 +900,7 @@ void launch_tiles(hipStream_t st, MmArgs a) {
   a.tm = (a.M + C::BM - 1) / C::BM;
   a.tn = (a.N + C::BN - 1) / C::BN;
   a.chunk = (a.tm * a.tn + 7) / 8;
-  hipLaunchKernelGGL((fp8_mm<C, SC, TO>), dim3(8u * (unsigned)a.chunk), dim3(64 * C::NW), 0, st, a);
+  hipLaunchKernelGGL((fp8_mm<C, SC, TO>), dim3(8u * (unsigned)a.chunk), dim3(64 * C::NW * C::KS), 0, st, a);
 }
 template <int MT, Scaling SC, typename TO>
 void launch_rows(hipStream_t st, const MmArgs& a) {
@@ -875,17 +915,22 @@ hipError_t launch_mm(hipStream_t st, const MmArgs& a) {
   auto tiles = [&](int bm, int bn) {
     return (((long long)a.M + bm - 1) / bm) * (((long long)a.N + bn - 1) / bn);
   };
-  // bfloat16 results in us, K = 4096 (8192 columns: K = 1024), of rows | 64 x 64 | 128 x 128:
-  //   17 x 4096       8 | 14 | 26         96 x 1024    8 | 14 | 26
-  //   64 x 4096      14 | 14 | 26        128 x 1024  8.5 | 14 | 26
-  //   96 x 4096      20 | 15 | 26        192 x 1024   14 | 14 | 26
-  //   768 x 4096      - | 25 | 34       2048 x 1024    - | 22 | 34
-  //   1024 x 4096     - | 41 | 35       4096 x 1024    - | 42 | 36
-  //   384 x 8192     37 | 9.5 | 11       512 x 8192   47 | 13 | 12
+  // bfloat16 results in us, K = 4096 (8192 columns: K = 1024), of rows | 64 x 64 in halves of k | 64 x 64
+  // | 128 x 128:
+  //   17 x 4096       8 |   - | 14 | 26       96 x 1024    8 |   - | 14 | 26
+  //   64 x 4096      14 |  10 | 14 | 26      128 x 1024  8.5 |   - | 14 | 26
+  //   96 x 4096      20 |  10 | 15 | 26      192 x 1024   14 |  10 | 14 | 26
+  //   256 x 4096     47 |  11 | 15 | 27     1024 x 1024    - |  11 | 15 | 34
+  //   768 x 4096      - |   - | 25 | 34     2048 x 1024    - |   - | 22 | 34
+  //   1024 x 4096     - |   - | 41 | 35     4096 x 1024    - |   - | 42 | 36
+  //   64 x 8192     8.7 | 5.5 |  6 |  9      384 x 8192   37 |   - | 9.5 | 11
+  //                                          512 x 8192   47 |   - | 13 | 12
   if (a.M <= 16)
     launch_rows<1, SC, TO>(st, a);
   else if (a.M <= 32 || tiles(32, 16) <= cus)
     launch_rows<2, SC, TO>(st, a);
+  else if (tiles(64, 64) <= cus && a.K >= 8 * kBK)        // a workgroup a CU: two halves of k
+    launch_tiles<Tile<64, 64, 2, 2, SC == kExponents ? 4 : 3, 1, 2>, SC, TO>(st, a);
   else if (sizeof(TO) == 4 || tiles(64, 64) <= 3 * cus)   // float32: registers for no more
     launch_tiles<Tile<64, 64, 2, 2, SC == kExponents ? 4 : 3, SC == kExponents ? 2 : 3>, SC, TO>(st, a);
   else if constexpr (sizeof(TO) == 2)

@@ -217,6 +217,18 @@ def test_product_of_many_tiles(dev, M, N, K, blocks):
         check(gp.gdn2_fp8_matmul(q, sx, w, sw, bias=b, out_dtype=dt), product(x64, w64, b), K)
 
 
+@pytest.mark.parametrize("blocks", [True, False])
+@pytest.mark.parametrize("M,N", [(130, 900), (200, 777), (260, 1300)])
+def test_product_of_few_tiles(dev, M, N, blocks):
+    """A tile for a CU at most: two halves of k of 4 and 4 slices up to 9 and 8, the last one whole,
+    of one value or in between."""
+    import gdn2_package as gp
+    for K in (1023, 1024, 1025, 1157, 1280, 1300, 2048, 2170):
+        q, sx, w, sw, bias, x64, w64 = operands(M, N, K, dev, M + K, blocks)
+        for dt, b in ((F32, bias), (BF16, None)):
+            check(gp.gdn2_fp8_matmul(q, sx, w, sw, bias=b, out_dtype=dt), product(x64, w64, b), K)
+
+
 def test_layouts(dev):
     """Padding that holds NaN, rows at odd offsets, transposes, batches, scales laid out either way."""
     import gdn2_package as gp
@@ -253,7 +265,8 @@ def test_layouts(dev):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 5, 7), (33, 130, 64), (130, 64, 300),
-                                   (257, 300, 129), (700, 520, 400)])
+                                   (257, 300, 129), (700, 520, 400), (130, 1160, 1157),
+                                   (1160, 130, 1030), (2200, 140, 1300)])
 def test_linear(dev, M, N, K, dtype):
     import gdn2_package as gp
     x, w, dy = (values(*s, dtype, dev, i) for i, s in enumerate(((M, K), (N, K), (M, N))))
