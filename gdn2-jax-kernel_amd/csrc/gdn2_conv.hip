@@ -9,8 +9,8 @@
 // of tokens for its V channels (8- or 16-byte accesses) with the taps in registers, the
 // next tokens' loads in flight.  The halo of a run, W - 1 tokens (twice that in the backward,
 // which forms the pre-activation values again), is read from cache.  Sums are float32.
-// 8 x 8192 x 768 in bfloat16: forward 35 to 41 us (5.8 to 4.9 TB/s), backward 81 (3.7 TB/s; its
-// operations bound it: the pre-activation again, its sigmoid, 2 W multiply-adds a value) and 4.5 for
+// 8 x 8192 x 768 in bfloat16: forward 35 to 41 us (5.8 to 4.9 TB/s), backward 75 packed (4.0 TB/s; its
+// operations bound it: the pre-activation again, its sigmoid, 2 W multiply-adds a value) and 4 for
 // its sums over runs.
 #include <limits.h>
 
@@ -497,7 +497,7 @@ struct Split {
 };
 // Lanes across the channels and tokens of a run, by sizes alone: the backward's workspace is
 // sized for one channel a thread or two, whichever needs more.
-Split split(int B, int T, int C, int V) {
+Split split(int B, int T, int C, int V, bool back) {
   Split s;
   const int groups = (C + V - 1) / V;
   // 16 lanes across the channels where 64 would leave over a third of the lanes without any (8 x 8192 x
@@ -508,8 +508,11 @@ Split split(int B, int T, int C, int V) {
   const int per = kThreads / s.ct;
   // runs of 32 tokens where they make two workgroups a CU, else of 16 or 8 (runs of 32, 16 and 8: 8 x
   // 8192 x 768 in bfloat16 34, 35 and 36 us, 1 x 4096 x 768 10, 7.0 and 6.3, 8 x 2048 x 64 9.9, 6.5 and 4.8)
-  s.run = 32;
-  while (s.run > 8 && (double)B * s.nct * ((T + per * s.run - 1ll) / (per * s.run)) < 512)
+  // The backward, whose first and last tokens of a run take longer, has runs of 64 where they make six
+  // (8 x 8192 x 768 packed 75 us, of 32 81; 6 x 8192 x 768 48 and 48)
+  s.run = back ? 64 : 32;
+  while (s.run > 8 && (double)B * s.nct * ((T + per * s.run - 1ll) / (per * s.run)) <
+                          (s.run == 64 ? 1536 : 512))
     s.run /= 2;
   s.runs = (int)((T + (long long)per * s.run - 1) / ((long long)per * s.run));
   return s;
@@ -520,7 +523,7 @@ int validate(int B, int T, int C, int W, int dtype) {
   // token numbers of a run and its halo stay within 31 bits, a launch's threads within 32
   if (T > INT_MAX - 1024 || C > (1 << 24)) return GDN2_ERR_SHAPE;
   for (int V : {1, 2, 4}) {
-    const Split s = split(B, T, C, V);
+    const Split s = split(B, T, C, V, false);   // the backward has no more
     if ((double)B * s.nct * (s.runs < 1 ? 1 : s.runs) > (double)(1 << 23)) return GDN2_ERR_SHAPE;
   }
   if (dtype != GDN2_F32 && dtype != GDN2_BF16) return GDN2_ERR_DTYPE;
@@ -555,7 +558,7 @@ void launch_width(hipStream_t st, ConvArgs& a, Mode mode) {
                        dim3(kThreads), 0, st, a);
     return;
   }
-  const Split s = split(a.B, a.T, a.C, mode == kBackward ? kBwd<V> : V);
+  const Split s = mode == kBackward ? split(a.B, a.T, a.C, kBwd<V>, true) : split(a.B, a.T, a.C, V, false);
   a.run = s.run, a.runs = s.runs, a.nct = s.nct;
   const dim3 grid((unsigned)((long long)a.B * s.runs * s.nct)), block(kThreads);
 #define GDN2_CONV(CT)                                                             \
@@ -594,7 +597,7 @@ extern "C" {
 
 size_t gdn2_short_conv_bwd_workspace_bytes(int B, int T, int C, int W) {
   if (validate(B, T, C, W, GDN2_F32) != GDN2_OK || T == 0) return 0;
-  const int r1 = split(B, T, C, 1).runs, r2 = split(B, T, C, 2).runs;
+  const int r1 = split(B, T, C, 1, true).runs, r2 = split(B, T, C, 2, true).runs;
   return (size_t)B * (r1 > r2 ? r1 : r2) * C * (W + 1) * sizeof(float);
 }
 

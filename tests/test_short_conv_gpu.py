@@ -16,7 +16,7 @@ ULP = 2.0 ** -24
 F32, BF16 = torch.float32, torch.bfloat16
 
 
-def reference(x, w, bias, state, starts, silu, dy=None, dlast=None):
+def reference(x, w, bias, state, starts, silu, dy=None, dlast=None, terms=128):
     """Values and the bounds of their errors (without the last rounding), in float64."""
     B, T, C = x.shape
     W = w.shape[1]
@@ -45,12 +45,12 @@ def reference(x, w, bias, state, starts, silu, dy=None, dlast=None):
         dline[:, k:k + T] += torch.where(same[k], dp, 0.0) * w[:, k]
         eline[:, k:k + T] += torch.where(same[k], ep + 8 * ULP * dp.abs(), 0.0) * w[:, k].abs()
         dw[:, k] = (dp * tap[k]).sum((0, 1))
-        ew[:, k] = ((ep + 128 * ULP * dp.abs()) * tap[k].abs()).sum((0, 1))
+        ew[:, k] = ((ep + terms * ULP * dp.abs()) * tap[k].abs()).sum((0, 1))
     dline[:, T:] += torch.where(kept, dlast, 0.0)
     eline += 4 * ULP * dline.abs()
     eline[:, T:] += 4 * ULP * dlast.abs()
     res.update(x=(dline[:, W - 1:], eline[:, W - 1:]), weight=(dw, ew),
-               bias=(dp.sum((0, 1)), (ep + 128 * ULP * dp.abs()).sum((0, 1))),
+               bias=(dp.sum((0, 1)), (ep + terms * ULP * dp.abs()).sum((0, 1))),
                state=(dline[:, :W - 1], eline[:, :W - 1]))
     return res
 
@@ -106,6 +106,25 @@ def test_forward_and_backward(dev, B, T, C, W, dtype):
                 again, same = gp.gdn2_short_conv(leaf["x"], leaf["weight"], bias=leaf.get("bias"),
                                                  state=leaf.get("state"), activation=act, starts=cut)
             assert torch.equal(again, y) and torch.equal(same, last)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,T,C,W", [(1540, 70, 12, 4), (1600, 133, 7, 3), (800, 1030, 6, 4)])
+def test_long_runs(dev, B, T, C, W, dtype):
+    """Enough workgroups for the backward's runs of 64 tokens.  A weight's sum: 64 tokens, 16 runs, at
+    most 1600 rows of partial sums of which a thread adds every 64th, 25, and 64 of those: 169."""
+    import gdn2_package as gp
+    for starts in (False, True):
+        t, cut, dy, dlast = inputs(B, T, C, W, dtype, dev, T, starts)
+        if starts:   # far from each other too
+            cut &= torch.arange(T, device=dev) % 32 < 3
+        leaf = [t[n].clone().requires_grad_() for n in ("x", "weight", "bias", "state")]
+        outs = gp.gdn2_short_conv(leaf[0], leaf[1], bias=leaf[2], state=leaf[3], starts=cut)
+        ref = reference(*map(d64, leaf), cut, True, d64(dy), d64(dlast), 192)
+        check(outs[0], ref["y"])
+        for n, g in zip(("x", "weight", "bias", "state"),
+                        torch.autograd.grad(outs, leaf, (dy, dlast))):
+            check(g, ref[n])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
