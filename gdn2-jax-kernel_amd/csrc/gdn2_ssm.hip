@@ -69,19 +69,17 @@ struct SsmArgs {
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
 
-// log(1 + e^v) = max(v, 0) + log1p(e^-|v|), log1p(u) = 2 artanh(s) with s = u / (2 + u) <= 1/3, and
-// artanh(s) = s (1 + s^2/3 + s^4/5 + ...), whose terms from s^16/17 on are below 2^-29.
+// log(1 + e^v) = max(v, 0) + log1p(e^-|v|), log1p(u) = 2 artanh(r) with r = u / (2 + u) <= 1/3.
+// artanh(r) = r p(r^2): p fitted for the least relative error up to 1/9, 2^-26.9 with these
+// coefficients.  NaN comes through u.
 __device__ __forceinline__ float softplus(float v) {
-  const float u = exp2_(-fabsf(v) * kLog2e), s = u * rcp_(2.f + u), q = s * s;
-  float p = 1.f / 15.f;
-  p = fmaf(p, q, 1.f / 13.f);
-  p = fmaf(p, q, 1.f / 11.f);
-  p = fmaf(p, q, 1.f / 9.f);
-  p = fmaf(p, q, 1.f / 7.f);
-  p = fmaf(p, q, 1.f / 5.f);
-  p = fmaf(p, q, 1.f / 3.f);
+  const float u = exp2_(-fabsf(v) * kLog2e), r = u * rcp_(2.f + u), q = r * r;
+  float p = 0.14089167f;
+  p = fmaf(p, q, 0.139803f);
+  p = fmaf(p, q, 0.20012455f);
+  p = fmaf(p, q, 0.33333158f);
   p = fmaf(p, q, 1.f);
-  return fmaf(2.f * s, p, v != v ? v : fmaxf(v, 0.f));
+  return fmaf(2.f * r, p, fmaxf(v, 0.f));
 }
 __device__ __forceinline__ float sigmoid(float v) { return rcp_(1.f + exp2_(-v * kLog2e)); }
 
