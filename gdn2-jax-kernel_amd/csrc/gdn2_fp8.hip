@@ -929,7 +929,7 @@ hipError_t launch_mm(hipStream_t st, const MmArgs& a) {
     launch_rows<1, SC, TO>(st, a);
   else if (a.M <= 32 || tiles(32, 16) <= cus)
     launch_rows<2, SC, TO>(st, a);
-  else if (tiles(64, 64) <= cus && a.K >= 8 * kBK)        // a workgroup a CU: two halves of k
+  else if (tiles(64, 64) <= cus && a.K > 7 * kBK)         // a workgroup a CU: two halves of k
     launch_tiles<Tile<64, 64, 2, 2, SC == kExponents ? 4 : 3, 1, 2>, SC, TO>(st, a);
   else if (sizeof(TO) == 4 || tiles(64, 64) <= 3 * cus)   // float32: registers for no more
     launch_tiles<Tile<64, 64, 2, 2, SC == kExponents ? 4 : 3, SC == kExponents ? 2 : 3>, SC, TO>(st, a);

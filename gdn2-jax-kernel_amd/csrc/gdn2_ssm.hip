@@ -14,8 +14,8 @@
 // the three to five operations around each at 4: a wave of 64 lanes has a channel a lane and all
 // its states in registers, so that nothing else is left to do but for B and C.  Those, the same for
 // all lanes, a small kernel lays out as float32 rows, which each wave brings to its part of LDS,
-// sixteen tokens at a time.  8 x 8192 x 768 x 16 in bfloat16, gated: rows 6 us, compositions 162,
-// join 12, outputs 215, where the exponentials, multiplies and additions for the states alone need
+// sixteen tokens at a time.  8 x 8192 x 768 x 16 in bfloat16, gated: rows 6 us, compositions 159,
+// join 12, outputs 209, where the exponentials, multiplies and additions for the states alone need
 // 28 and 32 cycles for 64 states, 143 and 164 us at 2.4 GHz; softplus and the gate, once for each
 // token and channel, are most of the rest.
 //
@@ -24,7 +24,7 @@
 // keeps them and their decays in registers, and walks back.  Here a lane has four states of a
 // channel, and sums over states and over channels are formed by lane exchanges.  A state takes one
 // exponential and about 20 operations, half of them for those sums, which bound it: 8 x 2048 x
-// 1536 x 16 in 375 us (forward 89, 11 and 127, reverse 97 and 12, sums over workgroups 23).
+// 1536 x 16 in 375 us (forward 86, 12 and 124, reverse 94 and 12, sums over workgroups 23).
 // Sums over workgroups are written as partial sums and added in a fixed order.
 // Everything is float32 between the inputs' and the outputs' types.
 #include <limits.h>
