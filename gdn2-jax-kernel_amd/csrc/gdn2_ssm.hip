@@ -952,11 +952,11 @@ Split split(int B, int T, int C, int G, int N) {
   s.btiles = (Cg + bwd_tile(s.np) - 1) / bwd_tile(s.np);
   // chunks of 128 tokens where they make four waves a SIMD, else of 64 or 32, and of 16 where those
   // would not give every SIMD one.  Forward in us, chunks of 16, 32, 64 and 128 tokens:
-  //   1 x 500 x 768 x 16     30   39   60  103     (waves: 384 of 16 tokens)
-  //   1 x 4001 x 1536 x 16  104   88   96  119     (3000 of 32)
-  //   4 x 2048 x 768 x 64   283  238  249  302     (3072 of 32)
-  //   8 x 2048 x 1536 x 16  259  222  212  215     (6144 of 64)
-  //   8 x 8192 x 768 x 16   522  425  396  394     (6144 of 128)
+  //   1 x 500 x 768 x 16     30   39   60  103     (0.4 waves a SIMD with 16 tokens)
+  //   1 x 4001 x 1536 x 16  104   88   96  119     (2.9 with 32)
+  //   4 x 2048 x 768 x 64   283  238  249  302     (3 with 32)
+  //   8 x 2048 x 1536 x 16  259  222  212  215     (6 with 64)
+  //   8 x 8192 x 768 x 16   522  425  396  394     (6 with 128)
   s.L = 128;
   auto waves = [&] { return (double)B * G * s.tiles * ((T + s.L - 1) / s.L); };
   while ((s.L > 32 && waves() < 4096) || (s.L > 16 && waves() < 1024)) s.L /= 2;
