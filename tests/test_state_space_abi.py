@@ -60,7 +60,7 @@ def test_conv_refusals_by_direction():
     assert size(2, 0, 64, 4) == 0 and size(2, 60, 64, 5) == 0 and size(-1, 60, 64, 4) == 0
     # a row of sums for each workgroup: 8 tokens and 4 runs (64 lanes), or 16 (16 lanes)
     assert size(2, 60, 64, 4) == 2 * 2 * 64 * 5 * 4
-    assert size(8, 8192, 768, 4) == 8 * 64 * 768 * 5 * 4
+    assert size(8, 8192, 768, 4) == 8 * 32 * 768 * 5 * 4   # 64 tokens
 
 
 def ssm_fwd(B=2, T=60, C=64, G=2, N=16, dt=F32, ddt=F32, sp=1, x=P[0], d=P[1], z=P[2], bm=P[3],
