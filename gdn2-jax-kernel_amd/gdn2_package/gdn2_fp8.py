@@ -144,8 +144,12 @@ def gdn2_fp8_matmul(q, scale, weight, weight_scale, bias=None, out_dtype=torch.b
 
     q (..., K) float8_e4m3fn with scale (..., ceil(K / 128)); weight (N, K) with weight_scale
     (ceil(N / 128), ceil(K / 128)) or, a scale for each row, (N, ceil(K / 128)); bias (N,) or
-    None.  Returns (..., N) in out_dtype (float32 or bfloat16): float32 sums of a block's
-    products, scaled and added in float32 and rounded once.  Inference only."""
+    None.  Returns (..., N) in out_dtype (float32 or bfloat16).  For float32 the products of a
+    block are added in float32.  For bfloat16 they are added by the 8-bit matrix instruction, which is
+    faster: of eight neighbouring products it drops, towards zero, what lies below 2^-13 of the
+    largest, so that small products are lost beside large ones that cancel.  A caller who
+    needs them takes a float32 result and rounds it.  Blocks are scaled and added in float32 and
+    the result is rounded once, for either type.  Inference only."""
     what = "gdn2_fp8_matmul"
     if out_dtype not in _SUPPORTED_IN:
         raise GDN2Error(f"{what}: out_dtype must be float32 or bfloat16; got {out_dtype}")
@@ -235,8 +239,9 @@ def gdn2_fp8_linear(x, weight, bias=None):
     are widened to float32).  Returns (..., N) in x's type.  Forward: x in rows of 1 x 128, the
     weight in blocks of 128 x 128.  Backward: the gradient of x from the output's in rows and the
     weight's blocks, that of the weight from the output's gradient and x in blocks of 128 tokens;
-    the bias's is the sum of the output's gradient as it comes.  Between the passes x and the
-    weight are kept in 8 bits.  Differentiable in x, weight and bias in reverse mode (tangents of
+    the bias's is the sum of the output's gradient as it comes.  All three products add as
+    gdn2_fp8_matmul does for results of that type: float32 inputs in float32, bfloat16 ones by the
+    8-bit matrix instruction.  Between the passes x and the weight are kept in 8 bits.  Differentiable in x, weight and bias in reverse mode (tangents of
     forward mode raise NotImplementedError): gradients pass through the roundings as if they were
     none.  To serve, quantise the weight once and call gdn2_fp8_matmul."""
     what = "gdn2_fp8_linear"
