@@ -438,27 +438,33 @@ __global__ void __launch_bounds__(kThreads, V == 2 ? 4 : 1) conv_bwd(ConvArgs a)
 }
 
 // The partial sums of dw and dbias added in their order: 16 columns a workgroup, 64 rows at a
-// time.
+// time.  A grid of kSumsMost workgroups walks on over the columns.
+constexpr unsigned kSumsMost = 1u << 20;   // a launch's threads stay within 32 bits
 __global__ void __launch_bounds__(1024) conv_sums(const float* part, long long rows, int C, int W,
                                                   float* dw, float* dbias) {
   __shared__ float s[64][16];
   const int col = threadIdx.x & 15, r = threadIdx.x >> 4;
-  const long long at = (long long)blockIdx.x * 16 + col, width = (long long)C * (W + 1);
-  float v = 0.f;
-  if (at < width)
-    for (long long k = r; k < rows; k += 64) v += part[k * width + at];
-  s[r][col] = v;
-  __syncthreads();
-  if (r || at >= width) return;
-  v = 0.f;
+  const long long width = (long long)C * (W + 1);
+  for (long long first = blockIdx.x * 16ll; first < width; first += gridDim.x * 16ll) {
+    const long long at = first + col;
+    float v = 0.f;
+    if (at < width)
+      for (long long k = r; k < rows; k += 64) v += part[k * width + at];
+    s[r][col] = v;
+    __syncthreads();
+    if (r == 0 && at < width) {
+      v = 0.f;
 #pragma unroll
-  for (int k = 0; k < 64; ++k) v += s[k][col];
-  const long long c = at / (W + 1);
-  const int k = (int)(at - c * (W + 1));
-  if (k < W)
-    dw[c * W + k] = v;
-  else if (dbias)
-    dbias[c] = v;
+      for (int k = 0; k < 64; ++k) v += s[k][col];
+      const long long c = at / (W + 1);
+      const int k = (int)(at - c * (W + 1));
+      if (k < W)
+        dw[c * W + k] = v;
+      else if (dbias)
+        dbias[c] = v;
+    }
+    __syncthreads();   // the next columns' rows are written over what was read here
+  }
 }
 
 // One token: a thread V channels of a batch entry; old and new state may be the same memory.
@@ -650,7 +656,8 @@ int gdn2_short_conv_bwd(void* stream, int B, int T, int C, int W, int dtype, int
   a.dy = dy, a.db = d[0], a.dt = d[1], a.dlast = dlast, a.dx = dx, a.dstate = dstate;
   a.part = (float*)ws, a.B = B, a.T = T, a.C = C, a.silu = silu;
   if ((rc = launch((hipStream_t)stream, a, W, dtype, vec, kBackward))) return rc;
-  const unsigned wgs = (unsigned)(((long long)C * (W + 1) + 15) / 16);
+  const long long sums = ((long long)C * (W + 1) + 15) / 16;
+  const unsigned wgs = sums < kSumsMost ? (unsigned)sums : kSumsMost;
   hipLaunchKernelGGL(conv_sums, dim3(wgs), dim3(1024), 0, (hipStream_t)stream, a.part,
                      (long long)B * a.runs, C, W, dw, dbias);
   return hipGetLastError() == hipSuccess ? GDN2_OK : GDN2_ERR_LAUNCH;
