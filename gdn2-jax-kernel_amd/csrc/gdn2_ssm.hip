@@ -825,8 +825,9 @@ __global__ void __launch_bounds__(kThreads, 2) ssm_bwd(SsmArgs a) {
 }
 
 // Partial sums added in their order.  The first workgroups: the gradients of A, D and dt_bias, 64
-// columns each (C NP of part_a, then 2 C of part_c), 16 rows at a time.  The others: those of B and
-// C, the tiles of a group for each value.
+// columns each (C NP of part_a, then 2 C of part_c), 16 rows at a time, walking on over the columns
+// where kSumsMost are too few.  The others: those of B and C, the tiles of a group for each value.
+constexpr int kSumsMost = 1 << 20;   // a launch's threads stay within 32 bits
 template <typename TX>
 __global__ void __launch_bounds__(1024) ssm_sums(SsmArgs a, int NP, int first) {
   if ((int)blockIdx.x >= first) {
@@ -847,27 +848,31 @@ __global__ void __launch_bounds__(1024) ssm_sums(SsmArgs a, int NP, int first) {
   __shared__ float sum[16][64];
   const int col = threadIdx.x & 63, r = threadIdx.x >> 6;
   const long long wa = (long long)a.C * NP, wc = 2ll * a.C, rows = (long long)a.B * a.chunks;
-  const long long at = (long long)blockIdx.x * 64 + col;
-  float v = 0.f;
-  if (at < wa) {
-    for (long long k = r; k < rows; k += 16) v += a.part_a[k * wa + at];
-  } else if (at < wa + wc) {
-    for (long long k = r; k < rows; k += 16) v += a.part_c[k * wc + at - wa];
-  }
-  sum[r][col] = v;
-  __syncthreads();
-  if (r) return;
-  v = 0.f;
+  for (long long c0 = blockIdx.x * 64ll; c0 < wa + wc; c0 += first * 64ll) {
+    const long long at = c0 + col;
+    float v = 0.f;
+    if (at < wa) {
+      for (long long k = r; k < rows; k += 16) v += a.part_a[k * wa + at];
+    } else if (at < wa + wc) {
+      for (long long k = r; k < rows; k += 16) v += a.part_c[k * wc + at - wa];
+    }
+    sum[r][col] = v;
+    __syncthreads();
+    if (r == 0) {
+      v = 0.f;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) v += sum[k][col];
-  if (at < wa) {
-    const long long c = at / NP;
-    const int n = (int)(at - c * NP);
-    if (n < a.N) a.dA[c * a.N + n] = v;
-  } else if (at < wa + a.C) {
-    if (a.dD) a.dD[at - wa] = v;
-  } else if (at < wa + wc) {
-    if (a.dbias) a.dbias[at - wa - a.C] = v;
+      for (int k = 0; k < 16; ++k) v += sum[k][col];
+      if (at < wa) {
+        const long long c = at / NP;
+        const int n = (int)(at - c * NP);
+        if (n < a.N) a.dA[c * a.N + n] = v;
+      } else if (at < wa + a.C) {
+        if (a.dD) a.dD[at - wa] = v;
+      } else if (at < wa + wc) {
+        if (a.dbias) a.dbias[at - wa - a.C] = v;
+      }
+    }
+    __syncthreads();   // the next columns' rows are written over what was read here
   }
 }
 
@@ -1041,7 +1046,7 @@ void launch_bwd(hipStream_t st, SsmArgs a) {
   hipLaunchKernelGGL((ssm_bwd<TX, TD, NP, STARTS>),
                      dim3((unsigned)((long long)a.B * a.G * a.tiles * a.chunks)), dim3(kThreads), 0,
                      st, a);
-  const int first = (int)(((long long)a.C * (NP + 2) + 63) / 64);
+  const int first = (int)groups_of((double)a.C * (NP + 2), 64, kSumsMost);
   hipLaunchKernelGGL((ssm_sums<TX>),
                      dim3(first + groups_of((double)a.B * a.T * a.G * 2 * NP, 1024, 16384)), dim3(1024),
                      0, st, a, NP, first);

@@ -1,5 +1,5 @@
-// The launches of the short convolution and the 8-bit floating-point operators over sizes up to
-// the largest that their entry points take, built with the kernels' host code alone by
+// The launches of the short convolution, the selective scan and the 8-bit floating-point operators
+// over sizes up to the largest that their entry points take, built with the kernels' host code alone by
 // tests/test_launch_sizes_host.py.  The runtime's launch is defined here: it only looks at the
 // grid, so no call needs a GPU and every pointer is a number that nothing follows.  A launch's threads
 // have to stay below 2^32 along each axis; one that does not would be refused after the launches
@@ -87,6 +87,31 @@ static void conv() {
           }
 }
 
+static void scan() {
+  const void* ins[5] = {p, p, p, p, p};
+  void* outs[5] = {p, p, p, p, p};
+  for (int B : kSizes)
+    for (int T : kSizes)
+      for (int C : kSizes)
+        for (int G : {1, 2, 100, 65536, 1 << 18})
+          for (int N : {1, 8, 16, 21, 64}) {
+            if (C % G) continue;
+            const bool fwd = call("scan_fwd", B, T, C, G * 100ll + N, gdn2_selective_scan_fwd(
+                nullptr, B, T, C, G, N, GDN2_BF16, GDN2_F32, 1, ins, nullptr, f, f, f, nullptr, nullptr,
+                p, f, f, p, kAll));
+            const bool bwd = call("scan_bwd", B, T, C, G * 100ll + N, gdn2_selective_scan_bwd(
+                nullptr, B, T, C, G, N, GDN2_F32, GDN2_F32, 1, ins, nullptr, f, f, f, nullptr, p,
+                nullptr, f, f, outs, f, f, f, f, p, kAll));
+            g_fail += fwd != bwd;
+            g_taken += fwd + bwd, g_calls += 2;
+            if (T == 1) {
+              g_taken += call("scan_step", B, C, G, N, gdn2_selective_scan_step(
+                  nullptr, B, C, G, N, GDN2_F32, GDN2_F32, 1, p, p, f, p, p, f, p, f, f, f, p));
+              ++g_calls;
+            }
+          }
+}
+
 static void fp8() {
   for (int M : kSizes)
     for (int N : kSizes) {
@@ -117,6 +142,7 @@ static void fp8() {
 
 int main() {
   conv();
+  scan();
   fp8();
   std::printf("%ld calls, %ld taken, %d failures\n", g_calls, g_taken, g_fail);
   return g_fail || !g_taken ? 1 : 0;

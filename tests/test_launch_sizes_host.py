@@ -9,7 +9,7 @@ import pytest
 
 ROOT = Path(__file__).resolve().parents[1]
 CSRC = ROOT / "gdn2-jax-kernel_amd" / "csrc"
-SOURCES = ["gdn2_conv.hip", "gdn2_fp8.hip"]
+SOURCES = ["gdn2_conv.hip", "gdn2_ssm.hip", "gdn2_fp8.hip"]
 
 
 def test_every_size_that_is_taken_can_be_launched(tmp_path):
