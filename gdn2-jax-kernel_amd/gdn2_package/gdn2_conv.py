@@ -193,4 +193,4 @@ def gdn2_short_conv_step(x, weight, bias=None, state=None, activation="silu", in
                          new.data_ptr(), y.data_ptr())
         if rc:
             _raise(rc, f"{what} (B,C,W)=({B},{C},{W})")
-    return _as(y, x.dtype), _as(new, x.dtype)
+    return _as(y, x.dtype), new if inplace else _as(new, x.dtype)
