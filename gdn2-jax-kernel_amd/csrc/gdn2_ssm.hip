@@ -429,8 +429,9 @@ __global__ void __launch_bounds__(kThreads, NP <= 16 ? 4 : 2) ssm_rev(SsmArgs a)
   a.sum[((long long)w.b * nch + w.chunk) * a.C + w.c] = fresh ? kNegInf : S;
 }
 
-// What enters each chunk, from the compositions: a thread a state of a channel, the chunks in
-// order (REV: from the last).
+// What enters each chunk but the first, from the compositions: a thread a state of a channel, the
+// chunks in order (REV: from the last).  What enters the first is h0 (the gradient of h_final), which
+// the walks read themselves.
 constexpr int kJoin = 64;   // threads: few states are to reach all CUs
 template <int NP, bool REV>
 __global__ void __launch_bounds__(kJoin) ssm_join(SsmArgs a) {
@@ -447,7 +448,6 @@ __global__ void __launch_bounds__(kJoin) ssm_join(SsmArgs a) {
   const long long at = ((long long)b * nch + (REV ? nch - 1 : 0)) * a.C + c;
   float* slot = a.slot + at * NP + n;
   const float* sum = a.sum + at;
-  if (REV) *slot = h;    // the forward's first chunk reads h0 itself
   // compositions are read sixteen at a time, the next while these are applied (1 x 4001 x 1536 x 16, 126
   // chunks: 13 us; eight at a time, each waited for, 17)
   constexpr int U = 16;
