@@ -11,8 +11,8 @@ nothing of what came before enters it, NaN included, and no gradient passes it. 
 in the reference.
 
 Sums are float32.  x is float32 or bfloat16 (other types are widened to float32), weight and
-bias are used in float32.  x may be strided as long as its channels are contiguous; otherwise it
-is copied.
+bias are used in float32.  The convolution's x may be strided as long as its channels are contiguous;
+otherwise it is copied, as the step's is wherever it is not dense.
 """
 from __future__ import annotations
 

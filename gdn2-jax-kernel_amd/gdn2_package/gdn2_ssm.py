@@ -14,9 +14,9 @@ nothing of what came before enters it, NaN included, and no gradient passes it. 
 counterpart in the reference.
 
 Arithmetic is float32.  x, B, C and z are float32 or bfloat16 (mixed or other types are widened
-to float32), dt is of x's type or float32; A, D, dt_bias and the states are float32.  Inputs may be
-strided as long as the values of a token are contiguous (the parts of one projection's output);
-others are copied.
+to float32), dt is of x's type or float32; A, D, dt_bias and the states are float32.  The scan's
+inputs may be strided as long as the values of a token are contiguous (the parts of one projection's
+output); others are copied.  The step's are copied wherever they are not dense, those parts too.
 """
 from __future__ import annotations
 
