@@ -9,8 +9,8 @@
 A block's scale is the smallest power of two s with max|t| <= 448 s, and its values are held as
 e4m3(t / s) (torch.float8_e4m3fn, ties to even): the one rounding there is.  A block of zeros has
 scale 0; one that holds NaN or an infinity has scale NaN and q = 0, so that all that is computed
-from it is NaN.  The product takes any float32 scales, so a weight may come from a checkpoint
-that was quantised otherwise.
+from it is NaN.  The product takes any float32 scales whose products with each other are zero or
+normal float32 numbers, so a weight may come from a checkpoint that was quantised otherwise.
 
 Rows of q start at multiples of 16 bytes: where the width is none, q is a view of a wider
 tensor; the scales of rows are laid out block by block (a transposed view).  The product takes both

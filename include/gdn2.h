@@ -542,7 +542,9 @@ int gdn2_dequantize_fp8(void* stream, int M, int C, int out_dtype, const void* q
 /* out[m][n] = sum_b x_scale[b][m] s[n][b] sum_{k in block b} x[m][k] w[n][k] + bias[n] (bias float32
  * or NULL), out (M,N) dense of out_dtype; x (M,K) and w (N,K).  s[n][b] is w_scale[b][n] with
  * w_row_block 1, w_scale[n / 128][b] with 128; *_scale_stride are the elements between rows of
- * the scales (at least M; N or ceil(K/128)); they may have any values.  Products of a block are
+ * the scales (at least M; N or ceil(K/128)).  A scale may have any value as long as its product with
+ * each of the other operand's is zero or a normal float32 number: the two may be multiplied
+ * first.  Products of a block are
  * summed by the matrix cores, blocks in float32: exactly as float32 sums for float32 results; for
  * bfloat16 ones at the 8-bit instruction's rate, which drops what lies below 2^-13 of the largest of
  * eight neighbouring products.  Otherwise as gdn2_int8_matmul. */
